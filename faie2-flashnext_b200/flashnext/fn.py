@@ -41,6 +41,7 @@ EXPORTS = [
     "fn_decoder_create", "fn_decoder_free", "fn_decoder_step", "fn_decoder_launches",
     "fn_load", "fn_forward", "fn_reset", "fn_free", "fn_debug_layers", "fn_use_graphs", "fn_n_past", "fn_last_ms",
     "fn_dev_gb", "fn_split", "fn_model_dims",
+    "fn_kv4_plan", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
 ]
 
 
@@ -58,6 +59,11 @@ class FnModel(C.Structure):
         ("final_norm", C.c_void_p), ("inv_freq", C.c_void_p), ("fuse_norm", C.c_int), ("prefetch", C.c_int)] + [
         (n, C.c_void_p) for n in ("hidden", "xnorm", "proj", "core", "Q", "att", "router_out", "logits", "tokens", "pos",
                                   "next", "prompt_len")]
+
+
+class FnKv4(C.Structure):
+    """fn_kv4_t (include/faie2fn.h): a paged 4-bit KV cache."""
+    _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_int), ("page_size", C.c_int), ("nkv", C.c_int), ("hd", C.c_int)]
 
 
 class FN:
@@ -128,6 +134,13 @@ class FN:
         d.fn_moe_prefetch_after.argtypes = [C.c_int, vp, C.c_uint64]
         d.fn_w_norm.argtypes = [C.c_int, vp, C.c_float]
         d.fn_moe_norm.argtypes = [C.c_int, vp, C.c_float]
+        i64, kv4 = C.c_int64, C.POINTER(FnKv4)
+        d.fn_kv4_plan.argtypes = [C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, vp, vp, C.c_int] + [vp] * 7
+        d.fn_kv4_store.argtypes = [kv4, C.c_uint32, vp, i64, i64, vp, i64, i64, vp, C.c_int, vp]
+        d.fn_kv4_load.argtypes = [kv4, C.c_uint32, vp, C.c_int, vp, vp, vp]
+        d.fn_kv4_attn_workspace.restype = C.c_uint64
+        d.fn_kv4_attn.argtypes = [kv4, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, i64, i64, vp, i64, i64, vp, i64, vp, vp,
+                                  vp, C.c_int, C.c_int, C.c_float, vp, C.c_uint64, vp]
         d.fn_tc_create.argtypes = [C.c_uint32, U8, C.c_int, C.c_int]
         d.fn_tc_free.argtypes = [C.c_int]
         d.fn_tc_gemv.argtypes = [C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp]
@@ -479,6 +492,27 @@ class FN:
         ms = C.c_float()
         self.check(self.d.fn_bench_tc_gemv(int(qtype), rows, cols, nt, iters, C.byref(ms)))
         return ms.value
+
+    # ---- paged KV cache in 4 bits (device pointers, 0 = null; flashnext/kv4.py is the layer over torch tensors) ----
+    def kv4_plan(self, n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out, max_tokens, cu,
+                 kv_len, slots, positions, requests, status, stream=0):
+        self.check(self.d.fn_kv4_plan(n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out,
+                                      max_tokens, cu, kv_len, slots, positions, requests, status, stream))
+
+    def kv4_store(self, cache, dtype, k, k_token, k_head, v, v_token, v_head, slots, nt, stream=0):
+        """cache: FnKv4; dtype: ggml type id of the rows (0 = F32, 30 = BF16); strides in elements."""
+        self.check(self.d.fn_kv4_store(cache, dtype, k, k_token, k_head, v, v_token, v_head, slots, nt, stream))
+
+    def kv4_load(self, cache, dtype, slots, nt, k, v, stream=0):
+        self.check(self.d.fn_kv4_load(cache, dtype, slots, nt, k, v, stream))
+
+    def kv4_attn_workspace(self) -> int:
+        return self.d.fn_kv4_attn_workspace()
+
+    def kv4_attn(self, cache, dtype, n, rows, nh, q, q_token, q_head, gate, gate_token, gate_head, out, out_token, cu,
+                 kv_len, table, max_pages, max_new, scale, ws, ws_bytes, stream=0):
+        self.check(self.d.fn_kv4_attn(cache, dtype, n, rows, nh, q, q_token, q_head, gate, gate_token, gate_head, out,
+                                      out_token, cu, kv_len, table, max_pages, max_new, scale, ws, ws_bytes, stream))
 
     # ---- L2 prefetch hints of a decode chain ----
     def w_weights(self, h):

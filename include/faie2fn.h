@@ -292,6 +292,50 @@ int fn_moe_prefetch_after(int h, const void *ptr, uint64_t bytes);
 int fn_w_norm(int h, const float *w, float eps);
 int fn_moe_norm(int h, const float *w, float eps);
 
+/* ---- paged KV cache in 4 bits (no counterpart in the reference, whose caches are dense; engine/faie2fn.cu:1452-1690) --
+ * For requests of different lengths: keys and values live in pages of page_size (16, 32 or 64) tokens, in 4-bit codes.
+ * pages: [n_pages][nkv][record], 16-byte aligned device memory; a record holds page_size tokens of one kv head as K codes
+ * [hd / 64][page_size][32 bytes], V codes likewise, K scales fp16 [hd / 64][page_size], V scales likewise
+ * (2 page_size (hd / 2 + hd / 32) bytes). 64 dims of a token share a scale d; dim i of them is nibble i of the 32 bytes
+ * (low nibble first), a code c that stands for d (c - 8). hd: 64, 128 or 256. A slot is page * page_size + place.
+ * Row types: F32 (0) or BF16 (30). All calls launch on the stream and allocate nothing; nothing is kept between them. */
+typedef struct fn_kv4_t {
+    uint8_t *pages;
+    int n_pages, page_size, nkv, hd;
+} fn_kv4_t;
+/* Plan a step of n (1..4096) requests from their lengths (everything device memory). ctx[r]: tokens already cached, in the
+ * first ceil(ctx / page_size) pages of table row r ([n][max_pages] page ids); add[r] > 0: new tokens, 0: idle, < 0: the
+ * request is finished. Finished requests' pages are pushed on the stack of free pages (free_ids [n_pages], *free_in of
+ * them), in request order; then new pages are popped from its top, in request order, and entered into the table;
+ * *free_out (may be free_in) = pages left. cu [n + 1]: first row of each request among the step's new tokens, clipped to
+ * max_tokens; kv_len [n] (an array of its own): the new length, 0 for a finished or refused request; slots, positions,
+ * requests [max_tokens]: each row's slot, position and request (-1 where there is none). A request is refused (nothing
+ * taken, its rows' slots and positions -1) when its pages exceed max_pages, its rows max_tokens, or the free pages run
+ * out; *status = how many were. Lengths below zero count as zero. */
+int fn_kv4_plan(int n, const int *ctx, const int *add, int *table, int max_pages, int page_size, int *free_ids,
+                int n_pages, const int *free_in, int *free_out, int max_tokens, int *cu, int *kv_len, int64_t *slots,
+                int *positions, int *requests, int *status, void *stream);
+/* Quantise nt rows of keys and values ([nt][nkv][hd], token and head strides in elements, the hd values of a head
+ * adjacent) into their slots (< 0: skipped; past the pages: skipped, reported by fn_sync). Per 64 dims d = m / -8 with m
+ * the value of largest magnitude (of two opposite ones the positive), c = clamp(trunc(x (1 / d) + 8.5), 0, 15) in fp32, d
+ * then rounded to fp16. A block that holds a NaN or an infinity, or whose scale exceeds fp16, reads back as NaN. */
+int fn_kv4_store(const fn_kv4_t *c, uint32_t type, const void *k, int64_t k_token, int64_t k_head, const void *v,
+                 int64_t v_token, int64_t v_head, const int64_t *slots, int nt, void *stream);
+/* The values that slots stand for, k and v [nt][nkv][hd] (either may be NULL; 16-byte aligned); zeros for slots < 0. */
+int fn_kv4_load(const fn_kv4_t *c, uint32_t type, const int64_t *slots, int nt, void *k, void *v, void *stream);
+/* out[i] = softmax(scale q[i] . k) v (* sigmoid(gate[i])) for the rows of n requests: row i of request r (rows cu[r] ..
+ * cu[r + 1]) stands at position kv_len[r] - (cu[r + 1] - cu[r]) + its index and sees the keys up to itself; a row that
+ * sees none, or belongs to no request, comes out zero. nh query heads, head h reading kv head h / (nh / nkv) (nh / nkv
+ * <= 64). q, gate (NULL: none): rows x nh x hd with token and head strides in elements; out: token stride, heads
+ * adjacent; all of `type`, fp32 inside. table: page ids as fn_kv4_plan makes them ([n][max_pages]). max_new: the most rows of a request,
+ * or an upper bound (it chooses the kernel, not the result's definition). ws: fn_kv4_attn_workspace() bytes of device
+ * memory, 256-byte aligned, zeroed once before its first use; calls that may overlap need one each. */
+uint64_t fn_kv4_attn_workspace(void);
+int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const void *q, int64_t q_token, int64_t q_head,
+                const void *gate, int64_t gate_token, int64_t gate_head, void *out, int64_t out_token, const int *cu,
+                const int *kv_len, const int *table, int max_pages, int max_new, float scale, void *ws, uint64_t ws_bytes,
+                void *stream);
+
 /* ---- the decode step (the reference's layer_forward + forward, engine/faie2fn.cu:2370-2490) --------------------
  * One step of the hybrid MoE decoder over resident handles (fn_w_create, fn_gdn_create, fn_moe_create) and device
  * buffers the caller owns: the embedding row of tokens[*pos], per layer the input projection, the gated-DeltaNet core
