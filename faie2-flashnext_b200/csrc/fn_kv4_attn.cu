@@ -8,12 +8,18 @@
 // c 2^-20 four bits higher), exact, and the tensor cores take it as it is. One mask per two codes replaces the
 // conversion; the offset's term enters as the product's initial accumulator (K) or is subtracted at the end (V).
 //
-// Precision. fp32 rows: q (scaled per row by a power of two so that its largest value is 2^10..2^11) and p dv are split
-// into two fp16 numbers, 22 bits together, in two of the 16 rows of a matrix instruction (rows g and g + 8 of the A
-// operand), so the second half costs no instruction: an 8-row tile fills the 16. Their sums are fp32. bf16 rows: q is
-// exact in fp16 after scaling, p dv is rounded once to 11 bits (the output has 8), and a tile holds 16 rows. The softmax
-// runs in base 2 with one reference per row, the running maximum plus the running exponent of the largest dv, so p dv uses
-// fp16's range whatever the size of V; the reference changes scale the sums exactly like a new maximum does.
+// Orientation. Codes are the A operand (16 tokens x 16 dims for K, 16 dims x 16 tokens for V) and the query rows the B
+// operand's 8 columns: a group of 8 heads fills the instruction. The weights p dv come out of the score product with tokens
+// down and rows across and are turned by movmatrix, 8 x 8 at a time, into the second product's B operand.
+//
+// Precision. bf16 rows: q is exact in fp16 after scaling, p dv is rounded once to 11 bits (the output has 8). fp32 rows: q
+// and p dv are split into two fp16 numbers, 22 bits together, which costs a second instruction each. A tensor core drops
+// what lies some 24 bits below the nominal size of its largest term, and a code as a subnormal fp16 number lies up to 10
+// bits below its nominal size; so both first halves are whole numbers up to 2^11 (q scaled per row by a power of two, p dv by
+// the softmax's reference): all their products and sums are multiples of one unit, and exact. Floating halves lost 2.5e-6
+// of the output where this form loses 3e-7. Sums over more than 32 tokens are added in fp32 outside the tensor core, whose
+// own accumulation cuts instead of rounding. The softmax runs in base 2 with one reference per row, the running maximum
+// plus the running exponent of the largest |dv|, so that p dv uses fp16's range whatever the size of V.
 //
 // Work. A unit is 64 tokens of one kv head for one row tile (8 or 16 rows: the heads of a group, token after token). All
 // units of the call in a row are cut into equal runs, one per CTA, whatever request they belong to: each CTA finds its run
@@ -40,7 +46,8 @@ constexpr int KA_THREADS = 256;               // the computing warpgroup, and on
 constexpr int KA_REG_COPY = 40, KA_REG_COMP = 216;
 constexpr int KA_CTAS = 2;                    // per SM
 constexpr int KA_FAN = 16;                    // partial results joined at once
-constexpr int KA_MAX_GRID = 2048;             // CTAs the workspace has room for
+constexpr int KA_JOIN = 32;                   // .. and at most in the second round
+constexpr int KA_MAX_GRID = KA_FAN * KA_JOIN; // CTAs at most
 
 struct Kv4AttnArgs {
     Kv4Lay l;
@@ -87,6 +94,18 @@ __device__ __forceinline__ uint32_t ka_pack(float a, float b) {
     return *(const uint32_t *)&h;
 }
 __device__ __forceinline__ float2 ka_unpack(uint32_t w) { return __half22float2(*(const __half2 *)&w); }
+// an 8 x 8 matrix of halves, row g columns 2t, 2t + 1 in lane 4 g + t, turned
+__device__ __forceinline__ uint32_t ka_turn(uint32_t w) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ float ka_half(const uint8_t *p) { return __half2float(*(const __half *)p); }
+// the weight of a part whose reference is `ref` beside the common one; a part without a key has none, and a row that has
+// nothing but NaN scores keeps them through the reference 0
+__device__ __forceinline__ float ka_weight(float ref, float common) {
+    return ka_exp2(ref == -INFINITY ? (common == -INFINITY ? 0.0f : -INFINITY) : ref - common);
+}
 __device__ __forceinline__ void ka_bar() { asm volatile("bar.sync 1, %0;" ::"n"(32 * KA_CONS) : "memory"); }
 // the same, and whether any thread brought `p`
 __device__ __forceinline__ bool ka_bar_or(bool p) {
@@ -105,35 +124,37 @@ template <typename T> __device__ __forceinline__ float ka_f(T x);
 template <> __device__ __forceinline__ float ka_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ float ka_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-template <int HD, bool HL> struct KaCfg {
+template <int HD, bool HL, int NT> struct KaCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
-    static constexpr int NG = HD / KV4_GROUP, ROWS = HL ? 8 : 16;
+    static constexpr int NG = HD / KV4_GROUP, ROWS = 8 * NT;
+    static constexpr int OS = HD + 1;                         // floats between rows of the merged sums (banks)
     static constexpr uint32_t STAGE = KA_TOK * HD / 16 * 17;  // bytes of 64 tokens of one head
-    static constexpr uint32_t QF = NG * 4 * 32 * 16;          // q as A operands: [group][step][lane] x 16 bytes
-    static constexpr uint32_t OB = ROWS * HD * 4;
+    static constexpr uint32_t QF = NT * NG * 4 * 32 * (HL ? 16 : 8);  // q as B operands: [n-tile][group][step][lane]
+    static constexpr uint32_t OB = (ROWS * OS * 4 + 127) / 128 * 128;
     // the merged sums share their place with q, which is rebuilt for the next row tile
     static constexpr uint32_t Q_OFF = 1024, ST_OFF = Q_OFF + (QF > OB ? QF : OB);
-    static constexpr uint32_t SMEM_MAX = 111 * 1024;          // of two CTAs on an SM (113 KB each, less static memory)
+    static constexpr uint32_t SMEM_MAX = 112 * 1024;          // of two CTAs on an SM (114 KB each, less static memory)
     // stages, an even number: a slot then always belongs to the same pair of warps, whose waits see each of its phases
     static constexpr int S = (SMEM_MAX - ST_OFF) / STAGE > 16 ? 16 : (SMEM_MAX - ST_OFF) / STAGE / 2 * 2;
     static constexpr uint32_t SMEM = ST_OFF + S * STAGE;
-    static constexpr int PART = ROWS * HD + 2 * ROWS;         // floats of a partial result
 };
 constexpr int KA_PART_MAX = 16 * 256 + 32;
 
-template <int HD, bool HL> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
-    using C = KaCfg<HD, HL>;
+template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
+    using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
-    constexpr int NG = C::NG, ROWS = C::ROWS, S = C::S;
+    constexpr int NG = C::NG, ROWS = C::ROWS, S = C::S, OS = C::OS;
+    using QF = std::conditional_t<HL, uint4, uint2>;
     extern __shared__ __align__(128) uint8_t sm_ka[];
     __shared__ long long red[KA_THREADS / 32], s_off;
     __shared__ int s_req;
     __shared__ volatile int s_fail;
-    __shared__ float s_rs[16], s_qs[16][NG], s_ref[KA_CONS][16], s_l[KA_CONS][16], s_mref[16], s_ml[16];
+    __shared__ float s_rs[ROWS], s_qs[2][ROWS][NG], s_ref[KA_CONS][ROWS], s_l[KA_CONS][ROWS], s_mref[ROWS], s_ml[ROWS];
+    __shared__ float s_join[KA_JOIN][ROWS];
     __shared__ int s_last;
     __shared__ uint32_t s_valid[S];
     uint64_t *full = (uint64_t *)sm_ka, *empty = full + S;
-    uint4 *qf = (uint4 *)(sm_ka + C::Q_OFF);
+    QF *qf = (QF *)(sm_ka + C::Q_OFF);
     float *ob = (float *)(sm_ka + C::Q_OFF);
     uint8_t *ring = sm_ka + C::ST_OFF;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -264,29 +285,27 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS
     // ---- compute
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KA_REG_COMP));
     const int g = lane >> 2, t = lane & 3, half = warp & 1, pair = warp >> 1;
-    // column n of an 8-token product is token n ^ (n >> 2): with it both the K reads (8 bytes of 4 tokens x 4 lanes) and
-    // the V reads (4 bytes of 4 tokens x 8 words) touch 32 different banks
+    // index n of 8 tokens is token n ^ (n >> 2): with it both the K reads (8 bytes of 8 tokens x 4 lanes, 16 lanes at a
+    // time) and the V reads (4 bytes of 4 tokens x 8 words) touch 32 different banks
     const int tk = g ^ (g >> 2);
-    const int tv0 = (2 * t) ^ (t >> 1), tv1 = (2 * t + 1) ^ (t >> 1);  // columns 2t, 2t + 1: one aligned pair of tokens
-    const bool swap = t >= 2;                                          // whose second is column 2t
-    const int tp = tv0 & ~1;
+    const int tv0 = (2 * t) ^ (t >> 1), tv1 = (2 * t + 1) ^ (t >> 1);
     int it = 0;
     for (long long u = u0; u < u1;) {
         const int kend = (int)min((long long)rq.tiles, k + (u1 - u)), kv = item / rq.rt, tile = item - kv * rq.rt;
         const int nrow = min(ROWS, rq.fresh * a.group - tile * ROWS);
-        // ---- q of the row tile into A operands
+        // ---- q of the row tile into B operands
         ka_bar();
         {
             constexpr int L = 32 * KA_CONS / ROWS, PG = KV4_GROUP / L;  // lanes of a row; dims of a group each takes
             const int i = tid / L, sub = tid % L, flat = tile * ROWS + i, tok = flat / a.group;
             const T *src = (const T *)after_wait(a.q) + (int64_t)(rq.first + tok) * a.qt +
-                           (int64_t)(kv * a.group + flat - tok * a.group) * a.qh;
+                           (int64_t)(kv * a.group + flat - tok * a.group) * a.qh + sub * PG;
             float x[NG][PG], mx = 0.0f;
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
                 for (int j = 0; j < PG; ++j) {
-                    x[gi][j] = i < nrow ? ka_f<T>(src[gi * KV4_GROUP + sub * PG + j]) : 0.0f;
+                    x[gi][j] = i < nrow ? ka_f<T>(src[gi * KV4_GROUP + j]) : 0.0f;
                     mx = fmaxf(mx, fabsf(x[gi][j]));
                 }
 #pragma unroll
@@ -295,49 +314,57 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
-                float sum = 0.0f;
+                float sum = 0.0f, sum_lo = 0.0f;
 #pragma unroll
                 for (int j = 0; j < PG; ++j) {
                     const int d = sub * PG + j, w = d >> 3, nib = d & 7, step = (w & 1) * 2 + ((nib & 3) >> 1);
-                    const float f = x[gi][j] * up * (nib & 1 ? 0.0625f : 1.0f);
-                    const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
-                    sum += (__half2float(hi) + (HL ? __half2float(lo) : 0.0f)) * (nib & 1 ? 16.0f : 1.0f);
-                    __half *dst = (__half *)&qf[(gi * 4 + step) * 32 + (i & 7) * 4 + (w >> 1)];
-                    // A registers: 0 = row g, 1 = row g + 8 (k low), 2, 3 the same (k high)
-                    const int reg = (nib & 1) * 2;
-                    if constexpr (HL) {
-                        dst[reg * 2 + (nib >> 2)] = hi;
-                        dst[(reg + 1) * 2 + (nib >> 2)] = lo;
-                    } else {
-                        dst[(reg + (i >> 3)) * 2 + (nib >> 2)] = hi;
-                    }
+                    const float f = x[gi][j] * up, fh = HL ? rintf(f) : f, fl = f - fh;
+                    const float sc = nib & 1 ? 0.0625f : 1.0f;  // odd nibbles stand 16 times as high
+                    const __half lo = __float2half_rn(fl);
+                    sum += fh;
+                    sum_lo += __half2float(lo);
+                    __half *dst = (__half *)&qf[(((i >> 3) * NG + gi) * 4 + step) * 32 + (i & 7) * 4 + (w >> 1)];
+                    dst[(nib & 1) * 2 + (nib >> 2)] = __float2half_rn(fh * sc);
+                    if constexpr (HL) dst[(2 + (nib & 1)) * 2 + (nib >> 2)] = __float2half_rn(__half2float(lo) * sc);
                 }
 #pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (sub == 0) s_qs[i][gi] = sum * (-8.0f / 16777216.0f);
+                for (int o = L / 2; o > 0; o >>= 1) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (HL) sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, o);
+                }
+                if (sub == 0) {
+                    s_qs[0][i][gi] = sum * (-8.0f / 16777216.0f);
+                    if (HL) s_qs[1][i][gi] = sum_lo * (-8.0f / 16777216.0f);
+                }
             }
             // scores in base 2: undo the scaling and the codes' 2^-24
             if (sub == 0) s_rs[i] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(24 - e + 127) << 23);
         }
         ka_bar();
-        // rows see tokens below lim; rows past the tile's last see what the last sees (their results are dropped)
+        // rows see tokens below their limit; rows past the tile's last see what the last sees (their results are dropped)
         auto limit = [&](int i) {
             const int f = tile * ROWS + min(i, nrow - 1);
             return min(max(rq.len - rq.fresh + f / a.group + 1, 0), rq.len);
         };
-        const int lim0 = limit(g), lim1 = HL ? lim0 : limit(g + 8), lo_lim = limit(0), hi_lim = limit(ROWS - 1);
-        const float rs0 = s_rs[g], rs1 = HL ? rs0 : s_rs[(g + 8) & (ROWS - 1)];
-        float qs0[NG], qs1[NG];
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) qs0[gi] = s_qs[g][gi], qs1[gi] = HL ? 0.0f : s_qs[(g + 8) & (ROWS - 1)][gi];
-        float o[NG][8][4], corr0[NG], corr1[NG], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        float ref0 = -INFINITY, ref1 = -INFINITY;
+        const int lo_lim = limit(0), hi_lim = limit(ROWS - 1);
+        int lim[NT][2];
+        // o[n-tile][group][byte]: rows 2t, 2t + 1 of the tile for dim 8 g + 2 byte, then for the dim after it
+        float o[NT][NG][4][4], corr[NT][NG][2], m[NT][2], l[NT][2], ref[NT][2];
         int ev = -40;
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-            corr0[gi] = corr1[gi] = 0.0f;
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[gi][i][0] = o[gi][i][1] = o[gi][i][2] = o[gi][i][3] = 0.0f;
+            for (int c = 0; c < 2; ++c) {
+                lim[n][c] = limit(8 * n + 2 * t + c);
+                m[n][c] = ref[n][c] = -INFINITY;
+                l[n][c] = 0.0f;
+            }
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+                corr[n][gi][0] = corr[n][gi][1] = 0.0f;
+#pragma unroll
+                for (int by = 0; by < 4; ++by) o[n][gi][by][0] = o[n][gi][by][1] = o[n][gi][by][2] = o[n][gi][by][3] = 0.0f;
+            }
         }
         bool alive = true;
         for (int j = k; j < kend; ++j, ++it) {
@@ -360,279 +387,318 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS
                 rec[b] = st + pg * a.l.rec;
                 pl[b] = at - pg * a.l.bs;
             }
-            // ---- scores: sc[n-tile][row g: columns 2t, 2t + 1 | row g + 8]
-            float sc[4][4];
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+            // ---- scores sc[n-tile][run][tokens tk, tk + 8][rows 2t, 2t + 1]
+            float sc[NT][2][2][2] = {};
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
-                uint4 A[4];
+                QF B[NT][4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) A[x] = qf[(gi * 4 + x) * 32 + lane];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const uint8_t *rc = rec[nt >> 1];
-                    const int line = gi * a.l.bs + pl[nt >> 1] + (nt & 1) * 8;
-                    const uint2 w = *(const uint2 *)(rc + (line + tk) * 32 + t * 8);
-                    float acc[4] = {qs0[gi], qs0[gi], qs1[gi], qs1[gi]};
-                    ka_mma(acc, A[0], w.x & 0x000f000fu, w.x & 0x00f000f0u);
-                    ka_mma(acc, A[1], (w.x >> 8) & 0x000f000fu, (w.x >> 8) & 0x00f000f0u);
-                    ka_mma(acc, A[2], w.y & 0x000f000fu, w.y & 0x00f000f0u);
-                    ka_mma(acc, A[3], (w.y >> 8) & 0x000f000fu, (w.y >> 8) & 0x00f000f0u);
-                    uint32_t dw = *(const uint32_t *)(rc + 2 * a.l.kb + (line + tp) * 2);
-                    if (swap) dw = __byte_perm(dw, 0, 0x1032);
-                    const float2 d = ka_unpack(dw);
-                    if constexpr (HL) {
-                        sc[nt][0] += (acc[0] + acc[2]) * d.x;
-                        sc[nt][1] += (acc[1] + acc[3]) * d.y;
-                    } else {
-                        sc[nt][0] += acc[0] * d.x;
-                        sc[nt][1] += acc[1] * d.y;
-                        sc[nt][2] += acc[2] * d.x;
-                        sc[nt][3] += acc[3] * d.y;
+                    for (int x = 0; x < 4; ++x) B[n][x] = qf[((n * NG + gi) * 4 + x) * 32 + lane];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int line = gi * a.l.bs + pl[b] + tk;
+                    const uint2 w = *(const uint2 *)(rec[b] + line * 32 + t * 8), v = *(const uint2 *)(rec[b] + (line + 8) * 32 + t * 8);
+                    const float d0 = ka_half(rec[b] + 2 * a.l.kb + line * 2), d1 = ka_half(rec[b] + 2 * a.l.kb + (line + 8) * 2);
+                    const uint4 A0 = make_uint4(w.x & 0x000f000fu, v.x & 0x000f000fu, w.x & 0x00f000f0u, v.x & 0x00f000f0u);
+                    const uint4 A1 = make_uint4((w.x >> 8) & 0x000f000fu, (v.x >> 8) & 0x000f000fu, (w.x >> 8) & 0x00f000f0u, (v.x >> 8) & 0x00f000f0u);
+                    const uint4 A2 = make_uint4(w.y & 0x000f000fu, v.y & 0x000f000fu, w.y & 0x00f000f0u, v.y & 0x00f000f0u);
+                    const uint4 A3 = make_uint4((w.y >> 8) & 0x000f000fu, (v.y >> 8) & 0x000f000fu, (w.y >> 8) & 0x00f000f0u, (v.y >> 8) & 0x00f000f0u);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float i0 = s_qs[0][8 * n + 2 * t][gi], i1 = s_qs[0][8 * n + 2 * t + 1][gi];
+                        float acc[4] = {i0, i1, i0, i1};
+                        ka_mma(acc, A0, B[n][0].x, B[n][0].y);
+                        ka_mma(acc, A1, B[n][1].x, B[n][1].y);
+                        ka_mma(acc, A2, B[n][2].x, B[n][2].y);
+                        ka_mma(acc, A3, B[n][3].x, B[n][3].y);
+                        if constexpr (HL) {
+                            const float j0 = s_qs[1][8 * n + 2 * t][gi], j1 = s_qs[1][8 * n + 2 * t + 1][gi];
+                            float low[4] = {j0, j1, j0, j1};
+                            ka_mma(low, A0, B[n][0].z, B[n][0].w);
+                            ka_mma(low, A1, B[n][1].z, B[n][1].w);
+                            ka_mma(low, A2, B[n][2].z, B[n][2].w);
+                            ka_mma(low, A3, B[n][3].z, B[n][3].w);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[x] += low[x];
+                        }
+                        sc[n][b][0][0] += acc[0] * d0;
+                        sc[n][b][0][1] += acc[1] * d0;
+                        sc[n][b][1][0] += acc[2] * d1;
+                        sc[n][b][1][1] += acc[3] * d1;
                     }
                 }
             }
-            // ---- V scales of this lane's tokens, and the largest exponent among the warp's
-            uint32_t dv[4][NG];
-            __half2 dmax = __float2half2_rn(0.0f);
+            // ---- V scales of this lane's tokens, and the largest among the warp's
+            float dv[2][2][NG], dm = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const int b = t0 + nt * 8;
-                uint32_t keep = 0xffffffffu;
-                if (masked) {
-                    const bool there = valid >> ((half * 32 + nt * 8) / a.l.bs) & 1u;
-                    keep = (there && b + tv0 < hi_lim ? 0xffffu : 0u) | (there && b + tv1 < hi_lim ? 0xffff0000u : 0u);
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int tok = t0 + b * 16 + h * 8 + tk;
+                    const bool drop = masked && (!(valid >> ((half * 32 + b * 16 + h * 8) / a.l.bs) & 1u) || tok >= hi_lim);
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) {
+                        const float d = ka_half(rec[b] + 2 * a.l.kb + a.l.sb + (gi * a.l.bs + pl[b] + h * 8 + tk) * 2);
+                        dv[b][h][gi] = drop ? 0.0f : d;  // what nobody sees counts for nothing, whatever is there
+                        dm = fmaxf(dm, fabsf(dv[b][h][gi]));
+                    }
                 }
 #pragma unroll
-                for (int gi = 0; gi < NG; ++gi) {
-                    uint32_t w = *(const uint32_t *)(rec[nt >> 1] + 2 * a.l.kb + a.l.sb + (gi * a.l.bs + pl[nt >> 1] + (nt & 1) * 8 + tp) * 2);
-                    if (swap) w = __byte_perm(w, 0, 0x1032);
-                    w &= keep;
-                    dv[nt][gi] = w;
-                    dmax = __hmax2(dmax, __habs2(*(const __half2 *)&w));
-                }
-            }
-            float dm = fmaxf(__low2float(dmax), __high2float(dmax));
-            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 1));
-            dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, 2));
+            for (int x = 4; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
             ev = max(ev, (int)(__float_as_uint(dm) >> 23) - 127);
-            // ---- running softmax in base 2
+            // ---- running softmax in base 2: p = exp2(s - reference), |p dv| < 2^11
+            bool moved = false;
+            float z[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                sc[nt][0] *= rs0;
-                sc[nt][1] *= rs0;
-                if constexpr (!HL) {
-                    sc[nt][2] *= rs1;
-                    sc[nt][3] *= rs1;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float rs = s_rs[8 * n + 2 * t + c];
+                    float mx = m[n][c];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float s = sc[n][b][h][c] * rs;
+                            if (masked) {
+                                const int tok = t0 + b * 16 + h * 8 + tk;
+                                if (!(valid >> ((half * 32 + b * 16 + h * 8) / a.l.bs) & 1u) || tok >= lim[n][c]) s = -INFINITY;
+                            }
+                            sc[n][b][h][c] = s;
+                            mx = fmaxf(mx, s);
+                        }
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    m[n][c] = mx;
+                    const float nr = mx + (float)(ev - 10);
+                    moved |= nr != ref[n][c];
+                    z[n][c] = nr == -INFINITY ? 0.0f : nr;
                 }
-                if (masked) {
-                    const int b = t0 + nt * 8;
-                    const bool there = valid >> ((half * 32 + nt * 8) / a.l.bs) & 1u;
-                    if (!there || b + tv0 >= lim0) sc[nt][0] = -INFINITY;
-                    if (!there || b + tv1 >= lim0) sc[nt][1] = -INFINITY;
-                    if constexpr (!HL) {
-                        if (!there || b + tv0 >= lim1) sc[nt][2] = -INFINITY;
-                        if (!there || b + tv1 >= lim1) sc[nt][3] = -INFINITY;
-                    }
-                }
-                m0 = fmaxf(m0, fmaxf(sc[nt][0], sc[nt][1]));
-                if constexpr (!HL) m1 = fmaxf(m1, fmaxf(sc[nt][2], sc[nt][3]));
-            }
-            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-            if constexpr (!HL) {
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-            }
-            const float n0 = m0 + (float)(ev - 11), n1 = m1 + (float)(ev - 11);
-            const bool moved = n0 != ref0 || (!HL && n1 != ref1);
-            const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;
             if (__any_sync(0xffffffffu, moved)) {
-                const float f0 = ka_exp2(ref0 - z0), f1 = HL ? f0 : ka_exp2(ref1 - z1);
-                l0 *= f0;
-                l1 *= f1;
 #pragma unroll
-                for (int gi = 0; gi < NG; ++gi) {
-                    corr0[gi] *= f0;
-                    corr1[gi] *= f1;
+                for (int n = 0; n < NT; ++n) {
+                    const float f0 = ka_exp2(ref[n][0] - z[n][0]), f1 = ka_exp2(ref[n][1] - z[n][1]);
+                    l[n][0] *= f0;
+                    l[n][1] *= f1;
+                    ref[n][0] = m[n][0] + (float)(ev - 10);
+                    ref[n][1] = m[n][1] + (float)(ev - 10);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        o[gi][i][0] *= f0;
-                        o[gi][i][1] *= f0;
-                        o[gi][i][2] *= f1;
-                        o[gi][i][3] *= f1;
+                    for (int gi = 0; gi < NG; ++gi) {
+                        corr[n][gi][0] *= f0;
+                        corr[n][gi][1] *= f1;
+#pragma unroll
+                        for (int by = 0; by < 4; ++by) {
+                            o[n][gi][by][0] *= f0;
+                            o[n][gi][by][1] *= f1;
+                            o[n][gi][by][2] *= f0;
+                            o[n][gi][by][3] *= f1;
+                        }
                     }
                 }
-                ref0 = n0;
-                ref1 = n1;
             }
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                sc[nt][0] = ka_exp2(sc[nt][0] - z0);
-                sc[nt][1] = ka_exp2(sc[nt][1] - z0);
-                l0 += sc[nt][0] + sc[nt][1];
-                if constexpr (!HL) {
-                    sc[nt][2] = ka_exp2(sc[nt][2] - z1);
-                    sc[nt][3] = ka_exp2(sc[nt][3] - z1);
-                    l1 += sc[nt][2] + sc[nt][3];
-                }
-            }
-            // ---- out += (p dv) c, 16 tokens at a time
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int gi = 0; gi < NG; ++gi) {
-                    const float2 da = ka_unpack(dv[2 * b][gi]), db = ka_unpack(dv[2 * b + 1][gi]);
-                    const float(&sa)[4] = sc[2 * b], (&sb)[4] = sc[2 * b + 1];
-                    // a token that a row does not see weighs nothing whatever its scale is (NaN)
-                    auto weigh = [&](float p, float d) { return masked && p == 0.0f ? 0.0f : p * d; };
-                    const float x0 = weigh(sa[0], da.x), x1 = weigh(sa[1], da.y), x2 = weigh(sb[0], db.x), x3 = weigh(sb[1], db.y);
-                    uint4 A;
-                    A.x = ka_pack(x0, x1);
-                    A.z = ka_pack(x2, x3);
-                    corr0[gi] += (x0 + x1) + (x2 + x3);
-                    if constexpr (HL) {
-                        const float2 h0 = ka_unpack(A.x), h1 = ka_unpack(A.z);
-                        A.y = ka_pack(x0 - h0.x, x1 - h0.y);
-                        A.w = ka_pack(x2 - h1.x, x3 - h1.y);
-                    } else {
-                        const float y0 = weigh(sa[2], da.x), y1 = weigh(sa[3], da.y), y2 = weigh(sb[2], db.x), y3 = weigh(sb[3], db.y);
-                        A.y = ka_pack(y0, y1);
-                        A.w = ka_pack(y2, y3);
-                        corr1[gi] += (y0 + y1) + (y2 + y3);
-                    }
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            sc[n][b][h][c] = ka_exp2(sc[n][b][h][c] - z[n][c]);
+                            l[n][c] += sc[n][b][h][c];
+                        }
+            // ---- out += c (p dv)
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+                uint32_t P[NT][2][2], Q[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g; second halves
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float p0 = sc[n][b][h][0], p1 = sc[n][b][h][1], d = dv[b][h][gi];
+                            // a token that a row does not see weighs nothing whatever its scale is (NaN)
+                            const float x0 = masked && p0 == 0.0f ? 0.0f : p0 * d, x1 = masked && p1 == 0.0f ? 0.0f : p1 * d;
+                            corr[n][gi][0] += x0;
+                            corr[n][gi][1] += x1;
+                            if constexpr (HL) {
+                                const float big = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers
+                                const float h0 = __fadd_rn(__fadd_rn(x0, big), -big), h1 = __fadd_rn(__fadd_rn(x1, big), -big);
+                                P[n][b][h] = ka_turn(ka_pack(h0, h1));
+                                Q[n][b][h] = ka_turn(ka_pack(x0 - h0, x1 - h1));
+                            } else {
+                                P[n][b][h] = ka_turn(ka_pack(x0, x1));
+                            }
+                        }
+                uint32_t w[2][4];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
                     const uint8_t *vc = rec[b] + a.l.kb + (gi * a.l.bs + pl[b]) * 32 + g * 4;
-                    const uint32_t w0 = *(const uint32_t *)(vc + tv0 * 32), w1 = *(const uint32_t *)(vc + tv1 * 32);
-                    const uint32_t w2 = *(const uint32_t *)(vc + (8 + tv0) * 32), w3 = *(const uint32_t *)(vc + (8 + tv1) * 32);
+                    w[b][0] = *(const uint32_t *)(vc + tv0 * 32);
+                    w[b][1] = *(const uint32_t *)(vc + tv1 * 32);
+                    w[b][2] = *(const uint32_t *)(vc + (8 + tv0) * 32);
+                    w[b][3] = *(const uint32_t *)(vc + (8 + tv1) * 32);
+                }
 #pragma unroll
-                    for (int by = 0; by < 4; ++by) {
-                        const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
-                        const uint32_t x = __byte_perm(w0, w1, sel), y = __byte_perm(w2, w3, sel);
-                        ka_mma(o[gi][2 * by], A, x & 0x000f000fu, y & 0x000f000fu);
-                        ka_mma(o[gi][2 * by + 1], A, x & 0x00f000f0u, y & 0x00f000f0u);
+                for (int by = 0; by < 4; ++by) {
+                    const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
+                    uint4 A[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t x = __byte_perm(w[b][0], w[b][1], sel), y = __byte_perm(w[b][2], w[b][3], sel);
+                        A[b] = make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if constexpr (HL) {
+                            float acc[4] = {};
+                            ka_mma(acc, A[0], P[n][0][0], P[n][0][1]);
+                            ka_mma(acc, A[1], P[n][1][0], P[n][1][1]);
+                            ka_mma(acc, A[0], Q[n][0][0], Q[n][0][1]);
+                            ka_mma(acc, A[1], Q[n][1][0], Q[n][1][1]);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[n][gi][by][x] += acc[x];
+                        } else {
+                            ka_mma(o[n][gi][by], A[0], P[n][0][0], P[n][0][1]);
+                            ka_mma(o[n][gi][by], A[1], P[n][1][0], P[n][1][1]);
+                        }
                     }
                 }
             }
             __syncwarp();
             if (lane == 0) ka_arrive(&empty[sl]);
         }
+
         // ---- merge the four warps: one reference per row, sums added quarter by quarter in a fixed order
 #pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+        for (int x = 4; x < 32; x <<= 1)
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-                corr0[gi] += __shfl_xor_sync(0xffffffffu, corr0[gi], x);
-                corr1[gi] += __shfl_xor_sync(0xffffffffu, corr1[gi], x);
-            }
-        }
-        if (t == 0) {
-            s_ref[warp][g] = ref0;
-            s_l[warp][g] = l0;
-            if constexpr (!HL) {
-                s_ref[warp][g + 8] = ref1;
-                s_l[warp][g + 8] = l1;
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) corr[n][gi][c] += __shfl_xor_sync(0xffffffffu, corr[n][gi][c], x);
+                }
+        if (g == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    s_ref[warp][8 * n + 2 * t + c] = ref[n][c];
+                    s_l[warp][8 * n + 2 * t + c] = l[n][c];
+                }
         }
         if (ka_bar_or(!alive)) return;  // a wait gave up: all warps leave here together
         auto top = [&](int i) { return fmaxf(fmaxf(s_ref[0][i], s_ref[1][i]), fmaxf(s_ref[2][i], s_ref[3][i])); };
-        const float t0 = top(g), t1 = HL ? t0 : top(g + 8);
-        // a warp without a key has nothing; a row whose scores are all NaN keeps them through the reference 0
-        const float f0 = ka_exp2((ref0 == -INFINITY ? (t0 == -INFINITY ? 0.0f : -INFINITY) : ref0 - t0));
-        const float f1 = HL ? f0 : ka_exp2((ref1 == -INFINITY ? (t1 == -INFINITY ? 0.0f : -INFINITY) : ref1 - t1));
+        float wf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) wf[n][c] = ka_weight(ref[n][c], top(8 * n + 2 * t + c));
         if (tid < ROWS) {
             const float tt = top(tid);
-            float l = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < KA_CONS; ++w)
-                l += s_l[w][tid] * ka_exp2(s_ref[w][tid] == -INFINITY ? (tt == -INFINITY ? 0.0f : -INFINITY) : s_ref[w][tid] - tt);
+            for (int w = 0; w < KA_CONS; ++w) sum += s_l[w][tid] * ka_weight(s_ref[w][tid], tt);
             s_mref[tid] = tt;
-            s_ml[tid] = l;
+            s_ml[tid] = sum;
         }
         for (int round = 0; round < 4; ++round) {
 #pragma unroll
-            for (int qd = 0; qd < 4; ++qd) {
-                if (((warp + round) & 3) != qd) continue;
+            for (int by = 0; by < 4; ++by) {
+                if (((warp + round) & 3) != by) continue;
 #pragma unroll
-                for (int x = qd * NG * 2; x < (qd + 1) * NG * 2; ++x) {  // 8 NG products of 8 columns, a quarter of them
-                    const int gi = x >> 3, i = x & 7;
-                    const float up = i & 1 ? 1048576.0f : 16777216.0f;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int cc = 0; cc < 2; ++cc) {
-                        const int d = gi * KV4_GROUP + 8 * (2 * t + cc) + i;
-                        const float v0 = ((HL ? o[gi][i][cc] + o[gi][i][2 + cc] : o[gi][i][cc]) * up - 8.0f * corr0[gi]) * f0;
-                        float *p = ob + g * HD + d;
-                        *p = round ? *p + v0 : v0;
-                        if constexpr (!HL) {
-                            const float v1 = (o[gi][i][2 + cc] * up - 8.0f * corr1[gi]) * f1;
-                            p += 8 * HD;
-                            *p = round ? *p + v1 : v1;
+                    for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float v = (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * corr[n][gi][x & 1]) * wf[n][x & 1];
+                            float *p = ob + (8 * n + 2 * t + (x & 1)) * OS + gi * KV4_GROUP + 8 * g + 2 * by + (x >> 1);
+                            *p = round ? *p + v : v;
                         }
-                    }
-                }
             }
             ka_bar();
         }
-        // the row tile's output, from sums and weights of any place
-        auto emit = [&](auto sums, auto weight) {
-            for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) {
-                const int i = e / HD, d = e - i * HD, f = tile * ROWS + i, tok = f / a.group, h = kv * a.group + f - tok * a.group;
+        // the row tile's output: a warp takes a row at a time
+        auto emit = [&]() {
+            for (int i = warp; i < nrow; i += KA_CONS) {
+                const int f = tile * ROWS + i, tok = f / a.group, h = kv * a.group + f - tok * a.group;
                 const int64_t row = rq.first + tok;
-                float y = 0.0f;
-                if (limit(i) > 0) {
-                    y = sums(i, d) / weight(i);
-                    if (a.gate) y *= sigm(ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + d]));
+                const bool sees = limit(i) > 0;
+                const float inv = s_ml[i];
+                for (int d = lane; d < HD; d += 32) {
+                    float y = sees ? ob[i * OS + d] / inv : 0.0f;
+                    if (a.gate && sees) y *= sigm(ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + d]));
+                    ((T *)a.out)[row * a.ot + (int64_t)h * HD + d] = (T)y;
                 }
-                ((T *)a.out)[row * a.ot + (int64_t)h * HD + d] = (T)y;
             }
         };
         if (k == 0 && kend == rq.tiles) {
-            emit([&](int i, int d) { return ob[i * HD + d]; }, [&](int i) { return s_ml[i]; });
+            emit();
         } else {
             // ---- a part of a row tile: into the workspace; the last CTA of 16 joins them, the last of those the rest
-            const long long first = u - k;  // the row tile's first unit (of this run's numbering)
+            const long long first = u - k;  // the row tile's first unit
             const int c0 = (int)(first / per), c1 = (int)((first + rq.tiles - 1) / per), c = blockIdx.x;
-            auto slot = [&](int cta) {  // a CTA's part lies at its run's start (0) or after it (1)
-                return a.part + ((size_t)cta * 2 + (cta == c0 && first != c0 * per)) * KA_PART_MAX;
-            };
-            float *my = slot(c);
-            for (int e = tid * 4; e < ROWS * HD; e += 32 * KA_CONS * 4) __stcg((float4 *)(my + e), *(const float4 *)(ob + e));
-            if (tid < ROWS) {
-                __stcg(my + ROWS * HD + tid, s_mref[tid]);
-                __stcg(my + ROWS * HD + ROWS + tid, s_ml[tid]);
-            }
-            // joins `count` parts at CTAs b, b + step, ..; into ob / s_mref / s_ml
-            auto join = [&](int b, int step, int count) {
+            const int edge = first != c0 * per;  // a CTA's part lies at its run's start (0) or after it (1)
+            auto slot = [&](int cta) { return a.part + ((size_t)cta * 2 + (cta == c0 ? edge : 0)) * KA_PART_MAX; };
+            auto put = [&](float *to) {
+                for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) __stcg(to + e, ob[e / HD * OS + e % HD]);
                 if (tid < ROWS) {
-                    float m = -INFINITY, l = 0.0f;
-                    for (int x = 0; x < count; ++x) m = fmaxf(m, __ldcg(slot(b + x * step) + ROWS * HD + tid));
-                    for (int x = 0; x < count; ++x) {
-                        const float *p = slot(b + x * step) + ROWS * HD;
-                        const float rf = __ldcg(p + tid);
-                        l += __ldcg(p + ROWS + tid) * ka_exp2(rf == -INFINITY ? (m == -INFINITY ? 0.0f : -INFINITY) : rf - m);
-                    }
-                    s_mref[tid] = m;
-                    s_ml[tid] = l;
+                    __stcg(to + ROWS * HD + tid, s_mref[tid]);
+                    __stcg(to + ROWS * HD + ROWS + tid, s_ml[tid]);
                 }
+            };
+            put(slot(c));
+            // joins the parts of CTAs b, b + step, .. into ob, s_mref and s_ml
+            auto join = [&](int b, int step, int count) {
+                for (int x = tid; x < count * ROWS; x += 32 * KA_CONS)
+                    s_join[x / ROWS][x % ROWS] = __ldcg(slot(b + x / ROWS * step) + ROWS * HD + x % ROWS);
                 ka_bar();
-                for (int e = tid * 4; e < ROWS * HD; e += 32 * KA_CONS * 4) {
-                    const float m = s_mref[e / HD];
-                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (tid < ROWS) {
+                    float mx = -INFINITY, sum = 0.0f;
+                    for (int x = 0; x < count; ++x) mx = fmaxf(mx, s_join[x][tid]);
 #pragma unroll 8
                     for (int x = 0; x < count; ++x) {
-                        const float *p = slot(b + x * step);
-                        const float rf = __ldcg(p + ROWS * HD + e / HD);
-                        const float f = ka_exp2(rf == -INFINITY ? (m == -INFINITY ? 0.0f : -INFINITY) : rf - m);
-                        const float4 v = __ldcg((const float4 *)(p + e));
-                        y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+                        const float f = ka_weight(s_join[x][tid], mx);
+                        s_join[x][tid] = f;
+                        sum += f * __ldcg(slot(b + x * step) + ROWS * HD + ROWS + tid);
                     }
-                    *(float4 *)(ob + e) = y;
+                    s_mref[tid] = mx;
+                    s_ml[tid] = sum;
+                }
+                ka_bar();
+                constexpr int E = ROWS * HD / (32 * KA_CONS * 4), U = E >= 8 ? 1 : E >= 4 ? 2 : 4;  // loads in flight: 8 at least
+                float4 y[E] = {};
+                for (int x0 = 0; x0 < count; x0 += U) {
+                    float4 v[U][E];
+#pragma unroll
+                    for (int x = 0; x < U; ++x)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (x0 + x < count) v[x][e] = __ldcg((const float4 *)(slot(b + (x0 + x) * step)) + tid + e * 32 * KA_CONS);
+#pragma unroll
+                    for (int x = 0; x < U; ++x)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (x0 + x < count) {
+                                const float f = s_join[x0 + x][(tid + e * 32 * KA_CONS) * 4 / HD];
+                                y[e].x += f * v[x][e].x, y[e].y += f * v[x][e].y, y[e].z += f * v[x][e].z, y[e].w += f * v[x][e].w;
+                            }
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int at = (tid + e * 32 * KA_CONS) * 4;
+                    float *p = ob + at / HD * OS + at % HD;
+                    p[0] = y[e].x, p[1] = y[e].y, p[2] = y[e].z, p[3] = y[e].w;
                 }
                 ka_bar();
             };
-            // true for the last of `count` arrivals (all of this CTA's stores before it are visible to that one)
+            // true for the last of `count` arrivals (all that the others stored before theirs is visible to it)
             auto last_of = [&](uint32_t *counter, int count) {
                 __threadfence();
                 ka_bar();
@@ -647,21 +713,15 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS
             };
             const int parts = c1 - c0 + 1, gr = (c - c0) / KA_FAN, gb = c0 + gr * KA_FAN, gn = min(KA_FAN, c1 - gb + 1);
             bool mineis = last_of(a.cnt + (gr ? KA_MAX_GRID : 0) + gb, gn);
-            if (mineis) {
-                join(gb, 1, gn);
-                if (parts > KA_FAN) {
-                    float *to = slot(gb);
-                    for (int e = tid * 4; e < ROWS * HD; e += 32 * KA_CONS * 4) __stcg((float4 *)(to + e), *(const float4 *)(ob + e));
-                    if (tid < ROWS) {
-                        __stcg(to + ROWS * HD + tid, s_mref[tid]);
-                        __stcg(to + ROWS * HD + ROWS + tid, s_ml[tid]);
-                    }
-                    const int groups = (parts + KA_FAN - 1) / KA_FAN;
-                    mineis = last_of(a.cnt + 2 * KA_MAX_GRID + c0, groups);
-                    if (mineis) join(c0, KA_FAN, groups);
-                }
+            int jb = gb, step = 1, count = gn;
+            while (mineis) {
+                join(jb, step, count);
+                if (step == KA_FAN || parts <= KA_FAN) break;
+                put(slot(gb));
+                jb = c0, step = KA_FAN, count = (parts + KA_FAN - 1) / KA_FAN;
+                mineis = last_of(a.cnt + 2 * KA_MAX_GRID + c0, count);
             }
-            if (mineis) emit([&](int i, int d) { return ob[i * HD + d]; }, [&](int i) { return s_ml[i]; });
+            if (mineis) emit();
         }
         u += kend - k;
         if (u < u1) next();
@@ -677,10 +737,21 @@ FN_API uint64_t fn_kv4_attn_workspace(void) {
     return 3 * KA_MAX_GRID * 4 + (uint64_t)std::min(num_sms() * KA_CTAS, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
 }
 
-template <int HD, bool HL> static cudaError_t attn_go(const Kv4AttnArgs &a, int grid, cudaStream_t s) {
-    const cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL>);
+template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long units, cudaStream_t s) {
+    const cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL, NT>);
     if (e != cudaSuccess) return e;
-    return launch_k(k_kv4_attn<HD, HL>, dim3(grid), dim3(KA_THREADS), KaCfg<HD, HL>::SMEM, s, a);
+    const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KA_CTAS, KA_MAX_GRID));
+    return launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KA_THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+}
+template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
+    // requests whose rows fill one column tile of 8 take the narrow form
+    const long long rows = (long long)std::min(max_new, a.rows) * a.group;
+    const int nt = rows <= 8 ? 1 : 2;
+    // the most units there can be: no more CTAs than pairs of them
+    const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
+    const long long units = (long long)a.n * a.l.nkv * std::max((rows + 8 * nt - 1) / (8 * nt), 1ll) * tiles;
+    if (nt == 1) return f32 ? attn_launch<HD, true, 1>(a, units, s) : attn_launch<HD, false, 1>(a, units, s);
+    return f32 ? attn_launch<HD, true, 2>(a, units, s) : attn_launch<HD, false, 2>(a, units, s);
 }
 
 FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const void *q, int64_t q_token,
@@ -707,16 +778,10 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         a.cnt = (uint32_t *)ws;
         a.part = (float *)((uint8_t *)ws + 3 * KA_MAX_GRID * 4);
         const bool f32 = type == T_F32;
-        // no more CTAs than there can be pairs of units
-        const long long tiles = ((long long)max_pages * c->page_size + KA_TOK - 1) / KA_TOK;
-        const long long rt = ((long long)std::min(max_new, rows) * a.group + (f32 ? 7 : 15)) / (f32 ? 8 : 16);
-        const long long most = std::max(1ll, (long long)n * c->nkv * rt * tiles / 2);
-        const int grid = (int)std::min(most, (long long)std::min(num_sms() * KA_CTAS, KA_MAX_GRID));
-        cudaError_t e;
         const cudaStream_t s = (cudaStream_t)stream;
-        if (c->hd == 64) e = f32 ? attn_go<64, true>(a, grid, s) : attn_go<64, false>(a, grid, s);
-        else if (c->hd == 128) e = f32 ? attn_go<128, true>(a, grid, s) : attn_go<128, false>(a, grid, s);
-        else e = f32 ? attn_go<256, true>(a, grid, s) : attn_go<256, false>(a, grid, s);
+        const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
+                            : c->hd == 128 ? attn_go<128>(a, f32, max_new, s)
+                                           : attn_go<256>(a, f32, max_new, s);
         if (e != cudaSuccess) return fail(std::string("kv4 attn launch: ") + cudaGetErrorString(e));
         return 0;
     });
