@@ -24,8 +24,9 @@
 // Work. A unit is 64 tokens of one kv head for one row tile (8 or 16 rows: the heads of a group, token after token). All
 // units of the call in a row are cut into equal runs, one per CTA, whatever request they belong to: each CTA finds its run
 // from the lengths by a prefix sum, so nothing about the lengths is known on the host and a captured call serves any.
-// A row tile whose units lie in several CTAs is joined by the last of them to finish (groups of 16 first, then the
-// groups), in the order of the CTAs, so the result does not depend on timing.
+// A row tile whose units lie in several CTAs leaves a partial result in each; a second small kernel joins them in the order
+// of the CTAs, so the result does not depend on timing (joining in the CTA that finishes last cost 20 us of latency chains
+// for 147 parts, beside 33 us of work; the second kernel takes a few).
 //
 // A CTA: one warp copies pages into a ring (one bulk copy per page and head: codes and scales of K and V), four warps
 // compute, two on each 64-token stage, 32 tokens each, with their own running softmax; they merge at the end of a run.
@@ -45,9 +46,7 @@ constexpr int KA_THREADS = 256;               // the computing warpgroup, and on
 // which holds 8 or 16 rows of 256 sums
 constexpr int KA_REG_COPY = 40, KA_REG_COMP = 216;
 constexpr int KA_CTAS = 2;                    // per SM
-constexpr int KA_FAN = 16;                    // partial results joined at once
-constexpr int KA_JOIN = 32;                   // .. and at most in the second round
-constexpr int KA_MAX_GRID = KA_FAN * KA_JOIN; // CTAs at most
+constexpr int KA_MAX_GRID = 512;              // CTAs at most
 
 struct Kv4AttnArgs {
     Kv4Lay l;
@@ -58,8 +57,13 @@ struct Kv4AttnArgs {
     const int *cu, *kv_len, *table;
     float scale;
     float *part;     // [CTA][2]: a row tile's sums [rows][hd], references [rows], sums of weights [rows]
-    uint32_t *cnt;   // [3][KA_MAX_GRID] arrivals, zero between calls
+    struct KaSplit *split;  // [CTA]: the row tile that starts in the CTA's run and goes on past it
     uint32_t *err;
+};
+
+struct KaSplit {
+    int parts, edge;        // CTAs it lies in (0: there is none); where the first one's part is
+    int req, kv, tile;
 };
 
 // a request's share of the work
@@ -79,7 +83,7 @@ template <int ROWS> __device__ __forceinline__ KaReq ka_req(const Kv4AttnArgs &a
 }
 
 __device__ __forceinline__ void ka_mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
@@ -140,6 +144,23 @@ template <int HD, bool HL, int NT> struct KaCfg {
 };
 constexpr int KA_PART_MAX = 16 * 256 + 32;
 
+// a row's output by one warp: value(d), gated
+template <typename T, int HD, typename V>
+__device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, int kv, int flat, int lane, bool sees, V value) {
+    const int tok = flat / a.group, h = kv * a.group + flat - tok * a.group;
+    const int64_t row = rq.first + tok;
+    float gate[HD / 32];
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x)
+        gate[x] = a.gate && sees ? ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + lane + 32 * x]) : 0.0f;
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) {
+        float y = sees ? value(lane + 32 * x) : 0.0f;
+        if (a.gate) y *= sigm(gate[x]);
+        ((T *)a.out)[row * a.ot + (int64_t)h * HD + lane + 32 * x] = (T)y;
+    }
+}
+
 template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
     using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
@@ -149,9 +170,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     __shared__ long long red[KA_THREADS / 32], s_off;
     __shared__ int s_req;
     __shared__ volatile int s_fail;
-    __shared__ float s_rs[ROWS], s_qs[2][ROWS][NG], s_ref[KA_CONS][ROWS], s_l[KA_CONS][ROWS], s_mref[ROWS], s_ml[ROWS];
-    __shared__ float s_join[KA_JOIN][ROWS];
-    __shared__ int s_last;
+    __shared__ __align__(8) float s_rs[ROWS], s_qs[2][NG][ROWS];
+    __shared__ float s_ref[KA_CONS][ROWS], s_l[KA_CONS][ROWS], s_mref[ROWS], s_ml[ROWS];
     __shared__ uint32_t s_valid[S];
     uint64_t *full = (uint64_t *)sm_ka, *empty = full + S;
     QF *qf = (QF *)(sm_ka + C::Q_OFF);
@@ -214,7 +234,10 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
         }
     }
     __syncthreads();
-    if (u0 >= u1) return;
+    if (u0 >= u1) {
+        if (tid == 0) a.split[blockIdx.x].parts = 0;
+        return;
+    }
 
     int r = s_req;
     KaReq rq = ka_req<ROWS>(a, r);
@@ -333,8 +356,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
                     if (HL) sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, o);
                 }
                 if (sub == 0) {
-                    s_qs[0][i][gi] = sum * (-8.0f / 16777216.0f);
-                    if (HL) s_qs[1][i][gi] = sum_lo * (-8.0f / 16777216.0f);
+                    s_qs[0][gi][i] = sum * (-8.0f / 16777216.0f);
+                    if (HL) s_qs[1][gi][i] = sum_lo * (-8.0f / 16777216.0f);
                 }
             }
             // scores in base 2: undo the scaling and the codes' 2^-24
@@ -349,23 +372,236 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
         const int lo_lim = limit(0), hi_lim = limit(ROWS - 1);
         int lim[NT][2];
         // o[n-tile][group][byte]: rows 2t, 2t + 1 of the tile for dim 8 g + 2 byte, then for the dim after it
-        float o[NT][NG][4][4], corr[NT][NG][2], m[NT][2], l[NT][2], ref[NT][2];
+        float o[NT][NG][4][4];
+        float2 corr[NT][NG], m[NT], l[NT], ref[NT];
         int ev = -40;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                lim[n][c] = limit(8 * n + 2 * t + c);
-                m[n][c] = ref[n][c] = -INFINITY;
-                l[n][c] = 0.0f;
-            }
+            lim[n][0] = limit(8 * n + 2 * t);
+            lim[n][1] = limit(8 * n + 2 * t + 1);
+            m[n] = ref[n] = make_float2(-INFINITY, -INFINITY);
+            l[n] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
-                corr[n][gi][0] = corr[n][gi][1] = 0.0f;
+                corr[n][gi] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int by = 0; by < 4; ++by) o[n][gi][by][0] = o[n][gi][by][1] = o[n][gi][by][2] = o[n][gi][by][3] = 0.0f;
             }
         }
+        // 32 tokens of a stage; M: some of them are hidden from some rows
+        auto step = [&](auto mk, const uint8_t *st, int t0, uint32_t valid) {
+            constexpr bool M = decltype(mk)::value;
+            // the run's first 16 tokens, and how far its second 16 are
+            const int at = half * 32, pg = at / a.l.bs, pl = at - pg * a.l.bs;
+            const uint8_t *rec = st + pg * a.l.rec;
+            const uint32_t code2 = a.l.bs == 16 ? a.l.rec : 512, scale2 = a.l.bs == 16 ? a.l.rec : 32;
+            const uint32_t cstep = a.l.bs * 32, sstep = a.l.bs * 2;  // to the next 64 dims
+            const uint8_t *kp = rec + (pl + tk) * 32 + t * 8, *ks = rec + 2 * a.l.kb + (pl + tk) * 2;
+            auto hidden = [&](int b, int h, int lm) {
+                return !(valid >> ((at + b * 16 + h * 8) / a.l.bs) & 1u) || t0 + b * 16 + h * 8 + tk >= lm;
+            };
+            // ---- scores of tokens tk, tk + 8 of both runs
+            float2 sc[NT][2][2] = {};
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+                QF B[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) B[n][x] = qf[((n * NG + gi) * 4 + x) * 32 + lane];
+                uint4 A[2][4];
+                float d[2][2], acc[NT][2][4], low[NT][2][4];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint8_t *c = kp + gi * cstep + b * code2, *s = ks + gi * sstep + b * scale2;
+                    const uint2 w = *(const uint2 *)c, v = *(const uint2 *)(c + 256);
+                    d[b][0] = ka_half(s), d[b][1] = ka_half(s + 16);
+                    const uint32_t w8 = w.x >> 8, v8 = v.x >> 8, x8 = w.y >> 8, y8 = v.y >> 8;
+                    A[b][0] = make_uint4(w.x & 0x000f000fu, v.x & 0x000f000fu, w.x & 0x00f000f0u, v.x & 0x00f000f0u);
+                    A[b][1] = make_uint4(w8 & 0x000f000fu, v8 & 0x000f000fu, w8 & 0x00f000f0u, v8 & 0x00f000f0u);
+                    A[b][2] = make_uint4(w.y & 0x000f000fu, v.y & 0x000f000fu, w.y & 0x00f000f0u, v.y & 0x00f000f0u);
+                    A[b][3] = make_uint4(x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 i0 = *(const float2 *)&s_qs[0][gi][8 * n + 2 * t];
+                        acc[n][b][0] = acc[n][b][2] = i0.x, acc[n][b][1] = acc[n][b][3] = i0.y;
+                        if constexpr (HL) {
+                            const float2 i1 = *(const float2 *)&s_qs[1][gi][8 * n + 2 * t];
+                            low[n][b][0] = low[n][b][2] = i1.x, low[n][b][1] = low[n][b][3] = i1.y;
+                        }
+                    }
+                }
+                // the sums of both runs (and halves) side by side: an instruction does not wait for the one before it
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            ka_mma(acc[n][b], A[b][x], B[n][x].x, B[n][x].y);
+                            if constexpr (HL) ka_mma(low[n][b], A[b][x], B[n][x].z, B[n][x].w);
+                        }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float2 s = make_float2(acc[n][b][2 * h], acc[n][b][2 * h + 1]);
+                            if constexpr (HL) s = __fadd2_rn(s, make_float2(low[n][b][2 * h], low[n][b][2 * h + 1]));
+                            sc[n][b][h] = __ffma2_rn(s, make_float2(d[b][h], d[b][h]), sc[n][b][h]);
+                        }
+            }
+            // ---- V scales of this lane's tokens, and the largest among the warp's
+            float dv[2][2][NG], dm = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bool drop = M && hidden(b, h, hi_lim);
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) {
+                        const float d = ka_half(ks + a.l.sb + gi * sstep + b * scale2 + h * 16);
+                        dv[b][h][gi] = drop ? 0.0f : d;  // what nobody sees counts for nothing, whatever is there
+                        dm = fmaxf(dm, fabsf(dv[b][h][gi]));
+                    }
+                }
+            // ---- running softmax in base 2: p = exp2(s - reference), |p dv| < 2^11
+            float2 mx[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 rs = *(const float2 *)&s_rs[8 * n + 2 * t];
+                mx[n] = m[n];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float2 s = __fmul2_rn(sc[n][b][h], rs);
+                        if constexpr (M) {
+                            if (hidden(b, h, lim[n][0])) s.x = -INFINITY;
+                            if (hidden(b, h, lim[n][1])) s.y = -INFINITY;
+                        }
+                        sc[n][b][h] = s;
+                        mx[n].x = fmaxf(mx[n].x, s.x);
+                        mx[n].y = fmaxf(mx[n].y, s.y);
+                    }
+            }
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mx[n].x = fmaxf(mx[n].x, __shfl_xor_sync(0xffffffffu, mx[n].x, x));
+                    mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, x));
+                }
+            }
+            ev = max(ev, (int)(__float_as_uint(dm) >> 23) - 127);
+            const float e = (float)(ev - 10);
+            bool moved = false;
+            float2 z[NT];  // minus the reference (0 for a row that has seen nothing)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                m[n] = mx[n];
+                const float2 nr = make_float2(mx[n].x + e, mx[n].y + e);
+                moved |= nr.x != ref[n].x || nr.y != ref[n].y;
+                z[n] = make_float2(nr.x == -INFINITY ? 0.0f : -nr.x, nr.y == -INFINITY ? 0.0f : -nr.y);
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float2 f = make_float2(ka_exp2(ref[n].x + z[n].x), ka_exp2(ref[n].y + z[n].y));
+                    l[n] = __fmul2_rn(l[n], f);
+                    ref[n] = make_float2(m[n].x + e, m[n].y + e);
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) {
+                        corr[n][gi] = __fmul2_rn(corr[n][gi], f);
+#pragma unroll
+                        for (int by = 0; by < 4; ++by)
+#pragma unroll
+                            for (int x = 0; x < 4; x += 2) {
+                                const float2 y = __fmul2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), f);
+                                o[n][gi][by][x] = y.x, o[n][gi][by][x + 1] = y.y;
+                            }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 x = __fadd2_rn(sc[n][b][h], z[n]);
+                        sc[n][b][h] = make_float2(ka_exp2(x.x), ka_exp2(x.y));
+                        l[n] = __fadd2_rn(l[n], sc[n][b][h]);
+                    }
+            // ---- out += c (p dv)
+            const uint8_t *vp0 = rec + a.l.kb + (pl + tv0) * 32 + g * 4, *vp1 = vp0 + (tv1 - tv0) * 32;
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+                uint32_t P[NT][2][2], Q[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g; second halves
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float d = dv[b][h][gi];
+                            float2 x = __fmul2_rn(sc[n][b][h], make_float2(d, d));
+                            // a token that a row does not see weighs nothing whatever its scale is (NaN)
+                            if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
+                            corr[n][gi] = __fadd2_rn(corr[n][gi], x);
+                            if constexpr (HL) {
+                                const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: rounds to whole numbers
+                                const float2 w = __fadd2_rn(__fadd2_rn(x, big), make_float2(-12582912.0f, -12582912.0f));
+                                const float2 r = __ffma2_rn(w, make_float2(-1.0f, -1.0f), x);
+                                P[n][b][h] = ka_turn(ka_pack(w.x, w.y));
+                                Q[n][b][h] = ka_turn(ka_pack(r.x, r.y));
+                            } else {
+                                P[n][b][h] = ka_turn(ka_pack(x.x, x.y));
+                            }
+                        }
+                uint4 A[4][2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint8_t *c0 = vp0 + gi * cstep + b * code2, *c1 = vp1 + gi * cstep + b * code2;
+                    const uint32_t w0 = *(const uint32_t *)c0, w1 = *(const uint32_t *)c1;
+                    const uint32_t w2 = *(const uint32_t *)(c0 + 256), w3 = *(const uint32_t *)(c1 + 256);
+#pragma unroll
+                    for (int by = 0; by < 4; ++by) {
+                        const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
+                        const uint32_t x = __byte_perm(w0, w1, sel), y = __byte_perm(w2, w3, sel);
+                        A[by][b] = make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (HL) {
+                        float acc[4][4] = {};
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int by = 0; by < 4; ++by) ka_mma(acc[by], A[by][b], P[n][b][0], P[n][b][1]);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int by = 0; by < 4; ++by) ka_mma(acc[by], A[by][b], Q[n][b][0], Q[n][b][1]);
+#pragma unroll
+                        for (int by = 0; by < 4; ++by)
+#pragma unroll
+                            for (int x = 0; x < 4; x += 2) {
+                                const float2 y = __fadd2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), make_float2(acc[by][x], acc[by][x + 1]));
+                                o[n][gi][by][x] = y.x, o[n][gi][by][x + 1] = y.y;
+                            }
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int by = 0; by < 4; ++by) ka_mma(o[n][gi][by], A[by][b], P[n][b][0], P[n][b][1]);
+                    }
+                }
+            }
+        };
         bool alive = true;
         for (int j = k; j < kend; ++j, ++it) {
             if ((it & 1) != pair) continue;
@@ -377,197 +613,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
             const uint8_t *st = ring + (size_t)sl * C::STAGE;
             const int t0 = j * KA_TOK + half * 32;  // this warp's first token
             const uint32_t valid = s_valid[sl];
-            const bool masked = t0 + 32 > lo_lim || valid != (1u << ppt) - 1u;
-            // record and place of this warp's two runs of 16 tokens
-            const uint8_t *rec[2];
-            int pl[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int at = half * 32 + b * 16, pg = at / a.l.bs;
-                rec[b] = st + pg * a.l.rec;
-                pl[b] = at - pg * a.l.bs;
-            }
-            // ---- scores sc[n-tile][run][tokens tk, tk + 8][rows 2t, 2t + 1]
-            float sc[NT][2][2][2] = {};
-#pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-                QF B[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) B[n][x] = qf[((n * NG + gi) * 4 + x) * 32 + lane];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int line = gi * a.l.bs + pl[b] + tk;
-                    const uint2 w = *(const uint2 *)(rec[b] + line * 32 + t * 8), v = *(const uint2 *)(rec[b] + (line + 8) * 32 + t * 8);
-                    const float d0 = ka_half(rec[b] + 2 * a.l.kb + line * 2), d1 = ka_half(rec[b] + 2 * a.l.kb + (line + 8) * 2);
-                    const uint4 A0 = make_uint4(w.x & 0x000f000fu, v.x & 0x000f000fu, w.x & 0x00f000f0u, v.x & 0x00f000f0u);
-                    const uint4 A1 = make_uint4((w.x >> 8) & 0x000f000fu, (v.x >> 8) & 0x000f000fu, (w.x >> 8) & 0x00f000f0u, (v.x >> 8) & 0x00f000f0u);
-                    const uint4 A2 = make_uint4(w.y & 0x000f000fu, v.y & 0x000f000fu, w.y & 0x00f000f0u, v.y & 0x00f000f0u);
-                    const uint4 A3 = make_uint4((w.y >> 8) & 0x000f000fu, (v.y >> 8) & 0x000f000fu, (w.y >> 8) & 0x00f000f0u, (v.y >> 8) & 0x00f000f0u);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float i0 = s_qs[0][8 * n + 2 * t][gi], i1 = s_qs[0][8 * n + 2 * t + 1][gi];
-                        float acc[4] = {i0, i1, i0, i1};
-                        ka_mma(acc, A0, B[n][0].x, B[n][0].y);
-                        ka_mma(acc, A1, B[n][1].x, B[n][1].y);
-                        ka_mma(acc, A2, B[n][2].x, B[n][2].y);
-                        ka_mma(acc, A3, B[n][3].x, B[n][3].y);
-                        if constexpr (HL) {
-                            const float j0 = s_qs[1][8 * n + 2 * t][gi], j1 = s_qs[1][8 * n + 2 * t + 1][gi];
-                            float low[4] = {j0, j1, j0, j1};
-                            ka_mma(low, A0, B[n][0].z, B[n][0].w);
-                            ka_mma(low, A1, B[n][1].z, B[n][1].w);
-                            ka_mma(low, A2, B[n][2].z, B[n][2].w);
-                            ka_mma(low, A3, B[n][3].z, B[n][3].w);
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) acc[x] += low[x];
-                        }
-                        sc[n][b][0][0] += acc[0] * d0;
-                        sc[n][b][0][1] += acc[1] * d0;
-                        sc[n][b][1][0] += acc[2] * d1;
-                        sc[n][b][1][1] += acc[3] * d1;
-                    }
-                }
-            }
-            // ---- V scales of this lane's tokens, and the largest among the warp's
-            float dv[2][2][NG], dm = 0.0f;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int tok = t0 + b * 16 + h * 8 + tk;
-                    const bool drop = masked && (!(valid >> ((half * 32 + b * 16 + h * 8) / a.l.bs) & 1u) || tok >= hi_lim);
-#pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) {
-                        const float d = ka_half(rec[b] + 2 * a.l.kb + a.l.sb + (gi * a.l.bs + pl[b] + h * 8 + tk) * 2);
-                        dv[b][h][gi] = drop ? 0.0f : d;  // what nobody sees counts for nothing, whatever is there
-                        dm = fmaxf(dm, fabsf(dv[b][h][gi]));
-                    }
-                }
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
-            ev = max(ev, (int)(__float_as_uint(dm) >> 23) - 127);
-            // ---- running softmax in base 2: p = exp2(s - reference), |p dv| < 2^11
-            bool moved = false;
-            float z[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float rs = s_rs[8 * n + 2 * t + c];
-                    float mx = m[n][c];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float s = sc[n][b][h][c] * rs;
-                            if (masked) {
-                                const int tok = t0 + b * 16 + h * 8 + tk;
-                                if (!(valid >> ((half * 32 + b * 16 + h * 8) / a.l.bs) & 1u) || tok >= lim[n][c]) s = -INFINITY;
-                            }
-                            sc[n][b][h][c] = s;
-                            mx = fmaxf(mx, s);
-                        }
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                    m[n][c] = mx;
-                    const float nr = mx + (float)(ev - 10);
-                    moved |= nr != ref[n][c];
-                    z[n][c] = nr == -INFINITY ? 0.0f : nr;
-                }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float f0 = ka_exp2(ref[n][0] - z[n][0]), f1 = ka_exp2(ref[n][1] - z[n][1]);
-                    l[n][0] *= f0;
-                    l[n][1] *= f1;
-                    ref[n][0] = m[n][0] + (float)(ev - 10);
-                    ref[n][1] = m[n][1] + (float)(ev - 10);
-#pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) {
-                        corr[n][gi][0] *= f0;
-                        corr[n][gi][1] *= f1;
-#pragma unroll
-                        for (int by = 0; by < 4; ++by) {
-                            o[n][gi][by][0] *= f0;
-                            o[n][gi][by][1] *= f1;
-                            o[n][gi][by][2] *= f0;
-                            o[n][gi][by][3] *= f1;
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            sc[n][b][h][c] = ka_exp2(sc[n][b][h][c] - z[n][c]);
-                            l[n][c] += sc[n][b][h][c];
-                        }
-            // ---- out += c (p dv)
-#pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-                uint32_t P[NT][2][2], Q[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g; second halves
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float p0 = sc[n][b][h][0], p1 = sc[n][b][h][1], d = dv[b][h][gi];
-                            // a token that a row does not see weighs nothing whatever its scale is (NaN)
-                            const float x0 = masked && p0 == 0.0f ? 0.0f : p0 * d, x1 = masked && p1 == 0.0f ? 0.0f : p1 * d;
-                            corr[n][gi][0] += x0;
-                            corr[n][gi][1] += x1;
-                            if constexpr (HL) {
-                                const float big = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers
-                                const float h0 = __fadd_rn(__fadd_rn(x0, big), -big), h1 = __fadd_rn(__fadd_rn(x1, big), -big);
-                                P[n][b][h] = ka_turn(ka_pack(h0, h1));
-                                Q[n][b][h] = ka_turn(ka_pack(x0 - h0, x1 - h1));
-                            } else {
-                                P[n][b][h] = ka_turn(ka_pack(x0, x1));
-                            }
-                        }
-                uint32_t w[2][4];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint8_t *vc = rec[b] + a.l.kb + (gi * a.l.bs + pl[b]) * 32 + g * 4;
-                    w[b][0] = *(const uint32_t *)(vc + tv0 * 32);
-                    w[b][1] = *(const uint32_t *)(vc + tv1 * 32);
-                    w[b][2] = *(const uint32_t *)(vc + (8 + tv0) * 32);
-                    w[b][3] = *(const uint32_t *)(vc + (8 + tv1) * 32);
-                }
-#pragma unroll
-                for (int by = 0; by < 4; ++by) {
-                    const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
-                    uint4 A[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t x = __byte_perm(w[b][0], w[b][1], sel), y = __byte_perm(w[b][2], w[b][3], sel);
-                        A[b] = make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if constexpr (HL) {
-                            float acc[4] = {};
-                            ka_mma(acc, A[0], P[n][0][0], P[n][0][1]);
-                            ka_mma(acc, A[1], P[n][1][0], P[n][1][1]);
-                            ka_mma(acc, A[0], Q[n][0][0], Q[n][0][1]);
-                            ka_mma(acc, A[1], Q[n][1][0], Q[n][1][1]);
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) o[n][gi][by][x] += acc[x];
-                        } else {
-                            ka_mma(o[n][gi][by], A[0], P[n][0][0], P[n][0][1]);
-                            ka_mma(o[n][gi][by], A[1], P[n][1][0], P[n][1][1]);
-                        }
-                    }
-                }
-            }
+            if (t0 + 32 > lo_lim || valid != (1u << ppt) - 1u) step(std::true_type{}, st, t0, valid);
+            else step(std::false_type{}, st, t0, valid);
             __syncwarp();
             if (lane == 0) ka_arrive(&empty[sl]);
         }
@@ -576,29 +623,28 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                l[n].x += __shfl_xor_sync(0xffffffffu, l[n].x, x);
+                l[n].y += __shfl_xor_sync(0xffffffffu, l[n].y, x);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
-#pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) corr[n][gi][c] += __shfl_xor_sync(0xffffffffu, corr[n][gi][c], x);
+                for (int gi = 0; gi < NG; ++gi) {
+                    corr[n][gi].x += __shfl_xor_sync(0xffffffffu, corr[n][gi].x, x);
+                    corr[n][gi].y += __shfl_xor_sync(0xffffffffu, corr[n][gi].y, x);
                 }
+            }
         if (g == 0) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    s_ref[warp][8 * n + 2 * t + c] = ref[n][c];
-                    s_l[warp][8 * n + 2 * t + c] = l[n][c];
-                }
+            for (int n = 0; n < NT; ++n) {
+                s_ref[warp][8 * n + 2 * t] = ref[n].x, s_ref[warp][8 * n + 2 * t + 1] = ref[n].y;
+                s_l[warp][8 * n + 2 * t] = l[n].x, s_l[warp][8 * n + 2 * t + 1] = l[n].y;
+            }
         }
         if (ka_bar_or(!alive)) return;  // a wait gave up: all warps leave here together
         auto top = [&](int i) { return fmaxf(fmaxf(s_ref[0][i], s_ref[1][i]), fmaxf(s_ref[2][i], s_ref[3][i])); };
-        float wf[NT][2];
+        float2 wf[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) wf[n][c] = ka_weight(ref[n][c], top(8 * n + 2 * t + c));
+            wf[n] = make_float2(ka_weight(ref[n].x, top(8 * n + 2 * t)), ka_weight(ref[n].y, top(8 * n + 2 * t + 1)));
         if (tid < ROWS) {
             const float tt = top(tid);
             float sum = 0.0f;
@@ -607,151 +653,148 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
             s_mref[tid] = tt;
             s_ml[tid] = sum;
         }
+        // (the quarter is a constant in each branch: as a variable index it would put the sums into local memory)
+        auto quarter = [&](auto q, int round) {
+            constexpr int by = decltype(q)::value;
+            float old[NT][NG][4];  // read together, then written together
+            auto at = [&](int n, int gi, int x) { return ob + (8 * n + 2 * t + (x & 1)) * OS + gi * KV4_GROUP + 8 * g + 2 * by + (x >> 1); };
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) old[n][gi][x] = round ? *at(n, gi, x) : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        *at(n, gi, x) = old[n][gi][x] + (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * (x & 1 ? corr[n][gi].y : corr[n][gi].x)) * (x & 1 ? wf[n].y : wf[n].x);
+        };
         for (int round = 0; round < 4; ++round) {
-#pragma unroll
-            for (int by = 0; by < 4; ++by) {
-                if (((warp + round) & 3) != by) continue;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int gi = 0; gi < NG; ++gi)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float v = (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * corr[n][gi][x & 1]) * wf[n][x & 1];
-                            float *p = ob + (8 * n + 2 * t + (x & 1)) * OS + gi * KV4_GROUP + 8 * g + 2 * by + (x >> 1);
-                            *p = round ? *p + v : v;
-                        }
-            }
+            const int q = (warp + round) & 3;
+            if (q == 0) quarter(std::integral_constant<int, 0>{}, round);
+            else if (q == 1) quarter(std::integral_constant<int, 1>{}, round);
+            else if (q == 2) quarter(std::integral_constant<int, 2>{}, round);
+            else quarter(std::integral_constant<int, 3>{}, round);
             ka_bar();
         }
-        // the row tile's output: a warp takes a row at a time
-        auto emit = [&]() {
+        const long long first = u - k;  // the row tile's first unit
+        const bool starts = k == 0, ends = kend == rq.tiles;
+        if (starts && ends) {
+            // the row tile's output: a warp takes a row at a time
             for (int i = warp; i < nrow; i += KA_CONS) {
-                const int f = tile * ROWS + i, tok = f / a.group, h = kv * a.group + f - tok * a.group;
-                const int64_t row = rq.first + tok;
-                const bool sees = limit(i) > 0;
-                const float inv = s_ml[i];
-                for (int d = lane; d < HD; d += 32) {
-                    float y = sees ? ob[i * OS + d] / inv : 0.0f;
-                    if (a.gate && sees) y *= sigm(ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + d]));
-                    ((T *)a.out)[row * a.ot + (int64_t)h * HD + d] = (T)y;
-                }
+                const float sum = s_ml[i];
+                ka_emit<T, HD>(a, rq, kv, tile * ROWS + i, lane, limit(i) > 0, [&](int d) { return ob[i * OS + d] / sum; });
             }
-        };
-        if (k == 0 && kend == rq.tiles) {
-            emit();
         } else {
-            // ---- a part of a row tile: into the workspace; the last CTA of 16 joins them, the last of those the rest
-            const long long first = u - k;  // the row tile's first unit
-            const int c0 = (int)(first / per), c1 = (int)((first + rq.tiles - 1) / per), c = blockIdx.x;
-            const int edge = first != c0 * per;  // a CTA's part lies at its run's start (0) or after it (1)
-            auto slot = [&](int cta) { return a.part + ((size_t)cta * 2 + (cta == c0 ? edge : 0)) * KA_PART_MAX; };
-            auto put = [&](float *to) {
-                for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) __stcg(to + e, ob[e / HD * OS + e % HD]);
-                if (tid < ROWS) {
-                    __stcg(to + ROWS * HD + tid, s_mref[tid]);
-                    __stcg(to + ROWS * HD + ROWS + tid, s_ml[tid]);
-                }
-            };
-            put(slot(c));
-            // joins the parts of CTAs b, b + step, .. into ob, s_mref and s_ml
-            auto join = [&](int b, int step, int count) {
-                for (int x = tid; x < count * ROWS; x += 32 * KA_CONS)
-                    s_join[x / ROWS][x % ROWS] = __ldcg(slot(b + x / ROWS * step) + ROWS * HD + x % ROWS);
-                ka_bar();
-                if (tid < ROWS) {
-                    float mx = -INFINITY, sum = 0.0f;
-                    for (int x = 0; x < count; ++x) mx = fmaxf(mx, s_join[x][tid]);
-#pragma unroll 8
-                    for (int x = 0; x < count; ++x) {
-                        const float f = ka_weight(s_join[x][tid], mx);
-                        s_join[x][tid] = f;
-                        sum += f * __ldcg(slot(b + x * step) + ROWS * HD + ROWS + tid);
-                    }
-                    s_mref[tid] = mx;
-                    s_ml[tid] = sum;
-                }
-                ka_bar();
-                constexpr int E = ROWS * HD / (32 * KA_CONS * 4), U = E >= 8 ? 1 : E >= 4 ? 2 : 4;  // loads in flight: 8 at least
-                float4 y[E] = {};
-                for (int x0 = 0; x0 < count; x0 += U) {
-                    float4 v[U][E];
-#pragma unroll
-                    for (int x = 0; x < U; ++x)
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            if (x0 + x < count) v[x][e] = __ldcg((const float4 *)(slot(b + (x0 + x) * step)) + tid + e * 32 * KA_CONS);
-#pragma unroll
-                    for (int x = 0; x < U; ++x)
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            if (x0 + x < count) {
-                                const float f = s_join[x0 + x][(tid + e * 32 * KA_CONS) * 4 / HD];
-                                y[e].x += f * v[x][e].x, y[e].y += f * v[x][e].y, y[e].z += f * v[x][e].z, y[e].w += f * v[x][e].w;
-                            }
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int at = (tid + e * 32 * KA_CONS) * 4;
-                    float *p = ob + at / HD * OS + at % HD;
-                    p[0] = y[e].x, p[1] = y[e].y, p[2] = y[e].z, p[3] = y[e].w;
-                }
-                ka_bar();
-            };
-            // true for the last of `count` arrivals (all that the others stored before theirs is visible to it)
-            auto last_of = [&](uint32_t *counter, int count) {
-                __threadfence();
-                ka_bar();
-                if (tid == 0) {
-                    const bool last = atomicAdd(counter, 1u) == (uint32_t)count - 1;
-                    if (last) *counter = 0;
-                    __threadfence();
-                    s_last = last;
-                }
-                ka_bar();
-                return s_last != 0;
-            };
-            const int parts = c1 - c0 + 1, gr = (c - c0) / KA_FAN, gb = c0 + gr * KA_FAN, gn = min(KA_FAN, c1 - gb + 1);
-            bool mineis = last_of(a.cnt + (gr ? KA_MAX_GRID : 0) + gb, gn);
-            int jb = gb, step = 1, count = gn;
-            while (mineis) {
-                join(jb, step, count);
-                if (step == KA_FAN || parts <= KA_FAN) break;
-                put(slot(gb));
-                jb = c0, step = KA_FAN, count = (parts + KA_FAN - 1) / KA_FAN;
-                mineis = last_of(a.cnt + 2 * KA_MAX_GRID + c0, count);
+            // a part of a row tile, at the run's start (0) or after it (1)
+            float *to = a.part + ((size_t)blockIdx.x * 2 + (u != u0)) * KA_PART_MAX;
+            for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) to[e] = ob[e / HD * OS + e % HD];
+            if (tid < ROWS) {
+                to[ROWS * HD + tid] = s_mref[tid];
+                to[ROWS * HD + ROWS + tid] = s_ml[tid];
             }
-            if (mineis) emit();
+        }
+        if (tid == 0 && u + kend - k == u1) {
+            KaSplit sp{0, 0, r, kv, tile};
+            if (starts && !ends) {
+                sp.parts = (int)((first + rq.tiles - 1) / per) - (int)blockIdx.x + 1;
+                sp.edge = u != u0;
+            }
+            a.split[blockIdx.x] = sp;
         }
         u += kend - k;
         if (u < u1) next();
     }
 }
 
+// ---- the join: CTA (c, row) adds the parts of the row tile that starts in run c and goes on past it. A warp takes every
+// fourth part (loads of many parts in flight), the four sums are added in the order of the warps.
+template <int HD, bool HL, int NT> __global__ void __launch_bounds__(128) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
+    using C = KaCfg<HD, HL, NT>;
+    using T = typename C::T;
+    constexpr int PER = HD / 32, U = 8;
+    __shared__ float s_w[KA_MAX_GRID], s_red[2][4], s_sum[4][HD];
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const KaSplit sp = after_wait(a.split)[c];
+    if (sp.parts == 0) return;
+    const KaReq rq = ka_req<C::ROWS>(a, sp.req);
+    const int flat = sp.tile * C::ROWS + i;
+    if (flat >= rq.fresh * a.group) return;
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0 ? sp.edge : 0)) * KA_PART_MAX; };
+    float mx = -INFINITY;
+    for (int x = tid; x < sp.parts; x += 128) {
+        const float rf = slot(x)[C::ROWS * HD + i];
+        s_w[x] = rf;
+        mx = fmaxf(mx, rf);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) s_red[0][warp] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    for (int x = tid; x < sp.parts; x += 128) s_w[x] = ka_weight(s_w[x], mx);
+    __syncthreads();
+    float y[PER] = {}, sum = 0.0f;
+    for (int x0 = warp; x0 < sp.parts; x0 += 4 * U) {
+        float v[U][PER], w[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const bool in = x0 + 4 * x < sp.parts;
+            const float *p = slot(in ? x0 + 4 * x : 0);
+            w[x] = in ? s_w[x0 + 4 * x] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
+            sum += in ? w[x] * p[C::ROWS * HD + C::ROWS + i] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x)
+#pragma unroll
+            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
+    }
+#pragma unroll
+    for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
+    if (lane == 0) s_red[1][warp] = sum;
+    __syncthreads();
+    if (warp) return;
+    sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
+    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees,
+                   [&](int d) { return ((s_sum[0][d] + s_sum[1][d]) + (s_sum[2][d] + s_sum[3][d])) / sum; });
+}
+
 }  // namespace fn
 
 using namespace fn;
 
-// counters, then every CTA's two partial results
+// every CTA's split row tile, then its two partial results
 FN_API uint64_t fn_kv4_attn_workspace(void) {
-    return 3 * KA_MAX_GRID * 4 + (uint64_t)std::min(num_sms() * KA_CTAS, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
+    return KA_MAX_GRID * sizeof(KaSplit) + (uint64_t)std::min(num_sms() * KA_CTAS, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
 }
 
-template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long units, cudaStream_t s) {
-    const cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL, NT>);
+template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
+    cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL, NT>);
     if (e != cudaSuccess) return e;
+    // no more CTAs than pairs of units there can be; a row tile of one pair is never split
+    const long long units = items * tiles;
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KA_CTAS, KA_MAX_GRID));
-    return launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KA_THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+    e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KA_THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+    if (e != cudaSuccess || grid == 1) return e;
+    return launch_k(k_kv4_join<HD, HL, NT>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(128), 0, s, a);
 }
 template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
     // requests whose rows fill one column tile of 8 take the narrow form
     const long long rows = (long long)std::min(max_new, a.rows) * a.group;
     const int nt = rows <= 8 ? 1 : 2;
-    // the most units there can be: no more CTAs than pairs of them
+    // the most row tiles, and units of one, that there can be
     const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
-    const long long units = (long long)a.n * a.l.nkv * std::max((rows + 8 * nt - 1) / (8 * nt), 1ll) * tiles;
-    if (nt == 1) return f32 ? attn_launch<HD, true, 1>(a, units, s) : attn_launch<HD, false, 1>(a, units, s);
-    return f32 ? attn_launch<HD, true, 2>(a, units, s) : attn_launch<HD, false, 2>(a, units, s);
+    const long long items = (long long)a.n * a.l.nkv * std::max((rows + 8 * nt - 1) / (8 * nt), 1ll);
+    if (nt == 1) return f32 ? attn_launch<HD, true, 1>(a, items, tiles, s) : attn_launch<HD, false, 1>(a, items, tiles, s);
+    return f32 ? attn_launch<HD, true, 2>(a, items, tiles, s) : attn_launch<HD, false, 2>(a, items, tiles, s);
 }
 
 FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const void *q, int64_t q_token,
@@ -775,8 +818,8 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         a.scale = scale;
         a.err = dev_error_ptr();
         a.group = nh / c->nkv;
-        a.cnt = (uint32_t *)ws;
-        a.part = (float *)((uint8_t *)ws + 3 * KA_MAX_GRID * 4);
+        a.split = (KaSplit *)ws;
+        a.part = (float *)((uint8_t *)ws + KA_MAX_GRID * sizeof(KaSplit));
         const bool f32 = type == T_F32;
         const cudaStream_t s = (cudaStream_t)stream;
         const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
