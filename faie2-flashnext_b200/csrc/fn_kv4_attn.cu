@@ -41,11 +41,10 @@ namespace fn {
 
 constexpr int KA_TOK = 64;                    // tokens of a stage
 constexpr int KA_CONS = 4;                    // computing warps
-constexpr int KA_THREADS = 256;               // the computing warpgroup, and one of which a warp copies
-// registers: 256 threads x 128 at launch; the copying warpgroup gives up what the computing one takes (40 + 216 = 2 x 128),
-// which holds 8 or 16 rows of 256 sums
+constexpr int KA_EXTRA = 4;                   // units that a row tile counts beside its own, for its start and end
+// registers of the wide form: 256 threads x 128 at launch; the copying warpgroup gives up what the computing one takes
+// (40 + 216 = 2 x 128)
 constexpr int KA_REG_COPY = 40, KA_REG_COMP = 216;
-constexpr int KA_CTAS = 2;                    // per SM
 constexpr int KA_MAX_GRID = 512;              // CTAs at most
 
 struct Kv4AttnArgs {
@@ -62,7 +61,7 @@ struct Kv4AttnArgs {
 };
 
 struct KaSplit {
-    int parts, edge;        // CTAs it lies in (0: there is none); where the first one's part is
+    int parts;              // CTAs it lies in (0: there is none)
     int req, kv, tile;
 };
 
@@ -131,13 +130,16 @@ template <> __device__ __forceinline__ float ka_f<__nv_bfloat16>(__nv_bfloat16 x
 template <int HD, bool HL, int NT> struct KaCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
     static constexpr int NG = HD / KV4_GROUP, ROWS = 8 * NT;
+    // CTAs per SM: three of 4 + 1 warps with 128 registers, or two with 216 for the computing warps where the sums are many
+    static constexpr bool WIDE = HD * NT >= 256;
+    static constexpr int CTAS = WIDE ? 2 : 3, THREADS = WIDE ? 256 : 160;
     static constexpr int OS = HD + 1;                         // floats between rows of the merged sums (banks)
     static constexpr uint32_t STAGE = KA_TOK * HD / 16 * 17;  // bytes of 64 tokens of one head
     static constexpr uint32_t QF = NT * NG * 4 * 32 * (HL ? 16 : 8);  // q as B operands: [n-tile][group][step][lane]
     static constexpr uint32_t OB = (ROWS * OS * 4 + 127) / 128 * 128;
     // the merged sums share their place with q, which is rebuilt for the next row tile
     static constexpr uint32_t Q_OFF = 1024, ST_OFF = Q_OFF + (QF > OB ? QF : OB);
-    static constexpr uint32_t SMEM_MAX = 112 * 1024;          // of two CTAs on an SM (114 KB each, less static memory)
+    static constexpr uint32_t SMEM_MAX = (WIDE ? 112 : 73) * 1024;  // 228 KB / CTAS, less static memory and 1 KB
     // stages, an even number: a slot then always belongs to the same pair of warps, whose waits see each of its phases
     static constexpr int S = (SMEM_MAX - ST_OFF) / STAGE > 16 ? 16 : (SMEM_MAX - ST_OFF) / STAGE / 2 * 2;
     static constexpr uint32_t SMEM = ST_OFF + S * STAGE;
@@ -161,13 +163,14 @@ __device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, i
     }
 }
 
-template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS, KA_CTAS) k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
+template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, HL, NT>::THREADS, KaCfg<HD, HL, NT>::CTAS)
+    k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
     using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
-    constexpr int NG = C::NG, ROWS = C::ROWS, S = C::S, OS = C::OS;
+    constexpr int NG = C::NG, ROWS = C::ROWS, S = C::S, OS = C::OS, THREADS = C::THREADS;
     using QF = std::conditional_t<HL, uint4, uint2>;
     extern __shared__ __align__(128) uint8_t sm_ka[];
-    __shared__ long long red[KA_THREADS / 32], s_off;
+    __shared__ long long red[THREADS / 32], s_off;
     __shared__ int s_req;
     __shared__ volatile int s_fail;
     __shared__ __align__(8) float s_rs[ROWS], s_qs[2][NG][ROWS];
@@ -190,11 +193,11 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     pdl_trigger();
 
     // ---- this CTA's run of units: prefix sum over the requests, a contiguous share of them per thread
-    const int per_t = (a.n + KA_THREADS - 1) / KA_THREADS, r0 = min(tid * per_t, a.n), r1 = min(r0 + per_t, a.n);
+    const int per_t = (a.n + THREADS - 1) / THREADS, r0 = min(tid * per_t, a.n), r1 = min(r0 + per_t, a.n);
     long long mine = 0;
     for (int r = r0; r < r1; ++r) {
         const KaReq q = ka_req<ROWS>(a, r);
-        mine += (long long)q.rt * a.l.nkv * q.tiles;
+        mine += (long long)q.rt * a.l.nkv * (q.tiles + KA_EXTRA);
     }
     long long incl = mine;
 #pragma unroll
@@ -205,17 +208,17 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     if (lane == 31) red[warp] = incl;
     __syncthreads();
     long long before = incl - mine, units = 0;
-    for (int w = 0; w < KA_THREADS / 32; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += red[w];
         units += red[w];
     }
-    const long long per = max((units + gridDim.x - 1) / gridDim.x, 2ll);
+    const long long per = max((units + gridDim.x - 1) / gridDim.x, 2ll + KA_EXTRA);
     const long long u0 = blockIdx.x * per, u1 = min(u0 + per, units);
     if (u0 < u1 && u0 >= before && u0 < before + mine) {
         long long at = before;
         for (int r = r0; r < r1; ++r) {
             const KaReq q = ka_req<ROWS>(a, r);
-            const long long w = (long long)q.rt * a.l.nkv * q.tiles;
+            const long long w = (long long)q.rt * a.l.nkv * (q.tiles + KA_EXTRA);
             if (u0 < at + w) {
                 s_req = r;
                 s_off = u0 - at;
@@ -228,24 +231,30 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     {
         const int live = min(max(after_wait(a.cu)[a.n], 0), a.rows);
         const long long left = (long long)(a.rows - live) * a.nh * HD;
-        for (long long i = (long long)blockIdx.x * KA_THREADS + tid; i < left; i += (long long)gridDim.x * KA_THREADS) {
+        for (long long i = (long long)blockIdx.x * THREADS + tid; i < left; i += (long long)gridDim.x * THREADS) {
             const long long row = i / (a.nh * HD);
             ((T *)a.out)[(live + row) * a.ot + (i - row * a.nh * HD)] = (T)0.0f;
         }
     }
+    if (tid == 0) a.split[blockIdx.x].parts = 0;
     __syncthreads();
-    if (u0 >= u1) {
-        if (tid == 0) a.split[blockIdx.x].parts = 0;
-        return;
-    }
+    if (u0 >= u1) return;
 
     int r = s_req;
     KaReq rq = ka_req<ROWS>(a, r);
-    int item = (int)(s_off / rq.tiles), k = (int)(s_off - (long long)item * rq.tiles);
-    // to the next row tile of the run
+    // the run is at place `off` of a row tile's units: its own follow KA_EXTRA that only count
+    int item = (int)(s_off / (rq.tiles + KA_EXTRA)), off = (int)(s_off - (long long)item * (rq.tiles + KA_EXTRA));
+    long long u = u0;
+    int k, kend;  // the tiles that the run has of the row tile (none: k = kend)
+    auto here = [&]() {
+        k = max(off - KA_EXTRA, 0);
+        kend = max((int)min((long long)(rq.tiles + KA_EXTRA), off + (u1 - u)) - KA_EXTRA, 0);
+    };
+    // to the next row tile of the run, if there is one
     auto next = [&]() {
-        k = 0;
-        if (++item < rq.rt * a.l.nkv) return;
+        u += rq.tiles + KA_EXTRA - off;
+        off = 0;
+        if (u >= u1 || ++item < rq.rt * a.l.nkv) return;
         item = 0;
         do rq = ka_req<ROWS>(a, ++r);
         while (rq.rt == 0);
@@ -260,12 +269,13 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     const int ppt = KA_TOK / a.l.bs;  // pages of a stage
 
     if (warp >= KA_CONS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KA_REG_COPY));
+        if constexpr (C::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KA_REG_COPY));
         if (warp > KA_CONS) return;
         // ---- copies: lane p fetches page p of a stage; a lane holds one entry of the next 32 pages' ids
         int it = 0;
-        for (long long u = u0; u < u1;) {
-            const int kend = (int)min((long long)rq.tiles, k + (u1 - u)), kv = item / rq.rt;
+        for (; u < u1; next()) {
+            here();
+            const int kv = item / rq.rt;
             const int pages = (rq.len + a.l.bs - 1) / a.l.bs;
             const int *tab = after_wait(a.table) + (size_t)r * a.max_pages;
             const int p0 = k * ppt;
@@ -295,8 +305,6 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
                     bulk_g2s(ring + (size_t)sl * C::STAGE + lane * a.l.rec,
                              a.l.pages + ((int64_t)id * a.l.nkv + kv) * (int64_t)a.l.rec, a.l.rec, &full[sl]);
             }
-            u += kend - k;
-            if (u < u1) next();
         }
     drained:
         // a CTA that gave up must not leave with copies into its shared memory in flight
@@ -306,15 +314,17 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
     }
 
     // ---- compute
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KA_REG_COMP));
+    if constexpr (C::WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KA_REG_COMP));
     const int g = lane >> 2, t = lane & 3, half = warp & 1, pair = warp >> 1;
     // index n of 8 tokens is token n ^ (n >> 2): with it both the K reads (8 bytes of 8 tokens x 4 lanes, 16 lanes at a
     // time) and the V reads (4 bytes of 4 tokens x 8 words) touch 32 different banks
     const int tk = g ^ (g >> 2);
     const int tv0 = (2 * t) ^ (t >> 1), tv1 = (2 * t + 1) ^ (t >> 1);
     int it = 0;
-    for (long long u = u0; u < u1;) {
-        const int kend = (int)min((long long)rq.tiles, k + (u1 - u)), kv = item / rq.rt, tile = item - kv * rq.rt;
+    for (; u < u1; next()) {
+        here();
+        if (k == kend) continue;
+        const int kv = item / rq.rt, tile = item - kv * rq.rt;
         const int nrow = min(ROWS, rq.fresh * a.group - tile * ROWS);
         // ---- q of the row tile into B operands
         ka_bar();
@@ -410,7 +420,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
 #pragma unroll
                     for (int x = 0; x < 4; ++x) B[n][x] = qf[((n * NG + gi) * 4 + x) * 32 + lane];
                 uint4 A[2][4];
-                float d[2][2], acc[NT][2][4], low[NT][2][4];
+                float d[2][2], acc[NT][2][4];
+                [[maybe_unused]] float low[NT][2][4];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const uint8_t *c = kp + gi * cstep + b * code2, *s = ks + gi * sstep + b * scale2;
@@ -539,7 +550,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
             const uint8_t *vp0 = rec + a.l.kb + (pl + tv0) * 32 + g * 4, *vp1 = vp0 + (tv1 - tv0) * 32;
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
-                uint32_t P[NT][2][2], Q[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g; second halves
+                uint32_t P[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g
+                [[maybe_unused]] uint32_t Q[NT][2][2];  // their second halves
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -680,7 +692,6 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
             else quarter(std::integral_constant<int, 3>{}, round);
             ka_bar();
         }
-        const long long first = u - k;  // the row tile's first unit
         const bool starts = k == 0, ends = kend == rq.tiles;
         if (starts && ends) {
             // the row tile's output: a warp takes a row at a time
@@ -689,34 +700,27 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KA_THREADS,
                 ka_emit<T, HD>(a, rq, kv, tile * ROWS + i, lane, limit(i) > 0, [&](int d) { return ob[i * OS + d] / sum; });
             }
         } else {
-            // a part of a row tile, at the run's start (0) or after it (1)
-            float *to = a.part + ((size_t)blockIdx.x * 2 + (u != u0)) * KA_PART_MAX;
+            // a part of a row tile: its start (1), or what goes on from the run before (0)
+            float *to = a.part + ((size_t)blockIdx.x * 2 + starts) * KA_PART_MAX;
             for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) to[e] = ob[e / HD * OS + e % HD];
             if (tid < ROWS) {
                 to[ROWS * HD + tid] = s_mref[tid];
                 to[ROWS * HD + ROWS + tid] = s_ml[tid];
             }
+            if (tid == 0 && starts)
+                a.split[blockIdx.x] = KaSplit{(int)((u - off + KA_EXTRA + rq.tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
         }
-        if (tid == 0 && u + kend - k == u1) {
-            KaSplit sp{0, 0, r, kv, tile};
-            if (starts && !ends) {
-                sp.parts = (int)((first + rq.tiles - 1) / per) - (int)blockIdx.x + 1;
-                sp.edge = u != u0;
-            }
-            a.split[blockIdx.x] = sp;
-        }
-        u += kend - k;
-        if (u < u1) next();
     }
 }
 
 // ---- the join: CTA (c, row) adds the parts of the row tile that starts in run c and goes on past it. A warp takes every
-// fourth part (loads of many parts in flight), the four sums are added in the order of the warps.
-template <int HD, bool HL, int NT> __global__ void __launch_bounds__(128) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
+// eighth part (loads of many parts in flight), the eight sums are added in the order of the warps.
+constexpr int KJ_WARPS = 8;
+template <int HD, bool HL, int NT> __global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
     using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
-    constexpr int PER = HD / 32, U = 8;
-    __shared__ float s_w[KA_MAX_GRID], s_red[2][4], s_sum[4][HD];
+    constexpr int PER = HD / 32, U = 8, W = KJ_WARPS;
+    __shared__ float s_w[KA_MAX_GRID], s_red[2][W], s_sum[W][HD];
     pdl_wait();
     pdl_trigger();
     const int c = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -725,9 +729,9 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(128) k_kv4_
     const KaReq rq = ka_req<C::ROWS>(a, sp.req);
     const int flat = sp.tile * C::ROWS + i;
     if (flat >= rq.fresh * a.group) return;
-    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0 ? sp.edge : 0)) * KA_PART_MAX; };
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * KA_PART_MAX; };
     float mx = -INFINITY;
-    for (int x = tid; x < sp.parts; x += 128) {
+    for (int x = tid; x < sp.parts; x += 32 * W) {
         const float rf = slot(x)[C::ROWS * HD + i];
         s_w[x] = rf;
         mx = fmaxf(mx, rf);
@@ -736,35 +740,44 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(128) k_kv4_
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) s_red[0][warp] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-    for (int x = tid; x < sp.parts; x += 128) s_w[x] = ka_weight(s_w[x], mx);
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
+    for (int x = tid; x < sp.parts; x += 32 * W) s_w[x] = ka_weight(s_w[x], mx);
     __syncthreads();
     float y[PER] = {}, sum = 0.0f;
-    for (int x0 = warp; x0 < sp.parts; x0 += 4 * U) {
-        float v[U][PER], w[U];
+    for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
+        float v[U][PER], l[U], w[U];
 #pragma unroll
         for (int x = 0; x < U; ++x) {
-            const bool in = x0 + 4 * x < sp.parts;
-            const float *p = slot(in ? x0 + 4 * x : 0);
-            w[x] = in ? s_w[x0 + 4 * x] : 0.0f;
+            const bool in = x0 + W * x < sp.parts;
+            const float *p = slot(in ? x0 + W * x : 0);
+            w[x] = in ? s_w[x0 + W * x] : 0.0f;
+            l[x] = in ? p[C::ROWS * HD + C::ROWS + i] : 0.0f;
 #pragma unroll
             for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
-            sum += in ? w[x] * p[C::ROWS * HD + C::ROWS + i] : 0.0f;
         }
 #pragma unroll
-        for (int x = 0; x < U; ++x)
+        for (int x = 0; x < U; ++x) {
+            sum += w[x] * l[x];
 #pragma unroll
             for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
+        }
     }
 #pragma unroll
     for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
     if (lane == 0) s_red[1][warp] = sum;
     __syncthreads();
     if (warp) return;
-    sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += s_red[1][w];
     const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
-    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees,
-                   [&](int d) { return ((s_sum[0][d] + s_sum[1][d]) + (s_sum[2][d] + s_sum[3][d])) / sum; });
+    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees, [&](int d) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += s_sum[w][d];
+        return s / sum;
+    });
 }
 
 }  // namespace fn
@@ -773,7 +786,7 @@ using namespace fn;
 
 // every CTA's split row tile, then its two partial results
 FN_API uint64_t fn_kv4_attn_workspace(void) {
-    return KA_MAX_GRID * sizeof(KaSplit) + (uint64_t)std::min(num_sms() * KA_CTAS, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
+    return KA_MAX_GRID * sizeof(KaSplit) + (uint64_t)std::min(num_sms() * 3, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
 }
 
 template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
@@ -781,10 +794,10 @@ template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnA
     if (e != cudaSuccess) return e;
     // no more CTAs than pairs of units there can be; a row tile of one pair is never split
     const long long units = items * tiles;
-    const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KA_CTAS, KA_MAX_GRID));
-    e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KA_THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+    const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KaCfg<HD, HL, NT>::CTAS, KA_MAX_GRID));
+    e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KaCfg<HD, HL, NT>::THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_k(k_kv4_join<HD, HL, NT>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(128), 0, s, a);
+    return launch_k(k_kv4_join<HD, HL, NT>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(32 * KJ_WARPS), 0, s, a);
 }
 template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
     // requests whose rows fill one column tile of 8 take the narrow form
