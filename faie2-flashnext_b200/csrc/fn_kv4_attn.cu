@@ -30,56 +30,14 @@
 //
 // A CTA: one warp copies pages into a ring (one bulk copy per page and head: codes and scales of K and V), four warps
 // compute, two on each 64-token stage, 32 tokens each, with their own running softmax; they merge at the end of a run.
-#include <cuda_bf16.h>
-
-#include <algorithm>
-#include <type_traits>
-
-#include "fn_kv4.h"
+#include "fn_kv4_attn.cuh"
 
 namespace fn {
 
-constexpr int KA_TOK = 64;                    // tokens of a stage
 constexpr int KA_CONS = 4;                    // computing warps
-constexpr int KA_EXTRA = 4;                   // units that a row tile counts beside its own, for its start and end
 // registers of the wide form: 256 threads x 128 at launch; the copying warpgroup gives up what the computing one takes
 // (40 + 216 = 2 x 128)
 constexpr int KA_REG_COPY = 40, KA_REG_COMP = 216;
-constexpr int KA_MAX_GRID = 512;              // CTAs at most
-
-struct Kv4AttnArgs {
-    Kv4Lay l;
-    int n, rows, nh, group, max_pages, vec;
-    const void *q, *gate;
-    int64_t qt, qh, gt, gh, ot;
-    void *out;
-    const int *cu, *kv_len, *table;
-    float scale;
-    float *part;     // [CTA][2]: a row tile's sums [rows][hd], references [rows], sums of weights [rows]
-    struct KaSplit *split;  // [CTA]: the row tile that starts in the CTA's run and goes on past it
-    uint32_t *err;
-};
-
-struct KaSplit {
-    int parts;              // CTAs it lies in (0: there is none)
-    int req, kv, tile;
-};
-
-// a request's share of the work
-struct KaReq {
-    int first, fresh, len, tiles, rt;  // first row, rows, tokens, 64-token tiles, row tiles
-};
-template <int ROWS> __device__ __forceinline__ KaReq ka_req(const Kv4AttnArgs &a, int r) {
-    KaReq q;
-    const int c0 = after_wait(a.cu)[r], c1 = after_wait(a.cu)[r + 1];
-    q.first = min(max(c0, 0), a.rows);
-    q.fresh = min(max(c1, q.first), a.rows) - q.first;
-    const long long cap = (long long)a.max_pages * a.l.bs;
-    q.len = (int)min((long long)max(after_wait(a.kv_len)[r], 0), cap);
-    q.tiles = max((q.len + KA_TOK - 1) / KA_TOK, 1);  // an empty request's rows are written too
-    q.rt = (int)(((long long)q.fresh * a.group + ROWS - 1) / ROWS);
-    return q;
-}
 
 __device__ __forceinline__ void ka_mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm(
@@ -87,27 +45,11 @@ __device__ __forceinline__ void ka_mma(float (&d)[4], const uint4 &a, uint32_t b
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ka_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t ka_pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *(const uint32_t *)&h;
-}
-__device__ __forceinline__ float2 ka_unpack(uint32_t w) { return __half22float2(*(const __half2 *)&w); }
 // an 8 x 8 matrix of halves, row g columns 2t, 2t + 1 in lane 4 g + t, turned
 __device__ __forceinline__ uint32_t ka_turn(uint32_t w) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
     return r;
-}
-__device__ __forceinline__ float ka_half(const uint8_t *p) { return __half2float(*(const __half *)p); }
-// the weight of a part whose reference is `ref` beside the common one; a part without a key has none, and a row that has
-// nothing but NaN scores keeps them through the reference 0
-__device__ __forceinline__ float ka_weight(float ref, float common) {
-    return ka_exp2(ref == -INFINITY ? (common == -INFINITY ? 0.0f : -INFINITY) : ref - common);
 }
 __device__ __forceinline__ void ka_bar() { asm volatile("bar.sync 1, %0;" ::"n"(32 * KA_CONS) : "memory"); }
 // the same, and whether any thread brought `p`
@@ -123,10 +65,6 @@ __device__ __forceinline__ bool ka_bar_or(bool p) {
 __device__ __forceinline__ void ka_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
-template <typename T> __device__ __forceinline__ float ka_f(T x);
-template <> __device__ __forceinline__ float ka_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ float ka_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
 template <int HD, bool HL, int NT> struct KaCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
     static constexpr int NG = HD / KV4_GROUP, ROWS = 8 * NT;
@@ -145,23 +83,6 @@ template <int HD, bool HL, int NT> struct KaCfg {
     static constexpr uint32_t SMEM = ST_OFF + S * STAGE;
 };
 constexpr int KA_PART_MAX = 16 * 256 + 32;
-
-// a row's output by one warp: value(d), gated
-template <typename T, int HD, typename V>
-__device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, int kv, int flat, int lane, bool sees, V value) {
-    const int tok = flat / a.group, h = kv * a.group + flat - tok * a.group;
-    const int64_t row = rq.first + tok;
-    float gate[HD / 32];
-#pragma unroll
-    for (int x = 0; x < HD / 32; ++x)
-        gate[x] = a.gate && sees ? ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + lane + 32 * x]) : 0.0f;
-#pragma unroll
-    for (int x = 0; x < HD / 32; ++x) {
-        float y = sees ? value(lane + 32 * x) : 0.0f;
-        if (a.gate) y *= sigm(gate[x]);
-        ((T *)a.out)[row * a.ot + (int64_t)h * HD + lane + 32 * x] = (T)y;
-    }
-}
 
 template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, HL, NT>::THREADS, KaCfg<HD, HL, NT>::CTAS)
     k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
@@ -701,7 +622,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
             }
         } else {
             // a part of a row tile: its start (1), or what goes on from the run before (0)
-            float *to = a.part + ((size_t)blockIdx.x * 2 + starts) * KA_PART_MAX;
+            float *to = a.part + ((size_t)blockIdx.x * 2 + starts) * a.stride;
             for (int e = tid; e < nrow * HD; e += 32 * KA_CONS) to[e] = ob[e / HD * OS + e % HD];
             if (tid < ROWS) {
                 to[ROWS * HD + tid] = s_mref[tid];
@@ -713,80 +634,14 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
     }
 }
 
-// ---- the join: CTA (c, row) adds the parts of the row tile that starts in run c and goes on past it. A warp takes every
-// eighth part (loads of many parts in flight), the eight sums are added in the order of the warps.
-constexpr int KJ_WARPS = 8;
-template <int HD, bool HL, int NT> __global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
-    using C = KaCfg<HD, HL, NT>;
-    using T = typename C::T;
-    constexpr int PER = HD / 32, U = 8, W = KJ_WARPS;
-    __shared__ float s_w[KA_MAX_GRID], s_red[2][W], s_sum[W][HD];
-    pdl_wait();
-    pdl_trigger();
-    const int c = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const KaSplit sp = after_wait(a.split)[c];
-    if (sp.parts == 0) return;
-    const KaReq rq = ka_req<C::ROWS>(a, sp.req);
-    const int flat = sp.tile * C::ROWS + i;
-    if (flat >= rq.fresh * a.group) return;
-    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * KA_PART_MAX; };
-    float mx = -INFINITY;
-    for (int x = tid; x < sp.parts; x += 32 * W) {
-        const float rf = slot(x)[C::ROWS * HD + i];
-        s_w[x] = rf;
-        mx = fmaxf(mx, rf);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) s_red[0][warp] = mx;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
-    for (int x = tid; x < sp.parts; x += 32 * W) s_w[x] = ka_weight(s_w[x], mx);
-    __syncthreads();
-    float y[PER] = {}, sum = 0.0f;
-    for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
-        float v[U][PER], l[U], w[U];
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-            const bool in = x0 + W * x < sp.parts;
-            const float *p = slot(in ? x0 + W * x : 0);
-            w[x] = in ? s_w[x0 + W * x] : 0.0f;
-            l[x] = in ? p[C::ROWS * HD + C::ROWS + i] : 0.0f;
-#pragma unroll
-            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
-        }
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-            sum += w[x] * l[x];
-#pragma unroll
-            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
-        }
-    }
-#pragma unroll
-    for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
-    if (lane == 0) s_red[1][warp] = sum;
-    __syncthreads();
-    if (warp) return;
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) sum += s_red[1][w];
-    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
-    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees, [&](int d) {
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) s += s_sum[w][d];
-        return s / sum;
-    });
-}
-
 }  // namespace fn
 
 using namespace fn;
 
 // every CTA's split row tile, then its two partial results
 FN_API uint64_t fn_kv4_attn_workspace(void) {
-    return KA_MAX_GRID * sizeof(KaSplit) + (uint64_t)std::min(num_sms() * 3, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
+    const uint64_t few = (uint64_t)std::min(num_sms() * 3, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
+    return KA_MAX_GRID * sizeof(KaSplit) + std::max(few, kv4_prompt_workspace());
 }
 
 template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
@@ -797,11 +652,14 @@ template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnA
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KaCfg<HD, HL, NT>::CTAS, KA_MAX_GRID));
     e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KaCfg<HD, HL, NT>::THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_k(k_kv4_join<HD, HL, NT>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(32 * KJ_WARPS), 0, s, a);
+    return launch_k(k_kv4_join<typename KaCfg<HD, HL, NT>::T, HD, KaCfg<HD, HL, NT>::ROWS>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(32 * KJ_WARPS), 0, s, a);
 }
+constexpr int KP_FROM = 48;  // rows of a request from which the prompts' kernel is faster
+
 template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
-    // requests whose rows fill one column tile of 8 take the narrow form
     const long long rows = (long long)std::min(max_new, a.rows) * a.group;
+    if (rows >= KP_FROM) return launch_kv4_prompt(a, f32, max_new, s);
+    // requests whose rows fill one column tile of 8 take the narrow form
     const int nt = rows <= 8 ? 1 : 2;
     // the most row tiles, and units of one, that there can be
     const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
@@ -822,6 +680,8 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         if (nh < 1 || nh % c->nkv || nh / c->nkv > 64) return fail("kv4 attn: bad head counts");
         if (rows < 0 || max_pages < 1 || max_new < 0) return fail("kv4 attn: bad row / page counts");
         if (rows == 0) return 0;
+        if ((uintptr_t)q % (type == T_F32 ? 4 : 2) || (uintptr_t)out % (type == T_F32 ? 4 : 2) || (uintptr_t)gate % (type == T_F32 ? 4 : 2))
+            return fail("kv4 attn: rows must be aligned to their type");
         if (!q || !out || !cu || !kv_len || !table || !ws) return fail("kv4 attn: null pointer");
         if (ws_bytes < fn_kv4_attn_workspace() || (uintptr_t)ws % 256) return fail("kv4 attn: workspace too small or unaligned");
         a.n = n, a.rows = rows, a.nh = nh, a.max_pages = max_pages;
@@ -832,8 +692,11 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         a.err = dev_error_ptr();
         a.group = nh / c->nkv;
         a.split = (KaSplit *)ws;
+        a.stride = KA_PART_MAX;
         a.part = (float *)((uint8_t *)ws + KA_MAX_GRID * sizeof(KaSplit));
         const bool f32 = type == T_F32;
+        const int64_t size = f32 ? 4 : 2;
+        a.vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0 && out_token * size % 16 == 0;
         const cudaStream_t s = (cudaStream_t)stream;
         const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
                             : c->hd == 128 ? attn_go<128>(a, f32, max_new, s)

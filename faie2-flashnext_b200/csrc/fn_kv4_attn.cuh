@@ -1,0 +1,160 @@
+// What the two attention kernels over the paged 4-bit cache share (fn_kv4_attn.cu: few rows per request, fn_kv4_prompt.cu:
+// prompts): arguments, the requests' share of the work, a row's output, the join of partial results.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "fn_kv4.h"
+
+namespace fn {
+
+constexpr int KA_TOK = 64;                    // tokens of a unit
+constexpr int KA_EXTRA = 4;                   // units that a row tile counts beside its own, for its start and end
+constexpr int KA_MAX_GRID = 512;              // CTAs at most
+
+struct Kv4AttnArgs {
+    Kv4Lay l;
+    int n, rows, nh, group, max_pages, vec;
+    const void *q, *gate;
+    int64_t qt, qh, gt, gh, ot;
+    void *out;
+    const int *cu, *kv_len, *table;
+    float scale;
+    float *part;     // [CTA][2]: a row tile's sums [rows][hd], references [rows], sums of weights [rows]
+    int64_t stride;  // floats of a partial result's place
+    struct KaSplit *split;  // [CTA]: the row tile that starts in the CTA's run and goes on past it
+    uint32_t *err;
+};
+
+struct KaSplit {
+    int parts;              // CTAs it lies in (0: there is none)
+    int req, kv, tile;
+};
+
+// a request's share of the work
+struct KaReq {
+    int first, fresh, len, tiles, rt;  // first row, rows, tokens, 64-token tiles, row tiles
+};
+template <int ROWS> __device__ __forceinline__ KaReq ka_req(const Kv4AttnArgs &a, int r) {
+    KaReq q;
+    const int c0 = after_wait(a.cu)[r], c1 = after_wait(a.cu)[r + 1];
+    q.first = min(max(c0, 0), a.rows);
+    q.fresh = min(max(c1, q.first), a.rows) - q.first;
+    const long long cap = (long long)a.max_pages * a.l.bs;
+    q.len = (int)min((long long)max(after_wait(a.kv_len)[r], 0), cap);
+    q.tiles = max((q.len + KA_TOK - 1) / KA_TOK, 1);  // an empty request's rows are written too
+    q.rt = (int)(((long long)q.fresh * a.group + ROWS - 1) / ROWS);
+    return q;
+}
+
+__device__ __forceinline__ float ka_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t ka_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ float2 ka_unpack(uint32_t w) { return __half22float2(*(const __half2 *)&w); }
+__device__ __forceinline__ float ka_half(const uint8_t *p) { return __half2float(*(const __half *)p); }
+// the weight of a part whose reference is `ref` beside the common one; a part without a key has none, and a row that has
+// nothing but NaN scores keeps them through the reference 0
+__device__ __forceinline__ float ka_weight(float ref, float common) {
+    return ka_exp2(ref == -INFINITY ? (common == -INFINITY ? 0.0f : -INFINITY) : ref - common);
+}
+template <typename T> __device__ __forceinline__ float ka_f(T x);
+template <> __device__ __forceinline__ float ka_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float ka_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// a row's output by one warp: value(d), gated
+template <typename T, int HD, typename V>
+__device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, int kv, int flat, int lane, bool sees, V value) {
+    const int tok = flat / a.group, h = kv * a.group + flat - tok * a.group;
+    const int64_t row = rq.first + tok;
+    float gate[HD / 32];
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x)
+        gate[x] = a.gate && sees ? ka_f<T>(((const T *)after_wait(a.gate))[row * a.gt + h * a.gh + lane + 32 * x]) : 0.0f;
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) {
+        float y = sees ? value(lane + 32 * x) : 0.0f;
+        if (a.gate) y *= sigm(gate[x]);
+        ((T *)a.out)[row * a.ot + (int64_t)h * HD + lane + 32 * x] = (T)y;
+    }
+}
+
+// ---- the join: the parts of the row tile that starts in run c = blockIdx.x and goes on past it, each a run of [ROWS][HD]
+// sums, [ROWS] references (base 2) and [ROWS] sums of weights, `stride` floats apart, two to a run. The warps of a CTA take a row
+// together, part by part (loads of many parts in flight), and add their sums in the order of the warps.
+constexpr int KJ_WARPS = 8;
+template <typename T, int HD, int ROWS> __global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
+    constexpr int PER = HD / 32, U = 8, W = KJ_WARPS;
+    __shared__ float s_w[KA_MAX_GRID], s_red[2][W], s_sum[W][HD];
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const KaSplit sp = after_wait(a.split)[c];
+    if (sp.parts == 0) return;
+    const KaReq rq = ka_req<ROWS>(a, sp.req);
+    const int flat = sp.tile * ROWS + i;
+    if (flat >= rq.fresh * a.group) return;
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
+    float mx = -INFINITY;
+    for (int x = tid; x < sp.parts; x += 32 * W) {
+        const float rf = slot(x)[ROWS * HD + i];
+        s_w[x] = rf;
+        mx = fmaxf(mx, rf);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) s_red[0][warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
+    for (int x = tid; x < sp.parts; x += 32 * W) s_w[x] = ka_weight(s_w[x], mx);
+    __syncthreads();
+    float y[PER] = {}, sum = 0.0f;
+    for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
+        float v[U][PER], l[U], w[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const bool in = x0 + W * x < sp.parts;
+            const float *p = slot(in ? x0 + W * x : 0);
+            w[x] = in ? s_w[x0 + W * x] : 0.0f;
+            l[x] = in ? p[ROWS * HD + ROWS + i] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            sum += w[x] * l[x];
+#pragma unroll
+            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
+    if (lane == 0) s_red[1][warp] = sum;
+    __syncthreads();
+    if (warp) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += s_red[1][w];
+    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
+    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees, [&](int d) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += s_sum[w][d];
+        return s / sum;
+    });
+}
+
+// host: prompts' kernel (fn_kv4_prompt.cu), and its share of the workspace
+cudaError_t launch_kv4_prompt(Kv4AttnArgs a, bool f32, int max_new, cudaStream_t s);
+uint64_t kv4_prompt_workspace();
+
+}  // namespace fn

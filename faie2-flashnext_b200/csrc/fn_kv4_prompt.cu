@@ -1,0 +1,771 @@
+// Attention over the paged 4-bit KV cache for prompts: many query rows per request (fn_kv4_attn.cu has few).
+//
+// A row tile is 128 rows of one kv head (the heads of its group, token after token), one per tensor-memory lane. Per 64
+// tokens the tensor cores (tcgen05, fp16 operands, fp32 sums in tensor memory) form S = Q K^T (128 x 64) and O = P V
+// (128 x hd). Here K and V are dequantised, once per 128 rows: 8192 products per code pay for it.
+//
+// Roles of the CTA's 16 warps, one CTA per SM:
+//   * warp 0 copies pages into rings (K and V parts apart: they are consumed at different times);
+//   * warp 1 issues the MMAs: S of tile j + 1 before O of tile j, so the softmax of one runs beside the products of the other;
+//   * warps 4..7 (a row a lane): scores out of tensor memory, running softmax, P back into tensor memory in S's place;
+//   * warps 8..15: Q into tensor memory, K and V codes into the MMAs' operands in shared memory, and the running output:
+//     each tile's O is read out of tensor memory and added in registers, o = o 2^.. + O, half a row a lane. So the sums
+//     over tokens are rounded fp32 additions, where the tensor core's own accumulation over a long context cuts, and a new
+//     maximum needs no pass over tensor memory.
+//
+// Scales. A tile's codes become (c - 8) d 2^-e with e the exponent of the tile's largest |d|, in fp16: in range whatever
+// the size of K or V; 2^e goes into the scores (K) and into the addition (V). Rows of q are scaled by a power of two.
+// bf16 rows: one product each; q is exact, K, P and V are rounded to 11 bits. fp32 rows: q, K, P and V are fp16 pairs (22
+// bits, K's and V's exact), three products each, the small ones first, so that the sum's cut bits are few.
+//
+// What no row of the tile sees becomes 0 in V, whatever its scale is. A visible token whose V scale is not finite also
+// becomes 0 and is noted: the rows that see it turn NaN in its 64 dims, the others must not (0 x NaN in the product).
+//
+// Work is cut into runs of 64-token units as in fn_kv4_attn.cu, one run per CTA; partial row tiles are joined after it.
+#include "fn_kv4_attn.cuh"
+#include "fn_umma.cuh"
+
+namespace fn {
+
+constexpr int KP_ROWS = 128, KP_THREADS = 512;
+constexpr int KP_REG_IO = 40, KP_REG_SM = 120, KP_REG_WORK = 176;  // 40 + 120 + 2 x 176 = 4 x 128 at launch
+constexpr int KP_W_SM = 4, KP_W_WORK = 8;
+
+template <int HD, bool HL> struct KpCfg {
+    using T = std::conditional_t<HL, float, __nv_bfloat16>;
+    static constexpr int NG = HD / KV4_GROUP, TERMS = HL ? 2 : 1;
+    static constexpr int NB = HL && HD == 256 ? 1 : 2;      // operand buffers of K and of V
+    static constexpr int RK = 2, RV = NB;                    // stages of the copies
+    static constexpr uint32_t KT = KA_TOK * HD * 2;          // K operand: [dim / 8][token] x 16 bytes
+    // V operand: [token / 8][dim] x 16 bytes, the token groups 16 bytes further apart (banks of the stores)
+    static constexpr uint32_t VG = HD * 16 + 16, VT = 8 * VG;
+    static constexpr uint32_t RAW = KA_TOK * (HD / 2 + HD / KV4_GROUP * 2);  // 64 tokens' codes and scales of K (or V)
+    static constexpr uint32_t QL = HL ? KP_ROWS * HD * 2 : 0;  // second halves of q: [dim / 8][row] x 16 bytes
+    static constexpr uint32_t K_OFF = 4096, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
+    static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAW, SMEM = RV_OFF + RV * RAW;
+    static constexpr int PART = KP_ROWS * HD + 2 * KP_ROWS;
+    // tensor memory: O, then q's first halves, then S / P twice (64 columns: P's halves 32 each)
+    static constexpr uint32_t TM_O = 0, TM_Q = HD, TM_S = HD + HD / 2;
+    static_assert(SMEM <= 227 * 1024 && TM_S + 128 <= 512);
+};
+
+// the fixed part of shared memory
+struct KpShared {
+    uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], ve[2], sf[2], pf[2], of, oe, qf, qe, lf, done;
+    long long red[KP_THREADS / 32], off;
+    uint32_t tmem, valid[8];
+    int req, fail;
+    float ek[4], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+};
+static_assert(sizeof(KpShared) <= 4096);
+
+// the workers' barrier, and whether any of them brought `p`
+__device__ __forceinline__ bool kp_bar_work_or(bool p) {
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 2, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(any)
+        : "r"((uint32_t)p)
+        : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void kp_bar_work() { asm volatile("bar.sync 2, 256;" ::: "memory"); }
+__device__ __forceinline__ float kp_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t kp_hsub2(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+__device__ __forceinline__ uint32_t kp_hmul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+// a b - c, rounded once
+__device__ __forceinline__ uint32_t kp_hrest2(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*(const __half2 *)&a, *(const __half2 *)&b, __hneg2(*(const __half2 *)&c));
+    return *(const uint32_t *)&r;
+}
+// the nibbles under 0x000f000f and 0x00f000f0 of w as halves c - 8
+__device__ __forceinline__ uint32_t kp_low(uint32_t w) { return kp_hsub2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
+__device__ __forceinline__ uint32_t kp_high(uint32_t w) { return kp_hsub2((w & 0x00f000f0u) | 0x54005400u, 0x54805480u); }
+
+// tiles of 64 tokens that row tile i of a request sees
+__device__ __forceinline__ int kp_tiles(const KaReq &q, int group, int i) {
+    const int last = min((int)min((long long)(i + 1) * KP_ROWS, (long long)q.fresh * group) - 1, INT32_MAX - 1) / group;
+    const int lim = min(max(q.len - q.fresh + last + 1, 0), q.len);
+    return max((lim + KA_TOK - 1) / KA_TOK, 1);
+}
+__device__ __forceinline__ KaReq kp_req(const Kv4AttnArgs &a, int r) { return ka_req<KP_ROWS>(a, r); }
+
+template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttnArgs a) {
+    using C = KpCfg<HD, HL>;
+    using T = typename C::T;
+    constexpr int NG = C::NG, NB = C::NB;
+    extern __shared__ __align__(1024) uint8_t sm_kp[];
+    KpShared &sh = *(KpShared *)sm_kp;
+    volatile int *const s_fail = &sh.fail;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 8), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 8);
+            mbar_init(&sh.kf[i], 8), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 8), mbar_init(&sh.ve[i], 1);
+            mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
+        }
+        mbar_init(&sh.of, 1), mbar_init(&sh.oe, 8), mbar_init(&sh.qf, 8), mbar_init(&sh.qe, 1), mbar_init(&sh.lf, 4);
+        mbar_init(&sh.done, 1);
+        mbar_fence_init();
+        sh.fail = 0;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this CTA's run of units
+    const int per_t = (a.n + KP_THREADS - 1) / KP_THREADS, r0 = min(tid * per_t, a.n), r1 = min(r0 + per_t, a.n);
+    auto weight = [&](int r) {
+        const KaReq q = kp_req(a, r);
+        long long w = 0;
+        for (int i = 0; i < q.rt; ++i) w += kp_tiles(q, a.group, i) + KA_EXTRA;
+        return w * a.l.nkv;
+    };
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) mine += weight(r);
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) sh.red[warp] = incl;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long before = incl - mine, units = 0;
+    for (int w = 0; w < KP_THREADS / 32; ++w) {
+        if (w < warp) before += sh.red[w];
+        units += sh.red[w];
+    }
+    const long long per = max((units + gridDim.x - 1) / gridDim.x, 2ll + KA_EXTRA);
+    const long long u0 = blockIdx.x * per, u1 = min(u0 + per, units);
+    if (u0 < u1 && u0 >= before && u0 < before + mine) {
+        long long at = before;
+        for (int r = r0; r < r1; ++r) {
+            const long long w = weight(r);
+            if (u0 < at + w) {
+                sh.req = r;
+                sh.off = u0 - at;
+                break;
+            }
+            at += w;
+        }
+    }
+    // rows that belong to no request
+    {
+        const int live = min(max(after_wait(a.cu)[a.n], 0), a.rows);
+        const long long left = (long long)(a.rows - live) * a.nh * HD;
+        for (long long i = (long long)blockIdx.x * KP_THREADS + tid; i < left; i += (long long)gridDim.x * KP_THREADS) {
+            const long long row = i / (a.nh * HD);
+            ((T *)a.out)[(live + row) * a.ot + (i - row * a.nh * HD)] = (T)0.0f;
+        }
+    }
+    if (tid == 0) a.split[blockIdx.x].parts = 0;
+    __syncthreads();
+    const uint32_t tmem = sh.tmem;
+
+    // the walk over the run's row tiles, the same in every role
+    int r = 0, tile = 0, kv = 0, tiles = 0, off = 0, k = 0, kend = 0;
+    long long u = u0;
+    KaReq rq{};
+    auto next = [&]() {
+        u += tiles + KA_EXTRA - off;
+        off = 0;
+        if (u >= u1 || ++kv < a.l.nkv) return;
+        kv = 0;
+        if (++tile >= rq.rt) {
+            tile = 0;
+            do rq = kp_req(a, ++r);
+            while (rq.rt == 0);
+        }
+        tiles = kp_tiles(rq, a.group, tile);
+    };
+    auto here = [&]() {
+        k = max(off - KA_EXTRA, 0);
+        kend = max((int)min((long long)(tiles + KA_EXTRA), off + (u1 - u)) - KA_EXTRA, 0);
+        return k < kend;
+    };
+    if (u0 < u1) {
+        r = sh.req;
+        rq = kp_req(a, r);
+        long long at = sh.off;
+        for (;; ++tile) {
+            tiles = kp_tiles(rq, a.group, tile);
+            const long long w = (long long)a.l.nkv * (tiles + KA_EXTRA);
+            if (at < w) break;
+            at -= w;
+        }
+        kv = (int)(at / (tiles + KA_EXTRA));
+        off = (int)(at - (long long)kv * (tiles + KA_EXTRA));
+    }
+    // rows of the tile see tokens below their limit; rows past its last see what the last sees (results dropped)
+    auto limit = [&](int i) {
+        const int nrow = (int)min((long long)KP_ROWS, (long long)rq.fresh * a.group - (long long)tile * KP_ROWS);
+        const int f = tile * KP_ROWS + min(i, nrow - 1);
+        return min(max(rq.len - rq.fresh + f / a.group + 1, 0), rq.len);
+    };
+    auto wt = [&](uint64_t *bar, int phase) {
+        if (*s_fail) return false;
+        if (mbar_park(bar, (uint32_t)phase & 1u)) return true;
+        *s_fail = 1;
+        dev_fail(a.err, DEV_WAIT_TIMEOUT);
+        return false;
+    };
+    const int ppt = KA_TOK / a.l.bs;  // pages of a tile
+    const uint32_t praw = a.l.kb + a.l.sb;  // bytes of a page's K (or V) part in a stage
+    int gt = 0, gi = 0;  // tiles and row tiles done by this role
+
+    if (warp < KP_W_SM) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_IO));
+        if (warp == 0) {
+            // ---- copies: lane p fetches page p of a tile
+            bool ok = true;
+            for (; u < u1 && ok; next()) {
+                if (!here()) continue;
+                const int pages = (rq.len + a.l.bs - 1) / a.l.bs;
+                const int *tab = after_wait(a.table) + (size_t)r * a.max_pages;
+                int ahead = lane < ppt && k * ppt + lane < pages ? tab[k * ppt + lane] : -1;
+                for (int j = k; j < kend && ok; ++j, ++gt) {
+                    const int pg = j * ppt + lane, id = ahead;
+                    const bool want = lane < ppt && pg < pages, good = want && id >= 0 && id < a.l.n_pages;
+                    ahead = lane < ppt && pg + ppt < pages ? tab[pg + ppt] : -1;
+                    if (want && !good) dev_fail(a.err, DEV_BAD_ARG);
+                    const uint32_t m = __ballot_sync(0xffffffffu, good);
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const int R = v ? C::RV : C::RK, sl = gt % R;
+                        uint64_t *full = v ? &sh.rvf[sl] : &sh.rkf[sl], *empty = v ? &sh.rve[sl] : &sh.rke[sl];
+                        if (lane == 0) {
+                            ok = gt < R || wt(empty, gt / R - 1);
+                            if (ok) {
+                                if (v == 0) sh.valid[gt & 7] = m;
+                                mbar_arrive_tx(full, (uint32_t)__popc(m) * praw);
+                            }
+                        }
+                        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+                        if (!ok) break;
+                        if (good) {
+                            const uint8_t *rec = a.l.pages + ((int64_t)id * a.l.nkv + kv) * (int64_t)a.l.rec;
+                            uint8_t *to = sm_kp + (v ? C::RV_OFF : C::RK_OFF) + sl * C::RAW + lane * praw;
+                            bulk_g2s(to, rec + v * a.l.kb, a.l.kb, full);
+                            bulk_g2s(to + a.l.kb, rec + 2 * a.l.kb + v * a.l.sb, a.l.sb, full);
+                        }
+                    }
+                }
+            }
+            // a CTA that gave up must not leave with copies into its shared memory in flight
+            if (*s_fail && lane == 0)
+                for (int v = 0; v < 2; ++v) {
+                    const int R = v ? C::RV : C::RK;
+                    for (int i = max(gt - R, 0); i <= gt; ++i)
+                        if (i < gt || v == 0) mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
+                }
+        } else if (warp == 1 && lane == 0) {
+            // ---- MMAs
+            constexpr uint32_t id_s = umma_idesc_f16(128, KA_TOK), id_o = umma_idesc_f16(128, HD);
+            const uint32_t kb = smem_u32(sm_kp + C::K_OFF), vb = smem_u32(sm_kp + C::V_OFF), ql = smem_u32(sm_kp + C::Q_OFF);
+            const uint32_t tq = tmem + C::TM_Q, to = tmem + C::TM_O;
+            auto scores = [&](int g) {  // S of tile g
+                const uint32_t ts = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, kt = kb + (uint32_t)(g % NB) * C::TERMS * C::KT;
+                uint32_t acc = 0;
+                if constexpr (HL) {
+                    for (int x = 0; x < HD / 16; ++x, acc = 1)
+                        umma_f16_smem_a(ts, umma_desc(ql + x * 4096u, 2048u, 128u), umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
+                    for (int x = 0; x < HD / 16; ++x)
+                        umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + C::KT + x * 2048u, 1024u, 128u), id_s, 1u);
+                }
+                for (int x = 0; x < HD / 16; ++x, acc = 1) umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
+            };
+            auto outputs = [&](int g) {  // O of tile g
+                const uint32_t tp = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, vt = vb + (uint32_t)(g % NB) * C::TERMS * C::VT;
+                uint32_t acc = 0;
+                if constexpr (HL) {
+                    for (int x = 0; x < KA_TOK / 16; ++x, acc = 1)
+                        umma_bf16_tmem_a(to, tp + 32u + 8u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+                    for (int x = 0; x < KA_TOK / 16; ++x)
+                        umma_bf16_tmem_a(to, tp + 8u * x, umma_desc(vt + C::VT + x * 2 * C::VG, C::VG, 128u), id_o, 1u);
+                }
+                for (int x = 0; x < KA_TOK / 16; ++x, acc = 1) umma_bf16_tmem_a(to, tp + 8u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+            };
+            bool ok = true;
+            for (; u < u1 && ok; next()) {
+                if (!here()) continue;
+                ok = wt(&sh.qf, gi);
+                const int n = kend - k, g0 = gt;
+                for (int j = 0; j <= n && ok; ++j) {
+                    if (j < n) {
+                        const int g = g0 + j;
+                        ok = wt(&sh.kf[g % NB], g / NB);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(g);
+                        umma_commit(&sh.sf[g & 1]);
+                        umma_commit(&sh.ke[g % NB]);
+                        if (j == n - 1) umma_commit(&sh.qe);
+                    }
+                    if (j > 0) {
+                        const int g = g0 + j - 1;
+                        ok = wt(&sh.pf[g & 1], g >> 1) && wt(&sh.vf[g % NB], g / NB) && (g == 0 || wt(&sh.oe, g - 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        outputs(g);
+                        umma_commit(&sh.of);
+                        umma_commit(&sh.ve[g % NB]);
+                    }
+                }
+                gt = g0 + n;
+                ++gi;
+            }
+            // every MMA issued has finished before the CTA gives its memory back
+            umma_commit(&sh.done);
+            mbar_park(&sh.done, 0);
+        }
+        __syncwarp();
+    } else if (warp < KP_W_WORK) {
+        // ---- softmax: row 32 (warp % 4) + lane
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_SM));
+        const int row = tid - 32 * KP_W_SM;
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::TM_S;
+        bool ok = true;
+        for (; u < u1 && ok; next()) {
+            if (!here()) continue;
+            const int lim = limit(row);
+            float m = -INFINITY, l = 0.0f;
+            float rs = 0.0f;
+            for (int j = k; j < kend; ++j, ++gt) {
+                const int b = gt & 1;
+                ok = wt(&sh.sf[b], gt >> 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                if (j == k) rs = sh.rs[row];
+                float s[64];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld16(tl + (uint32_t)b * 64u + 16u * c, *(float(*)[16]) & s[16 * c]);
+                const float f = rs * sh.ek[gt & 3];
+                const uint32_t valid = sh.valid[gt & 7];
+                const int t0 = j * KA_TOK;
+                if (t0 + KA_TOK > lim || valid != (1u << ppt) - 1u) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) {
+                        const bool gone = t0 + c >= lim || !(valid >> (c / a.l.bs) & 1u);
+                        s[c] = gone ? -INFINITY : s[c] * f;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) s[c] *= f;
+                }
+                float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // weights 2^10 exp2(s - maximum): fp16 keeps 11 bits down to 2^-24 of the largest
+                const float z = mn == -INFINITY ? 0.0f : 10.0f - mn;
+                const float fac = m == -INFINITY ? 0.0f : ka_exp2(m - mn);
+                m = mn;
+                sh.f[gt & 3][row] = fac;
+                float ls[4] = {};
+                uint32_t hi[32], lo[HL ? 32 : 1];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    const float p0 = ka_exp2(s[2 * c] + z), p1 = ka_exp2(s[2 * c + 1] + z);
+                    ls[c & 3] += p0 + p1;
+                    hi[c] = ka_pack(p0, p1);
+                    if constexpr (HL) {
+                        const float2 h = ka_unpack(hi[c]);
+                        lo[c] = ka_pack(p0 - h.x, p1 - h.y);
+                    }
+                }
+                l = l * fac + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    tmem_st16(tl + (uint32_t)b * 64u + 16u * c, *(uint32_t(*)[16]) & hi[16 * c]);
+                    if constexpr (HL) tmem_st16(tl + (uint32_t)b * 64u + 32u + 16u * c, *(uint32_t(*)[16]) & lo[16 * c]);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_arrive(&sh.pf[b]);
+            }
+            if (!ok) break;
+            if (k == 0 && kend == tiles) {
+                sh.l[row] = l;
+            } else {
+                float *to = a.part + ((size_t)blockIdx.x * 2 + (k == 0)) * a.stride + KP_ROWS * HD;
+                to[row] = m;
+                to[KP_ROWS + row] = l;
+                if (tid == 32 * KP_W_SM && k == 0)
+                    a.split[blockIdx.x] = KaSplit{(int)((u - off + KA_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
+            }
+            __syncwarp();
+            if (lane == 0) tc_arrive(&sh.lf);
+        }
+    } else {
+        // ---- workers: q, K, V into operands; the running output, dims [half HD / 2, + HD / 2) of row 32 (warp % 4) + lane
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_WORK));
+        const int wtid = tid - 32 * KP_W_WORK, half = (warp - KP_W_WORK) >> 2, row = 32 * (warp & 3) + lane;
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        constexpr int HH = HD / 2, NH = HH >= KV4_GROUP ? HH / KV4_GROUP : 1;  // this half's dims, and its 64-dim groups
+        const int g0 = half * HH / KV4_GROUP;
+        bool ok = true;
+        // a wait by all lanes, with one answer
+        auto wtw = [&](uint64_t *bar, int phase) { return __all_sync(0xffffffffu, wt(bar, phase)) != 0; };
+        for (; u < u1; next()) {
+            if (!here()) continue;
+            // a warp whose wait gave up goes on to this barrier, where all leave together
+            if (ok && gi > 0) ok = wtw(&sh.qe, gi - 1);
+            if (kp_bar_work_or(!ok)) break;
+            const int lim = limit(row), hi_lim = limit(KP_ROWS - 1);
+            const long long flat = (long long)tile * KP_ROWS + row;
+            const bool live = flat < (long long)rq.fresh * a.group;
+            const int tok_row = live ? (int)(flat / a.group) : 0, head = kv * a.group + (live ? (int)(flat - (long long)tok_row * a.group) : 0);
+            // ---- q: scaled so that the row's largest value is 2^10..2^11, dims in the order of the codes' nibbles
+            {
+                const T *src = (const T *)after_wait(a.q) + (int64_t)(rq.first + tok_row) * a.qt + (int64_t)head * a.qh + half * HH;
+                float mx = 0.0f;
+                if (live)
+#pragma unroll 8
+                    for (int d = 0; d < HH; d += 4) {
+                        float x[4];
+                        if (a.vec) {
+                            if constexpr (HL) *(float4 *)x = *(const float4 *)(src + d);
+                            else {
+                                const uint2 w = *(const uint2 *)(src + d);
+                                x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u);
+                                x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
+                            }
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) x[y] = ka_f<T>(src[d + y]);
+                        }
+                        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
+                    }
+                // both halves of the row agree on its exponent (K's place is free before the row tile's first K)
+                float *sx = (float *)(sm_kp + C::K_OFF);
+                sx[half * KP_ROWS + row] = mx;
+                kp_bar_work();
+                mx = fmaxf(mx, sx[(half ^ 1) * KP_ROWS + row]);
+                const int e = min(max(10 - ((int)(__float_as_uint(mx) >> 23) - 127), -90), 120);
+                const float up = kp_pow2(e);
+                if (half == 0) sh.rs[row] = a.scale * 1.44269504f * kp_pow2(-e);
+                kp_bar_work();
+#pragma unroll 1
+                for (int d = 0; d < HH; d += 32) {
+                    uint32_t hi[16];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        float x[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) x[y] = live ? ka_f<T>(src[d + 8 * w + y]) * up : 0.0f;
+                        uint32_t lo[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            hi[4 * w + y] = ka_pack(x[y], x[y + 4]);
+                            const float2 h = ka_unpack(hi[4 * w + y]);
+                            lo[y] = ka_pack(x[y] - h.x, x[y + 4] - h.y);
+                        }
+                        if constexpr (HL)
+                            *(uint4 *)(sm_kp + C::Q_OFF + ((half * HH + d) / 8 + w) * 2048 + row * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    tmem_st16(tl + C::TM_Q + (uint32_t)(half * HH + d) / 2u, hi);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) tc_arrive(&sh.qf);
+            }
+            float2 o[HH / 2];
+#pragma unroll
+            for (int c = 0; c < HH / 2; ++c) o[c] = make_float2(0.0f, 0.0f);
+            float ev_prev = 1.0f;
+            uint32_t bad_prev[NH][2] = {};
+            bool any_prev = false;
+
+            // what a tile's tokens may be used for: page there, and some row sees it
+            auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok / a.l.bs) & 1u) && j * KA_TOK + tok < hi_lim; };
+            // the exponent of the tile's largest finite |scale|
+            auto exponent = [&](const uint8_t *raw, int g, int j) {
+                float mx = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int tok = lane + 32 * h, pg = tok / a.l.bs;
+                    if (there(g, j, tok))
+#pragma unroll
+                        for (int x = 0; x < NG; ++x) {
+                            const float d = fabsf(ka_half(raw + pg * praw + a.l.kb + (x * a.l.bs + tok - pg * a.l.bs) * 2));
+                            if (d < INFINITY) mx = fmaxf(mx, d);
+                        }
+                }
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                return mx > 0.0f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
+            };
+            // K of tile g (the row tile's j): 16 bytes of codes (32 dims of a token) at a time
+            auto make_k = [&](int g, int j) {
+                if (!wtw(&sh.rkf[g % C::RK], g / C::RK)) return false;
+                if (g >= NB && !wtw(&sh.ke[g % NB], g / NB - 1)) return false;
+                const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAW;
+                uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT;
+                const int e = exponent(raw, g, j);
+                const float up = kp_pow2(-e);
+                if (wtid == 0) sh.ek[g & 3] = kp_pow2(e);
+#pragma unroll
+                for (int x = 0; x < (2 * NG * 64 + 255) / 256; ++x) {
+                    const int un = wtid + 256 * x, tok = un & 63, q = un >> 6;  // quarter q of 32 dims
+                    if (q < 2 * NG) {
+                        const int pg = tok / a.l.bs, line = (q >> 1) * a.l.bs + tok - pg * a.l.bs;
+                        const uint8_t *src = raw + pg * praw;
+                        const float d = there(g, j, tok) ? ka_half(src + a.l.kb + line * 2) * up : 0.0f;
+                        const uint32_t dd = ka_pack(d, d);
+                        const uint4 w4 = *(const uint4 *)(src + line * 32 + (q & 1) * 16);
+                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const uint32_t w = ws[y], c0 = kp_low(w), c1 = kp_high(w), c2 = kp_low(w >> 8), c3 = kp_high(w >> 8);
+                            const uint32_t h0 = kp_hmul2(c0, dd), h1 = kp_hmul2(c1, dd), h2 = kp_hmul2(c2, dd), h3 = kp_hmul2(c3, dd);
+                            uint8_t *at = to + (q * 4 + y) * 1024 + tok * 16;
+                            *(uint4 *)at = make_uint4(h0, h1, h2, h3);
+                            if constexpr (HL)
+                                *(uint4 *)(at + C::KT) = make_uint4(kp_hrest2(c0, dd, h0), kp_hrest2(c1, dd, h1), kp_hrest2(c2, dd, h2), kp_hrest2(c3, dd, h3));
+                        }
+                    }
+                }
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    tc_arrive(&sh.kf[g % NB]);
+                    tc_arrive(&sh.rke[g % C::RK]);
+                }
+                return true;
+            };
+            // V of tile g: 8 tokens x 8 dims at a time, turned
+            auto make_v = [&](int g, int j) {
+                if (!wtw(&sh.rvf[g % C::RV], g / C::RV)) return false;
+                if (g >= NB && !wtw(&sh.ve[g % NB], g / NB - 1)) return false;
+                const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
+                uint8_t *to = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT;
+                const int e = exponent(raw, g, j);
+                const float up = kp_pow2(-e);
+                ev_prev = kp_pow2(e);
+                // tokens whose scale is not finite, by group of this half's dims
+                uint32_t any = 0;
+#pragma unroll
+                for (int x = 0; x < NH; ++x)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int tok = lane + 32 * h, pg = tok / a.l.bs;
+                        const float d = fabsf(ka_half(raw + pg * praw + a.l.kb + ((g0 + x) * a.l.bs + tok - pg * a.l.bs) * 2));
+                        bad_prev[x][h] = __ballot_sync(0xffffffffu, there(g, j, tok) && !(d < INFINITY));
+                        any |= bad_prev[x][h];
+                    }
+                any_prev = any != 0;
+                if (wtid < HD) {
+                    const int ch = wtid & 7, wd = wtid >> 3, tok = ch * 8, pg = tok / a.l.bs;
+                    const int line = (wd >> 3) * a.l.bs + tok - pg * a.l.bs;
+                    const uint8_t *src = raw + pg * praw;
+                    const uint4 s4 = *(const uint4 *)(src + a.l.kb + line * 2);
+                    const uint32_t ss[4] = {s4.x, s4.y, s4.z, s4.w};
+                    uint32_t w[8], dd[4];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + (line + y) * 32 + (wd & 7) * 4);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        float2 d = ka_unpack(ss[y]);
+                        d.x = there(g, j, tok + 2 * y) && fabsf(d.x) < INFINITY ? d.x * up : 0.0f;
+                        d.y = there(g, j, tok + 2 * y + 1) && fabsf(d.y) < INFINITY ? d.y * up : 0.0f;
+                        dd[y] = ka_pack(d.x, d.y);
+                    }
+                    uint8_t *at = to + ch * C::VG + wd * 128;
+#pragma unroll
+                    for (int by = 0; by < 4; ++by) {
+                        const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
+                        uint32_t h[2][4], lo[2][4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const uint32_t x = __byte_perm(w[2 * y], w[2 * y + 1], sel), c0 = kp_low(x), c1 = kp_high(x);
+                            h[0][y] = kp_hmul2(c0, dd[y]), h[1][y] = kp_hmul2(c1, dd[y]);
+                            if constexpr (HL) lo[0][y] = kp_hrest2(c0, dd[y], h[0][y]), lo[1][y] = kp_hrest2(c1, dd[y], h[1][y]);
+                        }
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            *(uint4 *)(at + (2 * by + x) * 16) = make_uint4(h[x][0], h[x][1], h[x][2], h[x][3]);
+                            if constexpr (HL) *(uint4 *)(at + C::VT + (2 * by + x) * 16) = make_uint4(lo[x][0], lo[x][1], lo[x][2], lo[x][3]);
+                        }
+                    }
+                }
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    tc_arrive(&sh.vf[g % NB]);
+                    tc_arrive(&sh.rve[g % C::RV]);
+                }
+                return true;
+            };
+            // o = o f + O 2^e of tile g
+            auto add = [&](int g, int j) {
+                if (!wtw(&sh.of, g)) return false;
+                tc_fence_after();
+                const float f = sh.f[g & 3][row];
+                const float2 f2 = make_float2(f, f), e2 = make_float2(ev_prev, ev_prev);
+#pragma unroll
+                for (int c = 0; c < HH; c += 16) {
+                    float x[16];
+                    tmem_ld16(tl + C::TM_O + (uint32_t)(half * HH + c), x);
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        o[c / 2 + y] = __ffma2_rn(make_float2(x[2 * y], x[2 * y + 1]), e2, __fmul2_rn(o[c / 2 + y], f2));
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_arrive(&sh.oe);
+                if (any_prev) {
+                    const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
+                    const uint32_t m0 = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+                    const uint32_t m1 = left <= 32 ? 0u : left >= 64 ? 0xffffffffu : (1u << (left - 32)) - 1u;
+                    const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                    for (int x = 0; x < NH; ++x)
+                        if ((bad_prev[x][0] & m0) | (bad_prev[x][1] & m1))
+#pragma unroll
+                            for (int c = x * 32; c < (x + 1) * 32 && c < HH / 2; ++c) o[c] = make_float2(nan, nan);
+                }
+                return true;
+            };
+            for (int j = k; j < kend && ok; ++j) {
+                const int g = gt + j - k;
+                if (j == k) ok = make_k(g, j);
+                if (ok && j + 1 < kend) ok = make_k(g + 1, j + 1);
+                if (ok && j > k) ok = add(g - 1, j - 1);
+                if (ok) ok = make_v(g, j);
+            }
+            gt += kend - k;
+            ok = ok && add(gt - 1, kend - 1) && wtw(&sh.lf, gi);
+            ++gi;
+            if (!ok) continue;
+            if (k == 0 && kend == tiles) {
+                if (live) {
+                    const float inv = lim > 0 ? 1.0f / sh.l[row] : 0.0f;
+                    const int64_t at = rq.first + tok_row;
+                    T *dst = (T *)a.out + at * a.ot + (int64_t)head * HD + half * HH;
+                    const T *gate = a.gate ? (const T *)after_wait(a.gate) + at * a.gt + (int64_t)head * a.gh + half * HH : nullptr;
+#pragma unroll
+                    for (int c = 0; c < HH; c += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) y[2 * x] = lim > 0 ? o[c / 2 + x].x * inv : 0.0f, y[2 * x + 1] = lim > 0 ? o[c / 2 + x].y * inv : 0.0f;
+                        if (gate)
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) y[x] *= sigm(ka_f<T>(gate[c + x]));
+                        if (a.vec) {
+                            if constexpr (HL) {
+                                *(float4 *)(dst + c) = make_float4(y[0], y[1], y[2], y[3]);
+                                *(float4 *)(dst + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                            } else {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * x], y[2 * x + 1]);
+                                    w[x] = *(const uint32_t *)&h;
+                                }
+                                *(uint4 *)(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) dst[c + x] = (T)y[x];
+                        }
+                    }
+                }
+            } else {
+                float *to = a.part + ((size_t)blockIdx.x * 2 + (k == 0)) * a.stride + (size_t)row * HD + half * HH;
+#pragma unroll
+                for (int c = 0; c < HH / 2; c += 2) *(float4 *)(to + 2 * c) = make_float4(o[c].x, o[c].y, o[c + 1].x, o[c + 1].y);
+            }
+        }
+    }
+    // ---- everybody is here (the copies and MMAs of a CTA that gave up as well)
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// joins the parts of split row tiles: a warp takes a row, part after part
+template <typename T, int HD> __global__ void __launch_bounds__(256) k_kv4_prompt_join(const __grid_constant__ Kv4AttnArgs a) {
+    constexpr int PER = HD / 32, U = 4;
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const KaSplit sp = after_wait(a.split)[c];
+    if (sp.parts == 0) return;
+    const KaReq rq = kp_req(a, sp.req);
+    const long long flat = (long long)sp.tile * KP_ROWS + i;
+    if (flat >= (long long)rq.fresh * a.group) return;
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
+    float mx = -INFINITY, y[PER] = {}, sum = 0.0f;
+    for (int x = 0; x < sp.parts; ++x) mx = fmaxf(mx, slot(x)[KP_ROWS * HD + i]);
+    for (int x0 = 0; x0 < sp.parts; x0 += U) {
+        float v[U][PER], w[U], l[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const bool in = x0 + x < sp.parts;
+            const float *p = slot(in ? x0 + x : 0);
+            w[x] = in ? ka_weight(p[KP_ROWS * HD + i], mx) : 0.0f;
+            l[x] = in ? p[KP_ROWS * HD + KP_ROWS + i] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            sum += w[x] * l[x];
+#pragma unroll
+            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
+        }
+    }
+    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
+    ka_emit<T, HD>(a, rq, sp.kv, (int)flat, lane, sees, [&](int d) {
+        float r = 0.0f;
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+            if (d == lane + 32 * x) r = y[x];
+        return r / sum;
+    });
+}
+
+uint64_t kv4_prompt_workspace() {
+    return (uint64_t)std::min(num_sms(), KA_MAX_GRID) * 2 * KpCfg<256, true>::PART * 4;
+}
+
+template <int HD, bool HL> static cudaError_t prompt_go(Kv4AttnArgs a, int max_new, cudaStream_t s) {
+    using C = KpCfg<HD, HL>;
+    cudaError_t e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL>);
+    if (e != cudaSuccess) return e;
+    a.stride = C::PART;
+    const long long rt = ((long long)std::min(max_new, a.rows) * a.group + KP_ROWS - 1) / KP_ROWS;
+    const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
+    const long long units = (long long)a.n * a.l.nkv * std::max(rt, 1ll) * tiles;
+    const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms(), KA_MAX_GRID));
+    e = launch_k(k_kv4_prompt<HD, HL>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
+    if (e != cudaSuccess || grid == 1) return e;
+    return launch_k(k_kv4_prompt_join<typename C::T, HD>, dim3(grid, KP_ROWS / 8), dim3(256), 0, s, a);
+}
+
+cudaError_t launch_kv4_prompt(Kv4AttnArgs a, bool f32, int max_new, cudaStream_t s) {
+    switch (a.l.hd) {
+        case 64: return f32 ? prompt_go<64, true>(a, max_new, s) : prompt_go<64, false>(a, max_new, s);
+        case 128: return f32 ? prompt_go<128, true>(a, max_new, s) : prompt_go<128, false>(a, max_new, s);
+        default: return f32 ? prompt_go<256, true>(a, max_new, s) : prompt_go<256, false>(a, max_new, s);
+    }
+}
+
+}  // namespace fn
