@@ -264,8 +264,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv4_store(const K
         const int c = __float2int_rz(__fadd_rn(__fmul_rn(x[i], inv), 8.5f));
         w |= (uint32_t)min(max(c, 0), 15) << (4 * i);
     }
-    const int64_t page = slot / a.l.bs;
-    const int place = (int)(slot - page * a.l.bs);
+    const int64_t page = slot >> a.l.lbs;
+    const int place = (int)(slot & (a.l.bs - 1));
     uint8_t *rec = a.l.pages + (page * a.l.nkv + h) * (int64_t)a.l.rec;
     *(uint32_t *)(rec + part * a.l.kb + (uint32_t)(g * a.l.bs + place) * 32 + lane * 4) = w;
     if (lane == 0) {
@@ -289,8 +289,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv4_load(const Kv
     }
     float y[8] = {};
     if (slot >= 0) {
-        const int64_t page = slot / a.l.bs;
-        const int place = (int)(slot - page * a.l.bs);
+        const int64_t page = slot >> a.l.lbs;
+        const int place = (int)(slot & (a.l.bs - 1));
         const uint8_t *rec = after_wait(a.l.pages) + (page * a.l.nkv + h) * (int64_t)a.l.rec;
         const uint32_t w = *(const uint32_t *)(rec + part * a.l.kb + (uint32_t)(g * a.l.bs + place) * 32 + lane * 4);
         const float d = __half2float(*(const __half *)(rec + 2 * a.l.kb + part * a.l.sb + (uint32_t)(g * a.l.bs + place) * 2));

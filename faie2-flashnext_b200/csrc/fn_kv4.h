@@ -18,7 +18,7 @@ constexpr int KV4_MAX_REQ = 4096;   // requests per call (the planning CTA's off
 
 struct Kv4Lay {
     uint8_t *pages;
-    int n_pages, bs, nkv, hd, ng;   // ng = hd / 64
+    int n_pages, bs, lbs, nkv, hd, ng;  // lbs = log2 bs, ng = hd / 64
     uint32_t kb, sb, rec;           // bytes of a record's K codes (= V codes), of its K scales (= V scales), of all
 };
 
@@ -37,6 +37,7 @@ inline int kv4_layout(const fn_kv4_t *c, Kv4Lay &l, const char *who) {
     l.pages = c->pages;
     l.n_pages = c->n_pages;
     l.bs = c->page_size;
+    l.lbs = l.bs == 16 ? 4 : l.bs == 32 ? 5 : 6;
     l.nkv = c->nkv;
     l.hd = c->hd;
     l.ng = c->hd / KV4_GROUP;

@@ -187,7 +187,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         dev_fail(a.err, DEV_WAIT_TIMEOUT);
         return false;
     };
-    const int ppt = KA_TOK / a.l.bs;  // pages of a stage
+    const int ppt = KA_TOK >> a.l.lbs;  // pages of a stage
 
     if (warp >= KA_CONS) {
         if constexpr (C::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KA_REG_COPY));
@@ -197,7 +197,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         for (; u < u1; next()) {
             here();
             const int kv = item / rq.rt;
-            const int pages = (rq.len + a.l.bs - 1) / a.l.bs;
+            const int pages = (rq.len + a.l.bs - 1) >> a.l.lbs;
             const int *tab = after_wait(a.table) + (size_t)r * a.max_pages;
             const int p0 = k * ppt;
             int cur = p0 + lane < pages ? tab[p0 + lane] : -1, nxt = p0 + 32 + lane < pages ? tab[p0 + 32 + lane] : -1, base = p0;
@@ -323,13 +323,13 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         auto step = [&](auto mk, const uint8_t *st, int t0, uint32_t valid) {
             constexpr bool M = decltype(mk)::value;
             // the run's first 16 tokens, and how far its second 16 are
-            const int at = half * 32, pg = at / a.l.bs, pl = at - pg * a.l.bs;
+            const int at = half * 32, pg = at >> a.l.lbs, pl = at & (a.l.bs - 1);
             const uint8_t *rec = st + pg * a.l.rec;
             const uint32_t code2 = a.l.bs == 16 ? a.l.rec : 512, scale2 = a.l.bs == 16 ? a.l.rec : 32;
             const uint32_t cstep = a.l.bs * 32, sstep = a.l.bs * 2;  // to the next 64 dims
             const uint8_t *kp = rec + (pl + tk) * 32 + t * 8, *ks = rec + 2 * a.l.kb + (pl + tk) * 2;
             auto hidden = [&](int b, int h, int lm) {
-                return !(valid >> ((at + b * 16 + h * 8) / a.l.bs) & 1u) || t0 + b * 16 + h * 8 + tk >= lm;
+                return !(valid >> ((at + b * 16 + h * 8 >> a.l.lbs)) & 1u) || t0 + b * 16 + h * 8 + tk >= lm;
             };
             // ---- scores of tokens tk, tk + 8 of both runs
             float2 sc[NT][2][2] = {};
@@ -696,7 +696,8 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         a.part = (float *)((uint8_t *)ws + KA_MAX_GRID * sizeof(KaSplit));
         const bool f32 = type == T_F32;
         const int64_t size = f32 ? 4 : 2;
-        a.vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0 && out_token * size % 16 == 0;
+        a.vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0 && out_token * size % 16 == 0 &&
+                (!gate || ((uintptr_t)gate % 16 == 0 && gate_token * size % 16 == 0 && gate_head * size % 16 == 0));
         const cudaStream_t s = (cudaStream_t)stream;
         const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
                             : c->hd == 128 ? attn_go<128>(a, f32, max_new, s)

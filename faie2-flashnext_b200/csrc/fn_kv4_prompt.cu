@@ -6,6 +6,7 @@
 //
 // Roles of the CTA's 16 warps, one CTA per SM:
 //   * warp 0 copies pages into rings (K and V parts apart: they are consumed at different times);
+//   * warp 2 looks at each tile's V scales: their exponent, and which are not finite;
 //   * warp 1 issues the MMAs: S of tile j + 1 before O of tile j, so the softmax of one runs beside the products of the other;
 //   * warps 4..7 (a row a lane): scores out of tensor memory, running softmax, P back into tensor memory in S's place;
 //   * warps 8..15: Q into tensor memory, K and V codes into the MMAs' operands in shared memory, and the running output:
@@ -13,8 +14,10 @@
 //     over tokens are rounded fp32 additions, where the tensor core's own accumulation over a long context cuts, and a new
 //     maximum needs no pass over tensor memory.
 //
-// Scales. A tile's codes become (c - 8) d 2^-e with e the exponent of the tile's largest |d|, in fp16: in range whatever
-// the size of K or V; 2^e goes into the scores (K) and into the addition (V). Rows of q are scaled by a power of two.
+// Scales. V's codes of a tile become (c - 8) d 2^-e in fp16, e the exponent of the tile's largest |d|, and 2^e goes into
+// the addition: in range whatever the size of V (warp 2 finds e ahead of the workers). K's become (c - 8) d / 8: no fp16
+// scale overflows, and what a tiny K loses (2^-25 of its codes' fp16 grid) is nothing beside the other scores. Rows of q are
+// scaled by a power of two.
 // bf16 rows: one product each; q is exact, K, P and V are rounded to 11 bits. fp32 rows: q, K, P and V are fp16 pairs (22
 // bits, K's and V's exact), three products each, the small ones first, so that the sum's cut bits are few.
 //
@@ -28,7 +31,6 @@
 namespace fn {
 
 constexpr int KP_ROWS = 128, KP_THREADS = 512;
-constexpr int KP_REG_IO = 40, KP_REG_SM = 120, KP_REG_WORK = 176;  // 40 + 120 + 2 x 176 = 4 x 128 at launch
 constexpr int KP_W_SM = 4, KP_W_WORK = 8;
 
 template <int HD, bool HL> struct KpCfg {
@@ -43,6 +45,9 @@ template <int HD, bool HL> struct KpCfg {
     static constexpr uint32_t QL = HL ? KP_ROWS * HD * 2 : 0;  // second halves of q: [dim / 8][row] x 16 bytes
     static constexpr uint32_t K_OFF = 4096, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
     static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAW, SMEM = RV_OFF + RV * RAW;
+    // registers by warpgroup: IO + SM + 2 WORK <= 4 x 128 at launch; the workers hold HD / 2 sums
+    static constexpr int REG_IO = HD == 256 ? 40 : 72, REG_SM = HD == 256 ? 120 : 128, REG_WORK = HD == 256 ? 176 : 152;
+    static_assert(REG_IO + REG_SM + 2 * REG_WORK <= 512);
     static constexpr int PART = KP_ROWS * HD + 2 * KP_ROWS;
     // tensor memory: O, then q's first halves, then S / P twice (64 columns: P's halves 32 each)
     static constexpr uint32_t TM_O = 0, TM_Q = HD, TM_S = HD + HD / 2;
@@ -51,11 +56,13 @@ template <int HD, bool HL> struct KpCfg {
 
 // the fixed part of shared memory
 struct KpShared {
-    uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], ve[2], sf[2], pf[2], of, oe, qf, qe, lf, done;
+    uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[2], of, oe, qf, qe, lf, done;
     long long red[KP_THREADS / 32], off;
     uint32_t tmem, valid[8];
     int req, fail;
-    float ek[4], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    float ev[4], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    uint32_t bad[4][4][2];  // tokens whose V scale is not finite: [tile & 3][group][token / 32]
+    int any_bad[4];
 };
 static_assert(sizeof(KpShared) <= 4096);
 
@@ -68,6 +75,23 @@ __device__ __forceinline__ bool kp_bar_work_or(bool p) {
         : "r"((uint32_t)p)
         : "memory");
     return any != 0;
+}
+// tcgen05.ld without its wait; kp_tmem_got makes the values of a load usable after tmem_wait_ld
+__device__ __forceinline__ void kp_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void kp_tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void kp_tmem_got(uint32_t (&r)[16]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+__device__ __forceinline__ float2 kp_pair(const uint32_t (&r)[16], int i) {
+    return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 __device__ __forceinline__ void kp_bar_work() { asm volatile("bar.sync 2, 256;" ::: "memory"); }
 __device__ __forceinline__ float kp_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -88,6 +112,31 @@ __device__ __forceinline__ uint32_t kp_hrest2(uint32_t a, uint32_t b, uint32_t c
 __device__ __forceinline__ uint32_t kp_low(uint32_t w) { return kp_hsub2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
 __device__ __forceinline__ uint32_t kp_high(uint32_t w) { return kp_hsub2((w & 0x00f000f0u) | 0x54005400u, 0x54805480u); }
 
+// N adjacent values of a row (zeros unless `there`); vec: 16-byte aligned
+template <typename T, int N> __device__ __forceinline__ void kp_load(const T *p, bool there, bool vec, float (&x)[N]) {
+    if (!there) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) x[d] = 0.0f;
+    } else if (!vec) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) x[d] = ka_f<T>(p[d]);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int d = 0; d < N; d += 4) {
+            const float4 v = *(const float4 *)(p + d);
+            x[d] = v.x, x[d + 1] = v.y, x[d + 2] = v.z, x[d + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int d = 0; d < N; d += 8) {
+            const uint4 v = *(const uint4 *)(p + d);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[d + 2 * y] = __uint_as_float(w[y] << 16), x[d + 2 * y + 1] = __uint_as_float(w[y] & 0xffff0000u);
+        }
+    }
+}
+
 // tiles of 64 tokens that row tile i of a request sees
 __device__ __forceinline__ int kp_tiles(const KaReq &q, int group, int i) {
     const int last = min((int)min((long long)(i + 1) * KP_ROWS, (long long)q.fresh * group) - 1, INT32_MAX - 1) / group;
@@ -106,8 +155,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 8), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 8);
-            mbar_init(&sh.kf[i], 8), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 8), mbar_init(&sh.ve[i], 1);
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 8), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 9);
+            mbar_init(&sh.kf[i], 8), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 8), mbar_init(&sh.xf[i], 1);
             mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
         }
         mbar_init(&sh.of, 1), mbar_init(&sh.oe, 8), mbar_init(&sh.qf, 8), mbar_init(&sh.qe, 1), mbar_init(&sh.lf, 4);
@@ -222,18 +271,18 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         dev_fail(a.err, DEV_WAIT_TIMEOUT);
         return false;
     };
-    const int ppt = KA_TOK / a.l.bs;  // pages of a tile
+    const int ppt = KA_TOK >> a.l.lbs;  // pages of a tile
     const uint32_t praw = a.l.kb + a.l.sb;  // bytes of a page's K (or V) part in a stage
     int gt = 0, gi = 0;  // tiles and row tiles done by this role
 
     if (warp < KP_W_SM) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_IO));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_IO));
         if (warp == 0) {
             // ---- copies: lane p fetches page p of a tile
             bool ok = true;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
-                const int pages = (rq.len + a.l.bs - 1) / a.l.bs;
+                const int pages = (rq.len + a.l.bs - 1) >> a.l.lbs;
                 const int *tab = after_wait(a.table) + (size_t)r * a.max_pages;
                 int ahead = lane < ppt && k * ppt + lane < pages ? tab[k * ppt + lane] : -1;
                 for (int j = k; j < kend && ok; ++j, ++gt) {
@@ -271,6 +320,45 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     for (int i = max(gt - R, 0); i <= gt; ++i)
                         if (i < gt || v == 0) mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
                 }
+        } else if (warp == 2) {
+            // ---- V scales of a tile: the exponent of the largest finite one, and which are not
+            bool ok = true;
+            for (; u < u1 && ok; next()) {
+                if (!here()) continue;
+                const int hi_lim = limit(KP_ROWS - 1);
+                for (int j = k; j < kend && ok; ++j, ++gt) {
+                    ok = __all_sync(0xffffffffu, wt(&sh.rvf[gt % C::RV], gt / C::RV));
+                    if (!ok) break;
+                    const uint8_t *raw = sm_kp + C::RV_OFF + (gt % C::RV) * C::RAW + a.l.kb;
+                    const uint32_t valid = sh.valid[gt & 7];
+                    float mx = 0.0f;
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int tok = lane + 32 * h, pg = tok >> a.l.lbs;
+                        const bool here_ = (valid >> pg & 1u) && j * KA_TOK + tok < hi_lim;
+#pragma unroll
+                        for (int x = 0; x < NG; ++x) {
+                            const float d = fabsf(ka_half(raw + pg * praw + (x * a.l.bs + (tok & (a.l.bs - 1))) * 2));
+                            if (here_ && d < INFINITY) mx = fmaxf(mx, d);
+                            const uint32_t bad = __ballot_sync(0xffffffffu, here_ && !(d < INFINITY));
+                            if (lane == 0) sh.bad[gt & 3][x][h] = bad;
+                            any |= bad;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    if (lane == 0) {
+                        sh.ev[gt & 3] = mx > 0.0f ? kp_pow2((int)(__float_as_uint(mx) >> 23) - 127) : 1.0f;
+                        sh.any_bad[gt & 3] = any != 0;
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc_arrive(&sh.xf[gt & 1]);
+                        tc_arrive(&sh.rve[gt % C::RV]);
+                    }
+                }
+            }
         } else if (warp == 1 && lane == 0) {
             // ---- MMAs
             constexpr uint32_t id_s = umma_idesc_f16(128, KA_TOK), id_o = umma_idesc_f16(128, HD);
@@ -321,7 +409,6 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         tc_fence_after();
                         outputs(g);
                         umma_commit(&sh.of);
-                        umma_commit(&sh.ve[g % NB]);
                     }
                 }
                 gt = g0 + n;
@@ -334,7 +421,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         __syncwarp();
     } else if (warp < KP_W_WORK) {
         // ---- softmax: row 32 (warp % 4) + lane
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_SM));
+        if constexpr (C::REG_SM < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_SM));
         const int row = tid - 32 * KP_W_SM;
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::TM_S;
         bool ok = true;
@@ -350,44 +437,44 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 if (!ok) break;
                 tc_fence_after();
                 if (j == k) rs = sh.rs[row];
-                float s[64];
+                uint32_t sr[4][16];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld16(tl + (uint32_t)b * 64u + 16u * c, *(float(*)[16]) & s[16 * c]);
-                const float f = rs * sh.ek[gt & 3];
+                for (int c = 0; c < 4; ++c) kp_tmem_ld16(tl + (uint32_t)b * 64u + 16u * c, sr[c]);
+                kp_tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) kp_tmem_got(sr[c]);
                 const uint32_t valid = sh.valid[gt & 7];
                 const int t0 = j * KA_TOK;
                 if (t0 + KA_TOK > lim || valid != (1u << ppt) - 1u) {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        const bool gone = t0 + c >= lim || !(valid >> (c / a.l.bs) & 1u);
-                        s[c] = gone ? -INFINITY : s[c] * f;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) s[c] *= f;
+                    for (int c = 0; c < 64; ++c)
+                        if (t0 + c >= lim || !(valid >> (c >> a.l.lbs) & 1u)) sr[c >> 4][c & 15] = 0xff800000u;  // -inf
                 }
-                float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sr[c >> 4][c & 15]));
+                // rs > 0: the maximum may be taken before the scaling
+                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rs);
                 // weights 2^10 exp2(s - maximum): fp16 keeps 11 bits down to 2^-24 of the largest
                 const float z = mn == -INFINITY ? 0.0f : 10.0f - mn;
                 const float fac = m == -INFINITY ? 0.0f : ka_exp2(m - mn);
                 m = mn;
                 sh.f[gt & 3][row] = fac;
-                float ls[4] = {};
-                uint32_t hi[32], lo[HL ? 32 : 1];
+                const float2 rs2 = make_float2(rs, rs), z2 = make_float2(z, z);
+                float2 ls[2] = {};
+                uint32_t hi[32];
+                [[maybe_unused]] uint32_t lo[HL ? 32 : 1];
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
-                    const float p0 = ka_exp2(s[2 * c] + z), p1 = ka_exp2(s[2 * c + 1] + z);
-                    ls[c & 3] += p0 + p1;
-                    hi[c] = ka_pack(p0, p1);
+                    const float2 x = __ffma2_rn(kp_pair(sr[c >> 3], c & 7), rs2, z2), p = make_float2(ka_exp2(x.x), ka_exp2(x.y));
+                    ls[c & 1] = __fadd2_rn(ls[c & 1], p);
+                    hi[c] = ka_pack(p.x, p.y);
                     if constexpr (HL) {
                         const float2 h = ka_unpack(hi[c]);
-                        lo[c] = ka_pack(p0 - h.x, p1 - h.y);
+                        lo[c] = ka_pack(p.x - h.x, p.y - h.y);
                     }
                 }
-                l = l * fac + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+                l = l * fac + ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     tmem_st16(tl + (uint32_t)b * 64u + 16u * c, *(uint32_t(*)[16]) & hi[16 * c]);
@@ -413,7 +500,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         }
     } else {
         // ---- workers: q, K, V into operands; the running output, dims [half HD / 2, + HD / 2) of row 32 (warp % 4) + lane
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_WORK));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_WORK));
         const int wtid = tid - 32 * KP_W_WORK, half = (warp - KP_W_WORK) >> 2, row = 32 * (warp & 3) + lane;
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         constexpr int HH = HD / 2, NH = HH >= KV4_GROUP ? HH / KV4_GROUP : 1;  // this half's dims, and its 64-dim groups
@@ -433,47 +520,32 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             // ---- q: scaled so that the row's largest value is 2^10..2^11, dims in the order of the codes' nibbles
             {
                 const T *src = (const T *)after_wait(a.q) + (int64_t)(rq.first + tok_row) * a.qt + (int64_t)head * a.qh + half * HH;
-                float mx = 0.0f;
-                if (live)
-#pragma unroll 8
-                    for (int d = 0; d < HH; d += 4) {
-                        float x[4];
-                        if (a.vec) {
-                            if constexpr (HL) *(float4 *)x = *(const float4 *)(src + d);
-                            else {
-                                const uint2 w = *(const uint2 *)(src + d);
-                                x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u);
-                                x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
-                            }
-                        } else {
+                float x[HH], mx = 0.0f;
+                kp_load<T, HH>(src, live, a.vec, x);
 #pragma unroll
-                            for (int y = 0; y < 4; ++y) x[y] = ka_f<T>(src[d + y]);
-                        }
-                        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
-                    }
+                for (int d = 0; d < HH; ++d) mx = fmaxf(mx, fabsf(x[d]));
                 // both halves of the row agree on its exponent (K's place is free before the row tile's first K)
                 float *sx = (float *)(sm_kp + C::K_OFF);
                 sx[half * KP_ROWS + row] = mx;
                 kp_bar_work();
                 mx = fmaxf(mx, sx[(half ^ 1) * KP_ROWS + row]);
                 const int e = min(max(10 - ((int)(__float_as_uint(mx) >> 23) - 127), -90), 120);
-                const float up = kp_pow2(e);
-                if (half == 0) sh.rs[row] = a.scale * 1.44269504f * kp_pow2(-e);
+                const float up = a.scale < 0.0f ? -kp_pow2(e) : kp_pow2(e);
+                // scores in base 2: undo the scaling, and K's 1 / 8; positive also for a scale of zero
+                if (half == 0) sh.rs[row] = fmaxf(fabsf(a.scale) * 8.0f * 1.44269504f * kp_pow2(-e), 1e-30f);
                 kp_bar_work();
-#pragma unroll 1
+#pragma unroll
                 for (int d = 0; d < HH; d += 32) {
                     uint32_t hi[16];
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        float x[8];
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) x[y] = live ? ka_f<T>(src[d + 8 * w + y]) * up : 0.0f;
                         uint32_t lo[4];
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            hi[4 * w + y] = ka_pack(x[y], x[y + 4]);
+                            const float x0 = x[d + 8 * w + y] * up, x1 = x[d + 8 * w + y + 4] * up;
+                            hi[4 * w + y] = ka_pack(x0, x1);
                             const float2 h = ka_unpack(hi[4 * w + y]);
-                            lo[y] = ka_pack(x[y] - h.x, x[y + 4] - h.y);
+                            lo[y] = ka_pack(x0 - h.x, x1 - h.y);
                         }
                         if constexpr (HL)
                             *(uint4 *)(sm_kp + C::Q_OFF + ((half * HH + d) / 8 + w) * 2048 + row * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -489,51 +561,31 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             float2 o[HH / 2];
 #pragma unroll
             for (int c = 0; c < HH / 2; ++c) o[c] = make_float2(0.0f, 0.0f);
-            float ev_prev = 1.0f;
-            uint32_t bad_prev[NH][2] = {};
-            bool any_prev = false;
-
-            // what a tile's tokens may be used for: page there, and some row sees it
-            auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok / a.l.bs) & 1u) && j * KA_TOK + tok < hi_lim; };
-            // the exponent of the tile's largest finite |scale|
-            auto exponent = [&](const uint8_t *raw, int g, int j) {
-                float mx = 0.0f;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int tok = lane + 32 * h, pg = tok / a.l.bs;
-                    if (there(g, j, tok))
-#pragma unroll
-                        for (int x = 0; x < NG; ++x) {
-                            const float d = fabsf(ka_half(raw + pg * praw + a.l.kb + (x * a.l.bs + tok - pg * a.l.bs) * 2));
-                            if (d < INFINITY) mx = fmaxf(mx, d);
-                        }
-                }
-#pragma unroll
-                for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                return mx > 0.0f ? (int)(__float_as_uint(mx) >> 23) - 127 : 0;
-            };
+            // every token of the tile has its page and is seen by some row
+            auto whole = [&](int g, int j) { return sh.valid[g & 7] == (1u << ppt) - 1u && (j + 1) * KA_TOK <= hi_lim; };
+            auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
             // K of tile g (the row tile's j): 16 bytes of codes (32 dims of a token) at a time
             auto make_k = [&](int g, int j) {
                 if (!wtw(&sh.rkf[g % C::RK], g / C::RK)) return false;
-                if (g >= NB && !wtw(&sh.ke[g % NB], g / NB - 1)) return false;
+                // (with two buffers, the product that read this one came before an O that has been added)
+                if (NB == 1 && g >= 1 && !wtw(&sh.ke[0], g - 1)) return false;
                 const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAW;
                 uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT;
-                const int e = exponent(raw, g, j);
-                const float up = kp_pow2(-e);
-                if (wtid == 0) sh.ek[g & 3] = kp_pow2(e);
+                const bool all = whole(g, j);
 #pragma unroll
                 for (int x = 0; x < (2 * NG * 64 + 255) / 256; ++x) {
                     const int un = wtid + 256 * x, tok = un & 63, q = un >> 6;  // quarter q of 32 dims
                     if (q < 2 * NG) {
-                        const int pg = tok / a.l.bs, line = (q >> 1) * a.l.bs + tok - pg * a.l.bs;
+                        const int pg = tok >> a.l.lbs, line = (q >> 1) * a.l.bs + (tok & (a.l.bs - 1));
                         const uint8_t *src = raw + pg * praw;
-                        const float d = there(g, j, tok) ? ka_half(src + a.l.kb + line * 2) * up : 0.0f;
-                        const uint32_t dd = ka_pack(d, d);
                         const uint4 w4 = *(const uint4 *)(src + line * 32 + (q & 1) * 16);
+                        float d = ka_half(src + a.l.kb + line * 2) * 0.125f;
+                        if (!all && !there(g, j, tok)) d = 0.0f;
+                        const uint32_t dd = ka_pack(d, d);
                         const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            const uint32_t w = ws[y], c0 = kp_low(w), c1 = kp_high(w), c2 = kp_low(w >> 8), c3 = kp_high(w >> 8);
+                            const uint32_t w = ws[y], w8 = w >> 8, c0 = kp_low(w), c1 = kp_high(w), c2 = kp_low(w8), c3 = kp_high(w8);
                             const uint32_t h0 = kp_hmul2(c0, dd), h1 = kp_hmul2(c1, dd), h2 = kp_hmul2(c2, dd), h3 = kp_hmul2(c3, dd);
                             uint8_t *at = to + (q * 4 + y) * 1024 + tok * 16;
                             *(uint4 *)at = make_uint4(h0, h1, h2, h3);
@@ -550,48 +602,40 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 }
                 return true;
             };
-            // V of tile g: 8 tokens x 8 dims at a time, turned
+            // V of tile g: 8 tokens x 8 dims (4 where the dims are few) at a time, turned. Its buffer's last reader came before
+            // an O that has been added.
             auto make_v = [&](int g, int j) {
-                if (!wtw(&sh.rvf[g % C::RV], g / C::RV)) return false;
-                if (g >= NB && !wtw(&sh.ve[g % NB], g / NB - 1)) return false;
+                constexpr int BY = HD == 256 ? 4 : 2;  // bytes of a word that a thread takes
+                if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 1], g >> 1)) return false;
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
                 uint8_t *to = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT;
-                const int e = exponent(raw, g, j);
-                const float up = kp_pow2(-e);
-                ev_prev = kp_pow2(e);
-                // tokens whose scale is not finite, by group of this half's dims
-                uint32_t any = 0;
-#pragma unroll
-                for (int x = 0; x < NH; ++x)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int tok = lane + 32 * h, pg = tok / a.l.bs;
-                        const float d = fabsf(ka_half(raw + pg * praw + a.l.kb + ((g0 + x) * a.l.bs + tok - pg * a.l.bs) * 2));
-                        bad_prev[x][h] = __ballot_sync(0xffffffffu, there(g, j, tok) && !(d < INFINITY));
-                        any |= bad_prev[x][h];
-                    }
-                any_prev = any != 0;
-                if (wtid < HD) {
-                    const int ch = wtid & 7, wd = wtid >> 3, tok = ch * 8, pg = tok / a.l.bs;
-                    const int line = (wd >> 3) * a.l.bs + tok - pg * a.l.bs;
+                const int ch = wtid & 7, wd = (wtid >> 3) % (HD / 8), b0 = (wtid >> 3) / (HD / 8) * BY;
+                if (b0 < 4) {
+                    const int tok = ch * 8, pg = tok >> a.l.lbs, line = (wd >> 3) * a.l.bs + (tok & (a.l.bs - 1));
                     const uint8_t *src = raw + pg * praw;
                     const uint4 s4 = *(const uint4 *)(src + a.l.kb + line * 2);
                     const uint32_t ss[4] = {s4.x, s4.y, s4.z, s4.w};
                     uint32_t w[8], dd[4];
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + (line + y) * 32 + (wd & 7) * 4);
+                    for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + (line + y) * 32 + (wd & 7) * 4) >> (8 * b0);
+                    const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 3]));  // 1 / 2^e
+                    const bool all = whole(g, j) && !sh.any_bad[g & 3];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
                         float2 d = ka_unpack(ss[y]);
-                        d.x = there(g, j, tok + 2 * y) && fabsf(d.x) < INFINITY ? d.x * up : 0.0f;
-                        d.y = there(g, j, tok + 2 * y + 1) && fabsf(d.y) < INFINITY ? d.y * up : 0.0f;
+                        d.x *= up, d.y *= up;
+                        if (!all) {
+                            if (!(there(g, j, tok + 2 * y) && fabsf(d.x) < INFINITY)) d.x = 0.0f;
+                            if (!(there(g, j, tok + 2 * y + 1) && fabsf(d.y) < INFINITY)) d.y = 0.0f;
+                        }
                         dd[y] = ka_pack(d.x, d.y);
                     }
-                    uint8_t *at = to + ch * C::VG + wd * 128;
+                    uint8_t *at = to + ch * C::VG + wd * 128 + b0 * 32;
 #pragma unroll
-                    for (int by = 0; by < 4; ++by) {
+                    for (int by = 0; by < BY; ++by) {
                         const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
-                        uint32_t h[2][4], lo[2][4];
+                        uint32_t h[2][4];
+                        [[maybe_unused]] uint32_t lo[2][4];
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
                             const uint32_t x = __byte_perm(w[2 * y], w[2 * y + 1], sel), c0 = kp_low(x), c1 = kp_high(x);
@@ -613,31 +657,42 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 }
                 return true;
             };
-            // o = o f + O 2^e of tile g
-            auto add = [&](int g, int j) {
+            // o = o f + O 2^e of tile g, its tensor-memory loads two ahead; `between` runs while the first are on their way
+            auto add = [&](int g, int j, auto between) {
                 if (!wtw(&sh.of, g)) return false;
                 tc_fence_after();
-                const float f = sh.f[g & 3][row];
-                const float2 f2 = make_float2(f, f), e2 = make_float2(ev_prev, ev_prev);
+                const uint32_t to = tl + C::TM_O + (uint32_t)(half * HH);
+                uint32_t x[2][16];
+                kp_tmem_ld16(to, x[0]);
+                if (HH > 16) kp_tmem_ld16(to + 16u, x[1]);
+                if (!between()) return false;
+                const float f = sh.f[g & 3][row], e = sh.ev[g & 3];
+                const float2 f2 = make_float2(f, f), e2 = make_float2(e, e);
 #pragma unroll
-                for (int c = 0; c < HH; c += 16) {
-                    float x[16];
-                    tmem_ld16(tl + C::TM_O + (uint32_t)(half * HH + c), x);
+                for (int c = 0; c < HH; c += 32) {
+                    kp_tmem_wait_ld();
+                    kp_tmem_got(x[0]);
+                    kp_tmem_got(x[1]);
 #pragma unroll
-                    for (int y = 0; y < 8; ++y)
-                        o[c / 2 + y] = __ffma2_rn(make_float2(x[2 * y], x[2 * y + 1]), e2, __fmul2_rn(o[c / 2 + y], f2));
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(kp_pair(x[h], y), e2, __fmul2_rn(o[c / 2 + h * 8 + y], f2));
+                    if (c + 32 < HH) {
+                        kp_tmem_ld16(to + c + 32u, x[0]);
+                        kp_tmem_ld16(to + c + 48u, x[1]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc_arrive(&sh.oe);
-                if (any_prev) {
+                if (sh.any_bad[g & 3]) {
                     const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
                     const uint32_t m0 = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
                     const uint32_t m1 = left <= 32 ? 0u : left >= 64 ? 0xffffffffu : (1u << (left - 32)) - 1u;
                     const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
                     for (int x = 0; x < NH; ++x)
-                        if ((bad_prev[x][0] & m0) | (bad_prev[x][1] & m1))
+                        if ((sh.bad[g & 3][g0 + x][0] & m0) | (sh.bad[g & 3][g0 + x][1] & m1))
 #pragma unroll
                             for (int c = x * 32; c < (x + 1) * 32 && c < HH / 2; ++c) o[c] = make_float2(nan, nan);
                 }
@@ -646,12 +701,12 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             for (int j = k; j < kend && ok; ++j) {
                 const int g = gt + j - k;
                 if (j == k) ok = make_k(g, j);
-                if (ok && j + 1 < kend) ok = make_k(g + 1, j + 1);
-                if (ok && j > k) ok = add(g - 1, j - 1);
+                auto ahead = [&]() { return j + 1 < kend ? make_k(g + 1, j + 1) : true; };
+                if (ok) ok = j > k ? add(g - 1, j - 1, ahead) : ahead();
                 if (ok) ok = make_v(g, j);
             }
             gt += kend - k;
-            ok = ok && add(gt - 1, kend - 1) && wtw(&sh.lf, gi);
+            ok = ok && add(gt - 1, kend - 1, []() { return true; }) && wtw(&sh.lf, gi);
             ++gi;
             if (!ok) continue;
             if (k == 0 && kend == tiles) {
@@ -665,9 +720,12 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         float y[8];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) y[2 * x] = lim > 0 ? o[c / 2 + x].x * inv : 0.0f, y[2 * x + 1] = lim > 0 ? o[c / 2 + x].y * inv : 0.0f;
-                        if (gate)
+                        if (gate) {
+                            float gx[8];
+                            kp_load<T, 8>(gate + c, true, a.vec, gx);
 #pragma unroll
-                            for (int x = 0; x < 8; ++x) y[x] *= sigm(ka_f<T>(gate[c + x]));
+                            for (int x = 0; x < 8; ++x) y[x] *= sigm(gx[x]);
+                        }
                         if (a.vec) {
                             if constexpr (HL) {
                                 *(float4 *)(dst + c) = make_float4(y[0], y[1], y[2], y[3]);
