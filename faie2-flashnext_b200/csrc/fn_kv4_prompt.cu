@@ -58,14 +58,24 @@ template <int HD, bool HL> struct KpCfg {
 struct KpShared {
     uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[2], of, oe, qf, qe, lf, done;
     long long red[KP_THREADS / 32], off;
-    uint32_t tmem, valid[8];
+    uint32_t tmem, valid[8];  // pages there of tile & 7; bit 31: all of them, and every token seen by some row
     int req, fail;
-    float ev[4], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
-    uint32_t bad[4][4][2];  // tokens whose V scale is not finite: [tile & 3][group][token / 32]
-    int any_bad[4];
+    // rings as long as the fastest role can be ahead of the slowest reader
+    float ev[8], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    uint32_t bad[8][4][2];  // tokens whose V scale is not finite: [tile & 7][group][token / 32]
+    int any_bad[8];
 };
 static_assert(sizeof(KpShared) <= 4096);
 
+// whether a phase has completed, after a short wait in the hardware
+__device__ __forceinline__ bool kp_try(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
 // the workers' barrier, and whether any of them brought `p`
 __device__ __forceinline__ bool kp_bar_work_or(bool p) {
     uint32_t any;
@@ -155,8 +165,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 8), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 9);
-            mbar_init(&sh.kf[i], 8), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 8), mbar_init(&sh.xf[i], 1);
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 4), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 5);
+            mbar_init(&sh.kf[i], 4), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 4), mbar_init(&sh.xf[i], 1);
             mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
         }
         mbar_init(&sh.of, 1), mbar_init(&sh.oe, 8), mbar_init(&sh.qf, 8), mbar_init(&sh.qe, 1), mbar_init(&sh.lf, 4);
@@ -265,6 +275,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         return min(max(rq.len - rq.fresh + f / a.group + 1, 0), rq.len);
     };
     auto wt = [&](uint64_t *bar, int phase) {
+        if (kp_try(bar, (uint32_t)phase & 1u)) return true;
         if (*s_fail) return false;
         if (mbar_park(bar, (uint32_t)phase & 1u)) return true;
         *s_fail = 1;
@@ -282,7 +293,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             bool ok = true;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
-                const int pages = (rq.len + a.l.bs - 1) >> a.l.lbs;
+                const int pages = (rq.len + a.l.bs - 1) >> a.l.lbs, hi_lim = limit(KP_ROWS - 1);
                 const int *tab = after_wait(a.table) + (size_t)r * a.max_pages;
                 int ahead = lane < ppt && k * ppt + lane < pages ? tab[k * ppt + lane] : -1;
                 for (int j = k; j < kend && ok; ++j, ++gt) {
@@ -298,7 +309,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         if (lane == 0) {
                             ok = gt < R || wt(empty, gt / R - 1);
                             if (ok) {
-                                if (v == 0) sh.valid[gt & 7] = m;
+                                if (v == 0) sh.valid[gt & 7] = m | (m == (1u << ppt) - 1u && (j + 1) * KA_TOK <= hi_lim ? 0x80000000u : 0u);
                                 mbar_arrive_tx(full, (uint32_t)__popc(m) * praw);
                             }
                         }
@@ -342,15 +353,15 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                             const float d = fabsf(ka_half(raw + pg * praw + (x * a.l.bs + (tok & (a.l.bs - 1))) * 2));
                             if (here_ && d < INFINITY) mx = fmaxf(mx, d);
                             const uint32_t bad = __ballot_sync(0xffffffffu, here_ && !(d < INFINITY));
-                            if (lane == 0) sh.bad[gt & 3][x][h] = bad;
+                            if (lane == 0) sh.bad[gt & 7][x][h] = bad;
                             any |= bad;
                         }
                     }
 #pragma unroll
                     for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                     if (lane == 0) {
-                        sh.ev[gt & 3] = mx > 0.0f ? kp_pow2((int)(__float_as_uint(mx) >> 23) - 127) : 1.0f;
-                        sh.any_bad[gt & 3] = any != 0;
+                        sh.ev[gt & 7] = mx > 0.0f ? kp_pow2((int)(__float_as_uint(mx) >> 23) - 127) : 1.0f;
+                        sh.any_bad[gt & 7] = any != 0;
                     }
                     __syncwarp();
                     if (lane == 0) {
@@ -445,7 +456,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 for (int c = 0; c < 4; ++c) kp_tmem_got(sr[c]);
                 const uint32_t valid = sh.valid[gt & 7];
                 const int t0 = j * KA_TOK;
-                if (t0 + KA_TOK > lim || valid != (1u << ppt) - 1u) {
+                if (t0 + KA_TOK > lim || !(valid >> 31)) {
 #pragma unroll
                     for (int c = 0; c < 64; ++c)
                         if (t0 + c >= lim || !(valid >> (c >> a.l.lbs) & 1u)) sr[c >> 4][c & 15] = 0xff800000u;  // -inf
@@ -506,6 +517,16 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         constexpr int HH = HD / 2, NH = HH >= KV4_GROUP ? HH / KV4_GROUP : 1;  // this half's dims, and its 64-dim groups
         const int g0 = half * HH / KV4_GROUP;
         bool ok = true;
+        // Warps 8..11 make K, 12..15 V. A thread takes 16 bytes of codes (32 dims) of token k_tok at a time, from quarter k_q on,
+        // or word v_wd (8 dims) of tokens v_tok .. + 7: places in the stages and operands
+        constexpr int KU = NG, VU = HD >= 128 ? HD / 128 : 1;
+        const int gtid = wtid & 127;
+        const int k_tok = gtid & 63, k_q = gtid >> 6, k_line = k_tok & (a.l.bs - 1);
+        const uint32_t k_src = (k_tok >> a.l.lbs) * praw + k_line * 32 + k_q * 16, k_dst = k_q * 4096 + k_tok * 16;
+        const uint32_t k_sc = (k_tok >> a.l.lbs) * praw + a.l.kb + k_line * 2;
+        const int v_tok = (gtid & 7) * 8, v_wd = gtid >> 3, v_line = (v_wd >> 3) * a.l.bs + (v_tok & (a.l.bs - 1));
+        const uint32_t v_page = (v_tok >> a.l.lbs) * praw, v_src = v_page + v_line * 32 + (v_wd & 7) * 4, v_sc = v_page + a.l.kb + v_line * 2;
+        const uint32_t v_dst = (gtid & 7) * C::VG + v_wd * 128;
         // a wait by all lanes, with one answer
         auto wtw = [&](uint64_t *bar, int phase) { return __all_sync(0xffffffffu, wt(bar, phase)) != 0; };
         for (; u < u1; next()) {
@@ -561,37 +582,29 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             float2 o[HH / 2];
 #pragma unroll
             for (int c = 0; c < HH / 2; ++c) o[c] = make_float2(0.0f, 0.0f);
-            // every token of the tile has its page and is seen by some row
-            auto whole = [&](int g, int j) { return sh.valid[g & 7] == (1u << ppt) - 1u && (j + 1) * KA_TOK <= hi_lim; };
             auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
             // K of tile g (the row tile's j): 16 bytes of codes (32 dims of a token) at a time
             auto make_k = [&](int g, int j) {
                 if (!wtw(&sh.rkf[g % C::RK], g / C::RK)) return false;
-                // (with two buffers, the product that read this one came before an O that has been added)
-                if (NB == 1 && g >= 1 && !wtw(&sh.ke[0], g - 1)) return false;
+                if (g >= NB && !wtw(&sh.ke[g % NB], g / NB - 1)) return false;
                 const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAW;
-                uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT;
-                const bool all = whole(g, j);
+                uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT + k_dst;
+                const bool all = sh.valid[g & 7] >> 31;
 #pragma unroll
-                for (int x = 0; x < (2 * NG * 64 + 255) / 256; ++x) {
-                    const int un = wtid + 256 * x, tok = un & 63, q = un >> 6;  // quarter q of 32 dims
-                    if (q < 2 * NG) {
-                        const int pg = tok >> a.l.lbs, line = (q >> 1) * a.l.bs + (tok & (a.l.bs - 1));
-                        const uint8_t *src = raw + pg * praw;
-                        const uint4 w4 = *(const uint4 *)(src + line * 32 + (q & 1) * 16);
-                        float d = ka_half(src + a.l.kb + line * 2) * 0.125f;
-                        if (!all && !there(g, j, tok)) d = 0.0f;
-                        const uint32_t dd = ka_pack(d, d);
-                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+                for (int x = 0; x < KU; ++x) {  // a 64-dim group each
+                    const uint4 w4 = *(const uint4 *)(raw + k_src + x * a.l.bs * 32);
+                    float d = ka_half(raw + k_sc + x * a.l.bs * 2) * 0.125f;
+                    if (!all && !there(g, j, k_tok)) d = 0.0f;
+                    const uint32_t dd = ka_pack(d, d);
+                    const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const uint32_t w = ws[y], w8 = w >> 8, c0 = kp_low(w), c1 = kp_high(w), c2 = kp_low(w8), c3 = kp_high(w8);
-                            const uint32_t h0 = kp_hmul2(c0, dd), h1 = kp_hmul2(c1, dd), h2 = kp_hmul2(c2, dd), h3 = kp_hmul2(c3, dd);
-                            uint8_t *at = to + (q * 4 + y) * 1024 + tok * 16;
-                            *(uint4 *)at = make_uint4(h0, h1, h2, h3);
-                            if constexpr (HL)
-                                *(uint4 *)(at + C::KT) = make_uint4(kp_hrest2(c0, dd, h0), kp_hrest2(c1, dd, h1), kp_hrest2(c2, dd, h2), kp_hrest2(c3, dd, h3));
-                        }
+                    for (int y = 0; y < 4; ++y) {
+                        const uint32_t w = ws[y], w8 = w >> 8, c0 = kp_low(w), c1 = kp_high(w), c2 = kp_low(w8), c3 = kp_high(w8);
+                        const uint32_t h0 = kp_hmul2(c0, dd), h1 = kp_hmul2(c1, dd), h2 = kp_hmul2(c2, dd), h3 = kp_hmul2(c3, dd);
+                        uint8_t *at = to + (x * 8 + y) * 1024;
+                        *(uint4 *)at = make_uint4(h0, h1, h2, h3);
+                        if constexpr (HL)
+                            *(uint4 *)(at + C::KT) = make_uint4(kp_hrest2(c0, dd, h0), kp_hrest2(c1, dd, h1), kp_hrest2(c2, dd, h2), kp_hrest2(c3, dd, h3));
                     }
                 }
                 async_proxy_fence();
@@ -602,37 +615,34 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 }
                 return true;
             };
-            // V of tile g: 8 tokens x 8 dims (4 where the dims are few) at a time, turned. Its buffer's last reader came before
-            // an O that has been added.
+            // V of tile g: 8 tokens x 8 dims at a time, turned. Its buffer's last reader came before an O that has been added.
             auto make_v = [&](int g, int j) {
-                constexpr int BY = HD == 256 ? 4 : 2;  // bytes of a word that a thread takes
                 if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 1], g >> 1)) return false;
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
-                uint8_t *to = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT;
-                const int ch = wtid & 7, wd = (wtid >> 3) % (HD / 8), b0 = (wtid >> 3) / (HD / 8) * BY;
-                if (b0 < 4) {
-                    const int tok = ch * 8, pg = tok >> a.l.lbs, line = (wd >> 3) * a.l.bs + (tok & (a.l.bs - 1));
-                    const uint8_t *src = raw + pg * praw;
-                    const uint4 s4 = *(const uint4 *)(src + a.l.kb + line * 2);
+                const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 7]));  // 1 / 2^e
+                const bool all = (sh.valid[g & 7] >> 31) && !sh.any_bad[g & 7];
+#pragma unroll
+                for (int un = 0; un < VU; ++un) {
+                    if (HD < 128 && v_wd >= HD / 8) break;
+                    const uint8_t *src = raw + v_src + un * 2 * a.l.bs * 32;  // 16 words on: two groups
+                    const uint4 s4 = *(const uint4 *)(raw + v_sc + un * 2 * a.l.bs * 2);
                     const uint32_t ss[4] = {s4.x, s4.y, s4.z, s4.w};
                     uint32_t w[8], dd[4];
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + (line + y) * 32 + (wd & 7) * 4) >> (8 * b0);
-                    const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 3]));  // 1 / 2^e
-                    const bool all = whole(g, j) && !sh.any_bad[g & 3];
+                    for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + y * 32);
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        float2 d = ka_unpack(ss[y]);
-                        d.x *= up, d.y *= up;
+                        float2 d = __fmul2_rn(ka_unpack(ss[y]), make_float2(up, up));
                         if (!all) {
-                            if (!(there(g, j, tok + 2 * y) && fabsf(d.x) < INFINITY)) d.x = 0.0f;
-                            if (!(there(g, j, tok + 2 * y + 1) && fabsf(d.y) < INFINITY)) d.y = 0.0f;
+                            const int tok = v_tok + 2 * y;
+                            if (!(there(g, j, tok) && fabsf(d.x) < INFINITY)) d.x = 0.0f;
+                            if (!(there(g, j, tok + 1) && fabsf(d.y) < INFINITY)) d.y = 0.0f;
                         }
                         dd[y] = ka_pack(d.x, d.y);
                     }
-                    uint8_t *at = to + ch * C::VG + wd * 128 + b0 * 32;
+                    uint8_t *at = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT + v_dst + un * 2048;
 #pragma unroll
-                    for (int by = 0; by < BY; ++by) {
+                    for (int by = 0; by < 4; ++by) {
                         const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
                         uint32_t h[2][4];
                         [[maybe_unused]] uint32_t lo[2][4];
@@ -657,56 +667,63 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 }
                 return true;
             };
-            // o = o f + O 2^e of tile g, its tensor-memory loads two ahead; `between` runs while the first are on their way
-            auto add = [&](int g, int j, auto between) {
-                if (!wtw(&sh.of, g)) return false;
-                tc_fence_after();
+            // step j: K of tile j + 1 by half of the warps, V of tile j by the other half, then all add O of tile j - 1. (Every part
+            // appears once: the instruction cache holds the loop.)
+            for (int j = k - 1; j <= kend && ok; ++j) {
+                const int g = gt + j - k;
+                const bool adds = j > k;
+                if (half == 0) {
+                    if (j + 1 < kend) ok = make_k(g + 1, j + 1);
+                } else if (NB == 2 && j >= k && j < kend) {
+                    ok = make_v(g, j);
+                }
+                if (!ok) break;
+                if (adds && !wtw(&sh.of, g - 1)) {
+                    ok = false;
+                    break;
+                }
+                // with one buffer V has to wait for the O before it
+                if (NB == 1 && half == 1 && j >= k && j < kend) {
+                    ok = make_v(g, j);
+                    if (!ok) break;
+                }
                 const uint32_t to = tl + C::TM_O + (uint32_t)(half * HH);
-                uint32_t x[2][16];
-                kp_tmem_ld16(to, x[0]);
-                if (HH > 16) kp_tmem_ld16(to + 16u, x[1]);
-                if (!between()) return false;
-                const float f = sh.f[g & 3][row], e = sh.ev[g & 3];
-                const float2 f2 = make_float2(f, f), e2 = make_float2(e, e);
+                if (adds) {  // o = o f + O 2^e
+                    const int gp = (g - 1) & 7;
+                    const float f = sh.f[gp & 3][row], e = sh.ev[gp];
+                    const float2 f2 = make_float2(f, f), e2 = make_float2(e, e);
+                    uint32_t x[2][16];
+                    tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < HH; c += 32) {
-                    kp_tmem_wait_ld();
-                    kp_tmem_got(x[0]);
-                    kp_tmem_got(x[1]);
+                    for (int c = 0; c < HH; c += 32) {
+                        kp_tmem_ld16(to + c, x[0]);
+                        kp_tmem_ld16(to + c + 16u, x[1]);
+                        kp_tmem_wait_ld();
+                        kp_tmem_got(x[0]);
+                        kp_tmem_got(x[1]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(kp_pair(x[h], y), e2, __fmul2_rn(o[c / 2 + h * 8 + y], f2));
-                    if (c + 32 < HH) {
-                        kp_tmem_ld16(to + c + 32u, x[0]);
-                        kp_tmem_ld16(to + c + 48u, x[1]);
+                            for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(kp_pair(x[h], y), e2, __fmul2_rn(o[c / 2 + h * 8 + y], f2));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(&sh.oe);
+                    if (sh.any_bad[gp]) {
+                        const int left = lim - (j - 1) * KA_TOK;  // tokens of the tile that the row sees
+                        const uint32_t m0 = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+                        const uint32_t m1 = left <= 32 ? 0u : left >= 64 ? 0xffffffffu : (1u << (left - 32)) - 1u;
+                        const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                        for (int y = 0; y < NH; ++y)
+                            if ((sh.bad[gp][g0 + y][0] & m0) | (sh.bad[gp][g0 + y][1] & m1))
+#pragma unroll
+                                for (int c = y * 32; c < (y + 1) * 32 && c < HH / 2; ++c) o[c] = make_float2(nan, nan);
                     }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc_arrive(&sh.oe);
-                if (sh.any_bad[g & 3]) {
-                    const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
-                    const uint32_t m0 = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
-                    const uint32_t m1 = left <= 32 ? 0u : left >= 64 ? 0xffffffffu : (1u << (left - 32)) - 1u;
-                    const float nan = __uint_as_float(0x7fffffffu);
-#pragma unroll
-                    for (int x = 0; x < NH; ++x)
-                        if ((sh.bad[g & 3][g0 + x][0] & m0) | (sh.bad[g & 3][g0 + x][1] & m1))
-#pragma unroll
-                            for (int c = x * 32; c < (x + 1) * 32 && c < HH / 2; ++c) o[c] = make_float2(nan, nan);
-                }
-                return true;
-            };
-            for (int j = k; j < kend && ok; ++j) {
-                const int g = gt + j - k;
-                if (j == k) ok = make_k(g, j);
-                auto ahead = [&]() { return j + 1 < kend ? make_k(g + 1, j + 1) : true; };
-                if (ok) ok = j > k ? add(g - 1, j - 1, ahead) : ahead();
-                if (ok) ok = make_v(g, j);
             }
             gt += kend - k;
-            ok = ok && add(gt - 1, kend - 1, []() { return true; }) && wtw(&sh.lf, gi);
+            ok = ok && wtw(&sh.lf, gi);
             ++gi;
             if (!ok) continue;
             if (k == 0 && kend == tiles) {
