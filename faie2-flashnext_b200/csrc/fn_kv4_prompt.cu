@@ -49,7 +49,8 @@ template <int HD, bool HL> struct KpCfg {
     static constexpr int REG_IO = HD == 256 ? 40 : 72, REG_SM = HD == 256 ? 120 : 128, REG_WORK = HD == 256 ? 176 : 152;
     static_assert(REG_IO + REG_SM + 2 * REG_WORK <= 512);
     static constexpr int PART = KP_ROWS * HD + 2 * KP_ROWS;
-    // tensor memory: O, then q's first halves, then S / P twice (64 columns: P's halves 32 each)
+    // tensor memory: O, then q's first halves, then S / P twice (64 columns: of 16 tokens' scores,
+    // P's first halves take 8 and its second halves 8)
     static constexpr uint32_t TM_O = 0, TM_Q = HD, TM_S = HD + HD / 2;
     static_assert(SMEM <= 227 * 1024 && TM_S + 128 <= 512);
 };
@@ -94,6 +95,11 @@ __device__ __forceinline__ void kp_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) 
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+__device__ __forceinline__ void kp_tmem_st8(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ void kp_tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void kp_tmem_got(uint32_t (&r)[16]) {
@@ -379,23 +385,29 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 const uint32_t ts = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, kt = kb + (uint32_t)(g % NB) * C::TERMS * C::KT;
                 uint32_t acc = 0;
                 if constexpr (HL) {
+#pragma unroll 1
                     for (int x = 0; x < HD / 16; ++x, acc = 1)
                         umma_f16_smem_a(ts, umma_desc(ql + x * 4096u, 2048u, 128u), umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
+#pragma unroll 1
                     for (int x = 0; x < HD / 16; ++x)
                         umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + C::KT + x * 2048u, 1024u, 128u), id_s, 1u);
                 }
+#pragma unroll 1
                 for (int x = 0; x < HD / 16; ++x, acc = 1) umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
             };
             auto outputs = [&](int g) {  // O of tile g
                 const uint32_t tp = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, vt = vb + (uint32_t)(g % NB) * C::TERMS * C::VT;
                 uint32_t acc = 0;
                 if constexpr (HL) {
+#pragma unroll 1
                     for (int x = 0; x < KA_TOK / 16; ++x, acc = 1)
-                        umma_bf16_tmem_a(to, tp + 32u + 8u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+                        umma_bf16_tmem_a(to, tp + 8u + 16u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+#pragma unroll 1
                     for (int x = 0; x < KA_TOK / 16; ++x)
-                        umma_bf16_tmem_a(to, tp + 8u * x, umma_desc(vt + C::VT + x * 2 * C::VG, C::VG, 128u), id_o, 1u);
+                        umma_bf16_tmem_a(to, tp + 16u * x, umma_desc(vt + C::VT + x * 2 * C::VG, C::VG, 128u), id_o, 1u);
                 }
-                for (int x = 0; x < KA_TOK / 16; ++x, acc = 1) umma_bf16_tmem_a(to, tp + 8u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+#pragma unroll 1
+                for (int x = 0; x < KA_TOK / 16; ++x, acc = 1) umma_bf16_tmem_a(to, tp + 16u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
             };
             bool ok = true;
             for (; u < u1 && ok; next()) {
@@ -448,49 +460,60 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 if (!ok) break;
                 tc_fence_after();
                 if (j == k) rs = sh.rs[row];
-                uint32_t sr[4][16];
+                const uint32_t valid = sh.valid[gt & 7], ts = tl + (uint32_t)b * 64u;
+                const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
+                const bool masked = left < KA_TOK || !(valid >> 31);
+                // (16 columns at a time, read twice: a short loop stays in the instruction cache beside the other roles' loops,
+                // where 64 columns unrolled had every role wait for instructions)
+                auto hide = [&](uint32_t(&s)[16], int c) {
+                    if (masked) {
+                        const int n = valid >> (16 * c >> a.l.lbs) & 1u ? left - 16 * c : 0;  // a page is 16 tokens or more
 #pragma unroll
-                for (int c = 0; c < 4; ++c) kp_tmem_ld16(tl + (uint32_t)b * 64u + 16u * c, sr[c]);
-                kp_tmem_wait_ld();
+                        for (int i = 0; i < 16; ++i)
+                            if (i >= n) s[i] = 0xff800000u;  // -inf
+                    }
+                };
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[16];
+                    kp_tmem_ld16(ts + 16u * c, s);
+                    kp_tmem_wait_ld();
+                    kp_tmem_got(s);
+                    hide(s, c);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) kp_tmem_got(sr[c]);
-                const uint32_t valid = sh.valid[gt & 7];
-                const int t0 = j * KA_TOK;
-                if (t0 + KA_TOK > lim || !(valid >> 31)) {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (t0 + c >= lim || !(valid >> (c >> a.l.lbs) & 1u)) sr[c >> 4][c & 15] = 0xff800000u;  // -inf
+                    for (int i = 0; i < 16; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s[i]));
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sr[c >> 4][c & 15]));
                 // rs > 0: the maximum may be taken before the scaling
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rs);
+                const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * rs);
                 // weights 2^10 exp2(s - maximum): fp16 keeps 11 bits down to 2^-24 of the largest
                 const float z = mn == -INFINITY ? 0.0f : 10.0f - mn;
                 const float fac = m == -INFINITY ? 0.0f : ka_exp2(m - mn);
                 m = mn;
                 sh.f[gt & 3][row] = fac;
                 const float2 rs2 = make_float2(rs, rs), z2 = make_float2(z, z);
-                float2 ls[2] = {};
-                uint32_t hi[32];
-                [[maybe_unused]] uint32_t lo[HL ? 32 : 1];
+                float2 ls = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[16], p16[16];
+                    kp_tmem_ld16(ts + 16u * c, s);
+                    kp_tmem_wait_ld();
+                    kp_tmem_got(s);
+                    hide(s, c);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const float2 x = __ffma2_rn(kp_pair(sr[c >> 3], c & 7), rs2, z2), p = make_float2(ka_exp2(x.x), ka_exp2(x.y));
-                    ls[c & 1] = __fadd2_rn(ls[c & 1], p);
-                    hi[c] = ka_pack(p.x, p.y);
-                    if constexpr (HL) {
-                        const float2 h = ka_unpack(hi[c]);
-                        lo[c] = ka_pack(p.x - h.x, p.y - h.y);
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 x = __ffma2_rn(kp_pair(s, i), rs2, z2), p = make_float2(ka_exp2(x.x), ka_exp2(x.y));
+                        ls = __fadd2_rn(ls, p);
+                        p16[i] = ka_pack(p.x, p.y);
+                        if constexpr (HL) {
+                            const float2 h = ka_unpack(p16[i]);
+                            p16[8 + i] = ka_pack(p.x - h.x, p.y - h.y);
+                        }
                     }
+                    if constexpr (HL) tmem_st16(ts + 16u * c, p16);
+                    else kp_tmem_st8(ts + 16u * c, p16);
                 }
-                l = l * fac + ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y));
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    tmem_st16(tl + (uint32_t)b * 64u + 16u * c, *(uint32_t(*)[16]) & hi[16 * c]);
-                    if constexpr (HL) tmem_st16(tl + (uint32_t)b * 64u + 32u + 16u * c, *(uint32_t(*)[16]) & lo[16 * c]);
-                }
+                l = l * fac + (ls.x + ls.y);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -590,7 +613,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAW;
                 uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT + k_dst;
                 const bool all = sh.valid[g & 7] >> 31;
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < KU; ++x) {  // a 64-dim group each
                     const uint4 w4 = *(const uint4 *)(raw + k_src + x * a.l.bs * 32);
                     float d = ka_half(raw + k_sc + x * a.l.bs * 2) * 0.125f;
@@ -621,7 +644,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
                 const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 7]));  // 1 / 2^e
                 const bool all = (sh.valid[g & 7] >> 31) && !sh.any_bad[g & 7];
-#pragma unroll
+#pragma unroll 1
                 for (int un = 0; un < VU; ++un) {
                     if (HD < 128 && v_wd >= HD / 8) break;
                     const uint8_t *src = raw + v_src + un * 2 * a.l.bs * 32;  // 16 words on: two groups
@@ -641,9 +664,9 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         dd[y] = ka_pack(d.x, d.y);
                     }
                     uint8_t *at = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT + v_dst + un * 2048;
-#pragma unroll
+#pragma unroll 1
                     for (int by = 0; by < 4; ++by) {
-                        const uint32_t sel = (uint32_t)(by | by << 4 | (4 + by) << 8 | (4 + by) << 12);
+                        const uint32_t sel = 0x4400u + 0x1111u * (uint32_t)by;  // byte `by` of two tokens
                         uint32_t h[2][4];
                         [[maybe_unused]] uint32_t lo[2][4];
 #pragma unroll
