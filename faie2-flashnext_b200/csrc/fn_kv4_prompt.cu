@@ -68,6 +68,12 @@ struct KpShared {
 };
 static_assert(sizeof(KpShared) <= 4096);
 
+// true in one lane of the warp
+__device__ __forceinline__ bool kp_elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
 // whether a phase has completed, after a short wait in the hardware
 __device__ __forceinline__ bool kp_try(uint64_t *bar, uint32_t parity) {
     uint32_t done;
@@ -168,7 +174,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     extern __shared__ __align__(1024) uint8_t sm_kp[];
     KpShared &sh = *(KpShared *)sm_kp;
     volatile int *const s_fail = &sh.fail;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 4), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 5);
@@ -376,69 +382,76 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     }
                 }
             }
-        } else if (warp == 1 && lane == 0) {
-            // ---- MMAs
+        } else if (warp == 1) {
+            // ---- MMAs. The whole warp runs this and one elected lane issues: the operands' descriptors then live in uniform
+            // registers. (As one lane's own values each MMA took 120 cycles and more, whatever its size; so it takes what its size
+            // asks, 32 cycles at 64 columns.)
             constexpr uint32_t id_s = umma_idesc_f16(128, KA_TOK), id_o = umma_idesc_f16(128, HD);
-            const uint32_t kb = smem_u32(sm_kp + C::K_OFF), vb = smem_u32(sm_kp + C::V_OFF), ql = smem_u32(sm_kp + C::Q_OFF);
-            const uint32_t tq = tmem + C::TM_Q, to = tmem + C::TM_O;
+            const uint64_t kd0 = umma_desc(smem_u32(sm_kp + C::K_OFF), 1024u, 128u), qd = umma_desc(smem_u32(sm_kp + C::Q_OFF), 2048u, 128u);
+            const uint64_t vd0 = umma_desc(smem_u32(sm_kp + C::V_OFF), C::VG, 128u);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), tq = tm + C::TM_Q, to = tm + C::TM_O;
             auto scores = [&](int g) {  // S of tile g
-                const uint32_t ts = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, kt = kb + (uint32_t)(g % NB) * C::TERMS * C::KT;
-                uint32_t acc = 0;
+                const uint32_t ts = tm + C::TM_S + (uint32_t)(g & 1) * 64u;
+                const uint64_t kd = kd0 + (uint64_t)((g % NB) * (C::TERMS * C::KT >> 4));
                 if constexpr (HL) {
-#pragma unroll 1
-                    for (int x = 0; x < HD / 16; ++x, acc = 1)
-                        umma_f16_smem_a(ts, umma_desc(ql + x * 4096u, 2048u, 128u), umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
-#pragma unroll 1
-                    for (int x = 0; x < HD / 16; ++x)
-                        umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + C::KT + x * 2048u, 1024u, 128u), id_s, 1u);
+#pragma unroll
+                    for (int x = 0; x < HD / 16; ++x) umma_f16_smem_a(ts, qd + x * 256u, kd + x * 128u, id_s, x > 0);
+#pragma unroll
+                    for (int x = 0; x < HD / 16; ++x) umma_bf16_tmem_a(ts, tq + 8u * x, kd + (C::KT >> 4) + x * 128u, id_s, 1u);
                 }
-#pragma unroll 1
-                for (int x = 0; x < HD / 16; ++x, acc = 1) umma_bf16_tmem_a(ts, tq + 8u * x, umma_desc(kt + x * 2048u, 1024u, 128u), id_s, acc);
+#pragma unroll
+                for (int x = 0; x < HD / 16; ++x) umma_bf16_tmem_a(ts, tq + 8u * x, kd + x * 128u, id_s, HL || x > 0);
             };
             auto outputs = [&](int g) {  // O of tile g
-                const uint32_t tp = tmem + C::TM_S + (uint32_t)(g & 1) * 64u, vt = vb + (uint32_t)(g % NB) * C::TERMS * C::VT;
-                uint32_t acc = 0;
+                const uint32_t tp = tm + C::TM_S + (uint32_t)(g & 1) * 64u;
+                const uint64_t vd = vd0 + (uint64_t)((g % NB) * (C::TERMS * C::VT >> 4));
                 if constexpr (HL) {
-#pragma unroll 1
-                    for (int x = 0; x < KA_TOK / 16; ++x, acc = 1)
-                        umma_bf16_tmem_a(to, tp + 8u + 16u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
-#pragma unroll 1
-                    for (int x = 0; x < KA_TOK / 16; ++x)
-                        umma_bf16_tmem_a(to, tp + 16u * x, umma_desc(vt + C::VT + x * 2 * C::VG, C::VG, 128u), id_o, 1u);
+#pragma unroll
+                    for (int x = 0; x < KA_TOK / 16; ++x) umma_bf16_tmem_a(to, tp + 8u + 16u * x, vd + x * (C::VG >> 3), id_o, x > 0);
+#pragma unroll
+                    for (int x = 0; x < KA_TOK / 16; ++x) umma_bf16_tmem_a(to, tp + 16u * x, vd + (C::VT >> 4) + x * (C::VG >> 3), id_o, 1u);
                 }
-#pragma unroll 1
-                for (int x = 0; x < KA_TOK / 16; ++x, acc = 1) umma_bf16_tmem_a(to, tp + 16u * x, umma_desc(vt + x * 2 * C::VG, C::VG, 128u), id_o, acc);
+#pragma unroll
+                for (int x = 0; x < KA_TOK / 16; ++x) umma_bf16_tmem_a(to, tp + 16u * x, vd + x * (C::VG >> 3), id_o, HL || x > 0);
             };
+            auto wtw = [&](uint64_t *bar, int phase) { return __all_sync(0xffffffffu, wt(bar, phase)) != 0; };
             bool ok = true;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
-                ok = wt(&sh.qf, gi);
+                ok = wtw(&sh.qf, gi);
                 const int n = kend - k, g0 = gt;
                 for (int j = 0; j <= n && ok; ++j) {
                     if (j < n) {
                         const int g = g0 + j;
-                        ok = wt(&sh.kf[g % NB], g / NB);
+                        ok = wtw(&sh.kf[g % NB], g / NB);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(g);
-                        umma_commit(&sh.sf[g & 1]);
-                        umma_commit(&sh.ke[g % NB]);
-                        if (j == n - 1) umma_commit(&sh.qe);
+                        if (kp_elect()) {
+                            scores(g);
+                            umma_commit(&sh.sf[g & 1]);
+                            umma_commit(&sh.ke[g % NB]);
+                            if (j == n - 1) umma_commit(&sh.qe);
+                        }
+                        __syncwarp();
                     }
                     if (j > 0) {
                         const int g = g0 + j - 1;
-                        ok = wt(&sh.pf[g & 1], g >> 1) && wt(&sh.vf[g % NB], g / NB) && (g == 0 || wt(&sh.oe, g - 1));
+                        ok = wtw(&sh.pf[g & 1], g >> 1) && wtw(&sh.vf[g % NB], g / NB) && (g == 0 || wtw(&sh.oe, g - 1));
                         if (!ok) break;
                         tc_fence_after();
-                        outputs(g);
-                        umma_commit(&sh.of);
+                        if (kp_elect()) {
+                            outputs(g);
+                            umma_commit(&sh.of);
+                        }
+                        __syncwarp();
                     }
                 }
                 gt = g0 + n;
                 ++gi;
             }
             // every MMA issued has finished before the CTA gives its memory back
-            umma_commit(&sh.done);
+            if (kp_elect()) umma_commit(&sh.done);
+            __syncwarp();
             mbar_park(&sh.done, 0);
         }
         __syncwarp();
