@@ -31,6 +31,7 @@
 namespace fn {
 
 constexpr int KP_ROWS = 128, KP_THREADS = 512;
+constexpr int KP_EXTRA = 8;  // units that a row tile counts beside its own, for its start and end
 constexpr int KP_W_SM = 4, KP_W_WORK = 8;
 
 template <int HD, bool HL> struct KpCfg {
@@ -46,7 +47,7 @@ template <int HD, bool HL> struct KpCfg {
     static constexpr uint32_t K_OFF = 4096, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
     static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAW, SMEM = RV_OFF + RV * RAW;
     // registers by warpgroup: IO + SM + 2 WORK <= 4 x 128 at launch; the workers hold HD / 2 sums
-    static constexpr int REG_IO = HD == 256 ? 40 : 72, REG_SM = HD == 256 ? 120 : 128, REG_WORK = HD == 256 ? 176 : 152;
+    static constexpr int REG_IO = HD == 256 ? 56 : 72, REG_SM = HD == 256 ? 120 : 128, REG_WORK = HD == 256 ? 168 : 152;
     static_assert(REG_IO + REG_SM + 2 * REG_WORK <= 512);
     static constexpr int PART = KP_ROWS * HD + 2 * KP_ROWS;
     // tensor memory: O, then q's first halves, then S / P twice (64 columns: of 16 tokens' scores,
@@ -199,7 +200,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     auto weight = [&](int r) {
         const KaReq q = kp_req(a, r);
         long long w = 0;
-        for (int i = 0; i < q.rt; ++i) w += kp_tiles(q, a.group, i) + KA_EXTRA;
+        for (int i = 0; i < q.rt; ++i) w += kp_tiles(q, a.group, i) + KP_EXTRA;
         return w * a.l.nkv;
     };
     long long mine = 0;
@@ -219,7 +220,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         if (w < warp) before += sh.red[w];
         units += sh.red[w];
     }
-    const long long per = max((units + gridDim.x - 1) / gridDim.x, 2ll + KA_EXTRA);
+    const long long per = max((units + gridDim.x - 1) / gridDim.x, 2ll + KP_EXTRA);
     const long long u0 = blockIdx.x * per, u1 = min(u0 + per, units);
     if (u0 < u1 && u0 >= before && u0 < before + mine) {
         long long at = before;
@@ -251,7 +252,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     long long u = u0;
     KaReq rq{};
     auto next = [&]() {
-        u += tiles + KA_EXTRA - off;
+        u += tiles + KP_EXTRA - off;
         off = 0;
         if (u >= u1 || ++kv < a.l.nkv) return;
         kv = 0;
@@ -263,8 +264,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         tiles = kp_tiles(rq, a.group, tile);
     };
     auto here = [&]() {
-        k = max(off - KA_EXTRA, 0);
-        kend = max((int)min((long long)(tiles + KA_EXTRA), off + (u1 - u)) - KA_EXTRA, 0);
+        k = max(off - KP_EXTRA, 0);
+        kend = max((int)min((long long)(tiles + KP_EXTRA), off + (u1 - u)) - KP_EXTRA, 0);
         return k < kend;
     };
     if (u0 < u1) {
@@ -273,12 +274,12 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         long long at = sh.off;
         for (;; ++tile) {
             tiles = kp_tiles(rq, a.group, tile);
-            const long long w = (long long)a.l.nkv * (tiles + KA_EXTRA);
+            const long long w = (long long)a.l.nkv * (tiles + KP_EXTRA);
             if (at < w) break;
             at -= w;
         }
-        kv = (int)(at / (tiles + KA_EXTRA));
-        off = (int)(at - (long long)kv * (tiles + KA_EXTRA));
+        kv = (int)(at / (tiles + KP_EXTRA));
+        off = (int)(at - (long long)kv * (tiles + KP_EXTRA));
     }
     // rows of the tile see tokens below their limit; rows past its last see what the last sees (results dropped)
     auto limit = [&](int i) {
@@ -540,7 +541,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 to[row] = m;
                 to[KP_ROWS + row] = l;
                 if (tid == 32 * KP_W_SM && k == 0)
-                    a.split[blockIdx.x] = KaSplit{(int)((u - off + KA_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
+                    a.split[blockIdx.x] = KaSplit{(int)((u - off + KP_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
             }
             __syncwarp();
             if (lane == 0) tc_arrive(&sh.lf);
@@ -577,10 +578,14 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             // ---- q: scaled so that the row's largest value is 2^10..2^11, dims in the order of the codes' nibbles
             {
                 const T *src = (const T *)after_wait(a.q) + (int64_t)(rq.first + tok_row) * a.qt + (int64_t)head * a.qh + half * HH;
-                float x[HH], mx = 0.0f;
-                kp_load<T, HH>(src, live, a.vec, x);
+                float mx = 0.0f;
+#pragma unroll 2
+                for (int d = 0; d < HH; d += 16) {
+                    float x[16];
+                    kp_load<T, 16>(src + d, live, a.vec, x);
 #pragma unroll
-                for (int d = 0; d < HH; ++d) mx = fmaxf(mx, fabsf(x[d]));
+                    for (int y = 0; y < 16; ++y) mx = fmaxf(mx, fabsf(x[y]));
+                }
                 // both halves of the row agree on its exponent (K's place is free before the row tile's first K)
                 float *sx = (float *)(sm_kp + C::K_OFF);
                 sx[half * KP_ROWS + row] = mx;
@@ -591,15 +596,17 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 // scores in base 2: undo the scaling, and K's 1 / 8; positive also for a scale of zero
                 if (half == 0) sh.rs[row] = fmaxf(fabsf(a.scale) * 8.0f * 1.44269504f * kp_pow2(-e), 1e-30f);
                 kp_bar_work();
-#pragma unroll
+#pragma unroll 1
                 for (int d = 0; d < HH; d += 32) {
+                    float x[32];
+                    kp_load<T, 32>(src + d, live, a.vec, x);
                     uint32_t hi[16];
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         uint32_t lo[4];
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            const float x0 = x[d + 8 * w + y] * up, x1 = x[d + 8 * w + y + 4] * up;
+                            const float x0 = x[8 * w + y] * up, x1 = x[8 * w + y + 4] * up;
                             hi[4 * w + y] = ka_pack(x0, x1);
                             const float2 h = ka_unpack(hi[4 * w + y]);
                             lo[y] = ka_pack(x0 - h.x, x1 - h.y);
@@ -777,7 +784,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                             float gx[8];
                             kp_load<T, 8>(gate + c, true, a.vec, gx);
 #pragma unroll
-                            for (int x = 0; x < 8; ++x) y[x] *= sigm(gx[x]);
+                            for (int x = 0; x < 8; ++x) y[x] *= ka_gate(gx[x]);
                         }
                         if (a.vec) {
                             if constexpr (HL) {
