@@ -22,11 +22,11 @@ struct PlanArgs {
     int rows_here;  // 1: this kernel writes the rows; 0: k_kv4_rows does
 };
 
-constexpr int PLAN_T = 1024;
+constexpr int PLAN_T = 1024, PLAN_SMALL = 128;  // threads; the small form for steps of few requests and rows
 constexpr int PLAN_PER = KV4_MAX_REQ / PLAN_T;
 
-// exclusive prefix sum of v over the CTA's threads, and the total (PLAN_T threads)
-__device__ __forceinline__ long long plan_scan(long long v, long long *red, long long &total) {
+// exclusive prefix sum of v over the CTA's T threads, and the total
+template <int T> __device__ __forceinline__ long long plan_scan(long long v, long long *red, long long &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long s = v;
 #pragma unroll
@@ -36,7 +36,7 @@ __device__ __forceinline__ long long plan_scan(long long v, long long *red, long
     }
     if (lane == 31) red[warp] = s;
     __syncthreads();
-    long long w = red[lane], t = w;
+    long long w = lane < T / 32 ? red[lane] : 0, t = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, t, o);
@@ -69,12 +69,12 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, const int *cu, int s
     a.requests[i] = r;
 }
 
-__global__ void __launch_bounds__(PLAN_T) k_kv4_plan(const PlanArgs a) {
+template <int T> __global__ void __launch_bounds__(T) k_kv4_plan(const PlanArgs a) {
     extern __shared__ int sm_plan[];
     __shared__ long long red[32];
     __shared__ int s_taken, s_refused;
     int *cu = sm_plan, *need0 = cu + a.n + 1, *back0 = need0 + a.n + 1, *len = back0 + a.n + 1;
-    const int tid = threadIdx.x, per = (a.n + PLAN_T - 1) / PLAN_T, r0 = tid * per;
+    const int tid = threadIdx.x, per = (a.n + T - 1) / T, r0 = tid * per;
     if (tid == 0) s_taken = s_refused = 0;
     pdl_wait();
     pdl_trigger();
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(PLAN_T) k_kv4_plan(const PlanArgs a) {
         fresh[k] = max(add[k], 0);
         sum += fresh[k];
     }
-    long long end = plan_scan(sum, red, total);
+    long long end = plan_scan<T>(sum, red, total);
     // rows: offsets clipped to max_tokens; a request whose rows or pages do not fit its arrays takes nothing
     int need[PLAN_PER], back[PLAN_PER];
     bool fits[PLAN_PER];
@@ -109,9 +109,9 @@ __global__ void __launch_bounds__(PLAN_T) k_kv4_plan(const PlanArgs a) {
         backs += back[k];
     }
     if (tid == 0) cu[a.n] = (int)min(total, (long long)a.max_tokens);
-    long long nb = plan_scan(needs, red, total), bb, back_total;
+    long long nb = plan_scan<T>(needs, red, total), bb, back_total;
     if (tid == 0) need0[a.n] = (int)min(total, (long long)INT32_MAX);
-    bb = plan_scan(backs, red, back_total);
+    bb = plan_scan<T>(backs, red, back_total);
     const int returned = (int)min(back_total, (long long)(a.n_pages - top0)), top = top0 + returned;
     if (tid == 0) back0[a.n] = (int)min(back_total, (long long)INT32_MAX);
     int refused = 0, taken = 0;
@@ -134,24 +134,24 @@ __global__ void __launch_bounds__(PLAN_T) k_kv4_plan(const PlanArgs a) {
     if (refused) atomicAdd(&s_refused, refused);
     // the pages of finished requests go on top of the stack, in request order
     __syncthreads();
-    for (int j = tid; j < returned; j += PLAN_T) {
+    for (int j = tid; j < returned; j += T) {
         const int r = plan_find(back0, a.n, j);
         a.free_ids[top0 + j] = a.table[(size_t)r * a.max_pages + j - back0[r]];
     }
-    for (int r = tid; r <= a.n; r += PLAN_T) a.cu[r] = cu[r];
+    for (int r = tid; r <= a.n; r += T) a.cu[r] = cu[r];
     if (tid == 0) {
         *a.free_out = top - s_taken;
         *a.status = s_refused;
     }
     __syncthreads();
     // the new pages come from the top
-    for (int j = tid; j < s_taken; j += PLAN_T) {
+    for (int j = tid; j < s_taken; j += T) {
         const int r = plan_find(need0, a.n, j);
         a.table[(size_t)r * a.max_pages + plan_pages(max(a.ctx[r], 0), a.bs) + j - need0[r]] = a.free_ids[top - 1 - j];
     }
     if (!a.rows_here) return;
     __syncthreads();
-    for (int i = tid; i < a.max_tokens; i += PLAN_T) {
+    for (int i = tid; i < a.max_tokens; i += T) {
         if (i < cu[a.n]) {
             const int r = plan_find(cu, a.n, i);
             plan_row(a, cu, len[r], r, i);
@@ -162,16 +162,19 @@ __global__ void __launch_bounds__(PLAN_T) k_kv4_plan(const PlanArgs a) {
     }
 }
 
-// the rows of a large step, after k_kv4_plan: one thread a row
+// the rows of a large step, after k_kv4_plan: one thread a row, the offsets in shared memory (a bisection in global memory
+// took 8 round trips)
 __global__ void __launch_bounds__(256) k_kv4_rows(const PlanArgs a) {
+    extern __shared__ int sm_plan[];
     pdl_wait();
     pdl_trigger();
     const int i = blockIdx.x * 256 + threadIdx.x;
+    for (int r = threadIdx.x; r <= a.n; r += 256) sm_plan[r] = after_wait(a.cu)[r];
+    __syncthreads();
     if (i >= a.max_tokens) return;
-    const int *cu = after_wait(a.cu);
-    if (i < cu[a.n]) {
-        const int r = plan_find(cu, a.n, i);
-        plan_row(a, cu, after_wait(a.kv_len)[r], r, i);
+    if (i < sm_plan[a.n]) {
+        const int r = plan_find(sm_plan, a.n, i);
+        plan_row(a, sm_plan, after_wait(a.kv_len)[r], r, i);
     } else {
         a.slots[i] = -1;
         a.positions[i] = a.requests[i] = -1;
@@ -180,7 +183,8 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const PlanArgs a) {
 
 // ---- store / load --------------------------------------------------------------------------------------------------
 // A unit is 64 dims of one head of one token (K or V); eight lanes hold eight values each, so a warp covers four units:
-// reads of 32 (16) bytes a lane, codes written as one word a lane, 32 adjacent bytes a unit.
+// reads of 32 (16) bytes a lane, codes written as one word a lane, 32 adjacent bytes a unit. A thread takes four units, whose
+// loads are all under way before the first is used; blockIdx.y is the head of K or V, so that no index is divided.
 // d = m / -8 with m the value of largest magnitude (of two opposite ones the positive), c = clamp(trunc(x / d + 8.5), 0,
 // 15), so that m itself is the code 0 and all 16 codes are used; d is rounded to fp16 after the codes are chosen.
 template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]);
@@ -215,108 +219,128 @@ struct Kv4RowArgs {
     uint32_t *err;
 };
 
-// unit -> (token, part, head, group); false past the end
-__device__ __forceinline__ bool kv4_unit(const Kv4RowArgs &a, int &t, int &part, int &h, int &g) {
-    const int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+constexpr int ROW_UNITS = 4;  // of a thread
+
+// unit x of a thread -> token and group; false past the end
+__device__ __forceinline__ bool kv4_unit(const Kv4RowArgs &a, int x, int &t, int &g) {
+    const int64_t u = ((int64_t)blockIdx.x * ROW_UNITS + x) * 32 + (threadIdx.x >> 3);
+    const int lg = a.l.ng >> 1;  // log2 of 1, 2, 4
     g = (int)(u & (a.l.ng - 1));
-    const int64_t w = u / a.l.ng, row = w / a.l.nkv;
-    h = (int)(w - row * a.l.nkv);
-    part = (int)(row & 1);
-    t = (int)(row >> 1);
-    return (row >> 1) < a.nt;
+    t = (int)(u >> lg);
+    return (u >> lg) < a.nt;
+}
+// a slot's record, and the line of a group's codes and scale in it
+__device__ __forceinline__ uint8_t *kv4_place(const Kv4Lay &l, int64_t slot, int h, int g, uint32_t &line) {
+    line = (uint32_t)(g * l.bs) + (uint32_t)(slot & (l.bs - 1));
+    return l.pages + ((slot >> l.lbs) * l.nkv + h) * (int64_t)l.rec;
 }
 
 template <typename T> __global__ void __launch_bounds__(256) k_kv4_store(const Kv4RowArgs a) {
     pdl_wait();
     pdl_trigger();
-    int t, part, h, g;
-    const bool in = kv4_unit(a, t, part, h, g);
-    const int lane = threadIdx.x & 7;
-    int64_t slot = in ? after_wait(a.slots)[t] : -1;
-    if (slot >= (int64_t)a.l.n_pages * a.l.bs) {
-        dev_fail(a.err, DEV_BAD_ARG);
-        slot = -1;
-    }
-    float x[8] = {};
-    if (slot >= 0)
-        load8<T>((const T *)after_wait(a.x[part]) + t * a.token[part] + h * a.head[part] + g * KV4_GROUP + lane * 8, a.vec, x);
-    // NaN compares false: fminf / fmaxf would drop it, so non-finite values are counted apart
-    float big = x[0], small = x[0];
-    bool bad = false;
+    const int part = blockIdx.y >= a.l.nkv, h = blockIdx.y - part * a.l.nkv, lane = threadIdx.x & 7;
+    float v[ROW_UNITS][8];
+    int64_t slot[ROW_UNITS];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        big = fmaxf(big, x[i]);
-        small = fminf(small, x[i]);
-        bad |= !isfinite(x[i]);
+    for (int x = 0; x < ROW_UNITS; ++x) {
+        int t, g;
+        const bool in = kv4_unit(a, x, t, g);
+        slot[x] = in ? after_wait(a.slots)[t] : -1;
+        if (in) load8<T>((const T *)after_wait(a.x[part]) + t * a.token[part] + h * a.head[part] + g * KV4_GROUP + lane * 8, a.vec, v[x]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[x][i] = 0.0f;
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        small = fminf(small, __shfl_xor_sync(0xffffffffu, small, o));
-    }
-    bad = (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 24) & 255u) != 0;
-    if (slot < 0) return;
-    const float d = (big >= -small ? big : small) * -0.125f;
-    const float inv = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-    uint32_t w = 0;
+    for (int x = 0; x < ROW_UNITS; ++x) {
+        int t, g;
+        kv4_unit(a, x, t, g);
+        // fminf / fmaxf would drop a NaN, so values that are not finite are counted apart
+        float big = v[x][0], small = v[x][0];
+        bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = __float2int_rz(__fadd_rn(__fmul_rn(x[i], inv), 8.5f));
-        w |= (uint32_t)min(max(c, 0), 15) << (4 * i);
-    }
-    const int64_t page = slot >> a.l.lbs;
-    const int place = (int)(slot & (a.l.bs - 1));
-    uint8_t *rec = a.l.pages + (page * a.l.nkv + h) * (int64_t)a.l.rec;
-    *(uint32_t *)(rec + part * a.l.kb + (uint32_t)(g * a.l.bs + place) * 32 + lane * 4) = w;
-    if (lane == 0) {
-        // a block that holds a NaN or an infinity, or whose scale passes fp16, reads back as NaN
-        const bool over = bad || fabsf(d) > 65504.0f;
-        const __half s = over ? __ushort_as_half(0x7fffu) : __float2half_rn(d);
-        *(__half *)(rec + 2 * a.l.kb + part * a.l.sb + (uint32_t)(g * a.l.bs + place) * 2) = s;
+        for (int i = 0; i < 8; ++i) {
+            big = fmaxf(big, v[x][i]);
+            small = fminf(small, v[x][i]);
+            bad |= !isfinite(v[x][i]);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            small = fminf(small, __shfl_xor_sync(0xffffffffu, small, o));
+        }
+        bad = (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 24) & 255u) != 0;
+        if (slot[x] >= (int64_t)a.l.n_pages * a.l.bs) dev_fail(a.err, DEV_BAD_ARG);
+        else if (slot[x] >= 0) {
+            const float d = (big >= -small ? big : small) * -0.125f;
+            const float inv = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+            uint32_t w = 0, line;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = __float2int_rz(__fadd_rn(__fmul_rn(v[x][i], inv), 8.5f));
+                w |= (uint32_t)min(max(c, 0), 15) << (4 * i);
+            }
+            uint8_t *rec = kv4_place(a.l, slot[x], h, g, line);
+            *(uint32_t *)(rec + part * a.l.kb + line * 32 + lane * 4) = w;
+            if (lane == 0) {
+                // a block that holds a NaN or an infinity, or whose scale passes fp16, reads back as NaN
+                const bool over = bad || fabsf(d) > 65504.0f;
+                *(__half *)(rec + 2 * a.l.kb + part * a.l.sb + line * 2) = over ? __ushort_as_half(0x7fffu) : __float2half_rn(d);
+            }
+        }
     }
 }
 
 template <typename T> __global__ void __launch_bounds__(256) k_kv4_load(const Kv4RowArgs a) {
     pdl_wait();
     pdl_trigger();
-    int t, part, h, g;
-    if (!kv4_unit(a, t, part, h, g) || !a.y[part]) return;
-    const int lane = threadIdx.x & 7;
-    int64_t slot = after_wait(a.slots)[t];
-    if (slot >= (int64_t)a.l.n_pages * a.l.bs) {
-        dev_fail(a.err, DEV_BAD_ARG);
-        slot = -1;
-    }
-    float y[8] = {};
-    if (slot >= 0) {
-        const int64_t page = slot >> a.l.lbs;
-        const int place = (int)(slot & (a.l.bs - 1));
-        const uint8_t *rec = after_wait(a.l.pages) + (page * a.l.nkv + h) * (int64_t)a.l.rec;
-        const uint32_t w = *(const uint32_t *)(rec + part * a.l.kb + (uint32_t)(g * a.l.bs + place) * 32 + lane * 4);
-        const float d = __half2float(*(const __half *)(rec + 2 * a.l.kb + part * a.l.sb + (uint32_t)(g * a.l.bs + place) * 2));
+    const int part = blockIdx.y >= a.l.nkv, h = blockIdx.y - part * a.l.nkv, lane = threadIdx.x & 7;
+    if (!a.y[part]) return;
+    uint32_t w[ROW_UNITS];
+    float d[ROW_UNITS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (float)((int)(w >> (4 * i) & 15u) - 8) * d;
-    }
-    T *o = (T *)a.y[part] + ((int64_t)t * a.l.nkv + h) * a.l.hd + g * KV4_GROUP + lane * 8;
-    if constexpr (sizeof(T) == 4) {
-        *(float4 *)o = make_float4(y[0], y[1], y[2], y[3]);
-        *(float4 *)(o + 4) = make_float4(y[4], y[5], y[6], y[7]);
-    } else {
-        uint32_t b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-            b[i] = *(const uint32_t *)&p;
+    for (int x = 0; x < ROW_UNITS; ++x) {
+        int t, g;
+        int64_t slot = kv4_unit(a, x, t, g) ? after_wait(a.slots)[t] : -1;
+        if (slot >= (int64_t)a.l.n_pages * a.l.bs) {
+            dev_fail(a.err, DEV_BAD_ARG);
+            slot = -1;
         }
-        *(uint4 *)o = make_uint4(b[0], b[1], b[2], b[3]);
+        w[x] = 0x88888888u, d[x] = 0.0f;
+        if (slot >= 0) {
+            uint32_t line;
+            const uint8_t *rec = after_wait(kv4_place(a.l, slot, h, g, line));
+            w[x] = *(const uint32_t *)(rec + part * a.l.kb + line * 32 + lane * 4);
+            d[x] = __half2float(*(const __half *)(rec + 2 * a.l.kb + part * a.l.sb + line * 2));
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < ROW_UNITS; ++x) {
+        int t, g;
+        if (!kv4_unit(a, x, t, g)) continue;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (float)((int)(w[x] >> (4 * i) & 15u) - 8) * d[x];
+        T *o = (T *)a.y[part] + ((int64_t)t * a.l.nkv + h) * a.l.hd + g * KV4_GROUP + lane * 8;
+        if constexpr (sizeof(T) == 4) {
+            *(float4 *)o = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4 *)(o + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                b[i] = *(const uint32_t *)&p;
+            }
+            *(uint4 *)o = make_uint4(b[0], b[1], b[2], b[3]);
+        }
     }
 }
 
-static int rows_grid(const Kv4RowArgs &a, unsigned &grid) {
-    const int64_t threads = (int64_t)a.nt * 2 * a.l.nkv * a.l.ng * 8;
-    const int64_t g = (threads + 255) / 256;
+static int rows_grid(const Kv4RowArgs &a, dim3 &grid) {
+    const int64_t g = ((int64_t)a.nt * a.l.ng + 32 * ROW_UNITS - 1) / (32 * ROW_UNITS);
     if (g > INT32_MAX) return -1;
-    grid = (unsigned)g;
+    grid = dim3((unsigned)g, 2 * a.l.nkv);
     return 0;
 }
 
@@ -340,10 +364,13 @@ FN_API int fn_kv4_plan(int n, const int *ctx, const int *add, int *table, int ma
         // few rows: the planning CTA writes them itself; many: a second grid
         a.rows_here = max_tokens <= 4 * PLAN_T;
         const size_t smem = (size_t)4 * (n + 1) * sizeof(int);
-        cudaError_t e = allow_max_dynamic_smem(k_kv4_plan);
-        if (e == cudaSuccess) e = launch_k(k_kv4_plan, dim3(1), dim3(PLAN_T), smem, (cudaStream_t)stream, a);
+        cudaError_t e = allow_max_dynamic_smem(k_kv4_plan<PLAN_T>);
+        if (e == cudaSuccess && n <= PLAN_SMALL && max_tokens <= 4 * PLAN_SMALL)
+            e = launch_k(k_kv4_plan<PLAN_SMALL>, dim3(1), dim3(PLAN_SMALL), smem, (cudaStream_t)stream, a);
+        else if (e == cudaSuccess)
+            e = launch_k(k_kv4_plan<PLAN_T>, dim3(1), dim3(PLAN_T), smem, (cudaStream_t)stream, a);
         if (e == cudaSuccess && !a.rows_here)
-            e = launch_k(k_kv4_rows, dim3((max_tokens + 255) / 256), dim3(256), 0, (cudaStream_t)stream, a);
+            e = launch_k(k_kv4_rows, dim3((max_tokens + 255) / 256), dim3(256), (size_t)(n + 1) * sizeof(int), (cudaStream_t)stream, a);
         if (e != cudaSuccess) return fail(std::string("kv4 plan launch: ") + cudaGetErrorString(e));
         return 0;
     });
@@ -368,10 +395,10 @@ FN_API int fn_kv4_store(const fn_kv4_t *c, uint32_t type, const void *k, int64_t
         a.vec = 1;
         for (int i = 0; i < 2; ++i)
             a.vec &= (uintptr_t)a.x[i] % 16 == 0 && a.token[i] * size % 16 == 0 && a.head[i] * size % 16 == 0;
-        unsigned grid;
+        dim3 grid;
         if (rows_grid(a, grid)) return fail("kv4 store: too many rows");
-        const cudaError_t e = type == T_F32 ? launch_k(k_kv4_store<float>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, a)
-                                            : launch_k(k_kv4_store<__nv_bfloat16>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, a);
+        const cudaError_t e = type == T_F32 ? launch_k(k_kv4_store<float>, grid, dim3(256), 0, (cudaStream_t)stream, a)
+                                            : launch_k(k_kv4_store<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
         if (e != cudaSuccess) return fail(std::string("kv4 store launch: ") + cudaGetErrorString(e));
         return 0;
     });
@@ -390,10 +417,10 @@ FN_API int fn_kv4_load(const fn_kv4_t *c, uint32_t type, const int64_t *slots, i
         a.slots = slots;
         a.nt = nt;
         a.err = dev_error_ptr();
-        unsigned grid;
+        dim3 grid;
         if (rows_grid(a, grid)) return fail("kv4 load: too many rows");
-        const cudaError_t e = type == T_F32 ? launch_k(k_kv4_load<float>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, a)
-                                            : launch_k(k_kv4_load<__nv_bfloat16>, dim3(grid), dim3(256), 0, (cudaStream_t)stream, a);
+        const cudaError_t e = type == T_F32 ? launch_k(k_kv4_load<float>, grid, dim3(256), 0, (cudaStream_t)stream, a)
+                                            : launch_k(k_kv4_load<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, a);
         if (e != cudaSuccess) return fail(std::string("kv4 load launch: ") + cudaGetErrorString(e));
         return 0;
     });
