@@ -199,6 +199,19 @@ FN_API int fn_gdn_reset(int h, void *stream) {
     return 0;
 }
 
+// Zero one sequence's state and histories: sequence b's lie at b times their size.
+FN_API int fn_gdn_reset_seq(int h, int seq, void *stream) {
+    GdnH *g = gdn_get(h);
+    if (!g) return fail("fn_gdn_reset_seq: bad handle");
+    if (seq < 0 || seq >= g->batch) return fail("fn_gdn_reset_seq: no such sequence");
+    const size_t nS = (size_t)g->p.nvh * g->p.ds * g->p.ds, nv = (size_t)3 * g->p.nvh * g->p.ds, nqk = (size_t)g->p.nvh * 3 * 2 * g->p.ds;
+    cudaStream_t s = (cudaStream_t)stream;
+    FN_CK(cudaMemsetAsync(g->st.S + seq * nS, 0, nS * 4, s));
+    FN_CK(cudaMemsetAsync(g->st.conv_v + seq * nv, 0, nv * 4, s));
+    FN_CK(cudaMemsetAsync(g->st.conv_qk + seq * nqk, 0, nqk * 4, s));
+    return 0;
+}
+
 FN_API int fn_gdn_free(int h) {
     GdnH *g = gdn_get(h);
     if (!g) return fail("fn_gdn_free: bad handle");

@@ -42,6 +42,7 @@ EXPORTS = [
     "fn_load", "fn_forward", "fn_reset", "fn_free", "fn_debug_layers", "fn_use_graphs", "fn_n_past", "fn_last_ms",
     "fn_dev_gb", "fn_split", "fn_model_dims",
     "fn_kv4_plan", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
+    "fn_qk_rope_rows", "fn_gdn_reset_seq",
 ]
 
 
@@ -141,6 +142,8 @@ class FN:
         d.fn_kv4_attn_workspace.restype = C.c_uint64
         d.fn_kv4_attn.argtypes = [kv4, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, i64, i64, vp, i64, i64, vp, i64, vp, vp,
                                   vp, C.c_int, C.c_int, C.c_float, vp, C.c_uint64, vp]
+        d.fn_qk_rope_rows.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float, vp]
+        d.fn_gdn_reset_seq.argtypes = [C.c_int, C.c_int, vp]
         d.fn_tc_create.argtypes = [C.c_uint32, U8, C.c_int, C.c_int]
         d.fn_tc_free.argtypes = [C.c_int]
         d.fn_tc_gemv.argtypes = [C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp]
@@ -513,6 +516,16 @@ class FN:
                  kv_len, table, max_pages, max_new, scale, ws, ws_bytes, stream=0):
         self.check(self.d.fn_kv4_attn(cache, dtype, n, rows, nh, q, q_token, q_head, gate, gate_token, gate_head, out,
                                       out_token, cu, kv_len, table, max_pages, max_new, scale, ws, ws_bytes, stream))
+
+    def qk_rope_rows(self, q, q_token, q_head, k, k_token, k_head, wq, wk, inv_freq, positions, rows, nh, nkv, q_out, k_out,
+                     eps=1e-6, stream=0):
+        """q / k head RMSNorm and RoPE of rows at positions of their own (device pointers)."""
+        self.check(self.d.fn_qk_rope_rows(q, q_token, q_head, k, k_token, k_head, wq, wk, inv_freq, positions, rows, nh, nkv,
+                                          q_out, k_out, eps, stream))
+
+    def gdn_reset_seq(self, h, seq, stream=0):
+        """Zero one sequence's state of a batched DeltaNet handle."""
+        self.check(self.d.fn_gdn_reset_seq(h, seq, stream))
 
     # ---- L2 prefetch hints of a decode chain ----
     def w_weights(self, h):

@@ -281,7 +281,7 @@ class BatchDecodeModel:
             else:
                 o.update(w_qkv=tc(ty("w_q"), np.concatenate([L["w_q"], L["w_k"], L["w_v"]]), self.n_qkv, d),
                          w_o=tc(ty("w_o"), L["w_o"], d, nh * HD), q_norm=f32(L["q_norm"]), k_norm=f32(L["k_norm"]),
-                         Kc=torch.zeros(B, max_ctx, nkv, HD, device=dev), Vc=torch.zeros(B, max_ctx, nkv, HD, device=dev))
+                         **self._caches(dev))
             m = fn.moe_create(T.get("gate_up", cfg["gate_up"]), T.get("down", cfg["down"]), ne, cfg["k"], ffe, d, *L["moe"])
             self.moes.append(m)
             o["moe"] = m
@@ -311,11 +311,11 @@ class BatchDecodeModel:
     def launch_step(self, s: int):
         """One decode step of every sequence on stream s (device pointers only; capturable)."""
         fn, cfg, B = self.fn, self.cfg, self.B
-        d, nvh, nh, nkv, eps, ne1 = cfg["D"], cfg["nvh"], cfg["nh"], cfg["nkv"], cfg["eps"], cfg["ne"] + 1
+        d, nvh, nh, eps, ne1 = cfg["D"], cfg["nvh"], cfg["nh"], cfg["eps"], cfg["ne"] + 1
         p = lambda t: t.data_ptr()  # noqa: E731
         h, x, pr = p(self.h), p(self.x), p(self.proj)
         ps = self.proj.shape[1]
-        fn.embed_batch(cfg["embed"], p(self.E), d, p(self.tokens), self.max_ctx, p(self.pos), h, B, s)
+        self._embed(s)
         for L in self.layers:
             fn.rmsnorm_rows(h, p(L["norm1"]), x, d, B, eps, s)
             if L["kind"] == "G":
@@ -325,9 +325,7 @@ class BatchDecodeModel:
                 fn.tc_gemv(L["w_out"], p(self.core), nvh * DS, h, d, B, 1, s)  # h += W_out core
             else:
                 fn.tc_gemv(L["w_qkv"], x, d, pr, ps, B, 0, s)
-                fn.attn_decode_batch(pr, pr + 4 * nh * 2 * HD, pr + 4 * (nh * 2 * HD + nkv * HD), ps, p(L["q_norm"]),
-                                     p(L["k_norm"]), p(self.inv_freq), p(self.Q), p(L["Kc"]), p(L["Vc"]), p(self.att),
-                                     p(self.pos), nh, nkv, self.max_ctx, B, eps, s)
+                self._attention(L, s)
                 fn.tc_gemv(L["w_o"], p(self.att), nh * HD, h, d, B, 1, s)  # h += W_o o
             fn.rmsnorm_rows(h, p(L["norm2"]), x, d, B, eps, s)
             fn.tc_gemv(L["router"], x, d, p(self.lr), ne1, B, 0, s)
@@ -336,7 +334,31 @@ class BatchDecodeModel:
         vocab = cfg["vocab"]
         fn.tc_gemv(self.head, x, d, p(self.logits), vocab, B, 0, s)
         fn.argmax_dev(p(self.logits), vocab, vocab, B, p(self.next), s)
-        fn.step_advance_batch(p(self.pos), p(self.tokens), p(self.next), p(self.plen), self.max_ctx, B, s)
+        self._advance(s)
+
+    # what depends on where the sequences stand (flashnext/serve.py: each at a position of its own)
+    def _embed(self, s):
+        p = lambda t: t.data_ptr()  # noqa: E731
+        self.fn.embed_batch(self.cfg["embed"], p(self.E), self.cfg["D"], p(self.tokens), self.max_ctx, p(self.pos), p(self.h),
+                            self.B, s)
+
+    def _attention(self, L, s):
+        """self.att = the gated attention of the projections self.proj (q gate | k | v)."""
+        p, nh, nkv = (lambda t: t.data_ptr()), self.cfg["nh"], self.cfg["nkv"]
+        pr = p(self.proj)
+        self.fn.attn_decode_batch(pr, pr + 4 * nh * 2 * HD, pr + 4 * (nh * 2 * HD + nkv * HD), self.proj.shape[1],
+                                  p(L["q_norm"]), p(L["k_norm"]), p(self.inv_freq), p(self.Q), p(L["Kc"]), p(L["Vc"]),
+                                  p(self.att), p(self.pos), nh, nkv, self.max_ctx, self.B, self.cfg["eps"], s)
+
+    def _advance(self, s):
+        p = lambda t: t.data_ptr()  # noqa: E731
+        self.fn.step_advance_batch(p(self.pos), p(self.tokens), p(self.next), p(self.plen), self.max_ctx, self.B, s)
+
+    def _caches(self, dev):
+        """A layer's attention cache."""
+        import torch
+        shape = (self.B, self.max_ctx, self.cfg["nkv"], HD)
+        return dict(Kc=torch.zeros(shape, device=dev), Vc=torch.zeros(shape, device=dev))
 
     def start(self, prompts, stream):
         """New sequences: prompts [B][P] (one length for all), the position at 0, every DeltaNet state zeroed."""

@@ -336,6 +336,17 @@ int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const
                 const int *kv_len, const int *table, int max_pages, int max_new, float scale, void *ws, uint64_t ws_bytes,
                 void *stream);
 
+/* The attention layer's q / k head RMSNorm and RoPE (head dim 256, rotary on the first 64 dims) for rows at positions of
+ * their own: q [rows][nh][256] and k [rows][nkv][256] (fp32, token and head strides in floats, 16-byte aligned) ->
+ * q_out [rows][nh][256], k_out [rows][nkv][256]; rows with positions[i] < 0 come out zero. What fn_attn_decode does to q and
+ * k before its cache, without the one position for all (k_qk_norm_rope, engine/faie2fn.cu:1452-1478). */
+int fn_qk_rope_rows(const float *q, int64_t q_token, int64_t q_head, const float *k, int64_t k_token, int64_t k_head,
+                    const float *wq, const float *wk, const float *inv_freq, const int *positions, int rows, int nh, int nkv,
+                    float *q_out, float *k_out, float eps, void *stream);
+/* Zero the recurrent state and conv histories of one sequence of a batched DeltaNet handle (fn_gdn_create_batch), on a
+ * stream: its place is given to a new request. */
+int fn_gdn_reset_seq(int h, int seq, void *stream);
+
 /* ---- the decode step (the reference's layer_forward + forward, engine/faie2fn.cu:2370-2490) --------------------
  * One step of the hybrid MoE decoder over resident handles (fn_w_create, fn_gdn_create, fn_moe_create) and device
  * buffers the caller owns: the embedding row of tokens[*pos], per layer the input projection, the gated-DeltaNet core
