@@ -93,6 +93,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
     extern __shared__ __align__(128) uint8_t sm_ka[];
     __shared__ long long red[THREADS / 32], s_off;
     __shared__ int s_req;
+    __shared__ KaReq s_rq;
     __shared__ volatile int s_fail;
     __shared__ __align__(8) float s_rs[ROWS], s_qs[2][NG][ROWS];
     __shared__ float s_ref[KA_CONS][ROWS], s_l[KA_CONS][ROWS], s_mref[ROWS], s_ml[ROWS];
@@ -142,6 +143,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
             const long long w = (long long)q.rt * a.l.nkv * (q.tiles + KA_EXTRA);
             if (u0 < at + w) {
                 s_req = r;
+                s_rq = q;
                 s_off = u0 - at;
                 break;
             }
@@ -162,7 +164,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
     if (u0 >= u1) return;
 
     int r = s_req;
-    KaReq rq = ka_req<ROWS>(a, r);
+    KaReq rq = s_rq;
     // the run is at place `off` of a row tile's units: its own follow KA_EXTRA that only count
     int item = (int)(s_off / (rq.tiles + KA_EXTRA)), off = (int)(s_off - (long long)item * (rq.tiles + KA_EXTRA));
     long long u = u0;
@@ -629,7 +631,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                 to[ROWS * HD + ROWS + tid] = s_ml[tid];
             }
             if (tid == 0 && starts)
-                a.split[blockIdx.x] = KaSplit{(int)((u - off + KA_EXTRA + rq.tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
+                a.split[blockIdx.x] = KaSplit{(int)((u - off + KA_EXTRA + rq.tiles - 1) / per) - (int)blockIdx.x + 1, kv, tile, rq};
         }
     }
 }
@@ -647,14 +649,18 @@ FN_API uint64_t fn_kv4_attn_workspace(void) {
 template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
     cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL, NT>);
     if (e != cudaSuccess) return e;
-    // no more CTAs than pairs of units there can be; a row tile of one pair is never split
+    // no more CTAs than pairs of units there can be
     const long long units = items * tiles;
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KaCfg<HD, HL, NT>::CTAS, KA_MAX_GRID));
     e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KaCfg<HD, HL, NT>::THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
-    if (e != cudaSuccess || grid == 1) return e;
-    return launch_k(k_kv4_join<typename KaCfg<HD, HL, NT>::T, HD, KaCfg<HD, HL, NT>::ROWS>, dim3(grid, KaCfg<HD, HL, NT>::ROWS), dim3(32 * KJ_WARPS), 0, s, a);
+    // one request of at most two tiles: its row tiles weigh the same, 2 + KA_EXTRA units at most, which is the shortest run, so
+    // none is split
+    if (e != cudaSuccess || (a.n == 1 && tiles <= 2 && grid == units / 2)) return e;
+    const int runs_at_once = items <= KJ_GRID ? KJ_GRID : grid;  // few row tiles: few are split
+    return launch_k(k_kv4_join<typename KaCfg<HD, HL, NT>::T, HD, KaCfg<HD, HL, NT>::ROWS>, dim3(std::min(grid, runs_at_once), KaCfg<HD, HL, NT>::ROWS),
+                    dim3(32 * KJ_WARPS), 0, s, a, grid);
 }
-constexpr int KP_FROM = 48;  // rows of a request from which the prompts' kernel is faster
+constexpr int KP_FROM = 64;  // rows of a request from which the prompts' kernel takes it (16 requests: equal at 48 rows, 64 against 53 us at 64; one request of 16k tokens: 31 against 39 us at 64, equal near 112)
 
 template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
     const long long rows = (long long)std::min(max_new, a.rows) * a.group;

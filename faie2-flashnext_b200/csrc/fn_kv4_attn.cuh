@@ -29,14 +29,14 @@ struct Kv4AttnArgs {
     uint32_t *err;
 };
 
-struct KaSplit {
-    int parts;              // CTAs it lies in (0: there is none)
-    int req, kv, tile;
-};
-
 // a request's share of the work
 struct KaReq {
     int first, fresh, len, tiles, rt;  // first row, rows, tokens, 64-token tiles, row tiles
+};
+struct KaSplit {
+    int parts;  // CTAs it lies in (0: there is none)
+    int kv, tile;
+    KaReq rq;
 };
 template <int ROWS> __device__ __forceinline__ KaReq ka_req(const Kv4AttnArgs &a, int r) {
     KaReq q;
@@ -89,70 +89,89 @@ __device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, i
     }
 }
 
-// ---- the join: the parts of the row tile that starts in run c = blockIdx.x and goes on past it, each a run of [ROWS][HD]
-// sums, [ROWS] references (base 2) and [ROWS] sums of weights, `stride` floats apart, two to a run. The warps of a CTA take a row
-// together, part by part (loads of many parts in flight), and add their sums in the order of the warps.
-constexpr int KJ_WARPS = 8;
-template <typename T, int HD, int ROWS> __global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
-    constexpr int PER = HD / 32, U = 8, W = KJ_WARPS;
+// ---- the join of row tiles that lie in several runs: the parts of the one that starts in run c are [ROWS][HD] sums, [ROWS]
+// references (base 2) and [ROWS] sums of weights, a.stride floats apart, two to a run. CTA (x, row) takes the runs x, x +
+// gridDim.x, ..; its warps take a row together, part by part, the first of them
+// loaded before the weights are known, and add their sums in the order of the warps.
+constexpr int KJ_WARPS = 8, KJ_GRID = 32;
+template <typename T, int HD, int ROWS>
+__global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a, int runs) {
+    constexpr int PER = HD / 32, U = HD == 256 ? 6 : 8, W = KJ_WARPS;
     __shared__ float s_w[KA_MAX_GRID], s_red[2][W], s_sum[W][HD];
     pdl_wait();
     pdl_trigger();
-    const int c = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const KaSplit sp = after_wait(a.split)[c];
-    if (sp.parts == 0) return;
-    const KaReq rq = ka_req<ROWS>(a, sp.req);
-    const int flat = sp.tile * ROWS + i;
-    if (flat >= rq.fresh * a.group) return;
-    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
-    float mx = -INFINITY;
-    for (int x = tid; x < sp.parts; x += 32 * W) {
-        const float rf = slot(x)[ROWS * HD + i];
-        s_w[x] = rf;
-        mx = fmaxf(mx, rf);
-    }
+    const int i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const KaSplit *split = after_wait(a.split);
+    for (int base = blockIdx.x; base < runs; base += 32 * gridDim.x) {
+        const int mine = base + lane * gridDim.x;
+        uint32_t todo = __ballot_sync(0xffffffffu, mine < runs && split[mine].parts != 0);
+        for (; todo; todo &= todo - 1) {
+            const int c = base + (__ffs(todo) - 1) * gridDim.x;
+            const KaSplit sp = split[c];
+            const int flat = sp.tile * ROWS + i;
+            if (flat >= sp.rq.fresh * a.group) continue;
+            auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
+            float y[PER] = {}, v[U][PER];
+            auto fetch = [&](int x0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) s_red[0][warp] = mx;
-    __syncthreads();
+                for (int x = 0; x < U; ++x) {
+                    const bool in = x0 + W * x < sp.parts;
+                    const float *p = slot(in ? x0 + W * x : 0) + i * HD + lane;
 #pragma unroll
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
-    for (int x = tid; x < sp.parts; x += 32 * W) s_w[x] = ka_weight(s_w[x], mx);
-    __syncthreads();
-    float y[PER] = {}, sum = 0.0f;
-    for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
-        float v[U][PER], l[U], w[U];
+                    for (int d = 0; d < PER; ++d) v[x][d] = in ? p[32 * d] : 0.0f;
+                }
+            };
+            fetch(warp);
+            float rf[2], l[2], mx = -INFINITY, sum = 0.0f;  // 2 x 256 parts at most
 #pragma unroll
-        for (int x = 0; x < U; ++x) {
-            const bool in = x0 + W * x < sp.parts;
-            const float *p = slot(in ? x0 + W * x : 0);
-            w[x] = in ? s_w[x0 + W * x] : 0.0f;
-            l[x] = in ? p[ROWS * HD + ROWS + i] : 0.0f;
+            for (int x = 0; x < 2; ++x) {
+                const int q = tid + 32 * W * x;
+                rf[x] = q < sp.parts ? slot(q)[ROWS * HD + i] : -INFINITY;
+                l[x] = q < sp.parts ? slot(q)[ROWS * HD + ROWS + i] : 0.0f;
+                mx = fmaxf(mx, rf[x]);
+            }
 #pragma unroll
-            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (lane == 0) s_red[0][warp] = mx;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int q = tid + 32 * W * x;
+                const float f = q < sp.parts ? ka_weight(rf[x], mx) : 0.0f;
+                if (q < sp.parts) s_w[q] = f, sum += f * l[x];
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) s_red[1][warp] = sum;
+            __syncthreads();
+            for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
+                if (x0 != warp) fetch(x0);
+#pragma unroll
+                for (int x = 0; x < U; ++x) {
+                    const float w = x0 + W * x < sp.parts ? s_w[x0 + W * x] : 0.0f;
+#pragma unroll
+                    for (int d = 0; d < PER; ++d) y[d] += w * v[x][d];
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
+            __syncthreads();
+            sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) sum += s_red[1][w];
+            const bool sees = sp.rq.len - sp.rq.fresh + flat / a.group + 1 > 0 && sp.rq.len > 0;
+            if (warp == 0)
+                ka_emit<T, HD>(a, sp.rq, sp.kv, flat, lane, sees, [&](int d) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) s += s_sum[w][d];
+                    return s / sum;
+                });
+            __syncthreads();
         }
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-            sum += w[x] * l[x];
-#pragma unroll
-            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
-        }
     }
-#pragma unroll
-    for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
-    if (lane == 0) s_red[1][warp] = sum;
-    __syncthreads();
-    if (warp) return;
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) sum += s_red[1][w];
-    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
-    ka_emit<T, HD>(a, rq, sp.kv, flat, lane, sees, [&](int d) {
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) s += s_sum[w][d];
-        return s / sum;
-    });
 }
 
 // host: prompts' kernel (fn_kv4_prompt.cu), and its share of the workspace

@@ -541,7 +541,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 to[row] = m;
                 to[KP_ROWS + row] = l;
                 if (tid == 32 * KP_W_SM && k == 0)
-                    a.split[blockIdx.x] = KaSplit{(int)((u - off + KP_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, r, kv, tile};
+                    a.split[blockIdx.x] = KaSplit{(int)((u - off + KP_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, kv, tile, rq};
             }
             __syncwarp();
             if (lane == 0) tc_arrive(&sh.lf);
@@ -826,7 +826,7 @@ template <typename T, int HD> __global__ void __launch_bounds__(256) k_kv4_promp
     const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
     const KaSplit sp = after_wait(a.split)[c];
     if (sp.parts == 0) return;
-    const KaReq rq = kp_req(a, sp.req);
+    const KaReq rq = sp.rq;
     const long long flat = (long long)sp.tile * KP_ROWS + i;
     if (flat >= (long long)rq.fresh * a.group) return;
     auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
