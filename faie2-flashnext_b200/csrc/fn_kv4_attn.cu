@@ -619,8 +619,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         if (starts && ends) {
             // the row tile's output: a warp takes a row at a time
             for (int i = warp; i < nrow; i += KA_CONS) {
-                const float sum = s_ml[i];
-                ka_emit<T, HD>(a, rq, kv, tile * ROWS + i, lane, limit(i) > 0, [&](int d) { return ob[i * OS + d] / sum; });
+                const float inv = 1.0f / s_ml[i];
+                ka_emit<T, HD>(a, rq, kv, tile * ROWS + i, lane, limit(i) > 0, [&](int d) { return ob[i * OS + d] * inv; });
             }
         } else {
             // a part of a row tile: its start (1), or what goes on from the run before (0)

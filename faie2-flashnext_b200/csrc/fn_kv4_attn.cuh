@@ -162,12 +162,13 @@ __global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constan
 #pragma unroll
             for (int w = 0; w < W; ++w) sum += s_red[1][w];
             const bool sees = sp.rq.len - sp.rq.fresh + flat / a.group + 1 > 0 && sp.rq.len > 0;
+            const float inv = 1.0f / sum;
             if (warp == 0)
                 ka_emit<T, HD>(a, sp.rq, sp.kv, flat, lane, sees, [&](int d) {
                     float s = 0.0f;
 #pragma unroll
                     for (int w = 0; w < W; ++w) s += s_sum[w][d];
-                    return s / sum;
+                    return s * inv;
                 });
             __syncthreads();
         }

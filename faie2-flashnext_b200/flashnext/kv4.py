@@ -114,6 +114,7 @@ class KV4Cache:
         self.ws = workspace or KV4Workspace(fn)
         self.c = C.byref(FnKv4(pages.data_ptr(), pages.shape[0], page_size, nkv, hd))
         self.scale = 1.0 / math.sqrt(hd)
+        self._store, self._load, self._attn = fn.kv4_store, fn.kv4_load, fn.kv4_attn
 
     def _rows(self, name, x, heads):
         s = x.shape
@@ -131,7 +132,7 @@ class KV4Cache:
         self._slots(slots, nt)
         kt, kh, _ = k.stride()
         vt, vh, _ = v.stride()
-        self.fn.kv4_store(self.c, _TYPE[k.dtype], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), nt, _stream(self.dev))
+        self._store(self.c, _TYPE[k.dtype], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), nt, _stream(self.dev))
 
     def load(self, slots, dtype=torch.float32):
         """(k, v) [rows][nkv][hd], the values that slots stand for (zeros for slots < 0)."""
@@ -141,7 +142,7 @@ class KV4Cache:
         self._slots(slots, nt)
         k = torch.empty(nt, self.nkv, self.hd, dtype=dtype, device=self.dev)
         v = torch.empty_like(k)
-        self.fn.kv4_load(self.c, _TYPE[dtype], slots.data_ptr(), nt, k.data_ptr(), v.data_ptr(), _stream(self.dev))
+        self._load(self.c, _TYPE[dtype], slots.data_ptr(), nt, k.data_ptr(), v.data_ptr(), _stream(self.dev))
         return k, v
 
     def _slots(self, slots, nt):
@@ -170,7 +171,7 @@ class KV4Cache:
             if gate.shape != q.shape or gate.dtype != q.dtype:
                 raise ValueError("gate: q's shape and type is wanted")
             g, gt, gh = gate.data_ptr(), gate.stride(0), gate.stride(1)
-        self.fn.kv4_attn(self.c, _TYPE[q.dtype], n, rows, nh, q.data_ptr(), q.stride(0), q.stride(1), g, gt, gh,
+        self._attn(self.c, _TYPE[q.dtype], n, rows, nh, q.data_ptr(), q.stride(0), q.stride(1), g, gt, gh,
                          out.data_ptr(), out.stride(0), cu.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
                          table.shape[1], max_new, self.scale if scale is None else scale, self.ws.ptr, self.ws.bytes,
                          _stream(self.dev))

@@ -1,6 +1,6 @@
 """Float64 oracle of the paged 4-bit KV cache (csrc/fn_kv4.h): page records, planning, storing, loading, attention.
 
-Written from the definitions, one request, one block and one row at a time (numpy, no torch): the checker of
+Written from the definitions, one request, one block and one row at a time (numpy, no torch), for
 tests/test_kv4_gpu.py and tests/test_kv4_cpu.py.
 """
 
