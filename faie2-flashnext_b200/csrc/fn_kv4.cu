@@ -255,21 +255,20 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv4_store(const K
     for (int x = 0; x < ROW_UNITS; ++x) {
         int t, g;
         kv4_unit(a, x, t, g);
-        // fminf / fmaxf would drop a NaN, so values that are not finite are counted apart
-        float big = v[x][0], small = v[x][0];
-        bool bad = false;
+        // fminf / fmaxf would drop a NaN, so what is not finite shows in a sum of zeros
+        float big = v[x][0], small = v[x][0], zeros = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             big = fmaxf(big, v[x][i]);
             small = fminf(small, v[x][i]);
-            bad |= !isfinite(v[x][i]);
+            zeros = fmaf(v[x][i], 0.0f, zeros);
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             small = fminf(small, __shfl_xor_sync(0xffffffffu, small, o));
         }
-        bad = (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 24) & 255u) != 0;
+        const bool bad = (__ballot_sync(0xffffffffu, zeros != 0.0f) >> (threadIdx.x & 24) & 255u) != 0;
         if (slot[x] >= (int64_t)a.l.n_pages * a.l.bs) dev_fail(a.err, DEV_BAD_ARG);
         else if (slot[x] >= 0) {
             const float d = (big >= -small ? big : small) * -0.125f;
@@ -277,8 +276,10 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv4_store(const K
             uint32_t w = 0, line;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = __float2int_rz(__fadd_rn(__fmul_rn(v[x][i], inv), 8.5f));
-                w |= (uint32_t)min(max(c, 0), 15) << (4 * i);
+                // x / d + 8.5 is 0.5 .. 16.5: adding 2^23 cut towards zero leaves its whole part in the low bits (a conversion would
+                // go through the slow pipe)
+                const float t = __fadd_rn(__fmul_rn(v[x][i], inv), 8.5f);
+                w |= min(__float_as_uint(__fadd_rz(t, 8388608.0f)) & 31u, 15u) << (4 * i);
             }
             uint8_t *rec = kv4_place(a.l, slot[x], h, g, line);
             *(uint32_t *)(rec + part * a.l.kb + line * 32 + lane * 4) = w;
@@ -320,7 +321,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_kv4_load(const Kv
         if (!kv4_unit(a, x, t, g)) continue;
         float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (float)((int)(w[x] >> (4 * i) & 15u) - 8) * d[x];
+        for (int i = 0; i < 8; ++i)  // c as the float 2^23 + c, less 2^23 + 8
+            y[i] = (__uint_as_float((w[x] >> (4 * i) & 15u) | 0x4b000000u) - 8388616.0f) * d[x];
         T *o = (T *)a.y[part] + ((int64_t)t * a.l.nkv + h) * a.l.hd + g * KV4_GROUP + lane * 8;
         if constexpr (sizeof(T) == 4) {
             *(float4 *)o = make_float4(y[0], y[1], y[2], y[3]);

@@ -656,9 +656,12 @@ template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnA
     // one request of at most two tiles: its row tiles weigh the same, 2 + KA_EXTRA units at most, which is the shortest run, so
     // none is split
     if (e != cudaSuccess || (a.n == 1 && tiles <= 2 && grid == units / 2)) return e;
-    const int runs_at_once = items <= KJ_GRID ? KJ_GRID : grid;  // few row tiles: few are split
-    return launch_k(k_kv4_join<typename KaCfg<HD, HL, NT>::T, HD, KaCfg<HD, HL, NT>::ROWS>, dim3(std::min(grid, runs_at_once), KaCfg<HD, HL, NT>::ROWS),
-                    dim3(32 * KJ_WARPS), 0, s, a, grid);
+    using C = KaCfg<HD, HL, NT>;
+    using T = typename C::T;
+    // few row tiles may have many parts, many have few
+    if (items <= KJ_GRID)
+        return launch_k(k_kv4_join_few<T, HD, C::ROWS>, dim3(std::min(grid, KJ_GRID), C::ROWS), dim3(32 * KJ_WARPS), 0, s, a, grid);
+    return launch_k(k_kv4_join<T, HD, C::ROWS>, dim3(grid, C::ROWS / 8), dim3(256), 0, s, a);
 }
 constexpr int KP_FROM = 64;  // rows of a request from which the prompts' kernel takes it (16 requests: equal at 48 rows, 64 against 53 us at 64; one request of 16k tokens: 31 against 39 us at 64, equal near 112)
 

@@ -90,89 +90,159 @@ __device__ __forceinline__ void ka_emit(const Kv4AttnArgs &a, const KaReq &rq, i
 }
 
 // ---- the join of row tiles that lie in several runs: the parts of the one that starts in run c are [ROWS][HD] sums, [ROWS]
-// references (base 2) and [ROWS] sums of weights, a.stride floats apart, two to a run. CTA (x, row) takes the runs x, x +
-// gridDim.x, ..; its warps take a row together, part by part, the first of them
-// loaded before the weights are known, and add their sums in the order of the warps.
-constexpr int KJ_WARPS = 8, KJ_GRID = 32;
+// references (base 2) and [ROWS] sums of weights, a.stride floats apart, two to a run. Always in the order of the runs.
+template <int HD, int W> struct KjShared {
+    float w[KA_MAX_GRID], red[2][W], sum[W][HD];
+};
+
+// Row i of the tile by W warps: each takes every W-th part, the first of them loaded before the weights are known; their sums are
+// added in the order of the warps.
+template <typename T, int HD, int ROWS, int W>
+__device__ __forceinline__ void ka_join_row(const Kv4AttnArgs &a, int c, const KaSplit &sp, int i, KjShared<HD, W> &sh) {
+    constexpr int PER = HD / 32, U = 8, N = (KA_MAX_GRID + 32 * W - 1) / (32 * W);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long flat = (long long)sp.tile * ROWS + i;
+    if (flat >= (long long)sp.rq.fresh * a.group) return;
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
+    float y[PER] = {}, v[U][PER];
+    auto fetch = [&](int x0) {
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const bool in = x0 + W * x < sp.parts;
+            const float *p = slot(in ? x0 + W * x : 0) + i * HD + lane;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[32 * d] : 0.0f;
+        }
+    };
+    fetch(warp);
+    float rf[N], l[N], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        const int q = tid + 32 * W * x;
+        rf[x] = q < sp.parts ? slot(q)[ROWS * HD + i] : -INFINITY;
+        l[x] = q < sp.parts ? slot(q)[ROWS * HD + ROWS + i] : 0.0f;
+        mx = fmaxf(mx, rf[x]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) sh.red[0][warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, sh.red[0][w]);
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        const int q = tid + 32 * W * x;
+        if (q < sp.parts) {
+            const float f = ka_weight(rf[x], mx);
+            sh.w[q] = f;
+            sum += f * l[x];
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sh.red[1][warp] = sum;
+    __syncthreads();
+    for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
+        if (x0 != warp) fetch(x0);
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const float w = x0 + W * x < sp.parts ? sh.w[x0 + W * x] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) y[d] += w * v[x][d];
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < PER; ++d) sh.sum[warp][lane + 32 * d] = y[d];
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += sh.red[1][w];
+    const bool sees = sp.rq.len - sp.rq.fresh + flat / a.group + 1 > 0 && sp.rq.len > 0;
+    const float inv = 1.0f / sum;
+    if (warp == 0)
+        ka_emit<T, HD>(a, sp.rq, sp.kv, (int)flat, lane, sees, [&](int d) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += sh.sum[w][d];
+            return s * inv;
+        });
+    __syncthreads();
+}
+
+// few row tiles, perhaps of many parts: CTA (x, row) takes the runs x, x + gridDim.x, ..
+constexpr int KJ_WARPS = 16, KJ_GRID = 32;
 template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join(const __grid_constant__ Kv4AttnArgs a, int runs) {
-    constexpr int PER = HD / 32, U = HD == 256 ? 6 : 8, W = KJ_WARPS;
-    __shared__ float s_w[KA_MAX_GRID], s_red[2][W], s_sum[W][HD];
+__global__ void __launch_bounds__(32 * KJ_WARPS) k_kv4_join_few(const __grid_constant__ Kv4AttnArgs a, int runs) {
+    __shared__ KjShared<HD, KJ_WARPS> sh;
     pdl_wait();
     pdl_trigger();
-    const int i = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const KaSplit *split = after_wait(a.split);
     for (int base = blockIdx.x; base < runs; base += 32 * gridDim.x) {
-        const int mine = base + lane * gridDim.x;
+        const int mine = base + (threadIdx.x & 31) * gridDim.x;
         uint32_t todo = __ballot_sync(0xffffffffu, mine < runs && split[mine].parts != 0);
         for (; todo; todo &= todo - 1) {
             const int c = base + (__ffs(todo) - 1) * gridDim.x;
-            const KaSplit sp = split[c];
-            const int flat = sp.tile * ROWS + i;
-            if (flat >= sp.rq.fresh * a.group) continue;
-            auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
-            float y[PER] = {}, v[U][PER];
-            auto fetch = [&](int x0) {
-#pragma unroll
-                for (int x = 0; x < U; ++x) {
-                    const bool in = x0 + W * x < sp.parts;
-                    const float *p = slot(in ? x0 + W * x : 0) + i * HD + lane;
-#pragma unroll
-                    for (int d = 0; d < PER; ++d) v[x][d] = in ? p[32 * d] : 0.0f;
-                }
-            };
-            fetch(warp);
-            float rf[2], l[2], mx = -INFINITY, sum = 0.0f;  // 2 x 256 parts at most
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int q = tid + 32 * W * x;
-                rf[x] = q < sp.parts ? slot(q)[ROWS * HD + i] : -INFINITY;
-                l[x] = q < sp.parts ? slot(q)[ROWS * HD + ROWS + i] : 0.0f;
-                mx = fmaxf(mx, rf[x]);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            if (lane == 0) s_red[0][warp] = mx;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_red[0][w]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int q = tid + 32 * W * x;
-                const float f = q < sp.parts ? ka_weight(rf[x], mx) : 0.0f;
-                if (q < sp.parts) s_w[q] = f, sum += f * l[x];
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) s_red[1][warp] = sum;
-            __syncthreads();
-            for (int x0 = warp; x0 < sp.parts; x0 += W * U) {
-                if (x0 != warp) fetch(x0);
-#pragma unroll
-                for (int x = 0; x < U; ++x) {
-                    const float w = x0 + W * x < sp.parts ? s_w[x0 + W * x] : 0.0f;
-#pragma unroll
-                    for (int d = 0; d < PER; ++d) y[d] += w * v[x][d];
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < PER; ++d) s_sum[warp][lane + 32 * d] = y[d];
-            __syncthreads();
-            sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) sum += s_red[1][w];
-            const bool sees = sp.rq.len - sp.rq.fresh + flat / a.group + 1 > 0 && sp.rq.len > 0;
-            const float inv = 1.0f / sum;
-            if (warp == 0)
-                ka_emit<T, HD>(a, sp.rq, sp.kv, flat, lane, sees, [&](int d) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < W; ++w) s += s_sum[w][d];
-                    return s * inv;
-                });
-            __syncthreads();
+            ka_join_row<T, HD, ROWS, KJ_WARPS>(a, c, split[c], blockIdx.y, sh);
         }
     }
+}
+
+// many row tiles, mostly of few parts: CTA (c, eight rows), a warp a row, part after part; a row tile of many parts is taken row
+// after row by all eight warps
+template <typename T, int HD, int ROWS> __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4AttnArgs a) {
+    constexpr int PER = HD / 32, U = 4, ALONE = 24;
+    __shared__ KjShared<HD, 8> sh;
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const KaSplit sp = after_wait(a.split)[c];
+    if (sp.parts == 0) return;
+    if (sp.parts > ALONE) {
+        for (int x = 0; x < 8; ++x) ka_join_row<T, HD, ROWS, 8>(a, c, sp, blockIdx.y * 8 + x, sh);
+        return;
+    }
+    const long long flat = (long long)sp.tile * ROWS + i;
+    if (flat >= (long long)sp.rq.fresh * a.group) return;
+    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
+    // a part's reference and sum of weights a lane
+    const float rf = lane < sp.parts ? slot(lane)[ROWS * HD + i] : -INFINITY;
+    const float l = lane < sp.parts ? slot(lane)[ROWS * HD + ROWS + i] : 0.0f;
+    float v[U][PER], y[PER] = {};
+    auto fetch = [&](int x0) {
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const bool in = x0 + x < sp.parts;
+            const float *p = slot(in ? x0 + x : 0) + i * HD + lane;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[32 * d] : 0.0f;
+        }
+    };
+    fetch(0);
+    float mx = rf;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float w = lane < sp.parts ? ka_weight(rf, mx) : 0.0f;
+    float sum = w * l;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int x0 = 0; x0 < sp.parts; x0 += U) {
+        if (x0) fetch(x0);
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            const float f = __shfl_sync(0xffffffffu, w, x0 + x);
+#pragma unroll
+            for (int d = 0; d < PER; ++d) y[d] += f * v[x][d];
+        }
+    }
+    const bool sees = sp.rq.len - sp.rq.fresh + flat / a.group + 1 > 0 && sp.rq.len > 0;
+    const float inv = 1.0f / sum;
+    ka_emit<T, HD>(a, sp.rq, sp.kv, (int)flat, lane, sees, [&](int d) {
+        float r = 0.0f;
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+            if (d == lane + 32 * x) r = y[x];
+        return r * inv;
+    });
 }
 
 // host: prompts' kernel (fn_kv4_prompt.cu), and its share of the workspace

@@ -818,48 +818,6 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// joins the parts of split row tiles: a warp takes a row, part after part
-template <typename T, int HD> __global__ void __launch_bounds__(256) k_kv4_prompt_join(const __grid_constant__ Kv4AttnArgs a) {
-    constexpr int PER = HD / 32, U = 4;
-    pdl_wait();
-    pdl_trigger();
-    const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const KaSplit sp = after_wait(a.split)[c];
-    if (sp.parts == 0) return;
-    const KaReq rq = sp.rq;
-    const long long flat = (long long)sp.tile * KP_ROWS + i;
-    if (flat >= (long long)rq.fresh * a.group) return;
-    auto slot = [&](int x) { return after_wait(a.part) + ((size_t)(c + x) * 2 + (x == 0)) * a.stride; };
-    float mx = -INFINITY, y[PER] = {}, sum = 0.0f;
-    for (int x = 0; x < sp.parts; ++x) mx = fmaxf(mx, slot(x)[KP_ROWS * HD + i]);
-    for (int x0 = 0; x0 < sp.parts; x0 += U) {
-        float v[U][PER], w[U], l[U];
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-            const bool in = x0 + x < sp.parts;
-            const float *p = slot(in ? x0 + x : 0);
-            w[x] = in ? ka_weight(p[KP_ROWS * HD + i], mx) : 0.0f;
-            l[x] = in ? p[KP_ROWS * HD + KP_ROWS + i] : 0.0f;
-#pragma unroll
-            for (int d = 0; d < PER; ++d) v[x][d] = in ? p[i * HD + lane + 32 * d] : 0.0f;
-        }
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-            sum += w[x] * l[x];
-#pragma unroll
-            for (int d = 0; d < PER; ++d) y[d] += w[x] * v[x][d];
-        }
-    }
-    const bool sees = rq.len - rq.fresh + flat / a.group + 1 > 0 && rq.len > 0;
-    ka_emit<T, HD>(a, rq, sp.kv, (int)flat, lane, sees, [&](int d) {
-        float r = 0.0f;
-#pragma unroll
-        for (int x = 0; x < PER; ++x)
-            if (d == lane + 32 * x) r = y[x];
-        return r / sum;
-    });
-}
-
 uint64_t kv4_prompt_workspace() {
     return (uint64_t)std::min(num_sms(), KA_MAX_GRID) * 2 * KpCfg<256, true>::PART * 4;
 }
@@ -875,7 +833,7 @@ template <int HD, bool HL> static cudaError_t prompt_go(Kv4AttnArgs a, int max_n
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms(), KA_MAX_GRID));
     e = launch_k(k_kv4_prompt<HD, HL>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_k(k_kv4_prompt_join<typename C::T, HD>, dim3(grid, KP_ROWS / 8), dim3(256), 0, s, a);
+    return launch_k(k_kv4_join<typename C::T, HD, KP_ROWS>, dim3(grid, KP_ROWS / 8), dim3(256), 0, s, a);
 }
 
 cudaError_t launch_kv4_prompt(Kv4AttnArgs a, bool f32, int max_new, cudaStream_t s) {

@@ -277,6 +277,13 @@ def test_long_requests_are_split(fn, kv4, ws, dtype, hd, n, length):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_long_request_among_short_ones(fn, kv4, ws, dtype):
+    """Many row tiles, one of them in dozens of parts; the same for a prompt slice behind a long context."""
+    attn_case(fn, kv4, ws, 21, 64, 1, 8, 64, dtype, [20000] + [5 + i for i in range(39)], [1] * 40)
+    attn_case(fn, kv4, ws, 22, 64, 1, 1, 64, dtype, [20000], [100])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_prompt_slices(fn, kv4, ws, dtype):
     attn_case(fn, kv4, ws, 9, 128, 1, 2, 16, dtype, [2500, 900], [130, 333])
 
