@@ -26,7 +26,12 @@
 // from the lengths by a prefix sum, so nothing about the lengths is known on the host and a captured call serves any.
 // A row tile whose units lie in several CTAs leaves a partial result in each; a second small kernel joins them in the order
 // of the CTAs, so the result does not depend on timing (joining in the CTA that finishes last cost 20 us of latency chains
-// for 147 parts, beside 33 us of work; the second kernel takes a few).
+// for 147 parts, where the second kernel takes 6 to 8).
+//
+// What bounds it, and measured (device time): one request of 131071 tokens, bf16, 16 heads over 2 kv heads of 256 (71 MB) 27.8 us,
+// of which 15 us in the page loop (4.7 TB/s); 32 requests of 65 to 4096 tokens, fp32 25.1 us; 64 requests of 100 to 8192 tokens,
+// bf16, 32 heads over 8 of 128 (298 MB) 77 us (3.9 TB/s, issue of the page loop); one request of 77 tokens 8.2 us, a chain of round
+// trips to memory.
 //
 // A CTA: one warp copies pages into a ring (one bulk copy per page and head: codes and scales of K and V), four warps
 // compute, two on each 64-token stage, 32 tokens each, with their own running softmax; they merge at the end of a run.
