@@ -12,6 +12,7 @@ namespace fn {
 // - have further pages. Prefix sums over the requests give each its rows and its share of the free stack, so one CTA
 // with the requests' offsets in shared memory does all of it; the flat loops (returned pages, taken pages, rows) find
 // their request by bisection, so a prompt of thousands of rows spreads over all threads like many single tokens do.
+// Nothing but latency bounds it: 3.9 us for 32 requests of a token, 9.9 us for 256 requests with 7284 rows (two launches).
 struct PlanArgs {
     int n, max_pages, bs, n_pages, max_tokens;
     const int *ctx, *add;
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(const PlanArgs a) {
 // A unit is 64 dims of one head of one token (K or V); eight lanes hold eight values each, so a warp covers four units:
 // reads of 32 (16) bytes a lane, codes written as one word a lane, 32 adjacent bytes a unit. A thread takes four units, whose
 // loads are all under way before the first is used; blockIdx.y is the head of K or V, so that no index is divided.
+// Measured: 8192 rows of bf16, 8 heads of 128, store 20 and load 14 us (42 MB each; bound by instruction issue); 32 rows 3 us each.
 // d = m / -8 with m the value of largest magnitude (of two opposite ones the positive), c = clamp(trunc(x / d + 8.5), 0,
 // 15), so that m itself is the code 0 and all 16 codes are used; d is rounded to fp16 after the codes are chosen.
 template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]);

@@ -693,6 +693,8 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         if (n < 1 || n > KV4_MAX_REQ) return fail("kv4 attn: requests out of range (1..4096)");
         if (nh < 1 || nh % c->nkv || nh / c->nkv > 64) return fail("kv4 attn: bad head counts");
         if (rows < 0 || max_pages < 1 || max_new < 0) return fail("kv4 attn: bad row / page counts");
+        if ((long long)rows * (nh / c->nkv) > INT32_MAX - 256) return fail("kv4 attn: too many rows");
+        if ((long long)max_pages * c->page_size > INT32_MAX - 256) return fail("kv4 attn: table too wide");
         if (rows == 0) return 0;
         if ((uintptr_t)q % (type == T_F32 ? 4 : 2) || (uintptr_t)out % (type == T_F32 ? 4 : 2) || (uintptr_t)gate % (type == T_F32 ? 4 : 2))
             return fail("kv4 attn: rows must be aligned to their type");

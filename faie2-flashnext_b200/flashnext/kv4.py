@@ -96,7 +96,7 @@ class KV4Workspace:
 
     def __init__(self, fn):
         self.bytes = fn.kv4_attn_workspace()
-        self.tensor = torch.zeros(self.bytes, dtype=torch.uint8, device="cuda")
+        self.tensor = torch.empty(self.bytes, dtype=torch.uint8, device="cuda")
         self.ptr = self.tensor.data_ptr()
 
 

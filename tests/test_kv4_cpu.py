@@ -138,7 +138,8 @@ def attn_args(**k):
     (dict(type=8), "F32 or BF16"), (dict(n=0), "requests"), (dict(n=4097), "requests"), (dict(nh=5), "head counts"),
     (dict(nh=0), "head counts"), (dict(nh=130), "head counts"), (dict(rows=-1), "counts"), (dict(max_pages=0), "counts"),
     (dict(max_new=-1), "counts"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(ws=None), "null"),
-    (dict(table=None), "null"), (dict(wsb=8), "workspace"), (dict(ws=ONE + 16), "workspace")])
+    (dict(table=None), "null"), (dict(rows=1 << 30), "too many rows"), (dict(max_pages=1 << 28), "too wide"),
+    (dict(q=ONE + 2), "aligned"), (dict(gate=ONE + 1), "aligned"), (dict(wsb=8), "workspace"), (dict(ws=ONE + 16), "workspace")])
 def test_bad_attention_calls_are_refused(f, bad, word):
     refused(f.d.fn_kv4_attn(C.byref(cache()), *attn_args(**bad)), f, word)
 

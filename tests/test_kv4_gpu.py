@@ -276,6 +276,16 @@ def test_long_requests_are_split(fn, kv4, ws, dtype, hd, n, length):
         assert torch.equal(c.attn(q[..., :hd], dev(cu), dev(np.array(lens, np.int32)), dev(table), 1), out)
 
 
+@pytest.mark.parametrize("max_new", [1, 64])
+def test_more_requests_than_threads(fn, kv4, ws, max_new):
+    """Several requests a thread in the scan of the lengths (both kernels), idle and empty ones among them."""
+    rng = np.random.default_rng(23)
+    lens = rng.integers(0, 40, 1100).tolist()
+    news = rng.integers(0, 3, 1100).tolist()
+    lens[600], news[600] = 500, 2
+    attn_case(fn, kv4, ws, 24, 64, 1, 2, 16, "f32", lens, news, max_new=max_new, extra_rows=1)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_one_long_request_among_short_ones(fn, kv4, ws, dtype):
     """Many row tiles, one of them in dozens of parts; the same for a prompt slice behind a long context."""
