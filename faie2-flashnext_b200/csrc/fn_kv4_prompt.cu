@@ -6,7 +6,7 @@
 //
 // Roles of the CTA's 16 warps, one CTA per SM:
 //   * warp 0 copies pages into rings (K and V parts apart: they are consumed at different times);
-//   * warp 2 looks at each tile's V scales: their exponent, and which are not finite;
+//   * warp 2 looks at each tile's scales: K's and V's exponents, and which of V's are not finite;
 //   * warp 1 issues the MMAs: S of tile j + 1 before O of tile j, so the softmax of one runs beside the products of the other;
 //   * warps 4..7 (a row a lane): scores out of tensor memory, running softmax, P back into tensor memory in S's place;
 //   * warps 8..15: Q into tensor memory, K and V codes into the MMAs' operands in shared memory, and the running output:
@@ -15,9 +15,10 @@
 //     maximum needs no pass over tensor memory.
 //
 // Scales. V's codes of a tile become (c - 8) d 2^-e in fp16, e the exponent of the tile's largest |d|, and 2^e goes into
-// the addition: in range whatever the size of V (warp 2 finds e ahead of the workers). K's become (c - 8) d / 8: no fp16
-// scale overflows, and what a tiny K loses (2^-25 of its codes' fp16 grid) is nothing beside the other scores. Rows of q are
-// scaled by a power of two.
+// the addition: in range whatever the size of V (warp 2 finds e ahead of the workers). K's become (c - 8) d 2^(11 - e), e the
+// exponent of the tile's largest finite |d|, and the scores' unit takes 2^(e - 11): 8 d 2^(11 - e) is below 2^15, and scales down to
+// 2^-25 of the largest keep all their bits. In a tile where they lie further apart each token takes its own exponent, and its
+// column of scores is brought to the tile's. Rows of q are scaled by a power of two.
 // bf16 rows: one product each; q is exact, K, P and V are rounded to 11 bits. fp32 rows: q, K, P and V are fp16 pairs (22
 // bits, K's and V's exact), three products each, the small ones first, so that the sum's cut bits are few.
 //
@@ -38,6 +39,9 @@ namespace fn {
 constexpr int KP_ROWS = 128, KP_THREADS = 512;
 constexpr int KP_EXTRA = 8;  // units that a row tile counts beside its own, for its start and end
 constexpr int KP_W_SM = 4, KP_W_WORK = 8;
+constexpr int KP_POLLS = 1 << 17;         // of a wait before it gives up, 20 us at most each
+constexpr uint32_t KP_FIXED = 5120;       // bytes before the operands (KpShared)
+constexpr int KP_FAR = 25;                // binades between K scales of a tile from which tokens take their own exponents
 
 template <int HD, bool HL> struct KpCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
@@ -47,10 +51,11 @@ template <int HD, bool HL> struct KpCfg {
     static constexpr uint32_t KT = KA_TOK * HD * 2;          // K operand: [dim / 8][token] x 16 bytes
     // V operand: [token / 8][dim] x 16 bytes, the token groups 16 bytes further apart (banks of the stores)
     static constexpr uint32_t VG = HD * 16 + 16, VT = 8 * VG;
-    static constexpr uint32_t RAW = KA_TOK * (HD / 2 + HD / KV4_GROUP * 2);  // 64 tokens' codes and scales of K (or V)
+    // 64 tokens' codes and scales of V, and of K with V's scales beside its own (both are looked at before K is made)
+    static constexpr uint32_t RAW = KA_TOK * (HD / 2 + HD / KV4_GROUP * 2), RAWK = RAW + KA_TOK * HD / KV4_GROUP * 2;
     static constexpr uint32_t QL = HL ? KP_ROWS * HD * 2 : 0;  // second halves of q: [dim / 8][row] x 16 bytes
-    static constexpr uint32_t K_OFF = 4096, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
-    static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAW, SMEM = RV_OFF + RV * RAW;
+    static constexpr uint32_t K_OFF = KP_FIXED, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
+    static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAWK, SMEM = RV_OFF + RV * RAW;
     // registers by warpgroup: IO + SM + 2 WORK <= 4 x 128 at launch; the workers hold HD / 2 sums
     static constexpr int REG_IO = HD == 256 ? 56 : 72, REG_SM = HD == 256 ? 120 : 128, REG_WORK = HD == 256 ? 168 : 152;
     static_assert(REG_IO + REG_SM + 2 * REG_WORK <= 512);
@@ -63,16 +68,17 @@ template <int HD, bool HL> struct KpCfg {
 
 // the fixed part of shared memory
 struct KpShared {
-    uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[2], of, oe, qf, qe, lf, done;
+    uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[8], of, oe, qf, qe, lf, done;
     long long red[KP_THREADS / 32], off;
     uint32_t tmem, valid[8];  // pages there of tile & 7; bit 31: all of them, and every token seen by some row
     int req, fail;
     // rings as long as the fastest role can be ahead of the slowest reader
-    float ev[8], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    float ev[8], ek[8], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];  // ev: 2^e of V; ek: 2^(e - 11) of K, the scores' unit
     uint32_t bad[8][4][2];  // tokens whose V scale is not finite: [tile & 7][group][token / 32]
-    int any_bad[8];
+    int any_bad[8], far[8];  // far: K's exponents by token, below (biased by 127)
+    alignas(16) uint8_t kexp[8][KA_TOK];
 };
-static_assert(sizeof(KpShared) <= 4096);
+static_assert(sizeof(KpShared) <= KP_FIXED);
 
 // true in one lane of the warp
 __device__ __forceinline__ bool kp_elect() {
@@ -80,12 +86,12 @@ __device__ __forceinline__ bool kp_elect() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
     return p != 0;
 }
-// whether a phase has completed, after a short wait in the hardware
+// whether a phase has completed, after a wait of up to 20 us in the hardware
 __device__ __forceinline__ bool kp_try(uint64_t *bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(done)
-                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
                  : "memory");
     return done != 0;
 }
@@ -129,6 +135,14 @@ __device__ __forceinline__ uint32_t kp_hsub2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t kp_hmul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+__device__ __forceinline__ uint32_t kp_hmax2(uint32_t a, uint32_t b) {  // NaN where either is
+    const __half2 r = __hmax2_nan(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+__device__ __forceinline__ uint32_t kp_hmin2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmin2(*(const __half2 *)&a, *(const __half2 *)&b);
     return *(const uint32_t *)&r;
 }
 // a b - c, rounded once
@@ -183,12 +197,13 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 4), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 5);
-            mbar_init(&sh.kf[i], 4), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 4), mbar_init(&sh.xf[i], 1);
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 5), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 4);
+            mbar_init(&sh.kf[i], 4), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 4);
             mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
         }
         mbar_init(&sh.of, 1), mbar_init(&sh.oe, 8), mbar_init(&sh.qf, 8), mbar_init(&sh.qe, 1), mbar_init(&sh.lf, 4);
         mbar_init(&sh.done, 1);
+        for (int i = 0; i < 8; ++i) mbar_init(&sh.xf[i], 1);
         mbar_fence_init();
         sh.fail = 0;
     }
@@ -292,16 +307,20 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         const int f = tile * KP_ROWS + min(i, nrow - 1);
         return min(max(rq.len - rq.fresh + f / a.group + 1, 0), rq.len);
     };
+    // (few instructions, as it stands in every loop of every role: with a time limit by the clock each place had some 30 more, and the
+    // loops lost their places in the instruction cache)
     auto wt = [&](uint64_t *bar, int phase) {
-        if (kp_try(bar, (uint32_t)phase & 1u)) return true;
-        if (*s_fail) return false;
-        if (mbar_park(bar, (uint32_t)phase & 1u)) return true;
+#pragma unroll 1
+        for (int i = 0; i < KP_POLLS; ++i) {
+            if (kp_try(bar, (uint32_t)phase & 1u)) return true;
+            if (*s_fail) return false;
+        }
         *s_fail = 1;
         dev_fail(a.err, DEV_WAIT_TIMEOUT);
         return false;
     };
     const int ppt = KA_TOK >> a.l.lbs;  // pages of a tile
-    const uint32_t praw = a.l.kb + a.l.sb;  // bytes of a page's K (or V) part in a stage
+    const uint32_t praw = a.l.kb + a.l.sb, prawk = praw + a.l.sb;  // bytes of a page's V part in a stage, of its K part with V's scales
     int gt = 0, gi = 0;  // tiles and row tiles done by this role
 
     if (warp < KP_W_SM) {
@@ -328,16 +347,16 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                             ok = gt < R || wt(empty, gt / R - 1);
                             if (ok) {
                                 if (v == 0) sh.valid[gt & 7] = m | (m == (1u << ppt) - 1u && (j + 1) * KA_TOK <= hi_lim ? 0x80000000u : 0u);
-                                mbar_arrive_tx(full, (uint32_t)__popc(m) * praw);
+                                mbar_arrive_tx(full, (uint32_t)__popc(m) * (v ? praw : prawk));
                             }
                         }
                         ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                         if (!ok) break;
                         if (good) {
                             const uint8_t *rec = a.l.pages + ((int64_t)id * a.l.nkv + kv) * (int64_t)a.l.rec;
-                            uint8_t *to = sm_kp + (v ? C::RV_OFF : C::RK_OFF) + sl * C::RAW + lane * praw;
+                            uint8_t *to = sm_kp + (v ? C::RV_OFF + sl * C::RAW + lane * praw : C::RK_OFF + sl * C::RAWK + lane * prawk);
                             bulk_g2s(to, rec + v * a.l.kb, a.l.kb, full);
-                            bulk_g2s(to + a.l.kb, rec + 2 * a.l.kb + v * a.l.sb, a.l.sb, full);
+                            bulk_g2s(to + a.l.kb, rec + 2 * a.l.kb + v * a.l.sb, v ? a.l.sb : 2 * a.l.sb, full);
                         }
                     }
                 }
@@ -350,41 +369,72 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         if (i < gt || v == 0) mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
                 }
         } else if (warp == 2) {
-            // ---- V scales of a tile: the exponent of the largest finite one, and which are not
+            // ---- scales of a tile: the exponents of the largest finite K and V scale, which of V's are not finite, and whether K's
+            // lie so far apart that each token takes its own exponent
             bool ok = true;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
                 const int hi_lim = limit(KP_ROWS - 1);
                 for (int j = k; j < kend && ok; ++j, ++gt) {
-                    ok = __all_sync(0xffffffffu, wt(&sh.rvf[gt % C::RV], gt / C::RV));
+                    ok = __all_sync(0xffffffffu, wt(&sh.rkf[gt % C::RK], gt / C::RK));
                     if (!ok) break;
-                    const uint8_t *raw = sm_kp + C::RV_OFF + (gt % C::RV) * C::RAW + a.l.kb;
+                    const uint8_t *raw = sm_kp + C::RK_OFF + (gt % C::RK) * C::RAWK + a.l.kb;
                     const uint32_t valid = sh.valid[gt & 7];
-                    float mx = 0.0f;
-                    uint32_t any = 0;
+                    auto here_ = [&](int tok) { return (valid >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
+                    auto place = [&](int tok) { return raw + (tok >> a.l.lbs) * prawk + (tok & (a.l.bs - 1)) * 2; };
+                    // two tokens a lane, as halves (positive ones order as their bits do)
+                    const uint8_t *at = place(2 * lane);
+                    const uint32_t mask = (here_(2 * lane) ? 0x7fffu : 0u) | (here_(2 * lane + 1) ? 0x7fff0000u : 0u);
+                    uint32_t kw = 0, vw = 0, kn = 0x7bff7bffu;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int tok = lane + 32 * h, pg = tok >> a.l.lbs;
-                        const bool here_ = (valid >> pg & 1u) && j * KA_TOK + tok < hi_lim;
-#pragma unroll
-                        for (int x = 0; x < NG; ++x) {
-                            const float d = fabsf(ka_half(raw + pg * praw + (x * a.l.bs + (tok & (a.l.bs - 1))) * 2));
-                            if (here_ && d < INFINITY) mx = fmaxf(mx, d);
-                            const uint32_t bad = __ballot_sync(0xffffffffu, here_ && !(d < INFINITY));
-                            if (lane == 0) sh.bad[gt & 7][x][h] = bad;
-                            any |= bad;
-                        }
+                    for (int x = 0; x < NG; ++x) {
+                        const uint32_t dk = *(const uint32_t *)(at + x * a.l.bs * 2) & mask, dv = *(const uint32_t *)(at + a.l.sb + x * a.l.bs * 2) & mask;
+                        kw = kp_hmax2(kw, dk);
+                        vw = kp_hmax2(vw, dv);
+                        kn = kp_hmin2(kn, dk | (0x7bff7bffu & ~mask));
                     }
-#pragma unroll
-                    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    uint32_t kmax = __reduce_max_sync(0xffffffffu, max(kw & 0xffffu, kw >> 16));
+                    uint32_t vmax = __reduce_max_sync(0xffffffffu, max(vw & 0xffffu, vw >> 16));
+                    uint32_t kmin = __reduce_min_sync(0xffffffffu, min(kn & 0xffffu, kn >> 16));
+                    auto exponent = [](uint32_t h) { return (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) >> 23); };
+                    bool far = exponent(kmax) > exponent(kmin) + KP_FAR, any = false;
+                    if (far || max(kmax, vmax) >= 0x7c00u) [[unlikely]] {
+                        // a closer look, a token a lane: zeros and what is not finite set no exponent
+                        kmax = vmax = 0, kmin = 0x7bffu;
+                        uint32_t own[2] = {};
+#pragma unroll 1
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+                            for (int x = 0; x < NG; ++x) {
+                                const uint8_t *p = place(lane + 32 * h) + x * a.l.bs * 2;
+                                const bool in = here_(lane + 32 * h);
+                                const uint32_t dk = *(const uint16_t *)p & 0x7fffu, dv = *(const uint16_t *)(p + a.l.sb) & 0x7fffu;
+                                if (in && dv < 0x7c00u) vmax = max(vmax, dv);
+                                if (in && dk < 0x7c00u && dk > 0) {
+                                    kmax = max(kmax, dk), kmin = min(kmin, dk);
+                                    own[0] = h ? own[0] : max(own[0], dk), own[1] = h ? max(own[1], dk) : 0;
+                                }
+                                const uint32_t bad = __ballot_sync(0xffffffffu, in && dv >= 0x7c00u);
+                                if (lane == 0) sh.bad[gt & 7][x][h] = bad;
+                                any |= bad != 0;
+                            }
+                        kmax = __reduce_max_sync(0xffffffffu, kmax);
+                        vmax = __reduce_max_sync(0xffffffffu, vmax);
+                        kmin = __reduce_min_sync(0xffffffffu, kmin);
+                        far = exponent(kmax) > exponent(kmin) + KP_FAR;
+                        sh.kexp[gt & 7][lane] = (uint8_t)exponent(own[0] ? own[0] : kmax);
+                        sh.kexp[gt & 7][lane + 32] = (uint8_t)exponent(own[1] ? own[1] : kmax);
+                    }
                     if (lane == 0) {
-                        sh.ev[gt & 7] = mx > 0.0f ? kp_pow2((int)(__float_as_uint(mx) >> 23) - 127) : 1.0f;
-                        sh.any_bad[gt & 7] = any != 0;
+                        sh.ev[gt & 7] = vmax ? kp_pow2(exponent(vmax) - 127) : 1.0f;
+                        sh.ek[gt & 7] = kmax ? kp_pow2(exponent(kmax) - 138) : 1.0f;
+                        sh.any_bad[gt & 7] = any;
+                        sh.far[gt & 7] = far;
                     }
                     __syncwarp();
                     if (lane == 0) {
-                        tc_arrive(&sh.xf[gt & 1]);
-                        tc_arrive(&sh.rve[gt % C::RV]);
+                        tc_arrive(&sh.xf[gt & 7]);
+                        tc_arrive(&sh.rke[gt % C::RK]);
                     }
                 }
             }
@@ -478,10 +528,28 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
+                // (what warps 0 and 2 and the workers left for this tile is there: they came before the K and q of these scores)
                 if (j == k) rs = sh.rs[row];
                 const uint32_t valid = sh.valid[gt & 7], ts = tl + (uint32_t)b * 64u;
                 const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
                 const bool masked = left < KA_TOK || !(valid >> 31);
+                const float ek = sh.ek[gt & 7], rsj = rs * ek;
+                if (sh.far[gt & 7]) [[unlikely]] {  // the columns to the tile's unit, first of all
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[16];
+                        kp_tmem_ld16(ts + 16u * c, s);
+                        kp_tmem_wait_ld();
+                        kp_tmem_got(s);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {  // 2^(e - that of the unit)
+                            const uint32_t f = ((uint32_t)sh.kexp[gt & 7][16 * c + i] + 116u << 23) - __float_as_uint(ek);
+                            s[i] = __float_as_uint(__uint_as_float(s[i]) * __uint_as_float(f));
+                        }
+                        tmem_st16(ts + 16u * c, s);
+                        tmem_wait_st();
+                    }
+                }
                 // (16 columns at a time, read twice: a short loop stays in the instruction cache beside the other roles' loops,
                 // where 64 columns unrolled had every role wait for instructions)
                 auto hide = [&](uint32_t(&s)[16], int c) {
@@ -504,13 +572,13 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     for (int i = 0; i < 16; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s[i]));
                 }
                 // rs > 0: the maximum may be taken before the scaling
-                const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * rs);
+                const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * rsj);
                 // weights 2^10 exp2(s - maximum): fp16 keeps 11 bits down to 2^-24 of the largest
                 const float z = mn == -INFINITY ? 0.0f : 10.0f - mn;
                 const float fac = m == -INFINITY ? 0.0f : ka_exp2(m - mn);
                 m = mn;
                 sh.f[gt & 3][row] = fac;
-                const float2 rs2 = make_float2(rs, rs), z2 = make_float2(z, z);
+                const float2 rs2 = make_float2(rsj, rsj), z2 = make_float2(z, z);
                 float2 ls = make_float2(0.0f, 0.0f);
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -564,8 +632,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         constexpr int KU = NG, VU = HD >= 128 ? HD / 128 : 1;
         const int gtid = wtid & 127;
         const int k_tok = gtid & 63, k_q = gtid >> 6, k_line = k_tok & (a.l.bs - 1);
-        const uint32_t k_src = (k_tok >> a.l.lbs) * praw + k_line * 32 + k_q * 16, k_dst = k_q * 4096 + k_tok * 16;
-        const uint32_t k_sc = (k_tok >> a.l.lbs) * praw + a.l.kb + k_line * 2;
+        const uint32_t k_src = (k_tok >> a.l.lbs) * prawk + k_line * 32 + k_q * 16, k_dst = k_q * 4096 + k_tok * 16;
+        const uint32_t k_sc = (k_tok >> a.l.lbs) * prawk + a.l.kb + k_line * 2;
         const int v_tok = (gtid & 7) * 8, v_wd = gtid >> 3, v_line = (v_wd >> 3) * a.l.bs + (v_tok & (a.l.bs - 1));
         const uint32_t v_page = (v_tok >> a.l.lbs) * praw, v_src = v_page + v_line * 32 + (v_wd & 7) * 4, v_sc = v_page + a.l.kb + v_line * 2;
         const uint32_t v_dst = (gtid & 7) * C::VG + v_wd * 128;
@@ -598,8 +666,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 mx = fmaxf(mx, sx[(half ^ 1) * KP_ROWS + row]);
                 const int e = min(max(10 - ((int)(__float_as_uint(mx) >> 23) - 127), -90), 120);
                 const float up = a.scale < 0.0f ? -kp_pow2(e) : kp_pow2(e);
-                // scores in base 2: undo the scaling, and K's 1 / 8; positive also for a scale of zero
-                if (half == 0) sh.rs[row] = fmaxf(fabsf(a.scale) * 8.0f * 1.44269504f * kp_pow2(-e), 1e-30f);
+                // scores in base 2: undo the scaling; positive also for a scale of zero (beside K's unit, 2^-35 or more, too)
+                if (half == 0) sh.rs[row] = fmaxf(fabsf(a.scale) * 1.44269504f * kp_pow2(-e), 1e-26f);
                 kp_bar_work();
 #pragma unroll 1
                 for (int d = 0; d < HH; d += 32) {
@@ -633,15 +701,17 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
             // K of tile g (the row tile's j): 16 bytes of codes (32 dims of a token) at a time
             auto make_k = [&](int g, int j) {
-                if (!wtw(&sh.rkf[g % C::RK], g / C::RK)) return false;
+                if (!wtw(&sh.rkf[g % C::RK], g / C::RK) || !wtw(&sh.xf[g & 7], g >> 3)) return false;
                 if (g >= NB && !wtw(&sh.ke[g % NB], g / NB - 1)) return false;
-                const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAW;
+                const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAWK;
                 uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT + k_dst;
                 const bool all = sh.valid[g & 7] >> 31;
+                // 2^(11 - e)
+                const float up = __uint_as_float(sh.far[g & 7] ? 265u - sh.kexp[g & 7][k_tok] << 23 : 0x7f000000u - __float_as_uint(sh.ek[g & 7]));
 #pragma unroll 1
                 for (int x = 0; x < KU; ++x) {  // a 64-dim group each
                     const uint4 w4 = *(const uint4 *)(raw + k_src + x * a.l.bs * 32);
-                    float d = ka_half(raw + k_sc + x * a.l.bs * 2) * 0.125f;
+                    float d = ka_half(raw + k_sc + x * a.l.bs * 2) * up;
                     if (!all && !there(g, j, k_tok)) d = 0.0f;
                     const uint32_t dd = ka_pack(d, d);
                     const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -665,7 +735,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             };
             // V of tile g: 8 tokens x 8 dims at a time, turned. Its buffer's last reader came before an O that has been added.
             auto make_v = [&](int g, int j) {
-                if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 1], g >> 1)) return false;
+                if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 7], g >> 3)) return false;
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
                 const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 7]));  // 1 / 2^e
                 const bool all = (sh.valid[g & 7] >> 31) && !sh.any_bad[g & 7];

@@ -1,0 +1,128 @@
+"""GPU: attention over the paged 4-bit cache where keys and values differ in size, against a float64 softmax over the values that the
+cache holds (read back by load, whose values are exact).
+
+Tolerances, for a row and a 64-dim block, V the largest |v| of the block that the row sees, S the largest scale sum_d |q_d k_d| of a key
+that it sees. fp32 rows: products and sums keep some 22 bits, 2e-5 V as in tests/test_kv4_gpu.py; a score is kept to 2^-20 S, which
+changes a weight by that share and an output by twice that of V at most. bf16 rows: half an ulp of the output, 2^-8 |out| at
+most, P and V rounded to 11 bits each (2^-10 V), and keys rounded to 11 bits (2^-12 of each product, 2^-11 S V).
+"""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def kv4(fn):
+    import kv4 as m
+    return m
+
+
+@pytest.fixture(scope="module")
+def ws(fn, kv4):
+    return kv4.KV4Workspace(fn)
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Case:
+    """One request of `length` tokens, keys [length][nkv][hd] and values of any sizes, its last `new` tokens as rows."""
+
+    def __init__(self, fn, kv4, ws, k, v, q, bs=16, dtype="f32"):
+        self.length, self.nkv, self.hd = k.shape
+        n = -(-self.length // bs)
+        perm = torch.randperm(n, generator=torch.Generator().manual_seed(1))
+        self.c = kv4.KV4Cache(fn, self.nkv, self.hd, bs, n, ws)
+        self.table = perm.to(torch.int32).cuda()[None].contiguous()
+        slots = (perm[:, None] * bs + torch.arange(bs)[None]).reshape(-1)[:self.length].cuda()
+        self.c.store(torch.from_numpy(k).float().cuda(), torch.from_numpy(v).float().cuda(), slots)
+        self.q = torch.from_numpy(q).float().cuda().to(DT[dtype])
+        self.k, self.v = (x.double().cpu().numpy() for x in self.c.load(slots))
+        self.fn, self.dtype, self.new = fn, dtype, q.shape[0]
+
+    def run(self, scale=None, max_new=None):
+        out = self.c.attn(self.q, i32(0, self.new), i32(self.length), self.table, max_new or self.new, scale=scale)
+        self.fn.sync(torch.cuda.current_stream().cuda_stream)
+        return out.double().cpu().numpy()
+
+    def rows(self, scale=None):
+        """Per row and head: what it should be [hd], V per block, S."""
+        scale = 1 / np.sqrt(self.hd) if scale is None else scale
+        q = self.q.double().cpu().numpy()
+        group = q.shape[1] // self.nkv
+        for i in range(self.new):
+            see = self.length - self.new + i + 1
+            for h in range(q.shape[1]):
+                k, v = self.k[:see, h // group], self.v[:see, h // group]
+                s = scale * (k @ q[i, h])
+                p = np.exp(s - s.max())
+                yield i, h, p @ v / p.sum(), np.abs(v).reshape(see, -1, 64).max((0, 2)), abs(scale) * (np.abs(k) @ np.abs(q[i, h])).max()
+
+    def check(self, scale=None, max_new=None, cap=None):
+        """cap: rows whose S is above it are only looked at for finite outputs."""
+        got, worst = self.run(scale, max_new), 0.0
+        assert np.isfinite(got).all()
+        for i, h, want, V, S in self.rows(scale):
+            if cap is not None and S > cap:
+                continue
+            V = np.repeat(V, 64)
+            if self.dtype == "f32":
+                tol = (2e-5 + 2.0 ** -19 * S) * V
+            else:
+                tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -10 + 2.0 ** -11 * S) * V
+            worst = max(worst, float((np.abs(got[i, h] - want) / np.maximum(tol, 1e-300)).max()))
+        assert worst <= 1, worst
+
+
+# new tokens, heads of a group: the two forms of the kernel for few rows, the kernel for prompts
+FORMS = [pytest.param(1, 8, id="one"), pytest.param(5, 3, id="few"), pytest.param(70, 2, id="prompt")]
+
+
+def normal(rng, *shape):
+    return rng.standard_normal(shape)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("size", [1e-6, 1e-5, 1e-4, 1e-3, 1.0, 1e3, 3e4])
+def test_keys_of_any_size(fn, kv4, ws, size, new, group, dtype):
+    """Scores of the same spread from keys of any size. (Scales below fp16's normal numbers have few bits; those are the cache's values.)"""
+    rng = np.random.default_rng(1)
+    q = normal(rng, new, 2 * group, 128) * 2 / size
+    Case(fn, kv4, ws, normal(rng, 150, 2, 128) * size, normal(rng, 150, 2, 128), q, dtype=dtype).check()
+
+
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("scale", [0.3, -0.1, 0.0, -0.0, 1e-20])
+def test_scales_given(fn, kv4, ws, scale, new, group):
+    rng = np.random.default_rng(2)
+    for size in (1e-4, 1.0):
+        q = normal(rng, new, 2 * group, 64) / size
+        Case(fn, kv4, ws, normal(rng, 100, 2, 64) * size, normal(rng, 100, 2, 64), q, bs=32).check(scale)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("hd, spread", [(64, 2.0), (128, 4.0), (256, 3.0)])
+def test_keys_of_sizes_beside_each_other(fn, kv4, ws, hd, spread, new, group, dtype):
+    """Tokens whose keys differ by powers of ten, within a tile too: the scores stay right beside each other."""
+    rng = np.random.default_rng(3)
+    k = normal(rng, 200, 1, hd) * 10 ** rng.uniform(-spread, 0, (200, 1, 1))
+    Case(fn, kv4, ws, k, normal(rng, 200, 1, hd), normal(rng, new, group, hd) * 2, dtype=dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", [pytest.param(5, 3, id="few"), pytest.param(70, 2, id="prompt")])
+@pytest.mark.parametrize("factor", [1e4, 1e6, 1e8])
+def test_keys_hidden_from_a_row_do_not_matter(fn, kv4, ws, factor, new, group, dtype):
+    rng = np.random.default_rng(7)
+    k = normal(rng, 128, 1, 128) * 1e-3
+    k[-1] = np.clip(k[-1] * factor, -5e5, 5e5)
+    q = normal(rng, new, group, 128) * 1e3
+    Case(fn, kv4, ws, k, normal(rng, 128, 1, 128), q, dtype=dtype).check(cap=1e3)
