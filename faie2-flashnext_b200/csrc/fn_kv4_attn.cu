@@ -645,10 +645,12 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
 
 using namespace fn;
 
-// every CTA's split row tile, then its two partial results
+// every CTA's split row tile and note, then its two partial results
+constexpr size_t KA_HEAD = KA_MAX_GRID * (sizeof(KaSplit) + sizeof(int));
+static_assert(KA_HEAD % 256 == 0);
 FN_API uint64_t fn_kv4_attn_workspace(void) {
     const uint64_t few = (uint64_t)std::min(num_sms() * 3, KA_MAX_GRID) * 2 * KA_PART_MAX * 4;
-    return KA_MAX_GRID * sizeof(KaSplit) + std::max(few, kv4_prompt_workspace());
+    return KA_HEAD + std::max(few, kv4_prompt_workspace());
 }
 
 template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
@@ -709,11 +711,27 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         a.group = nh / c->nkv;
         a.split = (KaSplit *)ws;
         a.stride = KA_PART_MAX;
-        a.part = (float *)((uint8_t *)ws + KA_MAX_GRID * sizeof(KaSplit));
+        a.far = (int *)((uint8_t *)ws + KA_MAX_GRID * sizeof(KaSplit));
+        a.part = (float *)((uint8_t *)ws + KA_HEAD);
         const bool f32 = type == T_F32;
         const int64_t size = f32 ? 4 : 2;
         a.vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0 && out_token * size % 16 == 0 &&
                 (!gate || ((uintptr_t)gate % 16 == 0 && gate_token * size % 16 == 0 && gate_head * size % 16 == 0));
+        // whether rows of out may be rows of q or gate (by their first and last bytes)
+        struct Span {
+            intptr_t lo, hi;
+        };
+        auto span = [&](const void *p, int64_t token, int64_t head) {
+            const int64_t t = (rows - 1) * token, h = (nh - 1) * head;
+            return Span{(intptr_t)p + (std::min<int64_t>(t, 0) + std::min<int64_t>(h, 0)) * size,
+                        (intptr_t)p + (std::max<int64_t>(t, 0) + std::max<int64_t>(h, 0) + c->hd) * size};
+        };
+        const Span so = span(out, out_token, c->hd), sq = span(q, q_token, q_head);
+        a.always = so.lo < sq.hi && sq.lo < so.hi;
+        if (gate) {
+            const Span sg = span(gate, gate_token, gate_head);
+            a.always |= so.lo < sg.hi && sg.lo < so.hi;
+        }
         const cudaStream_t s = (cudaStream_t)stream;
         const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
                             : c->hd == 128 ? attn_go<128>(a, f32, max_new, s)

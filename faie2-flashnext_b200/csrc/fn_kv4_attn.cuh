@@ -26,6 +26,8 @@ struct Kv4AttnArgs {
     float *part;     // [CTA][2]: a row tile's sums [rows][hd], references [rows], sums of weights [rows]
     int64_t stride;  // floats of a partial result's place
     struct KaSplit *split;  // [CTA]: the row tile that starts in the CTA's run and goes on past it
+    int *far;    // prompts [CTA]: whether its run met what only the kernel's long form serves
+    int always;  // prompts: only the long form runs
     uint32_t *err;
 };
 

@@ -14,11 +14,17 @@
 //     over tokens are rounded fp32 additions, where the tensor core's own accumulation over a long context cuts, and a new
 //     maximum needs no pass over tensor memory.
 //
-// Scales. V's codes of a tile become (c - 8) d 2^-e in fp16, e the exponent of the tile's largest |d|, and 2^e goes into
-// the addition: in range whatever the size of V (warp 2 finds e ahead of the workers). K's become (c - 8) d 2^(11 - e), e the
-// exponent of the tile's largest finite |d|, and the scores' unit takes 2^(e - 11): 8 d 2^(11 - e) is below 2^15, and scales down to
-// 2^-25 of the largest keep all their bits. In a tile where they lie further apart each token takes its own exponent, and its
-// column of scores is brought to the tile's. Rows of q are scaled by a power of two.
+// Scales. Codes of a tile become (c - 8) d 2^(11 - e) in fp16, e the exponent of the tile's largest finite |d|, K's and V's for
+// themselves: 8 d 2^(11 - e) is below 2^15, and scales down to 2^-25 of the largest keep all their bits. K's e goes into the scores'
+// unit; in a tile whose K scales lie further apart (one huge key, hidden from some rows perhaps) each token takes its own. V's goes into the
+// weights: P = 2^10 2^(s + e - r), where a row's reference r is the running maximum of s + e, so what P's fp16 range holds is what
+// a tile adds to the row, and tiles that add little cost the others no bits, whatever their values' size. The sum of weights takes
+// 2^(11 - e) back. In a tile whose V scales lie more than 2^12 apart (one huge value, or block of it, beside small ones) no e serves
+// all: its weights stay fp32, and the workers add p v on the CUDA cores instead of the tensor core's O (some 15 times as slow).
+// Such tiles, and what is not finite, have a kernel of their own (FAR), the same with the code for them: with that code in it every
+// call would pay (the roles' loops share the instruction cache: 8 bf16 prompts 963 us beside 744). The first kernel notes whether it
+// met any; the second, launched behind it, returns at once or does the call again.
+// Rows of q are scaled by a power of two.
 // bf16 rows: one product each; q is exact, K, P and V are rounded to 11 bits. fp32 rows: q, K, P and V are fp16 pairs (22
 // bits, K's and V's exact), three products each, the small ones first, so that the sum's cut bits are few.
 //
@@ -41,7 +47,9 @@ constexpr int KP_EXTRA = 8;  // units that a row tile counts beside its own, for
 constexpr int KP_W_SM = 4, KP_W_WORK = 8;
 constexpr int KP_POLLS = 1 << 17;         // of a wait before it gives up, 20 us at most each
 constexpr uint32_t KP_FIXED = 5120;       // bytes before the operands (KpShared)
-constexpr int KP_FAR = 25;                // binades between K scales of a tile from which tokens take their own exponents
+// binades between the K, or the V scales of a tile from which it goes the long way. The operands are exact up to 25; but V's e stands
+// for every token and block of the tile, and P keeps 22 bits (11 for bf16 rows) down to 12 binades below the largest
+constexpr int KP_FAR_K = 25, KP_FAR_V = 12;
 
 template <int HD, bool HL> struct KpCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
@@ -71,12 +79,13 @@ struct KpShared {
     uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[8], of, oe, qf, qe, lf, done;
     long long red[KP_THREADS / 32], off;
     uint32_t tmem, valid[8];  // pages there of tile & 7; bit 31: all of them, and every token seen by some row
-    int req, fail;
+    int req, fail, met;  // met: what only the long way serves
     // rings as long as the fastest role can be ahead of the slowest reader
-    float ev[8], ek[8], f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];  // ev: 2^e of V; ek: 2^(e - 11) of K, the scores' unit
+    float f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    float ev[8], ek[8];  // e of V, 2^(e - 11) of K: the scores' unit
     uint32_t bad[8][4][2];  // tokens whose V scale is not finite: [tile & 7][group][token / 32]
-    int any_bad[8], far[8];  // far: K's exponents by token, below (biased by 127)
-    alignas(16) uint8_t kexp[8][KA_TOK];
+    uint8_t any_bad[8], kfar[8], vfar[8];
+    uint8_t kexp[8][KA_TOK];  // kfar: exponents by token (biased by 127)
 };
 static_assert(sizeof(KpShared) <= KP_FIXED);
 
@@ -127,6 +136,14 @@ __device__ __forceinline__ void kp_tmem_got(uint32_t (&r)[16]) {
 __device__ __forceinline__ float2 kp_pair(const uint32_t (&r)[16], int i) {
     return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
+__device__ __forceinline__ float kp_tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;\n" : "=r"(r) : "r"(taddr) : "memory");
+    return __uint_as_float(r);
+}
+__device__ __forceinline__ void kp_arrive2(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;\n" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void kp_bar_work() { asm volatile("bar.sync 2, 256;" ::: "memory"); }
 __device__ __forceinline__ float kp_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ uint32_t kp_hsub2(uint32_t a, uint32_t b) {
@@ -141,6 +158,7 @@ __device__ __forceinline__ uint32_t kp_hmax2(uint32_t a, uint32_t b) {  // NaN w
     const __half2 r = __hmax2_nan(*(const __half2 *)&a, *(const __half2 *)&b);
     return *(const uint32_t *)&r;
 }
+__device__ __forceinline__ uint32_t kp_hzero2(uint32_t a) { return __heq2_mask(*(const __half2 *)&a, __half2half2(__ushort_as_half(0))); }
 __device__ __forceinline__ uint32_t kp_hmin2(uint32_t a, uint32_t b) {
     const __half2 r = __hmin2(*(const __half2 *)&a, *(const __half2 *)&b);
     return *(const uint32_t *)&r;
@@ -187,7 +205,8 @@ __device__ __forceinline__ int kp_tiles(const KaReq &q, int group, int i) {
 }
 __device__ __forceinline__ KaReq kp_req(const Kv4AttnArgs &a, int r) { return ka_req<KP_ROWS>(a, r); }
 
-template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttnArgs a) {
+// FAR: the long way, for a call in which the other form met what it does not serve (it notes that in a.far, a place for each CTA)
+template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttnArgs a) {
     using C = KpCfg<HD, HL>;
     using T = typename C::T;
     constexpr int NG = C::NG, NB = C::NB;
@@ -197,7 +216,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 5), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 4);
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 5), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 8);
             mbar_init(&sh.kf[i], 4), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 4);
             mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
         }
@@ -206,14 +225,22 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         for (int i = 0; i < 8; ++i) mbar_init(&sh.xf[i], 1);
         mbar_fence_init();
         sh.fail = 0;
+        sh.met = 0;
+    }
+    if constexpr (FAR) {
+        pdl_wait();
+        pdl_trigger();
+        if (!__syncthreads_or(a.always || (tid < gridDim.x && after_wait(a.far)[tid]))) return;
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    pdl_wait();
-    pdl_trigger();
+    if constexpr (!FAR) {
+        pdl_wait();
+        pdl_trigger();
+    }
 
     // ---- this CTA's run of units
     const int per_t = (a.n + KP_THREADS - 1) / KP_THREADS, r0 = min(tid * per_t, a.n), r1 = min(r0 + per_t, a.n);
@@ -371,7 +398,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         } else if (warp == 2) {
             // ---- scales of a tile: the exponents of the largest finite K and V scale, which of V's are not finite, and whether K's
             // lie so far apart that each token takes its own exponent
-            bool ok = true;
+            bool ok = true, met = false;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
                 const int hi_lim = limit(KP_ROWS - 1);
@@ -382,54 +409,58 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     const uint32_t valid = sh.valid[gt & 7];
                     auto here_ = [&](int tok) { return (valid >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
                     auto place = [&](int tok) { return raw + (tok >> a.l.lbs) * prawk + (tok & (a.l.bs - 1)) * 2; };
-                    // two tokens a lane, as halves (positive ones order as their bits do)
+                    // two tokens a lane, as halves (positive ones order as their bits do); zeros set no exponent
                     const uint8_t *at = place(2 * lane);
                     const uint32_t mask = (here_(2 * lane) ? 0x7fffu : 0u) | (here_(2 * lane + 1) ? 0x7fff0000u : 0u);
-                    uint32_t kw = 0, vw = 0, kn = 0x7bff7bffu;
+                    uint32_t kw = 0, vw = 0, kn = 0x7bff7bffu, vn = kn;
 #pragma unroll
                     for (int x = 0; x < NG; ++x) {
                         const uint32_t dk = *(const uint32_t *)(at + x * a.l.bs * 2) & mask, dv = *(const uint32_t *)(at + a.l.sb + x * a.l.bs * 2) & mask;
                         kw = kp_hmax2(kw, dk);
                         vw = kp_hmax2(vw, dv);
-                        kn = kp_hmin2(kn, dk | (0x7bff7bffu & ~mask));
+                        kn = kp_hmin2(kn, dk | (kp_hzero2(dk) & 0x7bff7bffu));
+                        vn = kp_hmin2(vn, dv | (kp_hzero2(dv) & 0x7bff7bffu));
                     }
                     uint32_t kmax = __reduce_max_sync(0xffffffffu, max(kw & 0xffffu, kw >> 16));
                     uint32_t vmax = __reduce_max_sync(0xffffffffu, max(vw & 0xffffu, vw >> 16));
                     uint32_t kmin = __reduce_min_sync(0xffffffffu, min(kn & 0xffffu, kn >> 16));
+                    uint32_t vmin = __reduce_min_sync(0xffffffffu, min(vn & 0xffffu, vn >> 16));
                     auto exponent = [](uint32_t h) { return (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) >> 23); };
-                    bool far = exponent(kmax) > exponent(kmin) + KP_FAR, any = false;
-                    if (far || max(kmax, vmax) >= 0x7c00u) [[unlikely]] {
-                        // a closer look, a token a lane: zeros and what is not finite set no exponent
-                        kmax = vmax = 0, kmin = 0x7bffu;
-                        uint32_t own[2] = {};
+                    if constexpr (!FAR) {
+                        met |= exponent(kmax) > exponent(kmin) + KP_FAR_K || exponent(vmax) > exponent(vmin) + KP_FAR_V || max(kmax, vmax) >= 0x7c00u;
+                    } else {
+                        // a closer look, a token a lane: what is not finite sets no exponent either
+                        bool any = false;
+                        uint32_t own[2] = {};  // the token's largest K scale
+                        kmax = vmax = 0;
 #pragma unroll 1
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-                            for (int x = 0; x < NG; ++x) {
+                        for (int x = 0; x < NG; ++x)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
                                 const uint8_t *p = place(lane + 32 * h) + x * a.l.bs * 2;
                                 const bool in = here_(lane + 32 * h);
                                 const uint32_t dk = *(const uint16_t *)p & 0x7fffu, dv = *(const uint16_t *)(p + a.l.sb) & 0x7fffu;
+                                if (in && dk < 0x7c00u) own[h] = max(own[h], dk);
                                 if (in && dv < 0x7c00u) vmax = max(vmax, dv);
-                                if (in && dk < 0x7c00u && dk > 0) {
-                                    kmax = max(kmax, dk), kmin = min(kmin, dk);
-                                    own[0] = h ? own[0] : max(own[0], dk), own[1] = h ? max(own[1], dk) : 0;
-                                }
                                 const uint32_t bad = __ballot_sync(0xffffffffu, in && dv >= 0x7c00u);
                                 if (lane == 0) sh.bad[gt & 7][x][h] = bad;
                                 any |= bad != 0;
                             }
-                        kmax = __reduce_max_sync(0xffffffffu, kmax);
+                        kmax = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
                         vmax = __reduce_max_sync(0xffffffffu, vmax);
-                        kmin = __reduce_min_sync(0xffffffffu, kmin);
-                        far = exponent(kmax) > exponent(kmin) + KP_FAR;
-                        sh.kexp[gt & 7][lane] = (uint8_t)exponent(own[0] ? own[0] : kmax);
-                        sh.kexp[gt & 7][lane + 32] = (uint8_t)exponent(own[1] ? own[1] : kmax);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) sh.kexp[gt & 7][lane + 32 * h] = (uint8_t)exponent(own[h] ? own[h] : kmax);
+                        const bool vfar = vmax && exponent(vmax) > exponent(vmin) + KP_FAR_V;
+                        if (vfar) vmax = vmin;  // what is added in fp32 raises no reference
+                        if (lane == 0) {
+                            sh.any_bad[gt & 7] = any;
+                            sh.kfar[gt & 7] = kmax && exponent(kmax) > exponent(kmin) + KP_FAR_K;
+                            sh.vfar[gt & 7] = vfar;
+                        }
                     }
                     if (lane == 0) {
-                        sh.ev[gt & 7] = vmax ? kp_pow2(exponent(vmax) - 127) : 1.0f;
+                        sh.ev[gt & 7] = vmax ? (float)(exponent(vmax) - 127) : 0.0f;
                         sh.ek[gt & 7] = kmax ? kp_pow2(exponent(kmax) - 138) : 1.0f;
-                        sh.any_bad[gt & 7] = any;
-                        sh.far[gt & 7] = far;
                     }
                     __syncwarp();
                     if (lane == 0) {
@@ -438,6 +469,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     }
                 }
             }
+            if (met) sh.met = 1;
         } else if (warp == 1) {
             // ---- MMAs. The whole warp runs this and one elected lane issues: the operands' descriptors then live in uniform
             // registers. (As one lane's own values each MMA took 120 cycles and more, whatever its size; so it takes what its size
@@ -479,7 +511,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 for (int j = 0; j <= n && ok; ++j) {
                     if (j < n) {
                         const int g = g0 + j;
-                        ok = wtw(&sh.kf[g % NB], g / NB);
+                        // (S takes the place of P of tile g - 2, which the workers may still read)
+                        ok = wtw(&sh.kf[g % NB], g / NB) && (!FAR || g < 2 || !sh.vfar[(g - 2) & 7] || wtw(&sh.oe, g - 2));
                         if (!ok) break;
                         tc_fence_after();
                         if (kp_elect()) {
@@ -496,7 +529,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         if (!ok) break;
                         tc_fence_after();
                         if (kp_elect()) {
-                            outputs(g);
+                            if (!FAR || !sh.vfar[g & 7]) outputs(g);
                             umma_commit(&sh.of);
                         }
                         __syncwarp();
@@ -520,8 +553,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
         for (; u < u1 && ok; next()) {
             if (!here()) continue;
             const int lim = limit(row);
-            float m = -INFINITY, l = 0.0f;
-            float rs = 0.0f;
+            // the reference, as the score and the exponent that it came of: a large score would swallow the exponent
+            float sref = -INFINITY, eref = 0.0f, l = 0.0f, rs = 0.0f;
             for (int j = k; j < kend; ++j, ++gt) {
                 const int b = gt & 1;
                 ok = wt(&sh.sf[b], gt >> 1);
@@ -533,8 +566,9 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 const uint32_t valid = sh.valid[gt & 7], ts = tl + (uint32_t)b * 64u;
                 const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
                 const bool masked = left < KA_TOK || !(valid >> 31);
-                const float ek = sh.ek[gt & 7], rsj = rs * ek;
-                if (sh.far[gt & 7]) [[unlikely]] {  // the columns to the tile's unit, first of all
+                const float ek = sh.ek[gt & 7], ev = sh.ev[gt & 7];
+                float rsj = rs * ek;
+                if (FAR && sh.kfar[gt & 7]) {  // every column by its own unit
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t s[16];
@@ -542,13 +576,12 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         kp_tmem_wait_ld();
                         kp_tmem_got(s);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {  // 2^(e - that of the unit)
-                            const uint32_t f = ((uint32_t)sh.kexp[gt & 7][16 * c + i] + 116u << 23) - __float_as_uint(ek);
-                            s[i] = __float_as_uint(__uint_as_float(s[i]) * __uint_as_float(f));
-                        }
+                        for (int i = 0; i < 16; ++i)
+                            s[i] = __float_as_uint(__uint_as_float(s[i]) * (rs * kp_pow2((int)sh.kexp[gt & 7][16 * c + i] - 138)));
                         tmem_st16(ts + 16u * c, s);
                         tmem_wait_st();
                     }
+                    rsj = 1.0f;
                 }
                 // (16 columns at a time, read twice: a short loop stays in the instruction cache beside the other roles' loops,
                 // where 64 columns unrolled had every role wait for instructions)
@@ -572,14 +605,33 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     for (int i = 0; i < 16; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s[i]));
                 }
                 // rs > 0: the maximum may be taken before the scaling
-                const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * rsj);
-                // weights 2^10 exp2(s - maximum): fp16 keeps 11 bits down to 2^-24 of the largest
-                const float z = mn == -INFINITY ? 0.0f : 10.0f - mn;
-                const float fac = m == -INFINITY ? 0.0f : ka_exp2(m - mn);
-                m = mn;
+                const float top = fmaxf(mx[0], mx[1]) * rsj;
+                const bool higher = top - sref > eref - ev;  // (never so for -inf beside -inf)
+                const float ns = higher ? top : sref, ne = higher ? ev : eref;
+                const float fac = sref == -INFINITY ? 0.0f : ka_exp2((sref - ns) + (eref - ne));
+                sref = ns, eref = ne;
+                // P = 2^10 exp2(s + e - reference): fp16 keeps 11 bits down to 2^-24 of the largest
+                const float z = ns == -INFINITY ? 0.0f : (10.0f + ev - ne) - ns;
                 sh.f[gt & 3][row] = fac;
                 const float2 rs2 = make_float2(rsj, rsj), z2 = make_float2(z, z);
                 float2 ls = make_float2(0.0f, 0.0f);
+                if (FAR && sh.vfar[gt & 7]) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[16];
+                        kp_tmem_ld16(ts + 16u * c, s);
+                        kp_tmem_wait_ld();
+                        kp_tmem_got(s);
+                        hide(s, c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float p = ka_exp2(fmaf(__uint_as_float(s[i]), rsj, z));
+                            ls.x += p;
+                            s[i] = __float_as_uint(p);
+                        }
+                        tmem_st16(ts + 16u * c, s);
+                    }
+                } else {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t s[16], p16[16];
@@ -600,7 +652,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     if constexpr (HL) tmem_st16(ts + 16u * c, p16);
                     else kp_tmem_st8(ts + 16u * c, p16);
                 }
-                l = l * fac + (ls.x + ls.y);
+                }
+                l = l * fac + (ls.x + ls.y) * kp_pow2(11 - (int)ev);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -611,7 +664,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 sh.l[row] = l;
             } else {
                 float *to = a.part + ((size_t)blockIdx.x * 2 + (k == 0)) * a.stride + KP_ROWS * HD;
-                to[row] = m;
+                to[row] = sref + eref;
                 to[KP_ROWS + row] = l;
                 if (tid == 32 * KP_W_SM && k == 0)
                     a.split[blockIdx.x] = KaSplit{(int)((u - off + KP_EXTRA + tiles - 1) / per) - (int)blockIdx.x + 1, kv, tile, rq};
@@ -707,7 +760,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT + k_dst;
                 const bool all = sh.valid[g & 7] >> 31;
                 // 2^(11 - e)
-                const float up = __uint_as_float(sh.far[g & 7] ? 265u - sh.kexp[g & 7][k_tok] << 23 : 0x7f000000u - __float_as_uint(sh.ek[g & 7]));
+                const float up = __uint_as_float(FAR && sh.kfar[g & 7] ? 265u - sh.kexp[g & 7][k_tok] << 23 : 0x7f000000u - __float_as_uint(sh.ek[g & 7]));
 #pragma unroll 1
                 for (int x = 0; x < KU; ++x) {  // a 64-dim group each
                     const uint4 w4 = *(const uint4 *)(raw + k_src + x * a.l.bs * 32);
@@ -737,11 +790,11 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             auto make_v = [&](int g, int j) {
                 if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 7], g >> 3)) return false;
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
-                const float up = __uint_as_float(0x7f000000u - __float_as_uint(sh.ev[g & 7]));  // 1 / 2^e
-                const bool all = (sh.valid[g & 7] >> 31) && !sh.any_bad[g & 7];
+                const float up = kp_pow2(11 - (int)sh.ev[g & 7]);
+                const bool all = (sh.valid[g & 7] >> 31) && !(FAR && sh.any_bad[g & 7]), far = FAR && sh.vfar[g & 7];
 #pragma unroll 1
                 for (int un = 0; un < VU; ++un) {
-                    if (HD < 128 && v_wd >= HD / 8) break;
+                    if (far || (HD < 128 && v_wd >= HD / 8)) break;
                     const uint8_t *src = raw + v_src + un * 2 * a.l.bs * 32;  // 16 words on: two groups
                     const uint4 s4 = *(const uint4 *)(raw + v_sc + un * 2 * a.l.bs * 2);
                     const uint32_t ss[4] = {s4.x, s4.y, s4.z, s4.w};
@@ -753,8 +806,8 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                         float2 d = __fmul2_rn(ka_unpack(ss[y]), make_float2(up, up));
                         if (!all) {
                             const int tok = v_tok + 2 * y;
-                            if (!(there(g, j, tok) && fabsf(d.x) < INFINITY)) d.x = 0.0f;
-                            if (!(there(g, j, tok + 1) && fabsf(d.y) < INFINITY)) d.y = 0.0f;
+                            if (!there(g, j, tok) || (FAR && !(fabsf(d.x) < INFINITY))) d.x = 0.0f;
+                            if (!there(g, j, tok + 1) || (FAR && !(fabsf(d.y) < INFINITY))) d.y = 0.0f;
                         }
                         dd[y] = ka_pack(d.x, d.y);
                     }
@@ -781,7 +834,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                 __syncwarp();
                 if (lane == 0) {
                     tc_arrive(&sh.vf[g % NB]);
-                    tc_arrive(&sh.rve[g % C::RV]);
+                    if (!far) kp_arrive2(&sh.rve[g % C::RV]);
                 }
                 return true;
             };
@@ -790,6 +843,40 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
             for (int j = k - 1; j <= kend && ok; ++j) {
                 const int g = gt + j - k;
                 const bool adds = j > k;
+                // a tile whose V scales lie far apart: o = o f + p v in fp32, a token at a time. First of all, since the stage that it gives
+                // back may be the only one, and the next copies wait behind it.
+                const bool far = FAR && adds && sh.vfar[(g - 1) & 7];
+                if (far) {
+                    const int gp = g - 1;
+                    if (!wtw(&sh.rvf[gp % C::RV], gp / C::RV) || !wtw(&sh.pf[gp & 1], gp >> 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const float f = sh.f[gp & 3][row], up = kp_pow2(11 - (int)sh.ev[gp & 7]);
+#pragma unroll
+                    for (int c = 0; c < HH / 2; ++c) o[c].x *= f, o[c].y *= f;
+#pragma unroll 1
+                    for (int tok = 0; tok < KA_TOK; ++tok) {
+                        const float p = kp_tmem_ld1(tl + C::TM_S + (uint32_t)(gp & 1) * 64u + tok);
+                        const uint8_t *raw = sm_kp + C::RV_OFF + (gp % C::RV) * C::RAW + (tok >> a.l.lbs) * praw;
+                        const int line = tok & (a.l.bs - 1);
+                        const bool in = there(gp, j - 1, tok);
+#pragma unroll
+                        for (int w = 0; w < HH / 8; ++w) {
+                            const int at = (half * HH + 8 * w) / KV4_GROUP * a.l.bs + line;
+                            const float d = ka_half(raw + a.l.kb + at * 2), pd = in && fabsf(d) < INFINITY ? p * (d * up) : 0.0f;
+                            const uint32_t c = *(const uint32_t *)(raw + at * 32 + (half * HH / 8 + w) % 8 * 4);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                o[4 * w + x].x = fmaf((float)(int)(c >> (8 * x) & 15u) - 8.0f, pd, o[4 * w + x].x);
+                                o[4 * w + x].y = fmaf((float)(int)(c >> (8 * x + 4) & 15u) - 8.0f, pd, o[4 * w + x].y);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(&sh.rve[gp % C::RV]);
+                }
                 if (half == 0) {
                     if (j + 1 < kend) ok = make_k(g + 1, j + 1);
                 } else if (NB == 2 && j >= k && j < kend) {
@@ -806,12 +893,13 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
                     if (!ok) break;
                 }
                 const uint32_t to = tl + C::TM_O + (uint32_t)(half * HH);
-                if (adds) {  // o = o f + O 2^e
+                if (adds) {  // o = o f + O
                     const int gp = (g - 1) & 7;
-                    const float f = sh.f[gp & 3][row], e = sh.ev[gp];
-                    const float2 f2 = make_float2(f, f), e2 = make_float2(e, e);
+                    const float f = sh.f[gp & 3][row];
+                    const float2 f2 = make_float2(f, f);
                     uint32_t x[2][16];
                     tc_fence_after();
+                    if (!far)
 #pragma unroll
                     for (int c = 0; c < HH; c += 32) {
                         kp_tmem_ld16(to + c, x[0]);
@@ -822,12 +910,12 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(kp_pair(x[h], y), e2, __fmul2_rn(o[c / 2 + h * 8 + y], f2));
+                            for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(o[c / 2 + h * 8 + y], f2, kp_pair(x[h], y));
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) tc_arrive(&sh.oe);
-                    if (sh.any_bad[gp]) {
+                    if (FAR && sh.any_bad[gp]) {
                         const int left = lim - (j - 1) * KA_TOK;  // tokens of the tile that the row sees
                         const uint32_t m0 = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1u;
                         const uint32_t m1 = left <= 32 ? 0u : left >= 64 ? 0xffffffffu : (1u << (left - 32)) - 1u;
@@ -890,6 +978,7 @@ template <int HD, bool HL> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv
     // ---- everybody is here (the copies and MMAs of a CTA that gave up as well)
     tc_fence_before();
     __syncthreads();
+    if (!FAR && tid == 0) a.far[blockIdx.x] = sh.met;
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
 }
 
@@ -899,14 +988,17 @@ uint64_t kv4_prompt_workspace() {
 
 template <int HD, bool HL> static cudaError_t prompt_go(Kv4AttnArgs a, int max_new, cudaStream_t s) {
     using C = KpCfg<HD, HL>;
-    cudaError_t e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL>);
+    cudaError_t e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL, false>);
+    if (e == cudaSuccess) e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL, true>);
     if (e != cudaSuccess) return e;
     a.stride = C::PART;
     const long long rt = ((long long)std::min(max_new, a.rows) * a.group + KP_ROWS - 1) / KP_ROWS;
     const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
     const long long units = (long long)a.n * a.l.nkv * std::max(rt, 1ll) * tiles;
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms(), KA_MAX_GRID));
-    e = launch_k(k_kv4_prompt<HD, HL>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
+    // outputs over q or gate could not be made twice
+    if (!a.always) e = launch_k(k_kv4_prompt<HD, HL, false>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
+    if (e == cudaSuccess) e = launch_k(k_kv4_prompt<HD, HL, true>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
     if (e != cudaSuccess || grid == 1) return e;
     return launch_k(k_kv4_join<typename C::T, HD, KP_ROWS>, dim3(grid, KP_ROWS / 8), dim3(256), 0, s, a);
 }

@@ -118,6 +118,30 @@ def test_keys_of_sizes_beside_each_other(fn, kv4, ws, hd, spread, new, group, dt
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("hd, spread", [(64, 6.0), (128, 3.0), (256, 8.0)])
+def test_values_of_sizes_beside_each_other(fn, kv4, ws, hd, spread, new, group, dtype):
+    """Tokens, and 64-dim blocks, whose values differ by powers of ten: each block keeps its precision."""
+    rng = np.random.default_rng(4)
+    v = normal(rng, 200, 1, hd) * 10 ** rng.uniform(-spread / 2, spread / 2, (200, 1, 1))
+    v = np.clip((v.reshape(200, 1, -1, 64) * 10.0 ** rng.uniform(-2, 2, (1, 1, hd // 64, 1))).reshape(200, 1, hd), -5e5, 5e5)
+    Case(fn, kv4, ws, normal(rng, 200, 1, hd), v, normal(rng, new, group, hd), dtype=dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", [pytest.param(70, 2, id="prompt")])
+@pytest.mark.parametrize("base, factor", [(0.05, 1e6), (1e-3, 1e4), (1e-3, 1e6), (1e-3, 1e8)])
+def test_values_hidden_from_a_row_do_not_matter(fn, kv4, ws, base, factor, new, group, dtype):
+    """The last token's values (one block of them in the second case) are far larger; the rows before it do not see them."""
+    rng = np.random.default_rng(6)
+    for dims in (slice(0, 128), slice(64, 128)):
+        v = normal(rng, 128, 1, 128) * base
+        v[-1, 0, dims] *= factor
+        v = np.clip(v, -5e5, 5e5)  # scales within fp16
+        Case(fn, kv4, ws, normal(rng, 128, 1, 128), v, normal(rng, new, group, 128), dtype=dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("new, group", [pytest.param(5, 3, id="few"), pytest.param(70, 2, id="prompt")])
 @pytest.mark.parametrize("factor", [1e4, 1e6, 1e8])
 def test_keys_hidden_from_a_row_do_not_matter(fn, kv4, ws, factor, new, group, dtype):
@@ -126,3 +150,39 @@ def test_keys_hidden_from_a_row_do_not_matter(fn, kv4, ws, factor, new, group, d
     k[-1] = np.clip(k[-1] * factor, -5e5, 5e5)
     q = normal(rng, new, group, 128) * 1e3
     Case(fn, kv4, ws, k, normal(rng, 128, 1, 128), q, dtype=dtype).check(cap=1e3)
+
+
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("factor", [1e2, 1e5, 1e8])
+def test_large_values_of_no_weight(fn, kv4, ws, factor, new, group):
+    """A token that everyone sees, whose values are large and whose weight is nothing beside the others': the kernel for prompts keeps
+    the precision of what counts. The one for few rows is held to the largest value seen."""
+    rng = np.random.default_rng(8)
+    k, v = normal(rng, 128, 1, 128) * 0.1, normal(rng, 128, 1, 128) * 1e-3
+    q = np.abs(normal(rng, new, group, 128)) + 1
+    k[20], v[20] = -20.0, v[20] * factor  # scores of -200 and less
+    c = Case(fn, kv4, ws, k, v, q)
+    c.check()
+    if new >= 64:
+        got = c.run()
+        for i, h, want, _, S in c.rows():
+            # without that token the largest |v| is 5e-3 and S is at most a fortieth (keys of 0.5 beside its 20)
+            assert np.abs(got[i, h] - want).max() <= (2e-5 + 2.0 ** -19 * S / 40) * 5e-3
+
+
+def test_nan_and_infinite_values_beside_sizes(fn, kv4, ws):
+    """What is not finite reaches the rows that see it, whatever the sizes around it are."""
+    rng = np.random.default_rng(10)
+    for new, group in ((5, 3), (70, 2)):
+        k, v = normal(rng, 128, 1, 128), normal(rng, 128, 1, 128) * 10 ** rng.uniform(-4, 4, (128, 1, 1))
+        bad = 125
+        v[bad, 0, 70] = np.nan
+        c = Case(fn, kv4, ws, k, v, normal(rng, new, group, 128))
+        got = c.run()
+        sees = np.arange(128 - new, 128) >= bad
+        assert np.isnan(got[sees][..., 64:]).all() and np.isfinite(got[sees][..., :64]).all() and np.isfinite(got[~sees]).all()
+        # a key that is not finite: all of the rows that see it, none before
+        k[bad, 0, 3] = np.inf
+        c = Case(fn, kv4, ws, k, normal(rng, 128, 1, 128), normal(rng, new, group, 128))
+        got = c.run()
+        assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
