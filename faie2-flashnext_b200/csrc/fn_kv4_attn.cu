@@ -15,11 +15,12 @@
 // Precision. bf16 rows: q is exact in fp16 after scaling, p dv is rounded once to 11 bits (the output has 8). fp32 rows: q
 // and p dv are split into two fp16 numbers, 22 bits together, which costs a second instruction each. A tensor core drops
 // what lies some 24 bits below the nominal size of its largest term, and a code as a subnormal fp16 number lies up to 10
-// bits below its nominal size; so both first halves are whole numbers up to 2^11 (q scaled per row by a power of two, p dv by
-// the softmax's reference): all their products and sums are multiples of one unit, and exact. Floating halves lost 2.5e-6
+// bits below its nominal size; so both first halves are whole numbers up to 2^11 (q scaled per row by a power of two, p dv
+// by one per row and block): all their products and sums are multiples of one unit, and exact. Floating halves lost 2.5e-6
 // of the output where this form loses 3e-7. Sums over more than 32 tokens are added in fp32 outside the tensor core, whose
-// own accumulation cuts instead of rounding. The softmax runs in base 2 with one reference per row, the running maximum
-// plus the running exponent of the largest |dv|, so that p dv uses fp16's range whatever the size of V.
+// own accumulation cuts instead of rounding. The softmax runs in base 2 with the running
+// maximum of a row's scores as its reference; p dv is scaled by the exponent of the largest |dv| that the row has seen in the same 64
+// dims, so that it uses fp16's range whatever the size of V is, there, in other blocks, and in tokens that the row does not see.
 //
 // Work. A unit is 64 tokens of one kv head for one row tile (8 or 16 rows: the heads of a group, token after token). All
 // units of the call in a row are cut into equal runs, one per CTA, whatever request they belong to: each CTA finds its run
@@ -311,17 +312,18 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         int lim[NT][2];
         // o[n-tile][group][byte]: rows 2t, 2t + 1 of the tile for dim 8 g + 2 byte, then for the dim after it
         float o[NT][NG][4][4];
-        float2 corr[NT][NG], m[NT], l[NT], ref[NT];
-        int ev = -40;
+        // up: 2^(10 - e) of the largest |dv| that the row has seen in a group; -24 is the least e of an fp16 number
+        float2 corr[NT][NG], up[NT][NG], m[NT], l[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             lim[n][0] = limit(8 * n + 2 * t);
             lim[n][1] = limit(8 * n + 2 * t + 1);
-            m[n] = ref[n] = make_float2(-INFINITY, -INFINITY);
+            m[n] = make_float2(-INFINITY, -INFINITY);
             l[n] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
                 corr[n][gi] = make_float2(0.0f, 0.0f);
+                up[n][gi] = make_float2(17179869184.0f, 17179869184.0f);
 #pragma unroll
                 for (int by = 0; by < 4; ++by) o[n][gi][by][0] = o[n][gi][by][1] = o[n][gi][by][2] = o[n][gi][by][3] = 0.0f;
             }
@@ -391,21 +393,25 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                             sc[n][b][h] = __ffma2_rn(s, make_float2(d[b][h], d[b][h]), sc[n][b][h]);
                         }
             }
-            // ---- V scales of this lane's tokens, and the largest among the warp's
-            float dv[2][2][NG], dm = 0.0f;
+            // ---- V scales of this lane's tokens
+            float dv[2][2][NG];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bool drop = M && hidden(b, h, hi_lim);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) {
-                        const float d = ka_half(ks + a.l.sb + gi * sstep + b * scale2 + h * 16);
-                        dv[b][h][gi] = drop ? 0.0f : d;  // what nobody sees counts for nothing, whatever is there
-                        dm = fmaxf(dm, fabsf(dv[b][h][gi]));
-                    }
-                }
-            // ---- running softmax in base 2: p = exp2(s - reference), |p dv| < 2^11
+                    for (int gi = 0; gi < NG; ++gi) dv[b][h][gi] = ka_half(ks + a.l.sb + gi * sstep + b * scale2 + h * 16);
+            // the largest of a group that a row below `lm` sees (what it does not see counts for nothing, whatever is there)
+            auto largest = [&](int gi, int lm) {
+                float d = 0.0f;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (!M || !hidden(b, h, lm)) d = fmaxf(d, fabsf(dv[b][h][gi]));
+                return d;
+            };
+            // ---- running softmax in base 2: p = exp2(s - maximum), |p dv up| < 2^11
             float2 mx[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -427,38 +433,63 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
             }
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
-                dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mx[n].x = fmaxf(mx[n].x, __shfl_xor_sync(0xffffffffu, mx[n].x, x));
                     mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, x));
                 }
             }
-            ev = max(ev, (int)(__float_as_uint(dm) >> 23) - 127);
-            const float e = (float)(ev - 10);
             bool moved = false;
-            float2 z[NT];  // minus the reference (0 for a row that has seen nothing)
+            float2 z[NT];  // minus the maximum (0 for a row that has seen nothing)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                m[n] = mx[n];
-                const float2 nr = make_float2(mx[n].x + e, mx[n].y + e);
-                moved |= nr.x != ref[n].x || nr.y != ref[n].y;
-                z[n] = make_float2(nr.x == -INFINITY ? 0.0f : -nr.x, nr.y == -INFINITY ? 0.0f : -nr.y);
+                moved |= mx[n].x != m[n].x || mx[n].y != m[n].y;
+                z[n] = make_float2(mx[n].x == -INFINITY ? 0.0f : -mx[n].x, mx[n].y == -INFINITY ? 0.0f : -mx[n].y);
+            }
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+                if constexpr (M) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        moved |= largest(gi, lim[n][0]) * up[n][gi].x >= 2048.0f || largest(gi, lim[n][1]) * up[n][gi].y >= 2048.0f;
+                } else {
+                    float u = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) u = fmaxf(u, fmaxf(up[n][gi].x, up[n][gi].y));
+                    moved |= largest(gi, 0) * u >= 2048.0f;
+                }
             }
             if (__any_sync(0xffffffffu, moved)) {
+                auto over = [&](float d) {  // of the warp's tokens
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
+                    return fminf(d, 65504.0f);
+                };
+                // u where d fits it, else the power that d asks for
+                auto scaled = [](float u, float d) { return d * u < 2048.0f ? u : __uint_as_float(264u - (__float_as_uint(d) >> 23) << 23); };
+                auto ratio = [](float b, float a) { return b * __uint_as_float(0x7f000000u - __float_as_uint(a)); };  // powers of two
+                float2 f[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float2 f = make_float2(ka_exp2(ref[n].x + z[n].x), ka_exp2(ref[n].y + z[n].y));
-                    l[n] = __fmul2_rn(l[n], f);
-                    ref[n] = make_float2(m[n].x + e, m[n].y + e);
+                    f[n] = make_float2(ka_exp2(m[n].x + z[n].x), ka_exp2(m[n].y + z[n].y));
+                    l[n] = __fmul2_rn(l[n], f[n]);
+                    m[n] = mx[n];
+                }
 #pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) {
-                        corr[n][gi] = __fmul2_rn(corr[n][gi], f);
+                for (int gi = 0; gi < NG; ++gi) {
+                    [[maybe_unused]] const float all = M ? 0.0f : over(largest(gi, 0));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 d = M ? make_float2(over(largest(gi, lim[n][0])), over(largest(gi, lim[n][1]))) : make_float2(all, all);
+                        const float2 u = make_float2(scaled(up[n][gi].x, d.x), scaled(up[n][gi].y, d.y));
+                        const float2 fg = __fmul2_rn(f[n], make_float2(ratio(u.x, up[n][gi].x), ratio(u.y, up[n][gi].y)));
+                        up[n][gi] = u;
+                        corr[n][gi] = __fmul2_rn(corr[n][gi], fg);
 #pragma unroll
                         for (int by = 0; by < 4; ++by)
 #pragma unroll
                             for (int x = 0; x < 4; x += 2) {
-                                const float2 y = __fmul2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), f);
+                                const float2 y = __fmul2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), fg);
                                 o[n][gi][by][x] = y.x, o[n][gi][by][x + 1] = y.y;
                             }
                     }
@@ -487,7 +518,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float d = dv[b][h][gi];
-                            float2 x = __fmul2_rn(sc[n][b][h], make_float2(d, d));
+                            float2 x = __fmul2_rn(sc[n][b][h], __fmul2_rn(make_float2(d, d), up[n][gi]));
                             // a token that a row does not see weighs nothing whatever its scale is (NaN)
                             if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
                             corr[n][gi] = __fadd2_rn(corr[n][gi], x);
@@ -575,7 +606,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         if (g == 0) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                s_ref[warp][8 * n + 2 * t] = ref[n].x, s_ref[warp][8 * n + 2 * t + 1] = ref[n].y;
+                s_ref[warp][8 * n + 2 * t] = m[n].x, s_ref[warp][8 * n + 2 * t + 1] = m[n].y;
                 s_l[warp][8 * n + 2 * t] = l[n].x, s_l[warp][8 * n + 2 * t + 1] = l[n].y;
             }
         }
@@ -584,7 +615,14 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         float2 wf[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-            wf[n] = make_float2(ka_weight(ref[n].x, top(8 * n + 2 * t)), ka_weight(ref[n].y, top(8 * n + 2 * t + 1)));
+            wf[n] = make_float2(ka_weight(m[n].x, top(8 * n + 2 * t)), ka_weight(m[n].y, top(8 * n + 2 * t + 1)));
+        // the sums' own scales (2^-24 and 2^-20 of the codes are taken back below)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi)
+                up[n][gi] = make_float2(wf[n].x * __uint_as_float(0x7f000000u - __float_as_uint(up[n][gi].x)),
+                                        wf[n].y * __uint_as_float(0x7f000000u - __float_as_uint(up[n][gi].y)));
         if (tid < ROWS) {
             const float tt = top(tid);
             float sum = 0.0f;
@@ -610,7 +648,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                 for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        *at(n, gi, x) = old[n][gi][x] + (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * (x & 1 ? corr[n][gi].y : corr[n][gi].x)) * (x & 1 ? wf[n].y : wf[n].x);
+                        *at(n, gi, x) = old[n][gi][x] + (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * (x & 1 ? corr[n][gi].y : corr[n][gi].x)) * (x & 1 ? up[n][gi].y : up[n][gi].x);
         };
         for (int round = 0; round < 4; ++round) {
             const int q = (warp + round) & 3;

@@ -129,7 +129,20 @@ def test_values_of_sizes_beside_each_other(fn, kv4, ws, hd, spread, new, group, 
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("new, group", [pytest.param(70, 2, id="prompt")])
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("block", [1e-1, 1e-2, 1e-3, 1e-4])
+def test_blocks_of_small_values_beside_large_ones(fn, kv4, ws, block, new, group, dtype):
+    """One 64-dim block of every token is smaller: its outputs are right to their own size. Few tokens, whose errors do not average out,
+    and small scores, whose errors would cover it."""
+    rng = np.random.default_rng(5)
+    for length in (new + 2, new + 100):
+        v = normal(rng, length, 1, 256)
+        v[..., 64:128] *= block
+        Case(fn, kv4, ws, normal(rng, length, 1, 256), v, normal(rng, new, group, 256) * 0.05, dtype=dtype).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", [pytest.param(5, 3, id="few"), pytest.param(70, 2, id="prompt")])
 @pytest.mark.parametrize("base, factor", [(0.05, 1e6), (1e-3, 1e4), (1e-3, 1e6), (1e-3, 1e8)])
 def test_values_hidden_from_a_row_do_not_matter(fn, kv4, ws, base, factor, new, group, dtype):
     """The last token's values (one block of them in the second case) are far larger; the rows before it do not see them."""
