@@ -520,7 +520,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                             const float d = dv[b][h][gi];
                             float2 x = __fmul2_rn(sc[n][b][h], __fmul2_rn(make_float2(d, d), up[n][gi]));
                             // a token that a row does not see weighs nothing whatever its scale is (NaN)
-                            if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
+                            if constexpr (M) x = make_float2(hidden(b, h, lim[n][0]) ? 0.0f : x.x, hidden(b, h, lim[n][1]) ? 0.0f : x.y);
                             corr[n][gi] = __fadd2_rn(corr[n][gi], x);
                             if constexpr (HL) {
                                 const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: rounds to whole numbers

@@ -199,3 +199,16 @@ def test_nan_and_infinite_values_beside_sizes(fn, kv4, ws):
         c = Case(fn, kv4, ws, k, normal(rng, 128, 1, 128), normal(rng, new, group, 128))
         got = c.run()
         assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+
+
+@pytest.mark.parametrize("lead", [100.0, 300.0])
+def test_a_nan_value_of_no_weight_is_seen(fn, kv4, ws, lead):
+    """0 x NaN is NaN, in a tile that some rows see a part of as in one that all see: both kernels agree."""
+    rng = np.random.default_rng(11)
+    for new, group, length in ((1, 4, 20), (1, 4, 64), (3, 4, 60), (70, 2, 100), (70, 2, 128)):
+        k, v = normal(rng, length, 1, 64) * 1e-3, normal(rng, length, 1, 64)
+        q = np.ones((new, group, 64))
+        k[5], v[5, 0, 9] = -lead / 8, np.nan  # scale sum q k = 64 k / 8
+        got = Case(fn, kv4, ws, k, v, q).run()
+        sees = np.arange(length - new, length) >= 5
+        assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all(), (new, length)
