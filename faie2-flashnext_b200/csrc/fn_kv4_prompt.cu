@@ -21,7 +21,7 @@
 // a tile adds to the row, and tiles that add little cost the others no bits, whatever their values' size. The sum of weights takes
 // 2^(11 - e) back. In a tile whose V scales lie more than 2^12 apart (one huge value, or block of it, beside small ones) no e serves
 // all: its weights stay fp32, and the workers add p v on the CUDA cores instead of the tensor core's O (some 15 times as slow).
-// Such tiles, and what is not finite, have a kernel of their own (FAR), the same with the code for them: with that code in it every
+// Such tiles, what is not finite, and rows of scores past 2^20 have a kernel of their own (FAR), the same with the code for them: with that code in it every
 // call would pay (the roles' loops share the instruction cache: 8 bf16 prompts 963 us beside 744). The first kernel notes whether it
 // met any; the second, launched behind it, returns at once or does the call again.
 // Rows of q are scaled by a power of two.
@@ -555,6 +555,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
             const int lim = limit(row);
             // the reference, as the score and the exponent that it came of: a large score would swallow the exponent
             float sref = -INFINITY, eref = 0.0f, l = 0.0f, rs = 0.0f;
+            [[maybe_unused]] bool met = false;
             for (int j = k; j < kend; ++j, ++gt) {
                 const int b = gt & 1;
                 ok = wt(&sh.sf[b], gt >> 1);
@@ -611,7 +612,12 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 const float fac = sref == -INFINITY ? 0.0f : ka_exp2((sref - ns) + (eref - ne));
                 sref = ns, eref = ne;
                 // P = 2^10 exp2(s + e - reference): fp16 keeps 11 bits down to 2^-24 of the largest
-                const float z = ns == -INFINITY ? 0.0f : (10.0f + ev - ne) - ns;
+                // Beside a reference of 2^20 and more the 10 would be rounded, and at 2^27 a weight could pass fp16: the long way takes
+                // the exact difference to the best score first.
+                const float z0 = ns == -INFINITY ? 0.0f : -ns, z1 = 10.0f + ev - ne, z = z0 + z1;
+                // (one at a time: the packed product and sum would become one, and the rounding of the best score differ)
+                [[maybe_unused]] auto apart = [&](uint32_t x) { return __fadd_rn(__fadd_rn(__fmul_rn(__uint_as_float(x), rsj), z0), z1); };
+                if constexpr (!FAR) met |= fabsf(ns) > 1048576.0f && ns != -INFINITY;
                 sh.f[gt & 3][row] = fac;
                 const float2 rs2 = make_float2(rsj, rsj), z2 = make_float2(z, z);
                 float2 ls = make_float2(0.0f, 0.0f);
@@ -625,7 +631,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                         hide(s, c);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float p = ka_exp2(fmaf(__uint_as_float(s[i]), rsj, z));
+                            const float p = ka_exp2(apart(s[i]));
                             ls.x += p;
                             s[i] = __float_as_uint(p);
                         }
@@ -641,7 +647,10 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     hide(s, c);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float2 x = __ffma2_rn(kp_pair(s, i), rs2, z2), p = make_float2(ka_exp2(x.x), ka_exp2(x.y));
+                        float2 x;
+                        if constexpr (FAR) x = make_float2(apart(s[2 * i]), apart(s[2 * i + 1]));
+                        else x = __ffma2_rn(kp_pair(s, i), rs2, z2);
+                        const float2 p = make_float2(ka_exp2(x.x), ka_exp2(x.y));
                         ls = __fadd2_rn(ls, p);
                         p16[i] = ka_pack(p.x, p.y);
                         if constexpr (HL) {
@@ -660,6 +669,8 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 if (lane == 0) tc_arrive(&sh.pf[b]);
             }
             if (!ok) break;
+            if constexpr (!FAR)
+                if (met) sh.met = 1;
             if (k == 0 && kend == tiles) {
                 sh.l[row] = l;
             } else {

@@ -183,6 +183,24 @@ def test_large_values_of_no_weight(fn, kv4, ws, factor, new, group):
             assert np.abs(got[i, h] - want).max() <= (2e-5 + 2.0 ** -19 * S / 40) * 5e-3
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", FORMS)
+@pytest.mark.parametrize("qsize", [1e5, 1e7, 3e7, 1e8, 1e9, 1e12])
+def test_scores_of_any_size(fn, kv4, ws, qsize, new, group, dtype):
+    """Scores of up to 1e13: the row is its best key's value where that key's lead passes the scores' rounding (2^-18 S)."""
+    rng = np.random.default_rng(9)
+    c = Case(fn, kv4, ws, normal(rng, 150, 1, 64), normal(rng, 150, 1, 64), normal(rng, new, group, 64) * qsize, dtype=dtype)
+    got, q, led = c.run(), c.q.double().cpu().numpy(), 0
+    assert np.isfinite(got).all()
+    for i, h, want, V, S in c.rows():
+        s = np.sort(c.k[:c.length - new + i + 1, 0] @ q[i, h] / 8)
+        if s[-1] - s[-2] > (2.0 ** -18 if dtype == "f32" else 2.0 ** -10) * S + 60:
+            led += 1
+            tol = (2e-5 if dtype == "f32" else 2.0 ** -8) * V[0]
+            assert np.abs(got[i, h] - want).max() <= tol, (i, h)
+    assert led > 0
+
+
 def test_nan_and_infinite_values_beside_sizes(fn, kv4, ws):
     """What is not finite reaches the rows that see it, whatever the sizes around it are."""
     rng = np.random.default_rng(10)
