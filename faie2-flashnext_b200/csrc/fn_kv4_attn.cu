@@ -105,6 +105,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
     __shared__ float s_ref[KA_CONS][ROWS], s_l[KA_CONS][ROWS], s_mref[ROWS], s_ml[ROWS];
     __shared__ uint32_t s_valid[S];
     uint64_t *full = (uint64_t *)sm_ka, *empty = full + S;
+    uint8_t *s_up = sm_ka + 512;  // [warp][group][row]
+    static_assert(2 * S * 8 <= 512 && KA_CONS * NG * ROWS <= 512);
     QF *qf = (QF *)(sm_ka + C::Q_OFF);
     float *ob = (float *)(sm_ka + C::Q_OFF);
     uint8_t *ring = sm_ka + C::ST_OFF;
@@ -312,8 +314,19 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
         int lim[NT][2];
         // o[n-tile][group][byte]: rows 2t, 2t + 1 of the tile for dim 8 g + 2 byte, then for the dim after it
         float o[NT][NG][4][4];
-        // up: 2^(10 - e) of the largest |dv| that the row has seen in a group; -24 is the least e of an fp16 number
-        float2 corr[NT][NG], up[NT][NG], m[NT], l[NT];
+        float2 corr[NT][NG], m[NT], l[NT];
+        // p dv is scaled by ug = 2^(10 - e) of the largest |dv| that the row has seen in a group, the same for all rows until the tiles that
+        // some see a part of; from there on (own) each row's is in s_up, by its exponent. -24 is the least e of an fp16 number.
+        float ug[NG];
+        bool own = false;
+        auto inverse = [](float a) { return __uint_as_float(0x7f000000u - __float_as_uint(a)); };  // of a power of two
+        auto row_up = [&](int n, int gi) {
+            if (!own) return make_float2(ug[gi], ug[gi]);
+            const uint8_t *e = s_up + (warp * NG + gi) * ROWS + 8 * n + 2 * t;
+            return make_float2(__uint_as_float((uint32_t)e[0] << 23), __uint_as_float((uint32_t)e[1] << 23));
+        };
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) ug[gi] = 17179869184.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             lim[n][0] = limit(8 * n + 2 * t);
@@ -323,7 +336,6 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
                 corr[n][gi] = make_float2(0.0f, 0.0f);
-                up[n][gi] = make_float2(17179869184.0f, 17179869184.0f);
 #pragma unroll
                 for (int by = 0; by < 4; ++by) o[n][gi][by][0] = o[n][gi][by][1] = o[n][gi][by][2] = o[n][gi][by][3] = 0.0f;
             }
@@ -439,61 +451,97 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                     mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, x));
                 }
             }
-            bool moved = false;
+            [[maybe_unused]] float2 up[M ? NT : 1][M ? NG : 1];
+            if constexpr (M) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) up[n][gi] = row_up(n, gi);
+            }
+            bool moved = false, grown = false;
             float2 z[NT];  // minus the maximum (0 for a row that has seen nothing)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 moved |= mx[n].x != m[n].x || mx[n].y != m[n].y;
                 z[n] = make_float2(mx[n].x == -INFINITY ? 0.0f : -mx[n].x, mx[n].y == -INFINITY ? 0.0f : -mx[n].y);
             }
+            if constexpr (M) {
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-                if constexpr (M) {
+                for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        moved |= largest(gi, lim[n][0]) * up[n][gi].x >= 2048.0f || largest(gi, lim[n][1]) * up[n][gi].y >= 2048.0f;
-                } else {
-                    float u = 0.0f;
+                    for (int n = 0; n < NT; ++n) grown |= largest(gi, hi_lim) * fmaxf(up[n][gi].x, up[n][gi].y) >= 2048.0f;
+            } else {
+                float d = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) u = fmaxf(u, fmaxf(up[n][gi].x, up[n][gi].y));
-                    moved |= largest(gi, 0) * u >= 2048.0f;
-                }
+                for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            dv[b][h][gi] *= ug[gi];
+                            d = fmaxf(d, fabsf(dv[b][h][gi]));
+                        }
+                grown = d >= 2048.0f;
             }
-            if (__any_sync(0xffffffffu, moved)) {
-                auto over = [&](float d) {  // of the warp's tokens
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
-                    return fminf(d, 65504.0f);
-                };
-                // u where d fits it, else the power that d asks for
-                auto scaled = [](float u, float d) { return d * u < 2048.0f ? u : __uint_as_float(264u - (__float_as_uint(d) >> 23) << 23); };
-                auto ratio = [](float b, float a) { return b * __uint_as_float(0x7f000000u - __float_as_uint(a)); };  // powers of two
-                float2 f[NT];
+            // (what is rare is short too: the code of a step that runs once is fetched for it, and a part has some seven steps a warp)
+            if (__any_sync(0xffffffffu, moved | grown)) {
+                float2 f[NT][NG];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    f[n] = make_float2(ka_exp2(m[n].x + z[n].x), ka_exp2(m[n].y + z[n].y));
-                    l[n] = __fmul2_rn(l[n], f[n]);
+                    const float2 fm = make_float2(ka_exp2(m[n].x + z[n].x), ka_exp2(m[n].y + z[n].y));
+                    l[n] = __fmul2_rn(l[n], fm);
                     m[n] = mx[n];
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) f[n][gi] = fm;
+                }
+                if (__any_sync(0xffffffffu, grown)) {
+                    // u where d fits it, else the power that d asks for
+                    auto scaled = [](float u, float d) { return d * u < 2048.0f ? u : __uint_as_float(264u - (__float_as_uint(d) >> 23) << 23); };
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi) {
+                        if constexpr (M) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                auto over = [&](float d) {  // of the warp's tokens
+#pragma unroll
+                                    for (int x = 4; x < 32; x <<= 1) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
+                                    return fminf(d, 65504.0f);
+                                };
+                                const float2 u = make_float2(scaled(up[n][gi].x, over(largest(gi, lim[n][0]))), scaled(up[n][gi].y, over(largest(gi, lim[n][1]))));
+                                f[n][gi] = __fmul2_rn(f[n][gi], make_float2(u.x * inverse(up[n][gi].x), u.y * inverse(up[n][gi].y)));
+                                up[n][gi] = u;
+                                uint8_t *e = s_up + (warp * NG + gi) * ROWS + 8 * n + 2 * t;
+                                e[0] = (uint8_t)(__float_as_uint(u.x) >> 23), e[1] = (uint8_t)(__float_as_uint(u.y) >> 23);
+                            }
+                            ug[gi] = up[NT - 1][gi].y;  // (all rows' where whole pages are missing, and whole tiles come after it)
+                        } else {  // the same tokens, and factors, in all rows
+                            const float d = fminf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest(gi, 0)))), 65504.0f * ug[gi]);
+                            const float r = scaled(1.0f, d);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) f[n][gi] = __fmul2_rn(f[n][gi], make_float2(r, r));
+                            ug[gi] *= r;
+#pragma unroll
+                            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) dv[b][h][gi] *= r;
+                        }
+                    }
+                    own = M;
+                    __syncwarp();
                 }
 #pragma unroll
-                for (int gi = 0; gi < NG; ++gi) {
-                    [[maybe_unused]] const float all = M ? 0.0f : over(largest(gi, 0));
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float2 d = M ? make_float2(over(largest(gi, lim[n][0])), over(largest(gi, lim[n][1]))) : make_float2(all, all);
-                        const float2 u = make_float2(scaled(up[n][gi].x, d.x), scaled(up[n][gi].y, d.y));
-                        const float2 fg = __fmul2_rn(f[n], make_float2(ratio(u.x, up[n][gi].x), ratio(u.y, up[n][gi].y)));
-                        up[n][gi] = u;
-                        corr[n][gi] = __fmul2_rn(corr[n][gi], fg);
+                    for (int gi = 0; gi < NG; ++gi) {
+                        corr[n][gi] = __fmul2_rn(corr[n][gi], f[n][gi]);
 #pragma unroll
                         for (int by = 0; by < 4; ++by)
 #pragma unroll
                             for (int x = 0; x < 4; x += 2) {
-                                const float2 y = __fmul2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), fg);
+                                const float2 y = __fmul2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), f[n][gi]);
                                 o[n][gi][by][x] = y.x, o[n][gi][by][x + 1] = y.y;
                             }
                     }
-                }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -505,6 +553,30 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                         sc[n][b][h] = make_float2(ka_exp2(x.x), ka_exp2(x.y));
                         l[n] = __fadd2_rn(l[n], sc[n][b][h]);
                     }
+            if constexpr (M) {
+                // (below, what weighs nothing counts for nothing, hidden NaN scales among it; a NaN that a row sees counts)
+                bool odd = false;
+#pragma unroll
+                for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) odd |= !(fabsf(dv[b][h][gi]) < INFINITY) && !hidden(b, h, hi_lim);
+                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                    for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const float none = dv[b][h][gi] * 0.0f;
+                                    if (!hidden(b, h, lim[n][0])) corr[n][gi].x += none;
+                                    if (!hidden(b, h, lim[n][1])) corr[n][gi].y += none;
+                                }
+                }
+            }
             // ---- out += c (p dv)
             const uint8_t *vp0 = rec + a.l.kb + (pl + tv0) * 32 + g * 4, *vp1 = vp0 + (tv1 - tv0) * 32;
 #pragma unroll
@@ -512,16 +584,19 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                 uint32_t P[NT][2][2];  // B operands: tokens 2t, 2t + 1 (+ 8) of row g
                 [[maybe_unused]] uint32_t Q[NT][2][2];  // their second halves
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    float2 add[2][2];
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float d = dv[b][h][gi];
-                            float2 x = __fmul2_rn(sc[n][b][h], __fmul2_rn(make_float2(d, d), up[n][gi]));
+                            float2 x = make_float2(d, d);
+                            if constexpr (M) x = __fmul2_rn(x, up[n][gi]);
+                            x = __fmul2_rn(sc[n][b][h], x);
                             // a token that a row does not see weighs nothing whatever its scale is (NaN)
-                            if constexpr (M) x = make_float2(hidden(b, h, lim[n][0]) ? 0.0f : x.x, hidden(b, h, lim[n][1]) ? 0.0f : x.y);
-                            corr[n][gi] = __fadd2_rn(corr[n][gi], x);
+                            if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
+                            add[b][h] = x;
                             if constexpr (HL) {
                                 const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: rounds to whole numbers
                                 const float2 w = __fadd2_rn(__fadd2_rn(x, big), make_float2(-12582912.0f, -12582912.0f));
@@ -532,6 +607,8 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                                 P[n][b][h] = ka_turn(ka_pack(x.x, x.y));
                             }
                         }
+                    corr[n][gi] = __fadd2_rn(corr[n][gi], __fadd2_rn(__fadd2_rn(add[0][0], add[0][1]), __fadd2_rn(add[1][0], add[1][1])));
+                }
                 uint4 A[4][2];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -616,13 +693,15 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
 #pragma unroll
         for (int n = 0; n < NT; ++n)
             wf[n] = make_float2(ka_weight(m[n].x, top(8 * n + 2 * t)), ka_weight(m[n].y, top(8 * n + 2 * t + 1)));
-        // the sums' own scales (2^-24 and 2^-20 of the codes are taken back below)
+        // with the sums' own scales (2^-24 and 2^-20 of the codes are taken back below)
+        float2 back[NT][NG];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi)
-                up[n][gi] = make_float2(wf[n].x * __uint_as_float(0x7f000000u - __float_as_uint(up[n][gi].x)),
-                                        wf[n].y * __uint_as_float(0x7f000000u - __float_as_uint(up[n][gi].y)));
+            for (int gi = 0; gi < NG; ++gi) {
+                const float2 u = row_up(n, gi);
+                back[n][gi] = make_float2(wf[n].x * inverse(u.x), wf[n].y * inverse(u.y));
+            }
         if (tid < ROWS) {
             const float tt = top(tid);
             float sum = 0.0f;
@@ -648,7 +727,7 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                 for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        *at(n, gi, x) = old[n][gi][x] + (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * (x & 1 ? corr[n][gi].y : corr[n][gi].x)) * (x & 1 ? up[n][gi].y : up[n][gi].x);
+                        *at(n, gi, x) = old[n][gi][x] + (o[n][gi][by][x] * (x >= 2 ? 1048576.0f : 16777216.0f) - 8.0f * (x & 1 ? corr[n][gi].y : corr[n][gi].x)) * (x & 1 ? back[n][gi].y : back[n][gi].x);
         };
         for (int round = 0; round < 4; ++round) {
             const int q = (warp + round) & 3;
