@@ -18,7 +18,7 @@
 // bits below its nominal size; so both first halves are whole numbers up to 2^11 (q scaled per row by a power of two, p dv
 // by one per row and block): all their products and sums are multiples of one unit, and exact. Floating halves lost 2.5e-6
 // of the output where this form loses 3e-7. Sums over more than 32 tokens are added in fp32 outside the tensor core, whose
-// own accumulation cuts instead of rounding. The softmax runs in base 2 with the running
+// own accumulation cuts instead of rounding (bf16 rows: where a CTA has many tokens of a row, KA_LONG). The softmax runs in base 2 with the running
 // maximum of a row's scores as its reference; p dv is scaled by the exponent of the largest |dv| that the row has seen in the same 64
 // dims, so that it uses fp16's range whatever the size of V is, there, in other blocks, and in tokens that the row does not see.
 //
@@ -41,6 +41,10 @@
 namespace fn {
 
 constexpr int KA_CONS = 4;                    // computing warps
+// 64-token tiles that a CTA may have of one row from which bf16 rows take the LONG form. The tensor core's accumulation cuts: t tiles lose
+// up to t 2^-24 of the sum of |c p dv|, which may be twice the output and more; 2^21 tokens (32768 tiles) lost 0.6 % of it on average, so
+// 512 lose 1e-4, beside 2e-3 of the output's own rounding. The LONG form costs 3 to 4 % of the time.
+constexpr int KA_LONG = 512;
 // registers of the wide form: 256 threads x 128 at launch; the copying warpgroup gives up what the computing one takes
 // (40 + 216 = 2 x 128)
 constexpr int KA_REG_COPY = 40, KA_REG_COMP = 216;
@@ -90,7 +94,8 @@ template <int HD, bool HL, int NT> struct KaCfg {
 };
 constexpr int KA_PART_MAX = 16 * 256 + 32;
 
-template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, HL, NT>::THREADS, KaCfg<HD, HL, NT>::CTAS)
+// LONG: bf16 rows' sums leave the tensor core after every 32 tokens, as fp32 rows' always do
+template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(KaCfg<HD, HL, NT>::THREADS, KaCfg<HD, HL, NT>::CTAS)
     k_kv4_attn(const __grid_constant__ Kv4AttnArgs a) {
     using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
@@ -596,15 +601,18 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                             x = __fmul2_rn(sc[n][b][h], x);
                             // a token that a row does not see weighs nothing whatever its scale is (NaN)
                             if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
-                            add[b][h] = x;
                             if constexpr (HL) {
+                                add[b][h] = x;
                                 const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: rounds to whole numbers
                                 const float2 w = __fadd2_rn(__fadd2_rn(x, big), make_float2(-12582912.0f, -12582912.0f));
                                 const float2 r = __ffma2_rn(w, make_float2(-1.0f, -1.0f), x);
                                 P[n][b][h] = ka_turn(ka_pack(w.x, w.y));
                                 Q[n][b][h] = ka_turn(ka_pack(r.x, r.y));
                             } else {
-                                P[n][b][h] = ka_turn(ka_pack(x.x, x.y));
+                                // (of the rounded weights, so that the 8 of a code cancels and their rounding counts c - 8 times, not c)
+                                const uint32_t w = ka_pack(x.x, x.y);
+                                add[b][h] = ka_unpack(w);
+                                P[n][b][h] = ka_turn(w);
                             }
                         }
                     corr[n][gi] = __fadd2_rn(corr[n][gi], __fadd2_rn(__fadd2_rn(add[0][0], add[0][1]), __fadd2_rn(add[1][0], add[1][1])));
@@ -624,16 +632,18 @@ template <int HD, bool HL, int NT> __global__ void __launch_bounds__(KaCfg<HD, H
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    if constexpr (HL) {
+                    if constexpr (HL || LONG) {
                         float acc[4][4] = {};
 #pragma unroll
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
                             for (int by = 0; by < 4; ++by) ka_mma(acc[by], A[by][b], P[n][b][0], P[n][b][1]);
+                        if constexpr (HL) {
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
+                            for (int b = 0; b < 2; ++b)
 #pragma unroll
-                            for (int by = 0; by < 4; ++by) ka_mma(acc[by], A[by][b], Q[n][b][0], Q[n][b][1]);
+                                for (int by = 0; by < 4; ++by) ka_mma(acc[by], A[by][b], Q[n][b][0], Q[n][b][1]);
+                        }
 #pragma unroll
                         for (int by = 0; by < 4; ++by)
 #pragma unroll
@@ -771,12 +781,16 @@ FN_API uint64_t fn_kv4_attn_workspace(void) {
 }
 
 template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
-    cudaError_t e = allow_max_dynamic_smem(k_kv4_attn<HD, HL, NT>);
-    if (e != cudaSuccess) return e;
     // no more CTAs than pairs of units there can be
     const long long units = items * tiles;
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KaCfg<HD, HL, NT>::CTAS, KA_MAX_GRID));
-    e = launch_k(k_kv4_attn<HD, HL, NT>, dim3(grid), dim3(KaCfg<HD, HL, NT>::THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+    cudaError_t e;
+    auto go = [&](auto kernel) {
+        e = allow_max_dynamic_smem(kernel);
+        if (e == cudaSuccess) e = launch_k(kernel, dim3(grid), dim3(KaCfg<HD, HL, NT>::THREADS), KaCfg<HD, HL, NT>::SMEM, s, a);
+    };
+    if (!HL && std::min(tiles, units / grid) > KA_LONG) go(k_kv4_attn<HD, HL, NT, !HL>);
+    else go(k_kv4_attn<HD, HL, NT, false>);
     // one request of at most two tiles: its row tiles weigh the same, 2 + KA_EXTRA units at most, which is the shortest run, so
     // none is split
     if (e != cudaSuccess || (a.n == 1 && tiles <= 2 && grid == units / 2)) return e;

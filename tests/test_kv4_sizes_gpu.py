@@ -230,3 +230,27 @@ def test_a_nan_value_of_no_weight_is_seen(fn, kv4, ws, lead):
         got = Case(fn, kv4, ws, k, v, q).run()
         sees = np.arange(length - new, length) >= 5
         assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all(), (new, length)
+
+
+def test_long_sums_of_one_sign_keep_bf16_rows(fn, kv4, ws):
+    """Flat rows over two million tokens, one request to a CTA, all products of one sign: a sum that were cut at every step would
+    end low by 1e-3 and more. Averaged over 512 outputs, whose own rounding (2^-9 at most, spread) then counts 2^-9 / sqrt(512),
+    twice that allowed; the weights' common rounding to 11 bits is 2^-12."""
+    tokens, bs, hd, n = 1 << 21, 64, 64, 444
+    c = kv4.KV4Cache(fn, 1, hd, bs, tokens // bs, ws)
+    g = torch.Generator("cuda").manual_seed(3)
+    v = -0.55 - 0.4 * torch.arange(hd, device="cuda") / hd + 0.1 * torch.rand(tokens, 1, hd, device="cuda", generator=g)
+    v[..., 17] = 1.1  # the value of largest magnitude: the others' codes are 11 to 15 of 15
+    k = torch.zeros(tokens, 1, hd, device="cuda")
+    slots = torch.arange(tokens, device="cuda")
+    c.store(k, v, slots)
+    table = torch.arange(tokens // bs, dtype=torch.int32, device="cuda")[None].expand(n, -1).contiguous()
+    q = torch.randn(n, 8, hd, device="cuda", generator=g).bfloat16()
+    out = c.attn(q, torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.full((n,), tokens, dtype=torch.int32, device="cuda"),
+                 table, 1).double()
+    fn.sync(torch.cuda.current_stream().cuda_stream)
+    want = c.load(slots)[1].double().mean((0, 1))
+    rel = (out / want - 1)[..., torch.arange(hd) != 17]
+    # every request has the same answer; its 8 x 63 outputs round alike, so the dims are what is averaged over
+    tol = 2.0 ** -12 + 2 * 2.0 ** -9 / 63 ** 0.5
+    assert float(rel.mean((1, 2)).abs().max()) <= tol, rel.mean()
