@@ -780,7 +780,7 @@ FN_API uint64_t fn_kv4_attn_workspace(void) {
     return KA_HEAD + std::max(few, kv4_prompt_workspace());
 }
 
-template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, long long items, long long tiles, cudaStream_t s) {
+template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnArgs &a, int max_new, long long items, long long tiles, cudaStream_t s) {
     // no more CTAs than pairs of units there can be
     const long long units = items * tiles;
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms() * KaCfg<HD, HL, NT>::CTAS, KA_MAX_GRID));
@@ -792,8 +792,8 @@ template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnA
     if (!HL && std::min(tiles, units / grid) > KA_LONG) go(k_kv4_attn<HD, HL, NT, !HL>);
     else go(k_kv4_attn<HD, HL, NT, false>);
     // one request of at most two tiles: its row tiles weigh the same, 2 + KA_EXTRA units at most, which is the shortest run, so
-    // none is split
-    if (e != cudaSuccess || (a.n == 1 && tiles <= 2 && grid == units / 2)) return e;
+    // none is split (if there are no more of them than max_new says: a caller's bound is not trusted here)
+    if (e != cudaSuccess || (a.n == 1 && max_new >= a.rows && tiles <= 2 && grid == units / 2)) return e;
     using C = KaCfg<HD, HL, NT>;
     using T = typename C::T;
     // few row tiles may have many parts, many have few
@@ -811,8 +811,8 @@ template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int
     // the most row tiles, and units of one, that there can be
     const long long tiles = ((long long)a.max_pages * a.l.bs + KA_TOK - 1) / KA_TOK;
     const long long items = (long long)a.n * a.l.nkv * std::max((rows + 8 * nt - 1) / (8 * nt), 1ll);
-    if (nt == 1) return f32 ? attn_launch<HD, true, 1>(a, items, tiles, s) : attn_launch<HD, false, 1>(a, items, tiles, s);
-    return f32 ? attn_launch<HD, true, 2>(a, items, tiles, s) : attn_launch<HD, false, 2>(a, items, tiles, s);
+    if (nt == 1) return f32 ? attn_launch<HD, true, 1>(a, max_new, items, tiles, s) : attn_launch<HD, false, 1>(a, max_new, items, tiles, s);
+    return f32 ? attn_launch<HD, true, 2>(a, max_new, items, tiles, s) : attn_launch<HD, false, 2>(a, max_new, items, tiles, s);
 }
 
 FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const void *q, int64_t q_token,
