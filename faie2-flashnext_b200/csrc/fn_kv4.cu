@@ -20,6 +20,7 @@ struct PlanArgs {
     const int *free_in;
     int *free_out, *cu, *kv_len, *positions, *requests, *status;
     int64_t *slots;
+    int *next;      // the lengths that requests go on with (may be null)
     int rows_here;  // 1: this kernel writes the rows; 0: k_kv4_rows does
 };
 
@@ -130,6 +131,7 @@ template <int T> __global__ void __launch_bounds__(T) k_kv4_plan(const PlanArgs 
         const int l = add[k] < 0 || !ok ? 0 : (int)min(ctx[k] + fresh[k], (long long)INT32_MAX);
         len[r] = l;
         a.kv_len[r] = l;
+        if (a.next) a.next[r] = ok ? l : (int)ctx[k];  // a refused request stands where it stood
     }
     if (taken) atomicMax(&s_taken, taken);
     if (refused) atomicAdd(&s_refused, refused);
@@ -355,6 +357,13 @@ using namespace fn;
 FN_API int fn_kv4_plan(int n, const int *ctx, const int *add, int *table, int max_pages, int page_size, int *free_ids,
                        int n_pages, const int *free_in, int *free_out, int max_tokens, int *cu, int *kv_len,
                        int64_t *slots, int *positions, int *requests, int *status, void *stream) {
+    return fn_kv4_plan_next(n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out, max_tokens, cu, kv_len, slots,
+                            positions, requests, status, nullptr, stream);
+}
+
+FN_API int fn_kv4_plan_next(int n, const int *ctx, const int *add, int *table, int max_pages, int page_size, int *free_ids,
+                            int n_pages, const int *free_in, int *free_out, int max_tokens, int *cu, int *kv_len,
+                            int64_t *slots, int *positions, int *requests, int *status, int *next, void *stream) {
     return kv4_entry("kv4 plan", [&]() -> int {
         if (n < 1 || n > KV4_MAX_REQ) return fail("kv4 plan: requests out of range (1..4096)");
         if (page_size != 16 && page_size != 32 && page_size != 64) return fail("kv4 plan: page size must be 16, 32 or 64");
@@ -363,8 +372,9 @@ FN_API int fn_kv4_plan(int n, const int *ctx, const int *add, int *table, int ma
             (max_tokens && (!slots || !positions || !requests)))
             return fail("kv4 plan: null pointer");
         if (ctx == kv_len || add == kv_len) return fail("kv4 plan: kv_len must be an array of its own");
+        if (next && (next == ctx || next == add || next == kv_len)) return fail("kv4 plan: next must be an array of its own");
         PlanArgs a{n, max_pages, page_size, n_pages, max_tokens, ctx, add, table, free_ids, free_in, free_out, cu,
-                   kv_len, positions, requests, status, slots, 0};
+                   kv_len, positions, requests, status, slots, next, 0};
         // few rows: the planning CTA writes them itself; many: a second grid
         a.rows_here = max_tokens <= 4 * PLAN_T;
         const size_t smem = (size_t)4 * (n + 1) * sizeof(int);

@@ -41,7 +41,7 @@ EXPORTS = [
     "fn_decoder_create", "fn_decoder_free", "fn_decoder_step", "fn_decoder_launches",
     "fn_load", "fn_forward", "fn_reset", "fn_free", "fn_debug_layers", "fn_use_graphs", "fn_n_past", "fn_last_ms",
     "fn_dev_gb", "fn_split", "fn_model_dims",
-    "fn_kv4_plan", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
+    "fn_kv4_plan", "fn_kv4_plan_next", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
     "fn_qk_rope_rows", "fn_gdn_reset_seq",
 ]
 
@@ -137,6 +137,7 @@ class FN:
         d.fn_moe_norm.argtypes = [C.c_int, vp, C.c_float]
         i64, kv4 = C.c_int64, C.POINTER(FnKv4)
         d.fn_kv4_plan.argtypes = [C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, vp, vp, C.c_int] + [vp] * 7
+        d.fn_kv4_plan_next.argtypes = d.fn_kv4_plan.argtypes + [vp]
         d.fn_kv4_store.argtypes = [kv4, C.c_uint32, vp, i64, i64, vp, i64, i64, vp, C.c_int, vp]
         d.fn_kv4_load.argtypes = [kv4, C.c_uint32, vp, C.c_int, vp, vp, vp]
         d.fn_kv4_attn_workspace.restype = C.c_uint64
@@ -498,9 +499,10 @@ class FN:
 
     # ---- paged KV cache in 4 bits (device pointers, 0 = null; flashnext/kv4.py is the layer over torch tensors) ----
     def kv4_plan(self, n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out, max_tokens, cu,
-                 kv_len, slots, positions, requests, status, stream=0):
-        self.check(self.d.fn_kv4_plan(n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out,
-                                      max_tokens, cu, kv_len, slots, positions, requests, status, stream))
+                 kv_len, slots, positions, requests, status, stream=0, next=None):
+        """next: the lengths that requests go on with (None: not wanted)."""
+        self.check(self.d.fn_kv4_plan_next(n, ctx, add, table, max_pages, page_size, free_ids, n_pages, free_in, free_out,
+                                           max_tokens, cu, kv_len, slots, positions, requests, status, next, stream))
 
     def kv4_store(self, cache, dtype, k, k_token, k_head, v, v_token, v_head, slots, nt, stream=0):
         """cache: FnKv4; dtype: ggml type id of the rows (0 = F32, 30 = BF16); strides in elements."""

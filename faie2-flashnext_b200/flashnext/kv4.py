@@ -8,7 +8,8 @@ fn_kv4_*). The reference keeps one dense fp32 cache per layer and steps all toke
     step = planner.plan(ctx, add, table, free, free_count, max_tokens=32)
     cache.store(k, v, step.slots)                             # [rows][nkv][hd], fp32 or bf16, any token / head stride
     out = cache.attn(q, step.cu, step.kv_len, table, max_new=1, gate=g)
-    ctx, free_count = step.kv_len, step.free_count            # the next step's inputs: copy what you keep
+    ctx.copy_(step.ctx)                                       # the next step's inputs: a served request's new length, 0 of a
+    free_count.copy_(step.free_count)                         # finished one, the old one of a refused one (its pages stay its own)
 
 Everything runs on the current stream and returns at once; arguments that the kernels cannot check are the device-side
 lengths and page ids, which they clamp to the tensors' bounds.
@@ -46,15 +47,16 @@ def _ints(name, t, shape):
 
 
 class KV4Plan:
-    """A planned step (device tensors): cu [n + 1], kv_len [n], slots / positions / requests [max_tokens], free_count and
-    status (refused requests), one value each."""
+    """A planned step (device tensors): cu [n + 1], kv_len [n] (what attention reads: 0 for a refused request), ctx [n] (the lengths that
+    requests go on with: a refused one's is unchanged), slots / positions / requests [max_tokens], free_count and status (refused
+    requests), one value each."""
 
     def __init__(self, n, max_tokens, dev):
-        ints = torch.empty(2 * n + 3 + 2 * max_tokens, dtype=torch.int32, device=dev)
-        self.cu, self.kv_len, self.free_count, self.status, self.positions, self.requests = ints.split(
-            [n + 1, n, 1, 1, max_tokens, max_tokens])
+        ints = torch.empty(3 * n + 3 + 2 * max_tokens, dtype=torch.int32, device=dev)
+        self.cu, self.kv_len, self.ctx, self.free_count, self.status, self.positions, self.requests = ints.split(
+            [n + 1, n, n, 1, 1, max_tokens, max_tokens])
         self.slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-        self.ptrs = [t.data_ptr() for t in (self.cu, self.kv_len, self.slots, self.positions, self.requests, self.status)]
+        self.ptrs = [t.data_ptr() for t in (self.cu, self.kv_len, self.slots, self.positions, self.requests, self.status, self.ctx)]
 
 
 class KV4Planner:
@@ -83,10 +85,10 @@ class KV4Planner:
                 out = self.kept[key] = KV4Plan(n, max_tokens, ctx.device)
         elif out.kv_len.numel() != n or out.slots.numel() != max_tokens:
             raise ValueError("out: a plan of other sizes")
-        cu, kv_len, slots, positions, requests, status = out.ptrs
+        cu, kv_len, slots, positions, requests, status, following = out.ptrs
         self.fn.kv4_plan(n, ctx.data_ptr(), add.data_ptr(), table.data_ptr(), table.shape[1], self.page_size,
                          free.data_ptr(), free.numel(), free_count.data_ptr(), out.free_count.data_ptr(), max_tokens, cu,
-                         kv_len, slots, positions, requests, status, _stream(ctx.device))
+                         kv_len, slots, positions, requests, status, _stream(ctx.device), following)
         return out
 
 

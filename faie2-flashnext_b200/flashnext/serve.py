@@ -52,7 +52,7 @@ class ServeModel(BatchDecodeModel):
         """The step's plan (places that are dropped give their pages back, then every place gets a row), then its inputs."""
         f, p, d = self.planner, self.plan, self.free_plan
         f.plan(self.ctx, self.drop, self.table, self.free_ids, self.free_count, 0, out=d)
-        f.plan(d.kv_len, self.ones, self.table, self.free_ids, d.free_count, self.B, out=p)
+        f.plan(d.ctx, self.ones, self.table, self.free_ids, d.free_count, self.B, out=p)
         self.fn.embed_batch(self.cfg["embed"], self.E.data_ptr(), self.cfg["D"], self.inputs.data_ptr(), 1,
                             self.zero.data_ptr(), self.h.data_ptr(), self.B, s)
 
@@ -71,7 +71,7 @@ class ServeModel(BatchDecodeModel):
         """The lengths and the pool of the next step."""
         import torch
         with torch.cuda.stream(torch.cuda.ExternalStream(s)):
-            self.ctx.copy_(self.plan.kv_len)
+            self.ctx.copy_(self.plan.ctx)
             self.free_count.copy_(self.plan.free_count)
 
     def launch_step(self, s: int):

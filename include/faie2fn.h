@@ -311,10 +311,16 @@ typedef struct fn_kv4_t {
  * max_tokens; kv_len [n] (an array of its own): the new length, 0 for a finished or refused request; slots, positions,
  * requests [max_tokens]: each row's slot, position and request (-1 where there is none). A request is refused (nothing
  * taken, its rows' slots and positions -1) when its pages exceed max_pages, its rows max_tokens, or the free pages run
- * out; *status = how many were. Lengths below zero count as zero. */
+ * out; *status = how many were. Its rows stay its rows: cu counts every request's, so a caller lays out a step's tokens from add alone, and
+ * a request that alone passes max_tokens leaves none for those behind it. Lengths below zero count as zero. */
 int fn_kv4_plan(int n, const int *ctx, const int *add, int *table, int max_pages, int page_size, int *free_ids,
                 int n_pages, const int *free_in, int *free_out, int max_tokens, int *cu, int *kv_len, int64_t *slots,
                 int *positions, int *requests, int *status, void *stream);
+/* fn_kv4_plan, and next [n] (an array of its own, or NULL): the length that each request goes on with, the ctx of the next step: kv_len
+ * for a served or idle request, 0 for a finished one, the old ctx for a refused one (whose kv_len is 0, but whose pages it keeps). */
+int fn_kv4_plan_next(int n, const int *ctx, const int *add, int *table, int max_pages, int page_size, int *free_ids,
+                     int n_pages, const int *free_in, int *free_out, int max_tokens, int *cu, int *kv_len,
+                     int64_t *slots, int *positions, int *requests, int *status, int *next, void *stream);
 /* Quantise nt rows of keys and values ([nt][nkv][hd], token and head strides in elements, the hd values of a head
  * adjacent) into their slots (< 0: skipped; past the pages: skipped, reported by fn_sync). Per 64 dims d = m / -8 with m
  * the value of largest magnitude (of two opposite ones the positive), c = clamp(trunc(x (1 / d) + 8.5), 0, 15) in fp32, d
