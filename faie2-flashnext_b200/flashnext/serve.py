@@ -18,6 +18,14 @@ import numpy as np
 from model import HD, BatchDecodeModel
 
 
+class OutOfPages(RuntimeError):
+    """A step found too few free pages. outs: what generate would have returned, None for requests that were not finished."""
+
+    def __init__(self, message, outs):
+        super().__init__(message)
+        self.outs = outs
+
+
 class ServeModel(BatchDecodeModel):
     def __init__(self, fn, cfg: dict, W: dict, batch: int, pages: int, max_ctx: int = 512, page_size: int = 64):
         """pages: of the pool, for each attention layer (one table serves them all); idle places use one each."""
@@ -92,10 +100,12 @@ class ServeModel(BatchDecodeModel):
         for g in self.gdns:
             self.fn.gdn_reset(g, stream.cuda_stream)
 
-    def generate(self, prompts, n_new, stream, logits=None):
+    def generate(self, prompts, n_new, stream, logits=None, wait=False):
         """Greedy decode of any number of requests, as many at a time as the batch has places. prompts: a list of token id
         arrays (of any lengths); n_new: tokens to generate, one number or one per request. Returns a list of arrays, prompt
-        then new tokens. logits: an optional callback(request, position, row [vocab]) per step."""
+        then new tokens. logits: an optional callback(request, position, row [vocab]) per step. wait: a request is admitted, in order,
+        when the pages that it may come to need fit beside those of the requests before it and one for each idle place; without
+        it requests take places as they come free, and a step that finds no page raises OutOfPages."""
         import torch
         if self.graph is None:
             raise RuntimeError("capture() the step first")
@@ -103,6 +113,9 @@ class ServeModel(BatchDecodeModel):
         n_new = [n_new] * len(prompts) if np.ndim(n_new) == 0 else list(n_new)
         if len(n_new) != len(prompts) or any(len(p) < 1 or n < 1 or len(p) + n > self.max_ctx for p, n in zip(prompts, n_new)):
             raise ValueError("every request wants a prompt and new tokens within the context")
+        need = [-(-(len(p) + n - 1) // self.page_size) for p, n in zip(prompts, n_new)]  # the last token is not fed
+        if wait and max(need, default=0) + self.B - 1 > self.n_pages:
+            raise ValueError("a request wants more pages than there are beside one for each other place")
         self.start(None, stream)
         waiting, place, seq = list(range(len(prompts))), [None] * self.B, [p.tolist() for p in prompts]
         at = [0] * self.B  # tokens fed of the place's request
@@ -110,7 +123,9 @@ class ServeModel(BatchDecodeModel):
         while waiting or any(r is not None for r in place):
             for b in range(self.B):
                 drop[b] = -1 if place[b] is None else 0
-                if place[b] is None and waiting:
+                held = [need[r] for r in place if r is not None]
+                if place[b] is None and waiting and (
+                        not wait or sum(held) + need[waiting[0]] + self.B - len(held) - 1 <= self.n_pages):
                     place[b], at[b] = waiting.pop(0), 0
                     for g in self.gdns:
                         self.fn.gdn_reset_seq(g, b, stream.cuda_stream)
@@ -121,7 +136,8 @@ class ServeModel(BatchDecodeModel):
                 self.graph.replay()
             self.fn.sync(stream.cuda_stream)
             if int(self.plan.status):
-                raise RuntimeError(f"out of pages: {int(self.plan.status)} of the batch found none (of {self.n_pages})")
+                done = [np.array(s, np.int32) if len(s) == len(p) + n else None for s, p, n in zip(seq, prompts, n_new)]
+                raise OutOfPages(f"out of pages: {int(self.plan.status)} of the batch found none (of {self.n_pages})", done)
             new = self.next.cpu().numpy()
             for b, r in enumerate(place):
                 if r is None:
