@@ -1,9 +1,9 @@
 // Host-side interfaces shared by the engine's translation units.
 #pragma once
 
-#include <unordered_set>
 
 #include "fn_common.cuh"
+#include "fn_once.h"
 
 namespace fn {
 
@@ -125,16 +125,18 @@ struct DevBuf {
 // allow a kernel the largest dynamic shared memory the SM grants next to its static shared memory, and ask for the
 // SM's largest shared-memory carveout: an SM configured with a smaller carveout for one kernel cannot take a CTA of
 // the next kernel that needs more until it drains, which would keep consecutive small kernels from overlapping under
-// programmatic dependent launch (once per kernel)
+// programmatic dependent launch (once per kernel and device)
 template <typename K> cudaError_t allow_max_dynamic_smem(K *k) {
-    static std::unordered_set<const void *> done;
-    if (done.count((const void *)k)) return cudaSuccess;
+    static OncePerDevice done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || done.has((const void *)k, dev)) return e;
     cudaFuncAttributes fa;
-    cudaError_t e = cudaFuncGetAttributes(&fa, k);
+    e = cudaFuncGetAttributes(&fa, k);
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(227 * 1024 - fa.sharedSizeBytes));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e == cudaSuccess) done.insert((const void *)k);
+    if (e == cudaSuccess) done.add((const void *)k, dev);
     return e;
 }
 

@@ -1,4 +1,7 @@
-"""CPU: refusals of the paged 4-bit cache's later entries and layers, before any device work."""
+"""CPU: refusals of the paged 4-bit cache's later entries and layers, before any device work; what is done once per device."""
+
+import os
+import subprocess
 
 import pytest
 
@@ -18,3 +21,29 @@ def test_bad_plans_with_carried_lengths_are_refused(f, at, value, word):
     a = [1, ONE, ONE + 64, ONE, 4, 16, ONE, 4, ONE, ONE, 8, ONE, ONE + 128, ONE, ONE, ONE, ONE, None, None]
     a[at] = value
     assert f.d.fn_kv4_plan_next(*a) == -1 and word in f.d.fn_error().decode()
+
+
+def test_a_kernel_is_prepared_on_every_device(tmp_path):
+    """The shared-memory limit of a kernel is raised where it was not: on each device, and from several threads."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "faie2-flashnext_b200", "csrc")
+    (tmp_path / "once.cpp").write_text("""
+#include <thread>
+#include <vector>
+#include "fn_once.h"
+int main() {
+    fn::OncePerDevice once;
+    int k[2];
+    if (once.has(&k[0], 0)) return 1;
+    once.add(&k[0], 0);
+    if (!once.has(&k[0], 0) || once.has(&k[0], 1) || once.has(&k[1], 0)) return 2;
+    std::vector<std::thread> t;
+    for (int d = 0; d < 8; ++d) t.emplace_back([&, d] { for (int i = 0; i < 1000; ++i) once.add((char *)k + i, d); });
+    for (auto &x : t) x.join();
+    for (int d = 0; d < 8; ++d)
+        for (int i = 0; i < 1000; ++i)
+            if (!once.has((char *)k + i, d)) return 3;
+    return 0;
+}
+""")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-pthread", "-I", csrc, str(tmp_path / "once.cpp"), "-o", str(tmp_path / "once")], check=True)
+    assert subprocess.run([str(tmp_path / "once")]).returncode == 0
