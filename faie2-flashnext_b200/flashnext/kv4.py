@@ -41,9 +41,11 @@ def _stream(dev) -> int:
     return torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream().cuda_stream without its 2 us
 
 
-def _ints(name, t, shape):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name}: a contiguous int32 CUDA tensor {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)}")
+def _ints(name, t, shape, dev):
+    """dev: the index of the CUDA device that the call's tensors are on."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != dev or dev < 0:
+        raise ValueError(f"{name}: a contiguous int32 tensor {tuple(shape)} on cuda:{max(dev, 0)} is wanted, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
 
 
 class KV4Plan:
@@ -73,18 +75,19 @@ class KV4Planner:
         n = ctx.numel()
         if table.dim() != 2:
             raise ValueError("table: [requests][max_pages] is wanted")
-        _ints("ctx", ctx, (n,))
-        _ints("add", add, (n,))
-        _ints("table", table, (n, table.shape[1]))
-        _ints("free", free, (free.numel(),))
-        _ints("free_count", free_count, (1,))
+        dev = ctx.get_device()
+        _ints("ctx", ctx, (n,), dev)
+        _ints("add", add, (n,), dev)
+        _ints("table", table, (n, table.shape[1]), dev)
+        _ints("free", free, (free.numel(),), dev)
+        _ints("free_count", free_count, (1,), dev)
         if out is None:
             key = (n, max_tokens, ctx.device)
             out = self.kept.get(key)
             if out is None:
                 out = self.kept[key] = KV4Plan(n, max_tokens, ctx.device)
-        elif out.kv_len.numel() != n or out.slots.numel() != max_tokens:
-            raise ValueError("out: a plan of other sizes")
+        elif out.kv_len.numel() != n or out.slots.numel() != max_tokens or out.slots.get_device() != dev:
+            raise ValueError("out: a plan of other sizes, or on another device")
         cu, kv_len, slots, positions, requests, status, following = out.ptrs
         self.fn.kv4_plan(n, ctx.data_ptr(), add.data_ptr(), table.data_ptr(), table.shape[1], self.page_size,
                          free.data_ptr(), free.numel(), free_count.data_ptr(), out.free_count.data_ptr(), max_tokens, cu,
@@ -96,9 +99,9 @@ class KV4Workspace:
     """Scratch of the attention (split requests' partial results). Calls that may run at the same time, as on two
     streams, need one each."""
 
-    def __init__(self, fn):
+    def __init__(self, fn, device="cuda"):
         self.bytes = fn.kv4_attn_workspace()
-        self.tensor = torch.empty(self.bytes, dtype=torch.uint8, device="cuda")
+        self.tensor = torch.empty(self.bytes, dtype=torch.uint8, device=device)
         self.ptr = self.tensor.data_ptr()
 
 
@@ -113,7 +116,10 @@ class KV4Cache:
                 pages.shape[1:] != (nkv, record_bytes(hd, page_size)):
             raise ValueError("pages: a contiguous uint8 CUDA tensor [pages][nkv][record_bytes(hd, page_size)] is wanted")
         self.fn, self.nkv, self.hd, self.page_size, self.pages, self.dev = fn, nkv, hd, page_size, pages, pages.device
-        self.ws = workspace or KV4Workspace(fn)
+        self.ws = workspace or KV4Workspace(fn, self.dev)
+        if self.ws.tensor.device != self.dev:
+            raise ValueError(f"workspace: one on {self.dev} is wanted")
+        self.index = pages.get_device()
         self.c = C.byref(FnKv4(pages.data_ptr(), pages.shape[0], page_size, nkv, hd))
         self.scale = 1.0 / math.sqrt(hd)
         self._store, self._load, self._attn = fn.kv4_store, fn.kv4_load, fn.kv4_attn
@@ -158,9 +164,9 @@ class KV4Cache:
         rows, nh = q.shape[0], q.shape[1]
         self._rows("q", q, nh)
         n = kv_len.numel()
-        _ints("kv_len", kv_len, (n,))
-        _ints("cu", cu, (n + 1,))
-        _ints("table", table, (n, table.shape[-1]))
+        _ints("kv_len", kv_len, (n,), self.index)
+        _ints("cu", cu, (n + 1,), self.index)
+        _ints("table", table, (n, table.shape[-1]), self.index)
         if out is None:
             out = torch.empty(rows, nh, self.hd, dtype=q.dtype, device=self.dev)
         else:

@@ -2,6 +2,7 @@
 
 import os
 import subprocess
+from types import SimpleNamespace
 
 import pytest
 
@@ -47,3 +48,20 @@ int main() {
 """)
     subprocess.run(["g++", "-std=c++20", "-O1", "-pthread", "-I", csrc, str(tmp_path / "once.cpp"), "-o", str(tmp_path / "once")], check=True)
     assert subprocess.run([str(tmp_path / "once")]).returncode == 0
+
+
+def test_tensors_of_another_device_are_refused():
+    import kv4
+    import torch
+
+    def tensor(device, dtype=torch.int32):
+        return SimpleNamespace(dtype=dtype, shape=(3,), is_contiguous=lambda: True, get_device=lambda: device, device=f"cuda:{device}")
+
+    kv4._ints("cu", tensor(1), (3,), 1)
+    for t, dev in ((tensor(0), 1), (tensor(1), 0), (tensor(-1), 0), (tensor(-1), -1), (tensor(0, torch.int64), 0)):
+        with pytest.raises(ValueError, match="cu: a contiguous int32"):
+            kv4._ints("cu", t, (3,), dev)
+    # a planner's tensors have to be where its lengths are
+    z = [torch.zeros(s, dtype=torch.int32) for s in ((2,), (2,), (2, 3), (4,), (1,))]
+    with pytest.raises(ValueError, match="cuda"):
+        kv4.KV4Planner(None, 16).plan(*z, 4)
