@@ -243,8 +243,9 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
             }
         }
     drained:
-        // a CTA that gave up must not leave with copies into its shared memory in flight
-        if (s_fail && lane == 0)
+        // a CTA must not leave with copies into its shared memory in flight: the computing warps may give up after this warp is done, so
+        // it always stays until its last copies have landed
+        if (lane == 0)
             for (int i = max(it - S, 0); i < it; ++i) mbar_park(&full[i % S], (uint32_t)(i / S) & 1u);
         return;
     }

@@ -355,6 +355,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
         if (warp == 0) {
             // ---- copies: lane p fetches page p of a tile
             bool ok = true;
+            int begun[2] = {};  // stages of K, of V
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
                 const int pages = (rq.len + a.l.bs - 1) >> a.l.lbs, hi_lim = limit(KP_ROWS - 1);
@@ -379,6 +380,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                         }
                         ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                         if (!ok) break;
+                        ++begun[v];
                         if (good) {
                             const uint8_t *rec = a.l.pages + ((int64_t)id * a.l.nkv + kv) * (int64_t)a.l.rec;
                             uint8_t *to = sm_kp + (v ? C::RV_OFF + sl * C::RAW + lane * praw : C::RK_OFF + sl * C::RAWK + lane * prawk);
@@ -388,12 +390,13 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     }
                 }
             }
-            // a CTA that gave up must not leave with copies into its shared memory in flight
-            if (*s_fail && lane == 0)
+            // a CTA must not leave with copies into its shared memory in flight: other warps may give up after this one is done, so it always
+            // stays until its last copies have landed
+            if (lane == 0)
                 for (int v = 0; v < 2; ++v) {
                     const int R = v ? C::RV : C::RK;
-                    for (int i = max(gt - R, 0); i <= gt; ++i)
-                        if (i < gt || v == 0) mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
+                    for (int i = max(begun[v] - R, 0); i < begun[v]; ++i)
+                        mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
                 }
         } else if (warp == 2) {
             // ---- scales of a tile: the exponents of the largest finite K and V scale, which of V's are not finite, and whether K's
