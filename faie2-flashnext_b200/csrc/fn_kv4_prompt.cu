@@ -6,7 +6,7 @@
 //
 // Roles of the CTA's 16 warps, one CTA per SM:
 //   * warp 0 copies pages into rings (K and V parts apart: they are consumed at different times);
-//   * warp 2 looks at each tile's scales: K's and V's exponents, and which of V's are not finite;
+//   * warp 2 (only in the long form, below) looks at each tile's scales: K's and V's exponents, and which of V's are not finite;
 //   * warp 1 issues the MMAs: S of tile j + 1 before O of tile j, so the softmax of one runs beside the products of the other;
 //   * warps 4..7 (a row a lane): scores out of tensor memory, running softmax, P back into tensor memory in S's place;
 //   * warps 8..15: Q into tensor memory, K and V codes into the MMAs' operands in shared memory, and the running output:
@@ -14,26 +14,29 @@
 //     over tokens are rounded fp32 additions, where the tensor core's own accumulation over a long context cuts, and a new
 //     maximum needs no pass over tensor memory.
 //
-// Scales. Codes of a tile become (c - 8) d 2^(11 - e) in fp16, e the exponent of the tile's largest finite |d|, K's and V's for
-// themselves: 8 d 2^(11 - e) is below 2^15, and scales down to 2^-25 of the largest keep all their bits. K's e goes into the scores'
-// unit; in a tile whose K scales lie further apart (one huge key, hidden from some rows perhaps) each token takes its own. V's goes into the
-// weights: P = 2^10 2^(s + e - r), where a row's reference r is the running maximum of s + e, so what P's fp16 range holds is what
-// a tile adds to the row, and tiles that add little cost the others no bits, whatever their values' size. The sum of weights takes
-// 2^(11 - e) back. In a tile whose V scales lie more than 2^12 apart (one huge value, or block of it, beside small ones) no e serves
-// all: its weights stay fp32, and the workers add p v on the CUDA cores instead of the tensor core's O (some 15 times as slow).
-// Such tiles, what is not finite, and rows of scores past 2^20 have a kernel of their own (FAR), the same with the code for them: with that code in it every
-// call would pay (the roles' loops share the instruction cache: 8 bf16 prompts 963 us beside 744). The first kernel notes whether it
-// met any; the second, launched behind it, returns at once or does the call again.
-// Rows of q are scaled by a power of two.
+// Scales. Codes become (c - 8) d in fp16 as they are. The product has 15 bits, the last of them d's last, and that is 2^-24 or more, fp16's
+// own: at the small end nothing is lost, however small K and V are, so neither needs a scale of its own (dividing them by 8 lost
+// bits of keys below 4e-3; normalising V by its tile's largest lost those of everything 2^14 below it). At the large end 8 d fits up
+// to d = 8188. Weights are 2^10 exp2(s - maximum), 22 bits (11 for bf16 rows) of each down to 2^-12 of the largest and to 2^-35 of it
+// beyond, so that values which a row does not see, or hardly weighs, cost it nothing. Rows of q are scaled by a power of two.
 // bf16 rows: one product each; q is exact, K, P and V are rounded to 11 bits. fp32 rows: q, K, P and V are fp16 pairs (22
 // bits, K's and V's exact), three products each, the small ones first, so that the sum's cut bits are few.
 //
-// What no row of the tile sees becomes 0 in V, whatever its scale is. A visible token whose V scale is not finite also
-// becomes 0 and is noted: the rows that see it turn NaN in its 64 dims, the others must not (0 x NaN in the product).
+// The long form (FAR) is for what that does not serve: scales past 8188, scales that are not finite, scores past 2^20 (beside which the
+// weights' 2^10 would be rounded). It is a kernel of its own, the same code with more in it: in one kernel every call paid for it (the
+// roles' loops share the instruction cache: 8 bf16 prompts 963 us instead of 607). The first kernel notes whether it met any such thing;
+// the second, launched behind it, returns at once (2 us) or does the call again. There:
+//   * K's and V's codes of a tile become (c - 8) d 2^(11 - e), e the exponent of the tile's largest finite |d|; K's e goes into the scores'
+//     unit, V's into the weights: P = 2^10 2^(s + e - r), a row's reference r the running maximum of s + e. Scales down to 2^-25 of
+//     the largest keep all their bits.
+//   * Where a tile's K scales lie further apart each token takes its own e. Where its V scales lie more than 2^12 apart no e serves all:
+//     the weights stay fp32, and the workers add p v on the CUDA cores instead of the tensor core's O (some 15 times as slow).
+//   * What no row of the tile sees becomes 0 in V, whatever its scale is. A visible token whose V scale is not finite also becomes 0
+//     and is noted: the rows that see it turn NaN in its 64 dims, the others must not (0 x NaN in the product).
 //
-// What bounds it, and measured: 2048 new of 4096 tokens, fp32, 16 heads over 2 kv heads of 256 420 us (243 TFLOP/s of the case's
+// What bounds it, and measured: 2048 new of 4096 tokens, fp32, 16 heads over 2 kv heads of 256 423 us (244 TFLOP/s of the case's
 // products, three times that in the tensor cores): the workers, whose one operand buffer makes V wait for the O before it; 8
-// prompts, bf16, 32 heads over 8 of 128 635 us (310 TFLOP/s): issue and instruction fetch of softmax and workers, some 2500 cycles per 64
+// prompts, bf16, 32 heads over 8 of 128 607 us (327 TFLOP/s): issue and instruction fetch of softmax and workers, some 2400 cycles per 64
 // tokens beside 512 of products.
 //
 // Work is cut into runs of 64-token units as in fn_kv4_attn.cu, one run per CTA; partial row tiles are joined after it.
@@ -47,11 +50,12 @@ constexpr int KP_EXTRA = 8;  // units that a row tile counts beside its own, for
 constexpr int KP_W_SM = 4, KP_W_WORK = 8;
 constexpr int KP_POLLS = 1 << 17;         // of a wait before it gives up, 20 us at most each
 constexpr uint32_t KP_FIXED = 5120;       // bytes before the operands (KpShared)
-// binades between the K, or the V scales of a tile from which it goes the long way. The operands are exact up to 25; but V's e stands
-// for every token and block of the tile, and P keeps 22 bits (11 for bf16 rows) down to 12 binades below the largest
+// long form: binades between the K, or the V scales of a tile from which its tokens take their own exponents, or are added in fp32. The
+// operands are exact up to 25; but V's e stands for every token and block of the tile, and P keeps 22 bits down to 12 below the largest
 constexpr int KP_FAR_K = 25, KP_FAR_V = 12;
+constexpr uint32_t KP_MOST = 0x6fff;  // 8188 as a half: the scale of which 8 are fp16's largest number
 
-template <int HD, bool HL> struct KpCfg {
+template <int HD, bool HL, bool FAR> struct KpCfg {
     using T = std::conditional_t<HL, float, __nv_bfloat16>;
     static constexpr int NG = HD / KV4_GROUP, TERMS = HL ? 2 : 1;
     static constexpr int NB = HL && HD == 256 ? 1 : 2;      // operand buffers of K and of V
@@ -59,8 +63,8 @@ template <int HD, bool HL> struct KpCfg {
     static constexpr uint32_t KT = KA_TOK * HD * 2;          // K operand: [dim / 8][token] x 16 bytes
     // V operand: [token / 8][dim] x 16 bytes, the token groups 16 bytes further apart (banks of the stores)
     static constexpr uint32_t VG = HD * 16 + 16, VT = 8 * VG;
-    // 64 tokens' codes and scales of V, and of K with V's scales beside its own (both are looked at before K is made)
-    static constexpr uint32_t RAW = KA_TOK * (HD / 2 + HD / KV4_GROUP * 2), RAWK = RAW + KA_TOK * HD / KV4_GROUP * 2;
+    // 64 tokens' codes and scales of V, and of K (FAR: with V's scales beside its own, as both are looked at before K is made)
+    static constexpr uint32_t RAW = KA_TOK * (HD / 2 + HD / KV4_GROUP * 2), RAWK = RAW + FAR * KA_TOK * HD / KV4_GROUP * 2;
     static constexpr uint32_t QL = HL ? KP_ROWS * HD * 2 : 0;  // second halves of q: [dim / 8][row] x 16 bytes
     static constexpr uint32_t K_OFF = KP_FIXED, V_OFF = K_OFF + NB * TERMS * KT, Q_OFF = V_OFF + NB * TERMS * VT;
     static constexpr uint32_t RK_OFF = Q_OFF + QL, RV_OFF = RK_OFF + RK * RAWK, SMEM = RV_OFF + RV * RAW;
@@ -79,9 +83,10 @@ struct KpShared {
     uint64_t rkf[2], rke[2], rvf[2], rve[2], kf[2], ke[2], vf[2], sf[2], pf[2], xf[8], of, oe, qf, qe, lf, done;
     long long red[KP_THREADS / 32], off;
     uint32_t tmem, valid[8];  // pages there of tile & 7; bit 31: all of them, and every token seen by some row
-    int req, fail, met;  // met: what only the long way serves
+    int req, fail, met;  // met: what only the long form serves
     // rings as long as the fastest role can be ahead of the slowest reader
     float f[4][KP_ROWS], l[KP_ROWS], rs[KP_ROWS];
+    // long form
     float ev[8], ek[8];  // e of V, 2^(e - 11) of K: the scores' unit
     uint32_t bad[8][4][2];  // tokens whose V scale is not finite: [tile & 7][group][token / 32]
     uint8_t any_bad[8], kfar[8], vfar[8];
@@ -205,9 +210,9 @@ __device__ __forceinline__ int kp_tiles(const KaReq &q, int group, int i) {
 }
 __device__ __forceinline__ KaReq kp_req(const Kv4AttnArgs &a, int r) { return ka_req<KP_ROWS>(a, r); }
 
-// FAR: the long way, for a call in which the other form met what it does not serve (it notes that in a.far, a place for each CTA)
+// FAR: the long form, for a call in which the other met what it does not serve (it notes that in a.far, a place for each CTA)
 template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttnArgs a) {
-    using C = KpCfg<HD, HL>;
+    using C = KpCfg<HD, HL, FAR>;
     using T = typename C::T;
     constexpr int NG = C::NG, NB = C::NB;
     extern __shared__ __align__(1024) uint8_t sm_kp[];
@@ -216,7 +221,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], 5), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 8);
+            mbar_init(&sh.rkf[i], 1), mbar_init(&sh.rke[i], FAR ? 5 : 4), mbar_init(&sh.rvf[i], 1), mbar_init(&sh.rve[i], 8);
             mbar_init(&sh.kf[i], 4), mbar_init(&sh.ke[i], 1), mbar_init(&sh.vf[i], 4);
             mbar_init(&sh.sf[i], 1), mbar_init(&sh.pf[i], 4);
         }
@@ -347,7 +352,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
         return false;
     };
     const int ppt = KA_TOK >> a.l.lbs;  // pages of a tile
-    const uint32_t praw = a.l.kb + a.l.sb, prawk = praw + a.l.sb;  // bytes of a page's V part in a stage, of its K part with V's scales
+    const uint32_t praw = a.l.kb + a.l.sb, prawk = praw + FAR * a.l.sb;  // bytes of a page's V part in a stage, of its K part
     int gt = 0, gi = 0;  // tiles and row tiles done by this role
 
     if (warp < KP_W_SM) {
@@ -385,7 +390,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                             const uint8_t *rec = a.l.pages + ((int64_t)id * a.l.nkv + kv) * (int64_t)a.l.rec;
                             uint8_t *to = sm_kp + (v ? C::RV_OFF + sl * C::RAW + lane * praw : C::RK_OFF + sl * C::RAWK + lane * prawk);
                             bulk_g2s(to, rec + v * a.l.kb, a.l.kb, full);
-                            bulk_g2s(to + a.l.kb, rec + 2 * a.l.kb + v * a.l.sb, v ? a.l.sb : 2 * a.l.sb, full);
+                            bulk_g2s(to + a.l.kb, rec + 2 * a.l.kb + v * a.l.sb, FAR && !v ? 2 * a.l.sb : a.l.sb, full);
                         }
                     }
                 }
@@ -398,10 +403,10 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     for (int i = max(begun[v] - R, 0); i < begun[v]; ++i)
                         mbar_wait(v ? &sh.rvf[i % R] : &sh.rkf[i % R], (uint32_t)(i / R) & 1u, 1u << 16);
                 }
-        } else if (warp == 2) {
+        } else if (FAR && warp == 2) {
             // ---- scales of a tile: the exponents of the largest finite K and V scale, which of V's are not finite, and whether K's
             // lie so far apart that each token takes its own exponent
-            bool ok = true, met = false;
+            bool ok = true;
             for (; u < u1 && ok; next()) {
                 if (!here()) continue;
                 const int hi_lim = limit(KP_ROWS - 1);
@@ -415,53 +420,42 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     // two tokens a lane, as halves (positive ones order as their bits do); zeros set no exponent
                     const uint8_t *at = place(2 * lane);
                     const uint32_t mask = (here_(2 * lane) ? 0x7fffu : 0u) | (here_(2 * lane + 1) ? 0x7fff0000u : 0u);
-                    uint32_t kw = 0, vw = 0, kn = 0x7bff7bffu, vn = kn;
+                    uint32_t kn = 0x7bff7bffu, vn = kn, kmax = 0, vmax = 0;
 #pragma unroll
                     for (int x = 0; x < NG; ++x) {
                         const uint32_t dk = *(const uint32_t *)(at + x * a.l.bs * 2) & mask, dv = *(const uint32_t *)(at + a.l.sb + x * a.l.bs * 2) & mask;
-                        kw = kp_hmax2(kw, dk);
-                        vw = kp_hmax2(vw, dv);
                         kn = kp_hmin2(kn, dk | (kp_hzero2(dk) & 0x7bff7bffu));
                         vn = kp_hmin2(vn, dv | (kp_hzero2(dv) & 0x7bff7bffu));
                     }
-                    uint32_t kmax = __reduce_max_sync(0xffffffffu, max(kw & 0xffffu, kw >> 16));
-                    uint32_t vmax = __reduce_max_sync(0xffffffffu, max(vw & 0xffffu, vw >> 16));
-                    uint32_t kmin = __reduce_min_sync(0xffffffffu, min(kn & 0xffffu, kn >> 16));
-                    uint32_t vmin = __reduce_min_sync(0xffffffffu, min(vn & 0xffffu, vn >> 16));
+                    const uint32_t kmin = __reduce_min_sync(0xffffffffu, min(kn & 0xffffu, kn >> 16));
+                    const uint32_t vmin = __reduce_min_sync(0xffffffffu, min(vn & 0xffffu, vn >> 16));
                     auto exponent = [](uint32_t h) { return (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) >> 23); };
-                    if constexpr (!FAR) {
-                        met |= exponent(kmax) > exponent(kmin) + KP_FAR_K || exponent(vmax) > exponent(vmin) + KP_FAR_V || max(kmax, vmax) >= 0x7c00u;
-                    } else {
-                        // a closer look, a token a lane: what is not finite sets no exponent either
-                        bool any = false;
-                        uint32_t own[2] = {};  // the token's largest K scale
-                        kmax = vmax = 0;
+                    // a closer look, a token a lane: what is not finite sets no exponent either
+                    bool any = false;
+                    uint32_t own[2] = {};  // the token's largest K scale
 #pragma unroll 1
-                        for (int x = 0; x < NG; ++x)
+                    for (int x = 0; x < NG; ++x)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint8_t *p = place(lane + 32 * h) + x * a.l.bs * 2;
-                                const bool in = here_(lane + 32 * h);
-                                const uint32_t dk = *(const uint16_t *)p & 0x7fffu, dv = *(const uint16_t *)(p + a.l.sb) & 0x7fffu;
-                                if (in && dk < 0x7c00u) own[h] = max(own[h], dk);
-                                if (in && dv < 0x7c00u) vmax = max(vmax, dv);
-                                const uint32_t bad = __ballot_sync(0xffffffffu, in && dv >= 0x7c00u);
-                                if (lane == 0) sh.bad[gt & 7][x][h] = bad;
-                                any |= bad != 0;
-                            }
-                        kmax = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
-                        vmax = __reduce_max_sync(0xffffffffu, vmax);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) sh.kexp[gt & 7][lane + 32 * h] = (uint8_t)exponent(own[h] ? own[h] : kmax);
-                        const bool vfar = vmax && exponent(vmax) > exponent(vmin) + KP_FAR_V;
-                        if (vfar) vmax = vmin;  // what is added in fp32 raises no reference
-                        if (lane == 0) {
-                            sh.any_bad[gt & 7] = any;
-                            sh.kfar[gt & 7] = kmax && exponent(kmax) > exponent(kmin) + KP_FAR_K;
-                            sh.vfar[gt & 7] = vfar;
+                        for (int h = 0; h < 2; ++h) {
+                            const uint8_t *p = place(lane + 32 * h) + x * a.l.bs * 2;
+                            const bool in = here_(lane + 32 * h);
+                            const uint32_t dk = *(const uint16_t *)p & 0x7fffu, dv = *(const uint16_t *)(p + a.l.sb) & 0x7fffu;
+                            if (in && dk < 0x7c00u) own[h] = max(own[h], dk);
+                            if (in && dv < 0x7c00u) vmax = max(vmax, dv);
+                            const uint32_t bad = __ballot_sync(0xffffffffu, in && dv >= 0x7c00u);
+                            if (lane == 0) sh.bad[gt & 7][x][h] = bad;
+                            any |= bad != 0;
                         }
-                    }
+                    kmax = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
+                    vmax = __reduce_max_sync(0xffffffffu, vmax);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) sh.kexp[gt & 7][lane + 32 * h] = (uint8_t)exponent(own[h] ? own[h] : kmax);
+                    const bool vfar = vmax && exponent(vmax) > exponent(vmin) + KP_FAR_V;
+                    if (vfar) vmax = vmin;  // what is added in fp32 raises no reference
                     if (lane == 0) {
+                        sh.any_bad[gt & 7] = any;
+                        sh.kfar[gt & 7] = kmax && exponent(kmax) > exponent(kmin) + KP_FAR_K;
+                        sh.vfar[gt & 7] = vfar;
                         sh.ev[gt & 7] = vmax ? (float)(exponent(vmax) - 127) : 0.0f;
                         sh.ek[gt & 7] = kmax ? kp_pow2(exponent(kmax) - 138) : 1.0f;
                     }
@@ -472,7 +466,6 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     }
                 }
             }
-            if (met) sh.met = 1;
         } else if (warp == 1) {
             // ---- MMAs. The whole warp runs this and one elected lane issues: the operands' descriptors then live in uniform
             // registers. (As one lane's own values each MMA took 120 cycles and more, whatever its size; so it takes what its size
@@ -570,8 +563,8 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 const uint32_t valid = sh.valid[gt & 7], ts = tl + (uint32_t)b * 64u;
                 const int left = lim - j * KA_TOK;  // tokens of the tile that the row sees
                 const bool masked = left < KA_TOK || !(valid >> 31);
-                const float ek = sh.ek[gt & 7], ev = sh.ev[gt & 7];
-                float rsj = rs * ek;
+                const float ev = FAR ? sh.ev[gt & 7] : 0.0f;
+                float rsj = FAR ? rs * sh.ek[gt & 7] : rs;
                 if (FAR && sh.kfar[gt & 7]) {  // every column by its own unit
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
@@ -610,13 +603,13 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 }
                 // rs > 0: the maximum may be taken before the scaling
                 const float top = fmaxf(mx[0], mx[1]) * rsj;
-                const bool higher = top - sref > eref - ev;  // (never so for -inf beside -inf)
-                const float ns = higher ? top : sref, ne = higher ? ev : eref;
+                const bool higher = FAR ? top - sref > eref - ev : top > sref;  // (never so for -inf beside -inf)
+                const float ns = higher ? top : sref, ne = FAR && higher ? ev : eref;
                 const float fac = sref == -INFINITY ? 0.0f : ka_exp2((sref - ns) + (eref - ne));
                 sref = ns, eref = ne;
-                // P = 2^10 exp2(s + e - reference): fp16 keeps 11 bits down to 2^-24 of the largest
-                // Beside a reference of 2^20 and more the 10 would be rounded, and at 2^27 a weight could pass fp16: the long way takes
-                // the exact difference to the best score first.
+                // P = 2^10 exp2(s (+ e) - reference): fp16 keeps 11 bits down to 2^-24 of the largest. Beside a reference of 2^20 and more
+                // the 10 would be rounded, and at 2^27 a weight could pass fp16: the long form takes the exact difference to the best score
+                // first.
                 const float z0 = ns == -INFINITY ? 0.0f : -ns, z1 = 10.0f + ev - ne, z = z0 + z1;
                 // (one at a time: the packed product and sum would become one, and the rounding of the best score differ)
                 [[maybe_unused]] auto apart = [&](uint32_t x) { return __fadd_rn(__fadd_rn(__fmul_rn(__uint_as_float(x), rsj), z0), z1); };
@@ -640,9 +633,9 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                         }
                         tmem_st16(ts + 16u * c, s);
                     }
-                } else {
+                }
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = FAR && sh.vfar[gt & 7] ? 4 : 0; c < 4; ++c) {
                     uint32_t s[16], p16[16];
                     kp_tmem_ld16(ts + 16u * c, s);
                     kp_tmem_wait_ld();
@@ -664,8 +657,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     if constexpr (HL) tmem_st16(ts + 16u * c, p16);
                     else kp_tmem_st8(ts + 16u * c, p16);
                 }
-                }
-                l = l * fac + (ls.x + ls.y) * kp_pow2(11 - (int)ev);
+                l = l * fac + (FAR ? (ls.x + ls.y) * kp_pow2(11 - (int)ev) : ls.x + ls.y);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -694,6 +686,7 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
         constexpr int HH = HD / 2, NH = HH >= KV4_GROUP ? HH / KV4_GROUP : 1;  // this half's dims, and its 64-dim groups
         const int g0 = half * HH / KV4_GROUP;
         bool ok = true;
+        [[maybe_unused]] uint32_t seen = 0;  // the largest scales (NaN: one of them is)
         // Warps 8..11 make K, 12..15 V. A thread takes 16 bytes of codes (32 dims) of token k_tok at a time, from quarter k_q on,
         // or word v_wd (8 dims) of tokens v_tok .. + 7: places in the stages and operands
         constexpr int KU = NG, VU = HD >= 128 ? HD / 128 : 1;
@@ -768,19 +761,24 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
             auto there = [&](int g, int j, int tok) { return (sh.valid[g & 7] >> (tok >> a.l.lbs) & 1u) && j * KA_TOK + tok < hi_lim; };
             // K of tile g (the row tile's j): 16 bytes of codes (32 dims of a token) at a time
             auto make_k = [&](int g, int j) {
-                if (!wtw(&sh.rkf[g % C::RK], g / C::RK) || !wtw(&sh.xf[g & 7], g >> 3)) return false;
+                if (!wtw(&sh.rkf[g % C::RK], g / C::RK) || (FAR && !wtw(&sh.xf[g & 7], g >> 3))) return false;
                 if (g >= NB && !wtw(&sh.ke[g % NB], g / NB - 1)) return false;
                 const uint8_t *raw = sm_kp + C::RK_OFF + (g % C::RK) * C::RAWK;
                 uint8_t *to = sm_kp + C::K_OFF + (g % NB) * C::TERMS * C::KT + k_dst;
                 const bool all = sh.valid[g & 7] >> 31;
-                // 2^(11 - e)
-                const float up = __uint_as_float(FAR && sh.kfar[g & 7] ? 265u - sh.kexp[g & 7][k_tok] << 23 : 0x7f000000u - __float_as_uint(sh.ek[g & 7]));
+                const bool keep = all || there(g, j, k_tok);
+                [[maybe_unused]] float up;  // 2^(11 - e)
+                if constexpr (FAR) up = __uint_as_float(sh.kfar[g & 7] ? 265u - sh.kexp[g & 7][k_tok] << 23 : 0x7f000000u - __float_as_uint(sh.ek[g & 7]));
 #pragma unroll 1
                 for (int x = 0; x < KU; ++x) {  // a 64-dim group each
                     const uint4 w4 = *(const uint4 *)(raw + k_src + x * a.l.bs * 32);
-                    float d = ka_half(raw + k_sc + x * a.l.bs * 2) * up;
-                    if (!all && !there(g, j, k_tok)) d = 0.0f;
-                    const uint32_t dd = ka_pack(d, d);
+                    uint32_t dd = *(const uint16_t *)(raw + k_sc + x * a.l.bs * 2) * 0x10001u;
+                    if constexpr (FAR) {
+                        const float d = ka_unpack(dd).x * up;
+                        dd = ka_pack(d, d);
+                    }
+                    if (!keep) dd = 0;
+                    if constexpr (!FAR) seen = kp_hmax2(seen, dd & 0x7fff7fffu);
                     const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
@@ -802,9 +800,9 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
             };
             // V of tile g: 8 tokens x 8 dims at a time, turned. Its buffer's last reader came before an O that has been added.
             auto make_v = [&](int g, int j) {
-                if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || !wtw(&sh.xf[g & 7], g >> 3)) return false;
+                if (!wtw(&sh.rvf[g % C::RV], g / C::RV) || (FAR && !wtw(&sh.xf[g & 7], g >> 3))) return false;
                 const uint8_t *raw = sm_kp + C::RV_OFF + (g % C::RV) * C::RAW;
-                const float up = kp_pow2(11 - (int)sh.ev[g & 7]);
+                [[maybe_unused]] const float up = FAR ? kp_pow2(11 - (int)sh.ev[g & 7]) : 1.0f;
                 const bool all = (sh.valid[g & 7] >> 31) && !(FAR && sh.any_bad[g & 7]), far = FAR && sh.vfar[g & 7];
 #pragma unroll 1
                 for (int un = 0; un < VU; ++un) {
@@ -817,13 +815,19 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     for (int y = 0; y < 8; ++y) w[y] = *(const uint32_t *)(src + y * 32);
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        float2 d = __fmul2_rn(ka_unpack(ss[y]), make_float2(up, up));
-                        if (!all) {
-                            const int tok = v_tok + 2 * y;
-                            if (!there(g, j, tok) || (FAR && !(fabsf(d.x) < INFINITY))) d.x = 0.0f;
-                            if (!there(g, j, tok + 1) || (FAR && !(fabsf(d.y) < INFINITY))) d.y = 0.0f;
+                        const int tok = v_tok + 2 * y;
+                        if constexpr (FAR) {
+                            float2 d = __fmul2_rn(ka_unpack(ss[y]), make_float2(up, up));
+                            if (!all) {
+                                if (!(there(g, j, tok) && fabsf(d.x) < INFINITY)) d.x = 0.0f;
+                                if (!(there(g, j, tok + 1) && fabsf(d.y) < INFINITY)) d.y = 0.0f;
+                            }
+                            dd[y] = ka_pack(d.x, d.y);
+                        } else {
+                            dd[y] = ss[y];
+                            if (!all) dd[y] &= (there(g, j, tok) ? 0xffffu : 0u) | (there(g, j, tok + 1) ? 0xffff0000u : 0u);
+                            seen = kp_hmax2(seen, dd[y] & 0x7fff7fffu);
                         }
-                        dd[y] = ka_pack(d.x, d.y);
                     }
                     uint8_t *at = sm_kp + C::V_OFF + (g % NB) * C::TERMS * C::VT + v_dst + un * 2048;
 #pragma unroll 1
@@ -913,18 +917,19 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                     const float2 f2 = make_float2(f, f);
                     uint32_t x[2][16];
                     tc_fence_after();
-                    if (!far)
+                    if (!far) {
 #pragma unroll
-                    for (int c = 0; c < HH; c += 32) {
-                        kp_tmem_ld16(to + c, x[0]);
-                        kp_tmem_ld16(to + c + 16u, x[1]);
-                        kp_tmem_wait_ld();
-                        kp_tmem_got(x[0]);
-                        kp_tmem_got(x[1]);
+                        for (int c = 0; c < HH; c += 32) {
+                            kp_tmem_ld16(to + c, x[0]);
+                            kp_tmem_ld16(to + c + 16u, x[1]);
+                            kp_tmem_wait_ld();
+                            kp_tmem_got(x[0]);
+                            kp_tmem_got(x[1]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(o[c / 2 + h * 8 + y], f2, kp_pair(x[h], y));
+                                for (int y = 0; y < 8; ++y) o[c / 2 + h * 8 + y] = __ffma2_rn(o[c / 2 + h * 8 + y], f2, kp_pair(x[h], y));
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -988,6 +993,8 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 for (int c = 0; c < HH / 2; c += 2) *(float4 *)(to + 2 * c) = make_float4(o[c].x, o[c].y, o[c + 1].x, o[c + 1].y);
             }
         }
+        if constexpr (!FAR)
+            if ((seen & 0xffffu) > KP_MOST || (seen >> 16) > KP_MOST) sh.met = 1;
     }
     // ---- everybody is here (the copies and MMAs of a CTA that gave up as well)
     tc_fence_before();
@@ -997,11 +1004,11 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
 }
 
 uint64_t kv4_prompt_workspace() {
-    return (uint64_t)std::min(num_sms(), KA_MAX_GRID) * 2 * KpCfg<256, true>::PART * 4;
+    return (uint64_t)std::min(num_sms(), KA_MAX_GRID) * 2 * KpCfg<256, true, false>::PART * 4;
 }
 
 template <int HD, bool HL> static cudaError_t prompt_go(Kv4AttnArgs a, int max_new, cudaStream_t s) {
-    using C = KpCfg<HD, HL>;
+    using C = KpCfg<HD, HL, false>;
     cudaError_t e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL, false>);
     if (e == cudaSuccess) e = allow_max_dynamic_smem(k_kv4_prompt<HD, HL, true>);
     if (e != cudaSuccess) return e;
@@ -1012,7 +1019,7 @@ template <int HD, bool HL> static cudaError_t prompt_go(Kv4AttnArgs a, int max_n
     const int grid = (int)std::min(std::max(units / 2, 1ll), (long long)std::min(num_sms(), KA_MAX_GRID));
     // outputs over q or gate could not be made twice
     if (!a.always) e = launch_k(k_kv4_prompt<HD, HL, false>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
-    if (e == cudaSuccess) e = launch_k(k_kv4_prompt<HD, HL, true>, dim3(grid), dim3(KP_THREADS), C::SMEM, s, a);
+    if (e == cudaSuccess) e = launch_k(k_kv4_prompt<HD, HL, true>, dim3(grid), dim3(KP_THREADS), KpCfg<HD, HL, true>::SMEM, s, a);
     if (e != cudaSuccess || grid == 1) return e;
     return launch_k(k_kv4_join<typename C::T, HD, KP_ROWS>, dim3(grid, KP_ROWS / 8), dim3(256), 0, s, a);
 }

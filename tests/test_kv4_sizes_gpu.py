@@ -254,3 +254,20 @@ def test_long_sums_of_one_sign_keep_bf16_rows(fn, kv4, ws):
     # every request has the same answer; its 8 x 63 outputs round alike, so the dims are what is averaged over
     tol = 2.0 ** -12 + 2 * 2.0 ** -9 / 63 ** 0.5
     assert float(rel.mean((1, 2)).abs().max()) <= tol, rel.mean()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new, group", FORMS)
+def test_outputs_in_the_place_of_the_rows(fn, kv4, ws, new, group, dtype):
+    """out is q's own memory: the same values, also where the kernel for prompts has to do a call again (values past 65504)."""
+    rng = np.random.default_rng(12)
+    for size in (1.0, 2e5):
+        v = np.clip(normal(rng, 300, 1, 128) * size, -5e5, 5e5)  # scales within fp16
+        c = Case(fn, kv4, ws, normal(rng, 300, 1, 128), v, normal(rng, new, group, 128), dtype=dtype)
+        c.check()
+        want, q = c.run(), c.q.clone()
+        c.c.attn(q, i32(0, new), i32(300), c.table, new, out=q)
+        fn.sync(torch.cuda.current_stream().cuda_stream)
+        # another form of the kernel may round apart by twice what each is allowed
+        tol = (4e-5 + 2.0 ** -18 * 10 if dtype == "f32" else 2.0 ** -6) * 5 * size
+        assert np.abs(q.double().cpu().numpy() - want).max() <= tol
