@@ -507,8 +507,9 @@ template <int HD, bool HL, bool FAR> __global__ void __launch_bounds__(KP_THREAD
                 for (int j = 0; j <= n && ok; ++j) {
                     if (j < n) {
                         const int g = g0 + j;
-                        // (S takes the place of P of tile g - 2, which the workers may still read)
-                        ok = wtw(&sh.kf[g % NB], g / NB) && (!FAR || g < 2 || !sh.vfar[(g - 2) & 7] || wtw(&sh.oe, g - 2));
+                        // S takes the place of P of tile g - 2, which the workers may still read. (Not where that is of the row tile before: q came
+                        // after it had been added, and its phase of oe, two ago by now, would look like the one to come.)
+                        ok = wtw(&sh.kf[g % NB], g / NB) && (!FAR || j < 2 || !sh.vfar[(g - 2) & 7] || wtw(&sh.oe, g - 2));
                         if (!ok) break;
                         tc_fence_after();
                         if (kp_elect()) {

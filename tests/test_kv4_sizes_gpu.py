@@ -271,3 +271,53 @@ def test_outputs_in_the_place_of_the_rows(fn, kv4, ws, new, group, dtype):
         # another form of the kernel may round apart by twice what each is allowed
         tol = (4e-5 + 2.0 ** -18 * 10 if dtype == "f32" else 2.0 ** -6) * 5 * size
         assert np.abs(q.double().cpu().numpy() - want).max() <= tol
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd, bs", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("large", ["values", "keys", "scores", "none"])
+def test_many_prompts_with_large_values(fn, kv4, ws, hd, bs, dtype, large):
+    """Several row tiles and some 70 tiles to a CTA, split row tiles among them, with scales past 8188 here and there: both forms of the
+    kernel for prompts over long runs."""
+    n, nkv, group, new, length = 4, 4, 2, 600, 1500
+    g = torch.Generator("cuda").manual_seed(hd)
+    per = -(-length // bs)
+    table = torch.randperm(n * per, generator=torch.Generator().manual_seed(2)).to(torch.int32).reshape(n, per).cuda()
+    slots = (table.long()[:, :, None] * bs + torch.arange(bs, device="cuda")).reshape(n, -1)[:, :length].contiguous()
+    k, v = torch.randn(2, n, length, nkv, hd, device="cuda", generator=g)
+    few = (torch.rand(n, length, nkv, 1, device="cuda", generator=g) < 0.01).float()
+    q = torch.randn(n * new, nkv * group, hd, device="cuda", generator=g) * (1e7 if large == "scores" else 0.5)
+    if large == "values":
+        v *= 1 + 1e5 * few
+    if large == "keys":  # tiny but for a few, which only some rows weigh
+        k *= 1e-3 + 1e5 * few
+        q *= 1e-5
+    c = kv4.KV4Cache(fn, nkv, hd, bs, n * per, ws)
+    c.store(k.flatten(0, 1), v.flatten(0, 1), slots.flatten())
+    q = q.to(DT[dtype])
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda") * new
+    args = (cu, torch.full((n,), length, dtype=torch.int32, device="cuda"), table, new)
+    out = c.attn(q, *args)
+    fn.sync(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(out, c.attn(q, *args))  # the same bits again
+    hide = torch.arange(length, device="cuda")[None, :] > torch.arange(length - new, length, device="cuda")[:, None]
+    for r in range(n):
+        lk, lv = (x.double() for x in c.load(slots[r]))
+        for h in range(nkv * group):
+            qh, kh, vh = q[r * new:(r + 1) * new, h].double(), lk[:, h // group], lv[:, h // group]
+            s = (qh @ kh.T / hd ** 0.5).masked_fill(hide, float("-inf"))
+            want = torch.softmax(s, -1) @ vh
+            S = (qh.abs() @ kh.abs().T / hd ** 0.5).masked_fill(hide, 0.0).amax(-1, keepdim=True)
+            V = torch.cummax(vh.abs().reshape(length, -1, 64).amax(-1), 0).values[length - new:].repeat_interleave(64, 1)
+            got = out[r * new:(r + 1) * new, h].double()
+            assert got.isfinite().all()
+            if dtype == "f32":
+                tol = (2e-5 + 2.0 ** -19 * S) * V
+            else:
+                tol = 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -11 * S) * V
+            if large != "scores":
+                assert ((got - want).abs() <= tol).all(), (r, h)
+            else:  # rows whose best key leads by more than the scores' rounding are its value
+                two = s.topk(2, -1).values
+                led = two[:, 0] - two[:, 1] > (2.0 ** -18 if dtype == "f32" else 2.0 ** -10) * S[:, 0] + 60
+                assert led.any() and ((got - want).abs()[led] <= ((2e-5 if dtype == "f32" else 2.0 ** -8) * V)[led]).all(), (r, h)
