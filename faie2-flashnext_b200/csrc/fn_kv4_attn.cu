@@ -18,9 +18,10 @@
 // bits below its nominal size; so both first halves are whole numbers up to 2^11 (q scaled per row by a power of two, p dv
 // by one per row and block): all their products and sums are multiples of one unit, and exact. Floating halves lost 2.5e-6
 // of the output where this form loses 3e-7. Sums over more than 32 tokens are added in fp32 outside the tensor core, whose
-// own accumulation cuts instead of rounding (bf16 rows: where a CTA has many tokens of a row, KA_LONG). The softmax runs in base 2 with the running
-// maximum of a row's scores as its reference; p dv is scaled by the exponent of the largest |dv| that the row has seen in the same 64
-// dims, so that it uses fp16's range whatever the size of V is, there, in other blocks, and in tokens that the row does not see.
+// own accumulation cuts instead of rounding (bf16 rows: where a CTA may have many tokens of a row, KA_LONG). The softmax runs in
+// base 2 with the running maximum of a row's scores as its reference; p dv is scaled by the exponent of the largest |dv| that the row has
+// seen in the same 64 dims, so that it uses fp16's range whatever the size of V is, there, in other blocks, and in tokens that the row
+// does not see. (That scale, looked at for every 32 tokens, costs 2 to 5 % of the time beside one scale for the whole row tile.)
 //
 // Work. A unit is 64 tokens of one kv head for one row tile (8 or 16 rows: the heads of a group, token after token). All
 // units of the call in a row are cut into equal runs, one per CTA, whatever request they belong to: each CTA finds its run
@@ -29,9 +30,9 @@
 // of the CTAs, so the result does not depend on timing (joining in the CTA that finishes last cost 20 us of latency chains
 // for 147 parts, where the second kernel takes 6 to 8).
 //
-// What bounds it, and measured (device time): one request of 131071 tokens, bf16, 16 heads over 2 kv heads of 256 (71 MB) 27.8 us,
-// of which 15 us in the page loop (4.7 TB/s); 32 requests of 65 to 4096 tokens, fp32 25.1 us; 64 requests of 100 to 8192 tokens,
-// bf16, 32 heads over 8 of 128 (298 MB) 77 us (3.9 TB/s, issue of the page loop); one request of 77 tokens 8.2 us, a chain of round
+// What bounds it, and measured (device time): one request of 131071 tokens, bf16, 16 heads over 2 kv heads of 256 (71 MB) 28.9 us,
+// of which some 16 us in the page loop (4.4 TB/s); 32 requests of 65 to 4096 tokens, fp32 25.5 us; 64 requests of 100 to 8192 tokens,
+// bf16, 32 heads over 8 of 128 (298 MB) 79.6 us (3.7 TB/s, issue of the page loop); one request of 77 tokens 8.7 us, a chain of round
 // trips to memory.
 //
 // A CTA: one warp copies pages into a ring (one bulk copy per page and head: codes and scales of K and V), four warps
@@ -802,7 +803,12 @@ template <int HD, bool HL, int NT> static cudaError_t attn_launch(const Kv4AttnA
         return launch_k(k_kv4_join_few<T, HD, C::ROWS>, dim3(std::min(grid, KJ_GRID), C::ROWS), dim3(32 * KJ_WARPS), 0, s, a, grid);
     return launch_k(k_kv4_join<T, HD, C::ROWS>, dim3(grid, C::ROWS / 8), dim3(256), 0, s, a);
 }
-constexpr int KP_FROM = 64;  // rows of a request from which the prompts' kernel takes it (16 requests: equal at 48 rows, 64 against 53 us at 64; one request of 16k tokens: 31 against 39 us at 64, equal near 112)
+// Rows of a request (the largest, by max_new) from which the prompts' kernel takes the call. Measured with 128 dims, 8 heads to each of 4 kv
+// heads, fp32 (bf16), this kernel against the prompts': 16 requests of 2000 tokens, 64 rows 49 against 51 us (37 against 42), 80 rows 58
+// against 51 (44 against 43). It looks at rows alone: one request of 2000 tokens takes 19 against 34 us (16 against 29) at 64 rows and 29 against
+// 38 at 192, one of 16384 is equal at 128 (53 us), so single requests of 64 to some 128 rows get the slower kernel, and so do decoding
+// requests beside a prompt in the same call.
+constexpr int KP_FROM = 64;
 
 template <int HD> static cudaError_t attn_go(const Kv4AttnArgs &a, bool f32, int max_new, cudaStream_t s) {
     const long long rows = (long long)std::min(max_new, a.rows) * a.group;

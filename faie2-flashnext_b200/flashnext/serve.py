@@ -52,9 +52,10 @@ class ServeModel(BatchDecodeModel):
 
     def launches_per_step(self) -> int:
         """As the batched step's; two plans instead of the step counter, four attention kernels (norm + RoPE, store, attention
-        and its join) instead of two."""
+        and its join, which a single place of up to 128 tokens does without) instead of two."""
         attn = sum(L["kind"] != "G" for L in self.layers)
-        return super().launches_per_step() + 2 * attn + 1
+        join = self.B > 1 or self.table.shape[1] * self.page_size > 128
+        return super().launches_per_step() + (1 + join) * attn + 1
 
     def _embed(self, s):
         """The step's plan (places that are dropped give their pages back, then every place gets a row), then its inputs."""
