@@ -9,6 +9,7 @@
 #pragma once
 
 #include "fn_engine.h"
+#include "fn_rows.h"
 #include "faie2fn.h"
 
 namespace fn {

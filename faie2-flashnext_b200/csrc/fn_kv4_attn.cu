@@ -855,21 +855,8 @@ FN_API int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh
         const int64_t size = f32 ? 4 : 2;
         a.vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0 && out_token * size % 16 == 0 &&
                 (!gate || ((uintptr_t)gate % 16 == 0 && gate_token * size % 16 == 0 && gate_head * size % 16 == 0));
-        // whether rows of out may be rows of q or gate (by their first and last bytes)
-        struct Span {
-            intptr_t lo, hi;
-        };
-        auto span = [&](const void *p, int64_t token, int64_t head) {
-            const int64_t t = (rows - 1) * token, h = (nh - 1) * head;
-            return Span{(intptr_t)p + (std::min<int64_t>(t, 0) + std::min<int64_t>(h, 0)) * size,
-                        (intptr_t)p + (std::max<int64_t>(t, 0) + std::max<int64_t>(h, 0) + c->hd) * size};
-        };
-        const Span so = span(out, out_token, c->hd), sq = span(q, q_token, q_head);
-        a.always = so.lo < sq.hi && sq.lo < so.hi;
-        if (gate) {
-            const Span sg = span(gate, gate_token, gate_head);
-            a.always |= so.lo < sg.hi && sg.lo < so.hi;
-        }
+        a.always = kv4_rows_meet(out, out_token, c->hd, q, q_token, q_head, rows, nh, c->hd, size) ||
+                   (gate && kv4_rows_meet(out, out_token, c->hd, gate, gate_token, gate_head, rows, nh, c->hd, size));
         const cudaStream_t s = (cudaStream_t)stream;
         const cudaError_t e = c->hd == 64 ? attn_go<64>(a, f32, max_new, s)
                             : c->hd == 128 ? attn_go<128>(a, f32, max_new, s)

@@ -321,3 +321,22 @@ def test_many_prompts_with_large_values(fn, kv4, ws, hd, bs, dtype, large):
                 two = s.topk(2, -1).values
                 led = two[:, 0] - two[:, 1] > (2.0 ** -18 if dtype == "f32" else 2.0 ** -10) * S[:, 0] + 60
                 assert led.any() and ((got - want).abs()[led] <= ((2e-5 if dtype == "f32" else 2.0 ** -8) * V)[led]).all(), (r, h)
+
+
+@pytest.mark.parametrize("new, group", FORMS)
+def test_rows_and_outputs_as_columns_of_one_buffer(fn, kv4, ws, new, group):
+    """q, gate and out beside each other in the rows of one buffer: the same bits as apart."""
+    rng = np.random.default_rng(13)
+    c = Case(fn, kv4, ws, normal(rng, 300, 1, 128), normal(rng, 300, 1, 128), normal(rng, new, group, 128))
+    a = (i32(0, new), i32(300), c.table, new)
+    gate = torch.from_numpy(normal(rng, new, group, 128)).float().cuda()
+    want = c.c.attn(c.q, *a, gate=gate)
+    w = group * 128
+    for order in ((0, 1, 2), (2, 0, 1), (1, 2, 0)):
+        buf = torch.zeros(new, 3 * w, device="cuda")
+        q, g, out = (buf[:, i * w:(i + 1) * w].unflatten(1, (group, 128)) for i in order)
+        q.copy_(c.q)
+        g.copy_(gate)
+        c.c.attn(q, *a, gate=g, out=out)
+        fn.sync(torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out, want) and torch.equal(q, c.q) and torch.equal(g, gate)

@@ -65,3 +65,38 @@ def test_tensors_of_another_device_are_refused():
     z = [torch.zeros(s, dtype=torch.int32) for s in ((2,), (2,), (2, 3), (4,), (1,))]
     with pytest.raises(ValueError, match="cuda"):
         kv4.KV4Planner(None, 16).plan(*z, 4)
+
+
+def test_rows_that_may_meet_are_found(tmp_path):
+    """Whether outputs may lie over q or gate, against every element of small layouts: nothing that does is missed, and columns of one
+    buffer that do not are told apart."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "faie2-flashnext_b200", "csrc")
+    (tmp_path / "meet.cpp").write_text("""
+#include <random>
+#include <set>
+#include "fn_rows.h"
+int main() {
+    std::mt19937 g(1);
+    auto in = [&](int lo, int hi) { return (int64_t)(lo + (int)(g() % (unsigned)(hi - lo + 1))); };
+    int told = 0;
+    for (int i = 0; i < 200000; ++i) {
+        const int64_t rows = in(1, 4), nh = in(1, 3), hd = in(1, 4), ah = hd, bh = in(0, 3) ? hd + in(0, 3) : 2 * hd;
+        const int64_t wide = (nh - 1) * bh + hd, at = in(0, 2) ? wide + in(0, 12) : in(0, 20), bt = in(0, 1) ? at : in(0, 20);
+        const int64_t a = 1000 + in(-60, 60), b = 1000;
+        std::set<int64_t> s;
+        bool meet = false;
+        for (int r = 0; r < rows; ++r)
+            for (int h = 0; h < nh; ++h)
+                for (int d = 0; d < hd; ++d) s.insert(b + r * bt + h * bh + d);
+        for (int r = 0; r < rows; ++r)
+            for (int h = 0; h < nh; ++h)
+                for (int d = 0; d < hd; ++d) meet |= s.count(a + r * at + h * ah + d) != 0;
+        const bool said = fn::kv4_rows_meet((void *)(a * 4), at, ah, (void *)(b * 4), bt, bh, rows, nh, hd, 4);
+        if (meet && !said) return 1;
+        told += !said && a - b < (rows - 1) * bt && b - a < (rows - 1) * at;  // within one another's rows
+    }
+    return told > 1000 ? 0 : 2;
+}
+""")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-I", csrc, str(tmp_path / "meet.cpp"), "-o", str(tmp_path / "meet")], check=True)
+    assert subprocess.run([str(tmp_path / "meet")]).returncode == 0
