@@ -21,7 +21,9 @@
 // own accumulation cuts instead of rounding (bf16 rows: where a CTA may have many tokens of a row, KA_LONG). The softmax runs in
 // base 2 with the running maximum of a row's scores as its reference; p dv is scaled by the exponent of the largest |dv| that the row has
 // seen in the same 64 dims, so that it uses fp16's range whatever the size of V is, there, in other blocks, and in tokens that the row
-// does not see. (That scale, looked at for every 32 tokens, costs 2 to 5 % of the time beside one scale for the whole row tile.)
+// does not see. (That scale, looked at for every 32 tokens, costs 2 to 5 % of the time beside one scale for the whole row tile; fp32
+// rows' weights beside the largest of their own 32 tokens, and the sum of the rounded ones, another 1.5 %: errors against 64 bits 5.8e-7 ->
+// 3.8e-7 at 77 tokens, 1.7e-6 -> 5.2e-7 at 100 thousand.)
 //
 // Work. A unit is 64 tokens of one kv head for one row tile (8 or 16 rows: the heads of a group, token after token). All
 // units of the call in a row are cut into equal runs, one per CTA, whatever request they belong to: each CTA finds its run
@@ -30,9 +32,9 @@
 // of the CTAs, so the result does not depend on timing (joining in the CTA that finishes last cost 20 us of latency chains
 // for 147 parts, where the second kernel takes 6 to 8).
 //
-// What bounds it, and measured (device time): one request of 131071 tokens, bf16, 16 heads over 2 kv heads of 256 (71 MB) 28.9 us,
-// of which some 16 us in the page loop (4.4 TB/s); 32 requests of 65 to 4096 tokens, fp32 25.5 us; 64 requests of 100 to 8192 tokens,
-// bf16, 32 heads over 8 of 128 (298 MB) 79.6 us (3.7 TB/s, issue of the page loop); one request of 77 tokens 8.7 us, a chain of round
+// What bounds it, and measured (device time): one request of 131071 tokens, bf16, 16 heads over 2 kv heads of 256 (71 MB) 29.3 us,
+// of which some 16 us in the page loop (4.4 TB/s); 32 requests of 65 to 4096 tokens, fp32 26.0 us; 64 requests of 100 to 8192 tokens,
+// bf16, 32 heads over 8 of 128 (298 MB) 79.5 us (3.7 TB/s, issue of the page loop); one request of 77 tokens 9.0 us, a chain of round
 // trips to memory.
 //
 // A CTA: one warp copies pages into a ring (one bulk copy per page and head: codes and scales of K and V), four warps
@@ -430,12 +432,14 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
                         if (!M || !hidden(b, h, lm)) d = fmaxf(d, fabsf(dv[b][h][gi]));
                 return d;
             };
-            // ---- running softmax in base 2: p = exp2(s - maximum), |p dv up| < 2^11
+            // ---- running softmax in base 2: p = exp2(s - maximum), |p dv up| < 2^11. fp32 rows: the maximum of these 32 tokens, so that
+            // their weights have all of their bits beside one another, whatever came before; the sums of the 32 come to the running
+            // maximum's unit as they are added (100k tokens: 1.7e-6 off 64 bits otherwise)
             float2 mx[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float2 rs = *(const float2 *)&s_rs[8 * n + 2 * t];
-                mx[n] = m[n];
+                mx[n] = HL ? make_float2(-INFINITY, -INFINITY) : m[n];
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -467,10 +471,17 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
             }
             bool moved = false, grown = false;
             float2 z[NT];  // minus the maximum (0 for a row that has seen nothing)
+            [[maybe_unused]] float2 unit[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                if constexpr (HL) {
+                    const float2 here = mx[n];
+                    mx[n] = make_float2(fmaxf(m[n].x, here.x), fmaxf(m[n].y, here.y));
+                    unit[n] = make_float2(here.x == -INFINITY ? 0.0f : ka_exp2(here.x - mx[n].x), here.y == -INFINITY ? 0.0f : ka_exp2(here.y - mx[n].y));
+                    z[n] = make_float2(here.x == -INFINITY ? 0.0f : -here.x, here.y == -INFINITY ? 0.0f : -here.y);
+                }
                 moved |= mx[n].x != m[n].x || mx[n].y != m[n].y;
-                z[n] = make_float2(mx[n].x == -INFINITY ? 0.0f : -mx[n].x, mx[n].y == -INFINITY ? 0.0f : -mx[n].y);
+                if constexpr (!HL) z[n] = make_float2(mx[n].x == -INFINITY ? 0.0f : -mx[n].x, mx[n].y == -INFINITY ? 0.0f : -mx[n].y);
             }
             if constexpr (M) {
 #pragma unroll
@@ -495,7 +506,7 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
                 float2 f[NT][NG];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float2 fm = make_float2(ka_exp2(m[n].x + z[n].x), ka_exp2(m[n].y + z[n].y));
+                    const float2 fm = make_float2(m[n].x == -INFINITY ? 0.0f : ka_exp2(m[n].x - mx[n].x), m[n].y == -INFINITY ? 0.0f : ka_exp2(m[n].y - mx[n].y));
                     l[n] = __fmul2_rn(l[n], fm);
                     m[n] = mx[n];
 #pragma unroll
@@ -551,15 +562,17 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
                     }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float2 x = __fadd2_rn(sc[n][b][h], z[n]);
                         sc[n][b][h] = make_float2(ka_exp2(x.x), ka_exp2(x.y));
-                        l[n] = __fadd2_rn(l[n], sc[n][b][h]);
                     }
+                const float2 sum = __fadd2_rn(__fadd2_rn(sc[n][0][0], sc[n][0][1]), __fadd2_rn(sc[n][1][0], sc[n][1][1]));
+                l[n] = HL ? __ffma2_rn(sum, unit[n], l[n]) : __fadd2_rn(l[n], sum);
+            }
             if constexpr (M) {
                 // (below, what weighs nothing counts for nothing, hidden NaN scales among it; a NaN that a row sees counts)
                 bool odd = false;
@@ -603,21 +616,23 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
                             x = __fmul2_rn(sc[n][b][h], x);
                             // a token that a row does not see weighs nothing whatever its scale is (NaN)
                             if constexpr (M) x = make_float2(sc[n][b][h].x == 0.0f ? 0.0f : x.x, sc[n][b][h].y == 0.0f ? 0.0f : x.y);
+                            // (the sum is of the rounded weights, so that the 8 of a code cancels and their rounding counts c - 8 times, not c)
                             if constexpr (HL) {
-                                add[b][h] = x;
                                 const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 2^23: rounds to whole numbers
                                 const float2 w = __fadd2_rn(__fadd2_rn(x, big), make_float2(-12582912.0f, -12582912.0f));
                                 const float2 r = __ffma2_rn(w, make_float2(-1.0f, -1.0f), x);
+                                const uint32_t rest = ka_pack(r.x, r.y);
                                 P[n][b][h] = ka_turn(ka_pack(w.x, w.y));
-                                Q[n][b][h] = ka_turn(ka_pack(r.x, r.y));
+                                Q[n][b][h] = ka_turn(rest);
+                                add[b][h] = __fadd2_rn(w, ka_unpack(rest));
                             } else {
-                                // (of the rounded weights, so that the 8 of a code cancels and their rounding counts c - 8 times, not c)
                                 const uint32_t w = ka_pack(x.x, x.y);
                                 add[b][h] = ka_unpack(w);
                                 P[n][b][h] = ka_turn(w);
                             }
                         }
-                    corr[n][gi] = __fadd2_rn(corr[n][gi], __fadd2_rn(__fadd2_rn(add[0][0], add[0][1]), __fadd2_rn(add[1][0], add[1][1])));
+                    const float2 sum = __fadd2_rn(__fadd2_rn(add[0][0], add[0][1]), __fadd2_rn(add[1][0], add[1][1]));
+                    corr[n][gi] = HL ? __ffma2_rn(sum, unit[n], corr[n][gi]) : __fadd2_rn(corr[n][gi], sum);
                 }
                 uint4 A[4][2];
 #pragma unroll
@@ -650,7 +665,8 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
                         for (int by = 0; by < 4; ++by)
 #pragma unroll
                             for (int x = 0; x < 4; x += 2) {
-                                const float2 y = __fadd2_rn(make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]), make_float2(acc[by][x], acc[by][x + 1]));
+                                const float2 a2 = make_float2(acc[by][x], acc[by][x + 1]), o2 = make_float2(o[n][gi][by][x], o[n][gi][by][x + 1]);
+                                const float2 y = HL ? __ffma2_rn(a2, unit[n], o2) : __fadd2_rn(o2, a2);
                                 o[n][gi][by][x] = y.x, o[n][gi][by][x + 1] = y.y;
                             }
                     } else {

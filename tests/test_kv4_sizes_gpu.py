@@ -340,3 +340,29 @@ def test_rows_and_outputs_as_columns_of_one_buffer(fn, kv4, ws, new, group):
         c.c.attn(q, *a, gate=g, out=out)
         fn.sync(torch.cuda.current_stream().cuda_stream)
         assert torch.equal(out, want) and torch.equal(q, c.q) and torch.equal(g, gate)
+
+
+@pytest.mark.parametrize("new, group", [(1, 8), (6, 2)])
+def test_flat_rows_over_long_contexts(fn, kv4, ws, new, group):
+    """fp32 rows whose weights are spread over 60000 tokens, none near the largest: errors of a weight (exp2's 2^-22.5, its two halves' 2^-23
+    of the largest among 32 tokens) average out as the output itself does, which is some 2.5 times below the sum that the codes' 8 is
+    taken back from: 2.5 x 2^-22 = 6e-7 of the output's norm, 1e-6 allowed."""
+    n, nkv, hd, bs, length = 2, 1, 64, 64, 60000
+    per = -(-length // bs)
+    c = kv4.KV4Cache(fn, nkv, hd, bs, n * per, ws)
+    g = torch.Generator("cuda").manual_seed(1)
+    k, v = torch.randn(2, n * per * bs, nkv, hd, device="cuda", generator=g)
+    slots = torch.arange(n * per * bs, device="cuda")
+    c.store(k, v, slots)
+    q = torch.randn(n * new, nkv * group, hd, device="cuda", generator=g)
+    table = torch.arange(n * per, dtype=torch.int32, device="cuda").reshape(n, per)
+    out = c.attn(q, i32(0, new, 2 * new), i32(length, length), table, new).double()
+    fn.sync(torch.cuda.current_stream().cuda_stream)
+    hide = torch.arange(length, device="cuda")[None, :] > torch.arange(length - new, length, device="cuda")[:, None]
+    for r in range(n):
+        lk, lv = (x[:, 0].double() for x in c.load(slots[r * per * bs:r * per * bs + length]))
+        for h in range(group):
+            rows = slice(r * new, (r + 1) * new)
+            s = (q[rows, h].double() @ lk.T / 8).masked_fill(hide, float("-inf"))
+            want = torch.softmax(s, -1) @ lv
+            assert float((out[rows, h] - want).norm() / want.norm()) <= 1e-6
