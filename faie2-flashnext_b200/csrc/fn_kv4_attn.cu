@@ -327,6 +327,8 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
         // p dv is scaled by ug = 2^(10 - e) of the largest |dv| that the row has seen in a group, the same for all rows until the tiles that
         // some see a part of; from there on (own) each row's is in s_up, by its exponent. -24 is the least e of an fp16 number.
         float ug[NG];
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) ug[gi] = 17179869184.0f;
         bool own = false;
         auto inverse = [](float a) { return __uint_as_float(0x7f000000u - __float_as_uint(a)); };  // of a power of two
         auto row_up = [&](int n, int gi) {
@@ -334,8 +336,6 @@ template <int HD, bool HL, int NT, bool LONG> __global__ void __launch_bounds__(
             const uint8_t *e = s_up + (warp * NG + gi) * ROWS + 8 * n + 2 * t;
             return make_float2(__uint_as_float((uint32_t)e[0] << 23), __uint_as_float((uint32_t)e[1] << 23));
         };
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) ug[gi] = 17179869184.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             lim[n][0] = limit(8 * n + 2 * t);

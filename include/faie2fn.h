@@ -333,9 +333,10 @@ int fn_kv4_load(const fn_kv4_t *c, uint32_t type, const int64_t *slots, int nt, 
  * cu[r + 1]) stands at position kv_len[r] - (cu[r + 1] - cu[r]) + its index and sees the keys up to itself; a row that
  * sees none, or belongs to no request, comes out zero. nh query heads, head h reading kv head h / (nh / nkv) (nh / nkv
  * <= 64). q, gate (NULL: none): rows x nh x hd with token and head strides in elements; out: token stride, heads
- * adjacent; all of `type`, fp32 inside. table: page ids as fn_kv4_plan makes them ([n][max_pages]). max_new: the most rows of a request,
- * or a bound (it chooses the kernel and the number of its CTAs, not the result's definition; too small a one costs time only). ws: fn_kv4_attn_workspace() bytes of device
- * memory, 256-byte aligned, whatever they hold; calls that may overlap need one each. */
+ * adjacent; all of `type`, fp32 inside. table: page ids as fn_kv4_plan makes them ([n][max_pages]). max_new: the most
+ * rows of a request, or a bound (it chooses the kernel and the number of its CTAs, not the result's definition; too
+ * small a one costs time only). ws: fn_kv4_attn_workspace() bytes of device memory, 256-byte aligned, whatever they
+ * hold; calls that may overlap need one each. */
 uint64_t fn_kv4_attn_workspace(void);
 int fn_kv4_attn(const fn_kv4_t *c, uint32_t type, int n, int rows, int nh, const void *q, int64_t q_token, int64_t q_head,
                 const void *gate, int64_t gate_token, int64_t gate_head, void *out, int64_t out_token, const int *cu,
