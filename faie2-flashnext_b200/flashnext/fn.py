@@ -43,6 +43,7 @@ EXPORTS = [
     "fn_dev_gb", "fn_split", "fn_model_dims",
     "fn_kv4_plan", "fn_kv4_plan_next", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
     "fn_qk_rope_rows", "fn_gdn_reset_seq",
+    "fn_logprobs",
 ]
 
 
@@ -145,6 +146,7 @@ class FN:
                                   vp, C.c_int, C.c_int, C.c_float, vp, C.c_uint64, vp]
         d.fn_qk_rope_rows.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float, vp]
         d.fn_gdn_reset_seq.argtypes = [C.c_int, C.c_int, vp]
+        d.fn_logprobs.argtypes = [C.c_uint32, vp, i64, C.c_int, C.c_int] + [vp] * 4 + [C.c_int] + [vp] * 3
         d.fn_tc_create.argtypes = [C.c_uint32, U8, C.c_int, C.c_int]
         d.fn_tc_free.argtypes = [C.c_int]
         d.fn_tc_gemv.argtypes = [C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp]
@@ -528,6 +530,13 @@ class FN:
     def gdn_reset_seq(self, h, seq, stream=0):
         """Zero one sequence's state of a batched DeltaNet handle."""
         self.check(self.d.fn_gdn_reset_seq(h, seq, stream))
+
+    # ---- scores of tokens (device pointers, 0 = null; flashnext/logprobs.py is the layer over torch tensors) ----
+    def logprobs(self, dtype, logits, stride, rows, vocab, tokens, logprob, rank, entropy, top, top_ids, top_logprobs,
+                 stream=0):
+        """dtype: ggml type id of the logits (0 = F32, 30 = BF16); stride in elements."""
+        self.check(self.d.fn_logprobs(dtype, logits, stride, rows, vocab, tokens, logprob, rank, entropy, top, top_ids,
+                                      top_logprobs, stream))
 
     # ---- L2 prefetch hints of a decode chain ----
     def w_weights(self, h):

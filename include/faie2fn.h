@@ -354,6 +354,18 @@ int fn_qk_rope_rows(const float *q, int64_t q_token, int64_t q_head, const float
  * stream: its place is given to a new request. */
 int fn_gdn_reset_seq(int h, int seq, void *stream);
 
+/* ---- scores of tokens (no counterpart in the reference, which answers with the argmax alone, engine/faie2fn.cu:1910-1935) --
+ * Of every row of logits [rows][vocab] (device memory, F32 (0) or BF16 (30), `stride` elements from row to row, entries adjacent;
+ * vocab 1..2^30), in one launch: logprob [rows] = logits[t] - ln sum e^logits of the row's token t = tokens[row]; rank [rows] =
+ * the entries that stand before t, larger ones first, equal ones by the lower index (-0 equals +0); entropy [rows] = -sum p ln p;
+ * top_ids, top_logprobs [rows][top] = the first `top` (0..32) entries of that order. Any of logprob, rank, entropy may be NULL;
+ * tokens may be NULL if logprob and rank are. Entries at -inf have no probability and are no alternatives; places that stay empty
+ * hold -1 and -inf. tokens[row] < 0: no token, logprob 0 and rank -1; past the vocabulary: NaN and -1, reported by fn_sync. A row
+ * with a NaN or +inf has logprob, entropy and top_logprobs NaN (a NaN is no alternative, and its rank is -1); a row of nothing but
+ * -inf has log probabilities -inf and entropy 0. Sums are fp32. Allocates nothing, keeps nothing: calls may overlap. */
+int fn_logprobs(uint32_t type, const void *logits, int64_t stride, int rows, int vocab, const int *tokens, float *logprob,
+                int *rank, float *entropy, int top, int *top_ids, float *top_logprobs, void *stream);
+
 /* ---- the decode step (the reference's layer_forward + forward, engine/faie2fn.cu:2370-2490) --------------------
  * One step of the hybrid MoE decoder over resident handles (fn_w_create, fn_gdn_create, fn_moe_create) and device
  * buffers the caller owns: the embedding row of tokens[*pos], per layer the input projection, the gated-DeltaNet core
