@@ -43,7 +43,7 @@ EXPORTS = [
     "fn_dev_gb", "fn_split", "fn_model_dims",
     "fn_kv4_plan", "fn_kv4_plan_next", "fn_kv4_store", "fn_kv4_load", "fn_kv4_attn_workspace", "fn_kv4_attn",
     "fn_qk_rope_rows", "fn_gdn_reset_seq",
-    "fn_logprobs",
+    "fn_logprobs", "fn_fp8_rows", "fn_fp8_blocks", "fn_fp8_product",
 ]
 
 
@@ -66,6 +66,11 @@ class FnModel(C.Structure):
 class FnKv4(C.Structure):
     """fn_kv4_t (include/faie2fn.h): a paged 4-bit KV cache."""
     _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_int), ("page_size", C.c_int), ("nkv", C.c_int), ("hd", C.c_int)]
+
+
+class FnFp8(C.Structure):
+    """fn_fp8_t (include/faie2fn.h): an 8-bit weight."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int)]
 
 
 class FN:
@@ -147,6 +152,9 @@ class FN:
         d.fn_qk_rope_rows.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_float, vp]
         d.fn_gdn_reset_seq.argtypes = [C.c_int, C.c_int, vp]
         d.fn_logprobs.argtypes = [C.c_uint32, vp, i64, C.c_int, C.c_int] + [vp] * 4 + [C.c_int] + [vp] * 3
+        d.fn_fp8_rows.argtypes = [C.c_uint32, vp, i64, vp, i64, vp, C.c_float, C.c_int, C.c_int, vp, i64, vp, i64, vp, vp, vp]
+        d.fn_fp8_blocks.argtypes = [C.c_uint32, vp, i64, C.c_int, C.c_int, vp, vp, vp]
+        d.fn_fp8_product.argtypes = [C.POINTER(FnFp8), vp, vp, C.c_int, C.c_uint32, vp, i64, vp, i64, vp]
         d.fn_tc_create.argtypes = [C.c_uint32, U8, C.c_int, C.c_int]
         d.fn_tc_free.argtypes = [C.c_int]
         d.fn_tc_gemv.argtypes = [C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, vp]
@@ -530,6 +538,20 @@ class FN:
     def gdn_reset_seq(self, h, seq, stream=0):
         """Zero one sequence's state of a batched DeltaNet handle."""
         self.check(self.d.fn_gdn_reset_seq(h, seq, stream))
+
+    # ---- 8-bit rows and weights (device pointers, 0 = null; flashnext/fp8.py is the layer over torch tensors) ----
+    def fp8_rows(self, dtype, x, x_stride, add, add_stride, weight, eps, rows, cols, total, total_stride, normed, normed_stride,
+                 codes, scales, stream=0):
+        """dtype: ggml type id of the rows (0 = F32, 30 = BF16); strides in elements."""
+        self.check(self.d.fn_fp8_rows(dtype, x, x_stride, add, add_stride, weight, eps, rows, cols, total, total_stride, normed,
+                                      normed_stride, codes, scales, stream))
+
+    def fp8_blocks(self, dtype, w, stride, rows, cols, codes, scales, stream=0):
+        self.check(self.d.fn_fp8_blocks(dtype, w, stride, rows, cols, codes, scales, stream))
+
+    def fp8_product(self, weight, codes, scales, rows, dtype, add, add_stride, out, out_stride, stream=0):
+        """weight: FnFp8; dtype: of out and add."""
+        self.check(self.d.fn_fp8_product(weight, codes, scales, rows, dtype, add, add_stride, out, out_stride, stream))
 
     # ---- scores of tokens (device pointers, 0 = null; flashnext/logprobs.py is the layer over torch tensors) ----
     def logprobs(self, dtype, logits, stride, rows, vocab, tokens, logprob, rank, entropy, top, top_ids, top_logprobs,

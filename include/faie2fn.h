@@ -354,6 +354,32 @@ int fn_qk_rope_rows(const float *q, int64_t q_token, int64_t q_head, const float
  * stream: its place is given to a new request. */
 int fn_gdn_reset_seq(int h, int seq, void *stream);
 
+/* ---- 8-bit rows and weights (no counterpart in the reference, whose GEMVs take fp32 rows, engine/faie2fn.cu:690-1042) --------
+ * e4m3 codes, one byte each, with an fp32 scale for each 128 adjacent columns of a row (scales [rows][ceil(cols / 128)]), or for each
+ * 128 x 128 block of a weight (scales [ceil(rows / 128)][ceil(cols / 128)]); a code c stands for c * scale. Codes are [rows][cols],
+ * rows adjacent, 16-byte aligned; cols a multiple of 16. A scale is a / 448 with a = max(|y|, 2^-116) over the group, a code is
+ * y (448 / a) in fp32, rounded to the nearest e4m3 number, ties to even. A group that holds a NaN or an infinity reads back as NaN.
+ * All calls launch on the stream and allocate nothing; nothing is kept between them. */
+typedef struct fn_fp8_t {  /* a weight */
+    const uint8_t *codes;
+    const float *scales;
+    int rows, cols;
+} fn_fp8_t;
+/* Rows x [rows][cols] of `type` (F32 (0) or BF16 (30); strides in elements, columns adjacent) as codes and scales, in one pass with
+ * what comes before: h = x + add (add NULL: h = x), rounded to the type and written to total (NULL: not written); with weight [cols]
+ * (fp32, 16-byte aligned) y = h (mean h^2 + eps)^-1/2 weight, else y = h; y, rounded to the type, written to normed (NULL: not);
+ * y unrounded as codes and scales (both NULL: not). The sum of squares is held in 64 bits. total may be x or add. */
+int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const void *add, int64_t add_stride, const float *weight, float eps,
+                int rows, int cols, void *total, int64_t total_stride, void *normed, int64_t normed_stride, uint8_t *codes,
+                float *scales, void *stream);
+/* A weight [rows][cols] of `type` (row stride in elements) as codes and scales of 128 x 128 blocks. */
+int fn_fp8_blocks(uint32_t type, const void *w, int64_t stride, int rows, int cols, uint8_t *codes, float *scales, void *stream);
+/* out[i][j] = sum_g scales[i][g] w->scales[j / 128][g] sum_{k in group g} codes[i][k] w->codes[j][k] (+ add[i][j]) for i < rows,
+ * j < w->rows, on the tensor cores: fp32 sums, `type` F32 or BF16 for out and add (row strides in elements, columns adjacent; add may
+ * be NULL, or out itself). codes, scales: rows as fn_fp8_rows makes them, of w->cols columns. */
+int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *scales, int rows, uint32_t type, const void *add,
+                   int64_t add_stride, void *out, int64_t out_stride, void *stream);
+
 /* ---- scores of tokens (no counterpart in the reference, which answers with the argmax alone, engine/faie2fn.cu:1910-1935) --
  * Of every row of logits [rows][vocab] (device memory, F32 (0) or BF16 (30), `stride` elements from row to row, entries adjacent;
  * vocab 1..2^30), in one launch: logprob [rows] = logits[t] - ln sum e^logits of the row's token t = tokens[row]; rank [rows] =
