@@ -2,8 +2,8 @@
 // the residual's addition and RMSNorm in the same pass. The reference launches k_groupnorm (engine/faie2fn.cu:1222-1235) on fp32
 // rows and has no 8-bit activations.
 //
-//   h = x + add (rounded to its type), y = h (mean h^2 + eps)^-1/2 w, a = max(|y|, 2^-116) over a group, scale = a / 448,
-//   code = e4m3(y (448 / a)), to nearest, ties to even
+//   h = x + add (rounded to its type), y = h (mean h^2 + eps)^-1/2 w, a = max(|y|, 2^-116) over a group, scale = a (1 / 448),
+//   code = e4m3(y (448 (1 / a))), to nearest, ties to even; products and reciprocals in fp32
 //
 // 448 is e4m3's largest number; 2^-116 keeps 448 / a and a / 448 normal numbers (a group of zeros has codes 0). A NaN in a group
 // makes its scale NaN, an infinity its scale infinite and its codes NaN: both read back as NaN.
@@ -18,13 +18,14 @@
 namespace fn {
 
 constexpr int F8_T = 256;
-constexpr float F8_MAX = 448.0f, F8_TINY = 1.2037062152420224e-35f;  // 2^-116
+constexpr float F8_MAX = 448.0f, F8_TINY = 1.2037062152420224e-35f, F8_STEP = 1.0f / 448.0f;  // F8_TINY: 2^-116
 
 struct F8RowArgs {
     const void *x, *add;
     int64_t xs, adds;  // elements from row to row
     const float *w;
     float eps;
+    double per;  // 1 / cols
     int rows, cols, groups;
     void *total, *normed;
     int64_t totals, normeds;
@@ -93,6 +94,13 @@ template <typename T> __device__ __forceinline__ void f8_round(float (&v)[8]) {
     }
 }
 
+// v^-1/2 to well below a rounding of fp32: CUDA's approximation and a Newton step for v r^2 = 1 in 64 bits
+__device__ __forceinline__ float f8_rsqrt(double v) {
+    if (!(v > 1e-30 && v < 1e30)) return (float)rsqrt(v);
+    const double r = rsqrtf((float)v);
+    return (float)fma(0.5 * r, fma(-v * r, r, 1.0), r);
+}
+
 // 8 columns a thread, `tpr` threads a row, R rounds of them held in registers (0: any number, read twice if there is a norm)
 template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T) k_fp8_rows(const F8RowArgs a) {
     __shared__ double s_sum[F8_T / 32];
@@ -139,11 +147,11 @@ template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T) 
             if (a.tpr > 32) {
                 if ((threadIdx.x & 31) == 0) s_sum[warp] = ss;
                 __syncthreads();
-                const int w0 = warp & ~(a.tpr / 32 - 1);
-                ss = 0.0;
-                for (int i = 0; i < a.tpr / 32; ++i) ss += s_sum[w0 + i];
+                const int warps = a.tpr / 32;
+                ss = s_sum[(warp & ~(warps - 1)) + (threadIdx.x & (warps - 1))];
+                for (int o = 1; o < warps; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             }
-            r = (float)rsqrt(ss / a.cols + (double)a.eps);
+            r = f8_rsqrt(fma(ss, a.per, (double)a.eps));
         }
     }
 #pragma unroll
@@ -181,8 +189,8 @@ template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T) 
         for (int o = 8; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
         m = f8_max_nan(m, F8_TINY);
         if (!in) continue;
-        *(uint2 *)(codes + c) = f8_codes(y, F8_MAX / m);
-        if (t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m / F8_MAX;
+        *(uint2 *)(codes + c) = f8_codes(y, F8_MAX * __frcp_rn(m));
+        if (t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m * F8_STEP;
     }
 }
 
@@ -194,36 +202,55 @@ struct F8BlockArgs {
     float *scales;
 };
 
-// one CTA per 128 x 128 block, its values in registers between the maximum and the codes; 16 threads a row, 8 columns each
-template <typename T, bool WIDE> __global__ void __launch_bounds__(F8_T) k_fp8_blocks(const F8BlockArgs a) {
-    __shared__ float s_max[F8_T / 32];
-    const int c = blockIdx.x * FP8_GROUP + (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
-    const int64_t row0 = (int64_t)blockIdx.y * FP8_GROUP;
+// one CTA per 128 x 128 block, its values in registers (as they are stored) between the maximum and the codes; 16 threads a row, 8
+// columns each, four rows a thread
+constexpr int F8_BT = 512;
+template <typename T, bool WIDE> __global__ void __launch_bounds__(F8_BT, 2) k_fp8_blocks(const F8BlockArgs a) {
+    __shared__ float s_max[F8_BT / 32];
+    const int c = blockIdx.x * FP8_GROUP + (threadIdx.x & 15) * 8;
+    const int64_t row0 = (int64_t)blockIdx.y * FP8_GROUP + (threadIdx.x >> 4);
     pdl_wait();
     pdl_trigger();
-    const T *w = (const T *)after_wait(a.w);
-    float v[8][8] = {};
+    const T *w = (const T *)after_wait(a.w) + c;
+    T raw[4][8];
     float m = F8_TINY;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int64_t row = row0 + r0 + 16 * k;
-        if (row < a.rows && c < a.cols) f8_load<T, WIDE>(w + row * a.ws + c, v[k]);
+    for (int k = 0; k < 4; ++k) {
+        const int64_t row = row0 + 32 * k;
+        const bool in = row < a.rows && c < a.cols;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+                ((uint4 *)raw[k])[j] = in ? ((const uint4 *)(w + row * a.ws))[j] : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) raw[k][j] = in ? w[row * a.ws + j] : (T)0.0f;
+        }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = f8_max_nan(m, f8_amax(v[k]));
+    for (int k = 0; k < 4; ++k) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)raw[k][j];
+        m = f8_max_nan(m, f8_amax(v));
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
     __syncthreads();
+    m = s_max[threadIdx.x & 15];
 #pragma unroll
-    for (int i = 0; i < F8_T / 32; ++i) m = f8_max_nan(m, s_max[i]);
-    const float inv = F8_MAX / m;
+    for (int o = 8; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float inv = F8_MAX * __frcp_rn(m);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int64_t row = row0 + r0 + 16 * k;
-        if (row < a.rows && c < a.cols) *(uint2 *)(a.codes + row * a.cols + c) = f8_codes(v[k], inv);
+    for (int k = 0; k < 4; ++k) {
+        const int64_t row = row0 + 32 * k;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)raw[k][j];
+        if (row < a.rows && c < a.cols) *(uint2 *)(a.codes + row * a.cols + c) = f8_codes(v, inv);
     }
-    if (threadIdx.x == 0) a.scales[(int64_t)blockIdx.y * a.groups + blockIdx.x] = m / F8_MAX;
+    if (threadIdx.x == 0) a.scales[(int64_t)blockIdx.y * a.groups + blockIdx.x] = m * F8_STEP;
 }
 
 template <typename T, bool WIDE> static cudaError_t launch_rows(const F8RowArgs &a, dim3 grid, cudaStream_t s) {
@@ -258,7 +285,7 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
         while (tpr < F8_T && tpr * 8 < cols) tpr *= 2;
         const int64_t grid = ((int64_t)rows * tpr + F8_T - 1) / F8_T;
         if (grid > INT32_MAX) return fail("fp8 rows: too many rows");
-        const F8RowArgs a{x, add, x_stride, add_stride, weight, eps, rows, cols, fp8_groups(cols), total, normed, total_stride,
+        const F8RowArgs a{x, add, x_stride, add_stride, weight, eps, 1.0 / cols, rows, cols, fp8_groups(cols), total, normed, total_stride,
                           normed_stride, codes, scales, tpr};
         const dim3 g((unsigned)grid);
         const cudaStream_t s = (cudaStream_t)stream;
@@ -283,10 +310,10 @@ FN_API int fn_fp8_blocks(uint32_t type, const void *w, int64_t stride, int rows,
         const dim3 g((unsigned)a.groups, (unsigned)fp8_groups(rows));
         const bool wide = ((uintptr_t)w | (uint64_t)(stride * size)) % 16 == 0;
         const cudaStream_t s = (cudaStream_t)stream;
-        const cudaError_t e = type == T_F32 ? (wide ? launch_k(k_fp8_blocks<float, true>, g, dim3(F8_T), 0, s, a)
-                                                    : launch_k(k_fp8_blocks<float, false>, g, dim3(F8_T), 0, s, a))
-                                            : (wide ? launch_k(k_fp8_blocks<__nv_bfloat16, true>, g, dim3(F8_T), 0, s, a)
-                                                    : launch_k(k_fp8_blocks<__nv_bfloat16, false>, g, dim3(F8_T), 0, s, a));
+        const cudaError_t e = type == T_F32 ? (wide ? launch_k(k_fp8_blocks<float, true>, g, dim3(F8_BT), 0, s, a)
+                                                    : launch_k(k_fp8_blocks<float, false>, g, dim3(F8_BT), 0, s, a))
+                                            : (wide ? launch_k(k_fp8_blocks<__nv_bfloat16, true>, g, dim3(F8_BT), 0, s, a)
+                                                    : launch_k(k_fp8_blocks<__nv_bfloat16, false>, g, dim3(F8_BT), 0, s, a));
         if (e != cudaSuccess) return fail(std::string("fp8 blocks launch: ") + cudaGetErrorString(e));
         return 0;
     });

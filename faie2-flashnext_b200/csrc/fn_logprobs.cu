@@ -11,7 +11,8 @@
 //
 // The alternatives cost no second pass: the threads' maxima are there already, and their k-th largest is a bound that no
 // alternative of the CTA's part falls below, so only what can reach it is read again: the segments (of a thread's words) whose own
-// maximum does, about k of 4096. They are spread over all threads, and a warp keeps the best 32 entries that it meets sorted over its lanes.
+// maximum does, about k of 4096, spread over all threads, which list what reaches it. (If equal entries are too many to be listed, every
+// warp keeps its best 32 sorted over its lanes.)
 #include <cuda_bf16.h>
 
 #include "fn_argmax.cuh"
@@ -299,12 +300,12 @@ __device__ __forceinline__ bool lp_stands_before(float x, int i, int token, floa
 
 __device__ __forceinline__ uint32_t lp_order(float v) { return (uint32_t)(amax_key(v, 0) >> 32); }  // 0: no candidate
 
-// `list`: a warp's best entries, descending over the lanes (0: none); takes every lane's key
-__device__ __forceinline__ void lp_insert(unsigned long long &list, unsigned long long key, int lane, int top) {
+// `list`: a warp's best entries, descending over the lanes (0: none); takes every lane's key and returns the new list
+__device__ __noinline__ unsigned long long lp_insert(unsigned long long list, unsigned long long key, int lane, int top) {
     for (;;) {
         const unsigned long long last = __shfl_sync(0xffffffffu, list, top - 1);
         const uint32_t want = __ballot_sync(0xffffffffu, key > last);
-        if (!want) return;
+        if (!want) return list;
         const int from = __ffs(want) - 1;
         const unsigned long long k = __shfl_sync(0xffffffffu, key, from), up = __shfl_up_sync(0xffffffffu, list, 1);
         const int at = __popc(__ballot_sync(0xffffffffu, list > k));
@@ -352,8 +353,11 @@ template <int THREADS> struct LpShared {
     uint32_t most[SEGMENTS][THREADS];     // the largest entry (in order) of every segment
 };
 
+// What a CTA does once a row is out of line and rolled where it is called more than once: of a short call's time a good part is fetching
+// code that has not run yet.
+//
 // n keys (distinct, or 0) put in order: the first `top` into best, which holds zeros. THREADS / 256 neighbours count a key against the others.
-template <int THREADS> __device__ __forceinline__ void lp_rank_keys(const unsigned long long *keys, int n, int top, unsigned long long *best) {
+template <int THREADS> __device__ __noinline__ void lp_rank_keys(const unsigned long long *keys, int n, int top, unsigned long long *best) {
     constexpr int Q = THREADS / 256;
     for (int i0 = 0; i0 < n; i0 += 256) {
         const int i = i0 + threadIdx.x / Q;
@@ -415,7 +419,7 @@ template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, 1024 / L
             const int w = w0 + i * U * LP_T + tid;
             const uint4 *p = v + w;
             uint4 r[U];
-            if (w0 + (i + 1) * U * LP_T <= w1) {  // all words of all threads
+            if (LP_T < 1024 && w0 + (i + 1) * U * LP_T <= w1) {  // all words of all threads (of long loops; else it is more code to fetch)
 #pragma unroll
                 for (int u = 0; u < U; ++u) r[u] = p[u * LP_T];
                 most = LpAcc<T>::larger(most, acc.words(r));
@@ -494,48 +498,57 @@ template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, 1024 / L
                 }
         __syncthreads();
         const int n = sh.n_columns;
-        unsigned long long list = 0;
-        auto take = [&](unsigned long long key) {
-            if ((uint32_t)(key >> 32) < bound) key = 0;
-            lp_insert(list, key, lane, a.top);
-        };
         // segments that reach the bound, or all of them if they are too many to be listed
         const bool listed = n <= LP_T;
-        const int each = per * U, count = listed ? n : LP_T * ((rounds + per - 1) / per);  // words of a segment; segments
-        constexpr int B = 4;                                                              // words in flight per thread here
-        for (int i0 = 0; i0 < count * each; i0 += B * LP_T) {
-            uint4 word[B];
-            int at[B];
+        const int each = per * U, count = (listed ? n : LP_T * ((rounds + per - 1) / per)) * each;  // words of a segment; words to read
+        auto word = [&](int i) {  // word i of those to read, w1 if there is none
+            const int c = i / each, column = listed ? sh.columns[min(c, LP_T - 1)] : c;
+            return i < count ? w0 + (column / LP_T * each + i - c * each) * LP_T + column % LP_T : w1;
+        };
+        constexpr int KEYS = LP_W * LP_MAX_TOP;  // that sh.keys holds
+#pragma unroll 1
+        for (int i = tid; i < count; i += LP_T) {
+            const int w = word(i);
+            if (w >= w1) continue;
+            float e[N];
+            LpAcc<T>::unpack(v[w], e);
+            float m = e[0];
 #pragma unroll
-            for (int u = 0; u < B; ++u) {
-                const int i = i0 + u * LP_T + tid, c = i / each, j = i - c * each;
-                int w = w1;
-                if (c < count) {
-                    const int column = listed ? sh.columns[c] : c;
-                    w = w0 + (column / LP_T * each + j) * LP_T + column % LP_T;
-                }
-                at[u] = w < w1 ? w : -1;
-                if (at[u] >= 0) word[u] = v[w];
-            }
+            for (int j = 1; j < N; ++j) m = fmaxf(m, e[j]);
+            if (lp_order(m) < bound || !(m > -INFINITY)) continue;
+            uint32_t reach = 0;  // the entries that reach the bound
 #pragma unroll
-            for (int u = 0; u < B; ++u) {
-                if (i0 + u * LP_T + (tid & ~31) >= count * each) break;  // none of this warp
-                float e[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i) e[i] = NAN;
-                if (at[u] >= 0) LpAcc<T>::unpack(word[u], e);
-                float m = e[0];
-#pragma unroll
-                for (int i = 1; i < N; ++i) m = fmaxf(m, e[i]);
-                const uint32_t o = lp_order(m);
-                if (!__any_sync(0xffffffffu, o && o >= bound)) continue;
-#pragma unroll
-                for (int i = 0; i < N; ++i) take(amax_key(e[i], head + at[u] * N + i));
+            for (int j = 0; j < N; ++j)
+                if (const uint32_t o = lp_order(e[j]); o && o >= bound) reach |= 1u << j;
+#pragma unroll 1
+            for (; reach; reach &= reach - 1) {
+                const int j = __ffs(reach) - 1, at = atomicAdd(&sh.n_keys, 1);
+                if (at < KEYS) sh.keys[at] = amax_key((float)x[head + w * N + j], head + w * N + j);
             }
         }
-        if (part == 0 && warp == 0) take(lane < head + tail ? amax_key((float)x[odd], odd) : 0ull);
-        if (list && lane < a.top) sh.keys[atomicAdd(&sh.n_keys, 1)] = list;
+        if (odd >= 0) {
+            const unsigned long long key = amax_key((float)x[odd], odd);
+            if (key && (uint32_t)(key >> 32) >= bound) {
+                const int at = atomicAdd(&sh.n_keys, 1);
+                if (at < KEYS) sh.keys[at] = key;
+            }
+        }
         __syncthreads();
+        if (sh.n_keys > KEYS) {  // many equal entries: every warp keeps its best
+            __syncthreads();
+            if (tid == 0) sh.n_keys = 0;
+            unsigned long long list = 0;
+#pragma unroll 1
+            for (int i = tid; i - lane < count; i += LP_T) {
+                const int w = word(i);
+#pragma unroll 1
+                for (int j = 0; j < N; ++j) list = lp_insert(list, w < w1 ? amax_key((float)x[head + w * N + j], head + w * N + j) : 0ull, lane, a.top);
+            }
+            if (part == 0 && warp == 0) list = lp_insert(list, odd >= 0 ? amax_key((float)x[odd], odd) : 0ull, lane, a.top);
+            __syncthreads();
+            if (list && lane < a.top) sh.keys[atomicAdd(&sh.n_keys, 1)] = list;
+            __syncthreads();
+        }
         lp_rank_keys<LP_T>(sh.keys, sh.n_keys, a.top, sh.best);
     }
     __syncthreads();

@@ -29,35 +29,36 @@ class Logprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-def _make(rows, top, dev, tokens=True):
-    f = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev).split([rows, rows, rows * top])
-    i = torch.empty(rows * (1 + top), dtype=torch.int32, device=dev).split([rows, rows * top])
-    return Logprobs(f[0] if tokens else None, i[0] if tokens else None, f[1], i[1].view(rows, top), f[2].view(rows, top))
+def _make(rows, top, dev, tokens):
+    f, i = {"dtype": torch.float32, "device": dev}, {"dtype": torch.int32, "device": dev}
+    return Logprobs(torch.empty(rows, **f) if tokens else None, torch.empty(rows, **i) if tokens else None, torch.empty(rows, **f),
+                    torch.empty((rows, top), **i), torch.empty((rows, top), **f))
 
 
 def token_logprobs(fn, logits, tokens=None, top: int = 0, out: Logprobs | None = None) -> Logprobs:
     """logits: fp32 or bf16 [rows][vocab] on a CUDA device, any row stride; tokens: int32 [rows] (< 0: none) or None; top: how many
     alternatives (0..32). out: buffers of an earlier call of the same sizes, written again."""
-    if logits.dim() != 2 or logits.dtype not in _TYPE or not logits.is_cuda or (logits.stride(1) != 1 and logits.shape[1] > 1) or \
-            logits.shape[1] < 1:
-        raise ValueError(f"logits: fp32 or bf16 [rows][vocab] on a CUDA device with adjacent entries is wanted, got {logits.dtype} "
-                         f"{tuple(logits.shape)} on {logits.device}")
+    shape, dtype, dev = logits.shape, logits.dtype, logits.get_device()
+    if len(shape) != 2 or dtype not in _TYPE or dev < 0 or shape[1] < 1 or (logits.stride(1) != 1 and shape[1] > 1):
+        raise ValueError(f"logits: fp32 or bf16 [rows][vocab] on a CUDA device with adjacent entries is wanted, got {dtype} {tuple(shape)} "
+                         f"on {logits.device}")
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top: 0..{MAX_TOP} is wanted")
-    rows, vocab = logits.shape
-    dev = logits.get_device()
+    rows, vocab = shape
     if tokens is not None:
         _ints("tokens", tokens, (rows,), dev)
     if out is None:
         out = _make(rows, top, logits.device, tokens is not None)
     else:
-        for name, t, shape, dtype in (("logprob", out.logprob, (rows,), torch.float32), ("rank", out.rank, (rows,), torch.int32),
-                                      ("entropy", out.entropy, (rows,), torch.float32), ("top_ids", out.top_ids, (rows, top), torch.int32),
-                                      ("top_logprobs", out.top_logprobs, (rows, top), torch.float32)):
+        for name, t, want, kind in (("logprob", out.logprob, (rows,), torch.float32), ("rank", out.rank, (rows,), torch.int32),
+                                    ("entropy", out.entropy, (rows,), torch.float32), ("top_ids", out.top_ids, (rows, top), torch.int32),
+                                    ("top_logprobs", out.top_logprobs, (rows, top), torch.float32)):
             if (t is None) != (tokens is None and name in ("logprob", "rank")) or t is not None and (
-                    t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != dev):
+                    t.shape != want or t.dtype is not kind or not t.is_contiguous() or t.get_device() != dev):
                 raise ValueError(f"out.{name}: not of this call's sizes, type and device")
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    fn.logprobs(_TYPE[logits.dtype], logits.data_ptr(), logits.stride(0), rows, vocab, p(tokens), p(out.logprob), p(out.rank),
-                p(out.entropy), top, p(out.top_ids), p(out.top_logprobs), _stream(logits.device))
+    token = logprob = rank = None
+    if tokens is not None:
+        token, logprob, rank = tokens.data_ptr(), out.logprob.data_ptr(), out.rank.data_ptr()
+    fn.logprobs(_TYPE[dtype], logits.data_ptr(), logits.stride(0), rows, vocab, token, logprob, rank, out.entropy.data_ptr(), top,
+                out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _stream(logits.device))
     return out

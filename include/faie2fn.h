@@ -357,8 +357,8 @@ int fn_gdn_reset_seq(int h, int seq, void *stream);
 /* ---- 8-bit rows and weights (no counterpart in the reference, whose GEMVs take fp32 rows, engine/faie2fn.cu:690-1042) --------
  * e4m3 codes, one byte each, with an fp32 scale for each 128 adjacent columns of a row (scales [rows][ceil(cols / 128)]), or for each
  * 128 x 128 block of a weight (scales [ceil(rows / 128)][ceil(cols / 128)]); a code c stands for c * scale. Codes are [rows][cols],
- * rows adjacent, 16-byte aligned; cols a multiple of 16. A scale is a / 448 with a = max(|y|, 2^-116) over the group, a code is
- * y (448 / a) in fp32, rounded to the nearest e4m3 number, ties to even. A group that holds a NaN or an infinity reads back as NaN.
+ * rows adjacent, 16-byte aligned; cols a multiple of 16. With a = max(|y|, 2^-116) over the group the scale is a (1 / 448), a
+ * code is y (448 (1 / a)), all in fp32, rounded to the nearest e4m3 number, ties to even. A group that holds a NaN or an infinity reads back as NaN.
  * All calls launch on the stream and allocate nothing; nothing is kept between them. */
 typedef struct fn_fp8_t {  /* a weight */
     const uint8_t *codes;

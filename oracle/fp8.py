@@ -36,8 +36,8 @@ def groups(y, down, fp32=True):
             at = (slice(i * down, (i + 1) * down), slice(j * GROUP, (j + 1) * GROUP))
             a = t(np.maximum(np.abs(y[at]).max(), t(TINY)))
             with np.errstate(invalid="ignore"):
-                q[at] = e4m3(y[at] * (t(448) / a))
-            s[i, j] = a / t(448)
+                q[at] = e4m3(y[at] * (t(448) * (t(1) / a)))
+            s[i, j] = a * (t(1) / t(448))
     return q, s
 
 

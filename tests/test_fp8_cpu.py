@@ -33,7 +33,7 @@ def test_oracle_groups():
     y[2, 128:256] = 0
     y[3, 256:] = 1e-37
     q, s = O.groups(y, 1)
-    assert s.shape == (5, 3) and s[2, 1] == np.float32(O.TINY) / np.float32(448) and not q[2, 128:256].any()
+    assert s.shape == (5, 3) and s[2, 1] == np.float32(O.TINY) * (np.float32(1) / np.float32(448)) and not q[2, 128:256].any()
     assert np.abs(q).max(1).min() <= 448
     # half a step of e4m3 (2^-4 of the value) where codes are normal numbers, half the smallest step below; scales' and quotients' roundings
     off = np.abs(q * O.spread(s, 5, 272, 1) - y)
