@@ -13,6 +13,8 @@
 // that lie next to a border, and squares of fp32 values leave that type's range.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "fn_fp8.h"
 
 namespace fn {
@@ -54,20 +56,34 @@ __device__ __forceinline__ uint2 f8_codes(const float (&y)[8], float inv) {
     return make_uint2((uint32_t)p[0] | (uint32_t)p[1] << 16, (uint32_t)p[2] | (uint32_t)p[3] << 16);
 }
 
-// eight adjacent values; WIDE: 16-byte aligned
-template <typename T, bool WIDE> __device__ __forceinline__ void f8_load(const T *p, float (&v)[8]) {
-    if constexpr (!WIDE) {
+// eight adjacent values as they are stored; WIDE: 16-byte aligned
+template <typename T> struct F8Raw {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T, bool WIDE> __device__ __forceinline__ void f8_fetch(const T *p, F8Raw<T> &r) {
+    if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)p[i];
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) r.w[j] = ((const uint4 *)p)[j];
     } else {
-        const uint4 a = *(const uint4 *)p;
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
+        memcpy(&r, v, sizeof(r));
+    }
+}
+template <typename T> __device__ __forceinline__ void f8_unpack(const F8Raw<T> &r, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        memcpy(v, &r, sizeof(r));
+    } else {
+        const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
+}
+template <typename T, bool WIDE> __device__ __forceinline__ void f8_load(const T *p, float (&v)[8]) {
+    F8Raw<T> r;
+    f8_fetch<T, WIDE>(p, r);
+    f8_unpack<T>(r, v);
 }
 template <typename T, bool WIDE> __device__ __forceinline__ void f8_store(T *p, const float (&v)[8]) {
     if constexpr (!WIDE) {
@@ -101,96 +117,114 @@ __device__ __forceinline__ float f8_rsqrt(double v) {
     return (float)fma(0.5 * r, fma(-v * r, r, 1.0), r);
 }
 
-// 8 columns a thread, `tpr` threads a row, R rounds of them held in registers (0: any number, read twice if there is a norm)
-template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T) k_fp8_rows(const F8RowArgs a) {
-    __shared__ double s_sum[F8_T / 32];
-    const int t = threadIdx.x & (a.tpr - 1), warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * (F8_T / a.tpr) + threadIdx.x / a.tpr;
-    const bool live = row < a.rows;
+// 8 columns a thread, `tpr` threads a row, R rounds of them held in registers (0: any number, read twice if there is a norm). A CTA takes
+// rows at a stride of the grid, the next one's words on their way while one is summed and coded (R up to 2).
+template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T, R == 1 ? 6 : R == 2 ? 4 : 2) k_fp8_rows(const F8RowArgs a) {
+    constexpr bool AHEAD = R == 1 || R == 2;
+    __shared__ double s_sum[2][F8_T / 32];
+    const int t = threadIdx.x & (a.tpr - 1), warp = threadIdx.x >> 5, here = F8_T / a.tpr;  // rows a CTA at once
     const int span = a.tpr * 8, rounds = R ? R : (a.cols + span - 1) / span;
     pdl_wait();
     pdl_trigger();
-    const T *x = (const T *)after_wait(a.x) + row * a.xs, *add = a.add ? (const T *)after_wait(a.add) + row * a.adds : nullptr;
-    T *total = a.total ? (T *)a.total + row * a.totals : nullptr, *normed = a.normed ? (T *)a.normed + row * a.normeds : nullptr;
-    uint8_t *codes = a.codes ? a.codes + row * a.cols : nullptr;
-    float h[R ? R : 1][8] = {};
-    // the row's sum h in columns c .. c + 7
-    auto fetch = [&](int c, float (&v)[8]) {
-        f8_load<T, WIDE>(x + c, v);
-        if (add) {
-            float b[8];
-            f8_load<T, WIDE>(add + c, b);
+    const T *x = (const T *)after_wait(a.x), *add = (const T *)after_wait(a.add);
+    F8Raw<T> rx[AHEAD ? R : 1], ra[AHEAD ? R : 1];
+    auto ahead = [&](int64_t row) {
+        if (row < a.rows) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += b[i];
-            f8_round<T>(v);
+            for (int k = 0; k < (AHEAD ? R : 1); ++k) {
+                const int c = k * span + t * 8;
+                if (c < a.cols) {
+                    f8_fetch<T, WIDE>(x + row * a.xs + c, rx[k]);
+                    if (add) f8_fetch<T, WIDE>(add + row * a.adds + c, ra[k]);
+                }
+            }
         }
-        if (total) f8_store<T, WIDE>(total + c, v);
     };
-    float r = 1.0f;
-    if (R || a.w) {
-        double ss = 0.0;
+    const int64_t step = (int64_t)gridDim.x * here;
+    int64_t row = (int64_t)blockIdx.x * here + threadIdx.x / a.tpr;
+    if constexpr (AHEAD) ahead(row);
+    for (int turn = 0; row - threadIdx.x / a.tpr < a.rows; row += step, turn ^= 1) {
+        const bool live = row < a.rows;
+        T *total = a.total ? (T *)a.total + row * a.totals : nullptr, *normed = a.normed ? (T *)a.normed + row * a.normeds : nullptr;
+        uint8_t *codes = a.codes ? a.codes + row * a.cols : nullptr;
+        float h[R ? R : 1][8] = {};
+        // the row's sum h in columns c .. c + 7
+        auto fetch = [&](int c, float (&v)[8], const F8Raw<T> &wx, const F8Raw<T> &wa) {
+            f8_unpack<T>(wx, v);
+            if (add) {
+                float b[8];
+                f8_unpack<T>(wa, b);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += b[i];
+                f8_round<T>(v);
+            }
+        };
+        auto read = [&](int c, float (&v)[8]) {
+            F8Raw<T> wx, wa;
+            f8_fetch<T, WIDE>(x + row * a.xs + c, wx);
+            if (add) f8_fetch<T, WIDE>(add + row * a.adds + c, wa);
+            fetch(c, v, wx, wa);
+        };
+        float r = 1.0f;
+        if (R || a.w) {
+            double ss = 0.0;
+#pragma unroll
+            for (int k = 0; k < rounds; ++k) {
+                const int c = k * span + t * 8;
+                float(&v)[8] = h[R ? k : 0];
+                if (live && c < a.cols) {
+                    if constexpr (AHEAD) fetch(c, v, rx[k], ra[k]);
+                    else read(c, v);
+                    if (total) f8_store<T, WIDE>(total + c, v);
+                    if (a.w) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
+                    }
+                }
+            }
+            if constexpr (AHEAD) ahead(row + step);
+            if (a.w) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (a.tpr > 32) {
+                    if ((threadIdx.x & 31) == 0) s_sum[turn][warp] = ss;
+                    __syncthreads();
+                    const int warps = a.tpr / 32;
+                    ss = s_sum[turn][(warp & ~(warps - 1)) + (threadIdx.x & (warps - 1))];
+                    for (int o = 1; o < warps; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                }
+                r = f8_rsqrt(fma(ss, a.per, (double)a.eps));
+            }
+        }
 #pragma unroll
         for (int k = 0; k < rounds; ++k) {
             const int c = k * span + t * 8;
+            const bool in = live && c < a.cols;
             float(&v)[8] = h[R ? k : 0];
-            if (live && c < a.cols) {
-                fetch(c, v);
-                if (a.w) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
-                }
+            if (!R && in) {
+                if (a.w && total) f8_load<T, WIDE>(total + c, v);  // (x may be total: its sum is there already)
+                else read(c, v);
+                if (!a.w && total) f8_store<T, WIDE>(total + c, v);
             }
-        }
-        if (a.w) {
+            float y[8];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (a.tpr > 32) {
-                if ((threadIdx.x & 31) == 0) s_sum[warp] = ss;
-                __syncthreads();
-                const int warps = a.tpr / 32;
-                ss = s_sum[(warp & ~(warps - 1)) + (threadIdx.x & (warps - 1))];
-                for (int o = 1; o < warps; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            for (int i = 0; i < 8; ++i) y[i] = in ? v[i] : 0.0f;
+            if (a.w && in) {
+                float w[8];
+                f8_load<float, true>(a.w + c, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
             }
-            r = f8_rsqrt(fma(ss, a.per, (double)a.eps));
+            if (normed && in) f8_store<T, WIDE>(normed + c, y);
+            if (!codes) continue;
+            float m = f8_amax(y);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            m = f8_max_nan(m, F8_TINY);
+            if (!in) continue;
+            *(uint2 *)(codes + c) = f8_codes(y, F8_MAX * __frcp_rn(m));
+            if (t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m * F8_STEP;
         }
-    }
-#pragma unroll
-    for (int k = 0; k < rounds; ++k) {
-        const int c = k * span + t * 8;
-        const bool in = live && c < a.cols;
-        float(&v)[8] = h[R ? k : 0];
-        if (!R && in) {
-            if (!a.w) fetch(c, v);
-            else if (total) f8_load<T, WIDE>(total + c, v);
-            else {
-                f8_load<T, WIDE>(x + c, v);
-                if (add) {
-                    float b[8];
-                    f8_load<T, WIDE>(add + c, b);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] += b[i];
-                    f8_round<T>(v);
-                }
-            }
-        }
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = in ? v[i] : 0.0f;
-        if (a.w && in) {
-            float w[8];
-            f8_load<float, true>(a.w + c, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
-        }
-        if (normed && in) f8_store<T, WIDE>(normed + c, y);
-        if (!codes) continue;
-        float m = f8_amax(y);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        m = f8_max_nan(m, F8_TINY);
-        if (!in) continue;
-        *(uint2 *)(codes + c) = f8_codes(y, F8_MAX * __frcp_rn(m));
-        if (t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m * F8_STEP;
     }
 }
 
@@ -283,8 +317,8 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
                            (uint64_t)(add_stride * size) | (uint64_t)(total_stride * size) | (uint64_t)(normed_stride * size)) % 16 == 0;
         int tpr = 32;
         while (tpr < F8_T && tpr * 8 < cols) tpr *= 2;
-        const int64_t grid = ((int64_t)rows * tpr + F8_T - 1) / F8_T;
-        if (grid > INT32_MAX) return fail("fp8 rows: too many rows");
+        // as many CTAs as the SMs hold (6 of 256 threads where a row's 8 columns a thread are one round, 4 else)
+        const int64_t grid = std::min<int64_t>(((int64_t)rows * tpr + F8_T - 1) / F8_T, (int64_t)num_sms() * (cols <= 8 * tpr ? 6 : 4));
         const F8RowArgs a{x, add, x_stride, add_stride, weight, eps, 1.0 / cols, rows, cols, fp8_groups(cols), total, normed, total_stride,
                           normed_stride, codes, scales, tpr};
         const dim3 g((unsigned)grid);
