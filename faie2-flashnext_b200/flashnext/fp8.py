@@ -5,6 +5,7 @@ columns of a row, or each 128 x 128 block of a weight. The reference's GEMVs tak
     w = Fp8Weight.quantise(fn, weight)                 # [n][k] fp32 or bf16, once; or Fp8Weight(fn, codes, scales)
     x = quantise_rows(fn, h, add=y, total=h, weight=norm, eps=1e-6)    # h += y; rows = 8-bit RMSNorm(h) * norm
     out = w.product(x, dtype=torch.bfloat16)           # [rows][n]; add=: added in
+    add_norm(fn, h, y, norm, 1e-6, h, n)               # the residual's addition and the norm alone: h += y, n = RMSNorm(h) * norm
 
 Everything runs on the current stream and returns at once.
 """
@@ -96,6 +97,20 @@ def quantise_rows(fn, x, add=None, total=None, weight=None, eps: float = 1e-6, n
     fn.fp8_rows(_TYPE[dtype], x.data_ptr(), x.stride(0), a, at, w, eps, rows, cols, t, tt, n, nt, out.q.data_ptr(), out.scale.data_ptr(),
                 _stream(x.device))
     return out
+
+
+def add_norm(fn, x, add, weight, eps: float, total, normed) -> None:
+    """total = x + add (rounded to x's type; total may be x or add), normed = RMSNorm(total) * weight, without 8-bit rows. All fp32 or bf16
+    [rows][cols] of one type, any row stride; weight fp32 [cols]."""
+    shape, dtype, index = x.shape, x.dtype, x.get_device()
+    if len(shape) != 2 or dtype not in _TYPE or index < 0 or x.stride(1) != 1 or shape[1] % 16 or shape[1] < 16:
+        _wants("x (columns in multiples of 16)", x, None, None, -1)
+    for name, t in (("add", add), ("total", total), ("normed", normed)):
+        _like(name, t, shape, dtype, index)
+    if weight.shape != (shape[1],) or weight.dtype is not torch.float32 or not weight.is_contiguous() or weight.get_device() != index:
+        raise ValueError(f"weight: contiguous fp32 [{shape[1]}] on cuda:{index} is wanted")
+    fn.fp8_rows(_TYPE[dtype], x.data_ptr(), x.stride(0), add.data_ptr(), add.stride(0), weight.data_ptr(), eps, shape[0], shape[1], total.data_ptr(),
+                total.stride(0), normed.data_ptr(), normed.stride(0), None, None, _stream(x.device))
 
 
 class Fp8Weight:

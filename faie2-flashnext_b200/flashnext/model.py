@@ -242,13 +242,19 @@ class BatchDecodeModel:
     batch's tokens), the MoE layer for all the batch's tokens in one call, one DeltaNet state and one attention cache per
     sequence. The argmax of each sequence's logits feeds its next input, so a generation is again one CUDA graph
     replayed per position. Results are those of DecodeModel within the tensor-core GEMV's tolerance (1e-4 of max |y|
-    per projection)."""
+    per projection).
 
-    def __init__(self, fn, cfg: dict, W: dict, batch: int, max_ctx: int = 512):
+    dense="fp8": the input and output projections and the lm_head as 8-bit weights (flashnext/fp8.py: the GGUF rows' values,
+    quantised again in blocks of 128 x 128) on 8-bit rows, which need no decoding; each rounding of rows and weights to 3 mantissa
+    bits is off by up to 2^-4 of a value. The router and the experts keep their formats."""
+
+    def __init__(self, fn, cfg: dict, W: dict, batch: int, max_ctx: int = 512, dense: str = "gguf"):
         import torch
         if not 1 <= batch <= 32:
             raise ValueError("batch out of range (1..32)")
-        self.fn, self.cfg, self.B, self.max_ctx = fn, cfg, batch, max_ctx
+        if dense not in ("gguf", "fp8"):
+            raise ValueError("dense: gguf or fp8 is wanted")
+        self.fn, self.cfg, self.B, self.max_ctx, self.dense = fn, cfg, batch, max_ctx, dense
         dev = torch.device("cuda", torch.cuda.current_device())
         f32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(dev)  # noqa: E731
         d, nkh, nvh, nh, nkv = cfg["D"], cfg["nkh"], cfg["nvh"], cfg["nh"], cfg["nkv"]
@@ -258,8 +264,9 @@ class BatchDecodeModel:
         self.n_qkv = nh * 2 * HD + 2 * nkv * HD
         self.tcs, self.moes, self.gdns = [], [], []
         tc = lambda q, raw, r, c: self._tc(q, raw, r, c)  # noqa: E731
+        wide = self._fp8 if dense == "fp8" else tc
         self.E = torch.from_numpy(np.ascontiguousarray(W["embed"]).reshape(-1)).to(dev)
-        self.head = tc(cfg["head"], W["head"], cfg["vocab"], d)
+        self.head = wide(cfg["head"], W["head"], cfg["vocab"], d)
         self.final_norm = f32(W["final_norm"])
         self.inv_freq = f32(rope_inv_freq(cfg["rope_base"]))
         self.layers = []
@@ -273,14 +280,14 @@ class BatchDecodeModel:
             o = dict(kind=L["kind"], norm1=f32(L["norm1"]), norm2=f32(L["norm2"]),
                      router=tc(T.get("router", cfg["router"]), L["router"], ne + 1, d))
             if L["kind"] == "G":
-                o["w_in"] = tc(ty("w_in"), np.concatenate([L["w_in"], L["w_ab"]]), self.n_in, d)
-                o["w_out"] = tc(ty("w_out"), L["w_out"], d, nvh * DS)
+                o["w_in"] = wide(ty("w_in"), np.concatenate([L["w_in"], L["w_ab"]]), self.n_in, d)
+                o["w_out"] = wide(ty("w_out"), L["w_out"], d, nvh * DS)
                 g = fn.gdn_create_batch(nkh, nvh, L["conv_w"], L["dt_bias"], L["ssm_a"], L["gnorm"], B)
                 self.gdns.append(g)
                 o["gdn"] = g
             else:
-                o.update(w_qkv=tc(ty("w_q"), np.concatenate([L["w_q"], L["w_k"], L["w_v"]]), self.n_qkv, d),
-                         w_o=tc(ty("w_o"), L["w_o"], d, nh * HD), q_norm=f32(L["q_norm"]), k_norm=f32(L["k_norm"]),
+                o.update(w_qkv=wide(ty("w_q"), np.concatenate([L["w_q"], L["w_k"], L["w_v"]]), self.n_qkv, d),
+                         w_o=wide(ty("w_o"), L["w_o"], d, nh * HD), q_norm=f32(L["q_norm"]), k_norm=f32(L["k_norm"]),
                          **self._caches(dev))
             m = fn.moe_create(T.get("gate_up", cfg["gate_up"]), T.get("down", cfg["down"]), ne, cfg["k"], ffe, d, *L["moe"])
             self.moes.append(m)
@@ -290,6 +297,11 @@ class BatchDecodeModel:
         self.h, self.x, self.proj = z(B, d), z(B, d), z(B, max(self.n_in, self.n_qkv))
         self.core, self.Q, self.att, self.lr = z(B, nvh * DS), z(B, nh * HD), z(B, nh * HD), z(B, ne + 1)
         self.logits = z(B, cfg["vocab"])
+        if dense == "fp8":
+            import fp8
+            self.y = z(B, d)  # an output projection's rows, before they join the residual
+            fn.sync(torch.cuda.current_stream().cuda_stream)  # the weights were quantised there; a step may run on another
+            self.rows8 = {n: fp8.empty_rows(B, n, dev) for n in {d, nvh * DS, nh * HD}}
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self.next = torch.zeros(B, dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(B, max_ctx, dtype=torch.int32, device=dev)
@@ -301,38 +313,74 @@ class BatchDecodeModel:
         self.tcs.append(h)
         return h
 
+    def _fp8(self, qtype, raw, rows, cols):
+        import fp8
+        import torch
+        values = self.fn.dequant(qtype, np.ascontiguousarray(raw), rows, cols)
+        return fp8.Fp8Weight.quantise(self.fn, torch.from_numpy(values.reshape(rows, cols)).cuda())
+
     def launches_per_step(self) -> int:
         """The embedding; per layer two norms, the input GEMV, the DeltaNet core or the two attention kernels, the output
         GEMV, the router GEMV and the MoE layer's three kernels; the final norm, the lm_head, the argmax and the step
-        counter."""
+        counter. 8-bit dense weights: the norms are the rows' quantising or the residual's addition, and a mixer's output is quantised."""
         moe = 3
-        return 1 + sum(2 + 1 + (1 if L["kind"] == "G" else 2) + 1 + 1 + moe for L in self.layers) + 4
+        return 1 + sum(2 + 1 + (1 if L["kind"] == "G" else 2) + (self.dense == "fp8") + 1 + 1 + moe for L in self.layers) + 4
+
+    # a step's dense projections: rows normed for the input projections, those, the output projections into the residual with the norm
+    # of the router's and the experts' input, the lm_head
+    def _norm(self, norm, s):
+        if self.dense == "fp8":
+            import fp8
+            fp8.quantise_rows(self.fn, self.h, weight=norm, eps=self.cfg["eps"], out=self.rows8[self.cfg["D"]])
+        else:
+            self.fn.rmsnorm_rows(self.h.data_ptr(), norm.data_ptr(), self.x.data_ptr(), self.cfg["D"], self.B, self.cfg["eps"], s)
+
+    def _project(self, w, out, s):
+        """out [B][..] = W of the normed rows."""
+        if self.dense == "fp8":
+            w.product(self.rows8[self.cfg["D"]], out=out[:, :w.rows])
+        else:
+            self.fn.tc_gemv(w, self.x.data_ptr(), self.cfg["D"], out.data_ptr(), out.stride(0), self.B, 0, s)
+
+    def _join(self, w, rows, norm, s):
+        """h += W rows, x = the normed h."""
+        fn, d, B, eps = self.fn, self.cfg["D"], self.B, self.cfg["eps"]
+        if self.dense == "fp8":
+            import fp8
+            w.product(fp8.quantise_rows(fn, rows, out=self.rows8[rows.shape[1]]), out=self.y)
+            fp8.add_norm(fn, self.h, self.y, norm, eps, self.h, self.x)
+        else:
+            fn.tc_gemv(w, rows.data_ptr(), rows.shape[1], self.h.data_ptr(), d, B, 1, s)
+            fn.rmsnorm_rows(self.h.data_ptr(), norm.data_ptr(), self.x.data_ptr(), d, B, eps, s)
 
     def launch_step(self, s: int):
         """One decode step of every sequence on stream s (device pointers only; capturable)."""
+        import torch
+        with torch.cuda.stream(torch.cuda.ExternalStream(s)):  # the layers over torch tensors launch on the current stream
+            self._launch_step(s)
+
+    def _launch_step(self, s: int):
         fn, cfg, B = self.fn, self.cfg, self.B
-        d, nvh, nh, eps, ne1 = cfg["D"], cfg["nvh"], cfg["nh"], cfg["eps"], cfg["ne"] + 1
+        nvh, ne1 = cfg["nvh"], cfg["ne"] + 1
         p = lambda t: t.data_ptr()  # noqa: E731
-        h, x, pr = p(self.h), p(self.x), p(self.proj)
-        ps = self.proj.shape[1]
+        pr, ps = p(self.proj), self.proj.shape[1]
         self._embed(s)
         for L in self.layers:
-            fn.rmsnorm_rows(h, p(L["norm1"]), x, d, B, eps, s)
+            self._norm(L["norm1"], s)
             if L["kind"] == "G":
-                fn.tc_gemv(L["w_in"], x, d, pr, ps, B, 0, s)
+                self._project(L["w_in"], self.proj, s)
                 fn.gdn_run_batch(L["gdn"], pr, ps, pr + 4 * self.convch, ps, pr + 4 * (self.convch + nvh * DS), ps,
                                  p(self.core), nvh * DS, 1, s)
-                fn.tc_gemv(L["w_out"], p(self.core), nvh * DS, h, d, B, 1, s)  # h += W_out core
+                self._join(L["w_out"], self.core, L["norm2"], s)  # h += W_out core
             else:
-                fn.tc_gemv(L["w_qkv"], x, d, pr, ps, B, 0, s)
+                self._project(L["w_qkv"], self.proj, s)
                 self._attention(L, s)
-                fn.tc_gemv(L["w_o"], p(self.att), nh * HD, h, d, B, 1, s)  # h += W_o o
-            fn.rmsnorm_rows(h, p(L["norm2"]), x, d, B, eps, s)
-            fn.tc_gemv(L["router"], x, d, p(self.lr), ne1, B, 0, s)
-            fn.moe_run(L["moe"], p(self.lr), ne1, x, h, B, 1, s)  # every sequence's token in one call; h += moe(x)
-        fn.rmsnorm_rows(h, p(self.final_norm), x, d, B, eps, s)
+                self._join(L["w_o"], self.att, L["norm2"], s)  # h += W_o o
+            fn.tc_gemv(L["router"], p(self.x), cfg["D"], p(self.lr), ne1, B, 0, s)
+            fn.moe_run(L["moe"], p(self.lr), ne1, p(self.x), p(self.h), B, 1, s)  # every sequence's token in one call; h += moe(x)
         vocab = cfg["vocab"]
-        fn.tc_gemv(self.head, x, d, p(self.logits), vocab, B, 0, s)
+        self._norm(self.final_norm, s)
+        self._project(self.head, self.logits, s)
         fn.argmax_dev(p(self.logits), vocab, vocab, B, p(self.next), s)
         self._advance(s)
 

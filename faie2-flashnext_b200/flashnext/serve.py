@@ -7,11 +7,14 @@ on the GPU, so a step is one CUDA graph whatever the lengths are.
 
     m = ServeModel(fn, cfg, W, batch=8, pages=512, max_ctx=4096)
     outs = m.generate(prompts, n_new=[64, 200, ...])        # any number of requests; a list of token arrays
+    outs, scores = m.generate(prompts, 64, scores=5)        # and the log probabilities of their tokens, with 5 alternatives
 
 A prompt is fed a token per step, as in the other decode models (the DeltaNet core and the MoE layer take a token per
 sequence and step)."""
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import numpy as np
 
@@ -26,9 +29,21 @@ class OutOfPages(RuntimeError):
         self.outs = outs
 
 
+class Scores(NamedTuple):
+    """Of a request's tokens 1, 2, ..: log probability, rank (0: the largest logit), the entropy of the distribution that the token was taken from,
+    and its best alternatives (flashnext/logprobs.py); numpy arrays [tokens - 1], the last two [tokens - 1][alternatives]."""
+    logprob: np.ndarray
+    rank: np.ndarray
+    entropy: np.ndarray
+    top_ids: np.ndarray
+    top_logprobs: np.ndarray
+
+
 class ServeModel(BatchDecodeModel):
-    def __init__(self, fn, cfg: dict, W: dict, batch: int, pages: int, max_ctx: int = 512, page_size: int = 64):
-        """pages: of the pool, for each attention layer (one table serves them all); idle places use one each."""
+    def __init__(self, fn, cfg: dict, W: dict, batch: int, pages: int, max_ctx: int = 512, page_size: int = 64,
+                 dense: str = "gguf"):
+        """pages: of the pool, for each attention layer (one table serves them all); idle places use one each. dense: as the batched
+        step's."""
         import torch
 
         import kv4
@@ -36,7 +51,7 @@ class ServeModel(BatchDecodeModel):
         self.ws, self.planner = kv4.KV4Workspace(fn), kv4.KV4Planner(fn, page_size)
         if pages < batch:
             raise ValueError("a page per place of the batch is wanted at least")
-        super().__init__(fn, cfg, W, batch, max_ctx)
+        super().__init__(fn, cfg, W, batch, max_ctx, dense)
         dev = self.h.device
         i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)  # noqa: E731
         self.inputs, self.zero, self.drop, self.ones, self.ctx = i32(batch), i32(1), i32(batch), i32(batch) + 1, i32(batch)
@@ -83,11 +98,6 @@ class ServeModel(BatchDecodeModel):
             self.ctx.copy_(self.plan.ctx)
             self.free_count.copy_(self.plan.free_count)
 
-    def launch_step(self, s: int):
-        import torch
-        with torch.cuda.stream(torch.cuda.ExternalStream(s)):  # the kv4 layer launches on the current stream
-            super().launch_step(s)
-
     def start(self, prompts, stream):
         """Every place idle: no request, no pages taken."""
         import torch
@@ -101,13 +111,17 @@ class ServeModel(BatchDecodeModel):
         for g in self.gdns:
             self.fn.gdn_reset(g, stream.cuda_stream)
 
-    def generate(self, prompts, n_new, stream, logits=None, wait=False):
+    def generate(self, prompts, n_new, stream, logits=None, wait=False, scores=None):
         """Greedy decode of any number of requests, as many at a time as the batch has places. prompts: a list of token id
         arrays (of any lengths); n_new: tokens to generate, one number or one per request. Returns a list of arrays, prompt
         then new tokens. logits: an optional callback(request, position, row [vocab]) per step. wait: a request is admitted, in order,
         when the pages that it may come to need fit beside those of the requests before it and one for each idle place; without
-        it requests take places as they come free, and a step that finds no page raises OutOfPages."""
+        it requests take places as they come free, and a step that finds no page raises OutOfPages. scores: with a number of alternatives
+        (0..32) what the model said of every token after a request's first, the prompt's among them, is returned beside the tokens: a
+        list of Scores, one per request."""
         import torch
+
+        import logprobs as lp
         if self.graph is None:
             raise RuntimeError("capture() the step first")
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
@@ -120,6 +134,10 @@ class ServeModel(BatchDecodeModel):
         self.start(None, stream)
         waiting, place, seq = list(range(len(prompts))), [None] * self.B, [p.tolist() for p in prompts]
         at = [0] * self.B  # tokens fed of the place's request
+        if scores is not None:
+            if not 0 <= scores <= lp.MAX_TOP:
+                raise ValueError(f"scores: 0..{lp.MAX_TOP} alternatives are wanted")
+            said, kept, known = [[] for _ in prompts], None, np.full(self.B, -1, np.int32)  # known: the token that follows, if it is given
         inputs, drop = np.zeros(self.B, np.int32), np.full(self.B, -1, np.int32)
         while waiting or any(r is not None for r in place):
             for b in range(self.B):
@@ -131,23 +149,33 @@ class ServeModel(BatchDecodeModel):
                     for g in self.gdns:
                         self.fn.gdn_reset_seq(g, b, stream.cuda_stream)
                 inputs[b] = 0 if place[b] is None else seq[place[b]][at[b]]
+                if scores is not None:
+                    known[b] = seq[place[b]][at[b] + 1] if place[b] is not None and at[b] + 1 < len(seq[place[b]]) else -1
             with torch.cuda.stream(stream):
                 self.inputs.copy_(torch.from_numpy(inputs))
                 self.drop.copy_(torch.from_numpy(drop))
                 self.graph.replay()
+                if scores is not None:
+                    given = torch.from_numpy(known).to(self.next.device)
+                    kept = lp.token_logprobs(self.fn, self.logits, torch.where(given < 0, self.next, given), scores, out=kept)
             self.fn.sync(stream.cuda_stream)
             if int(self.plan.status):
                 done = [np.array(s, np.int32) if len(s) == len(p) + n else None for s, p, n in zip(seq, prompts, n_new)]
                 raise OutOfPages(f"out of pages: {int(self.plan.status)} of the batch found none (of {self.n_pages})", done)
             new = self.next.cpu().numpy()
+            if scores is not None:
+                step = [t.cpu().numpy() for t in kept]
             for b, r in enumerate(place):
                 if r is None:
                     continue
                 if logits is not None:
                     logits(r, at[b], self.logits[b])
+                if scores is not None:
+                    said[r].append([t[b] for t in step])
                 at[b] += 1
                 if at[b] == len(seq[r]):
                     seq[r].append(int(new[b]))
                 if len(seq[r]) == len(prompts[r]) + n_new[r]:
                     place[b] = None
-        return [np.array(s, np.int32) for s in seq]
+        outs = [np.array(s, np.int32) for s in seq]
+        return outs if scores is None else (outs, [Scores(*(np.array(v) for v in zip(*t))) for t in said])

@@ -106,16 +106,20 @@ def test_rows_of_any_size(fn, fp8):
         assert (off <= np.abs(want[r]) * (2.0 ** -4 + 2.0 ** -20) + O.spread(s, 1, 640, 1)[0] * 2.0 ** -9.9).all(), r
 
 
-def test_rows_without_codes(fn, fp8):
-    """The residual's addition and the norm alone, through the C entry."""
-    x, add, w = rand(5, 2048, "f32", 9), rand(5, 2048, "f32", 10), rand(1, 2048, "f32", 11)[0]
-    total, y = torch.empty_like(x), torch.empty_like(x)
-    s = torch.cuda.current_stream().cuda_stream
-    fn.fp8_rows(0, x.data_ptr(), 2048, add.data_ptr(), 2048, w.data_ptr(), 1e-6, 5, 2048, total.data_ptr(), 2048, y.data_ptr(), 2048, None,
-                None, s)
-    fn.sync(s)
-    assert torch.equal(total, x + add)
-    assert np.array_equal(np64(y), O.rms(np64(total), np64(w), 1e-6).astype(np.float64))
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, cols", [(5, 2048), (1, 48), (700, 512)])
+def test_rows_without_codes(fn, fp8, rows, cols, dtype):
+    """The residual's addition and the norm alone."""
+    x, add, w = rand(rows, cols, dtype, 9), rand(rows, cols, dtype, 10), rand(1, cols, "f32", 11)[0]
+    y, want = torch.empty_like(x), (x.float() + add.float()).to(x.dtype)
+    fp8.add_norm(fn, x, add, w, 1e-6, x, y)
+    sync(fn)
+    assert torch.equal(x, want)
+    assert np.array_equal(np64(y), np64(torch.from_numpy(O.rms(np64(want), np64(w), 1e-6)).to(x.dtype)))
+    with pytest.raises(ValueError, match="normed"):
+        fp8.add_norm(fn, x, add, w, 1e-6, x, y[:, :16])
+    with pytest.raises(ValueError, match="weight"):
+        fp8.add_norm(fn, x, add, w[:16], 1e-6, x, y)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -152,7 +156,8 @@ def exact_product(xq, xs, wq, ws):
 PRODUCTS = [(1, 1, 16), (1, 8, 128), (2, 129, 144), (1, 12352, 256), (5, 513, 2048), (16, 128, 4096), (17, 2048, 2048), (32, 1000, 1040),
             (33, 257, 384), (50, 3000, 512), (64, 640, 272), (65, 130, 128), (80, 19000, 128), (97, 255, 656), (128, 128, 8192), (129, 384, 256),
             (200, 2048, 512), (333, 2048, 4096), (257, 100, 2064), (512, 512, 512), (1000, 1111, 1024), (2000, 4100, 384), (4096, 24, 128),
-            (8192, 513, 256), (300, 20000, 144)]
+            (8192, 513, 256), (300, 20000, 144), (1500, 12352, 256), (2305, 5001, 1040), (3000, 8200, 144), (40, 12352, 128), (20, 30011, 384),
+            (31, 9000, 1168)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
