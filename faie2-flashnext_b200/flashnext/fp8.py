@@ -120,9 +120,11 @@ class Fp8Weight:
         _codes("weight", q, scale, GROUP, q.get_device())
         if q.shape[0] < 1 or q.data_ptr() % 16:
             raise ValueError("weight: rows are wanted, codes aligned to 16 bytes")
-        self.fn, self.q, self.scale, self.dev, self.index = fn, q, scale, q.device, q.get_device()
+        self._keep(fn, q, scale)
+
+    def _keep(self, fn, q, scale):
+        self.fn, self.q, self.scale, self.dev, self.index, self.c = fn, q, scale, q.device, q.get_device(), None
         self.rows, self.cols = q.shape
-        self.c = C.byref(FnFp8(q.data_ptr(), scale.data_ptr(), self.rows, self.cols))
 
     @classmethod
     def quantise(cls, fn, w):
@@ -135,7 +137,9 @@ class Fp8Weight:
         q = torch.empty(rows, cols, dtype=CODES, device=w.device)
         scale = torch.empty(-(-rows // GROUP), -(-cols // GROUP), dtype=torch.float32, device=w.device)
         fn.fp8_blocks(_TYPE[w.dtype], w.data_ptr(), w.stride(0), rows, cols, q.data_ptr(), scale.data_ptr(), _stream(w.device))
-        return cls(fn, q, scale)
+        self = cls.__new__(cls)
+        self._keep(fn, q, scale)
+        return self
 
     def values(self) -> torch.Tensor:
         """What the codes stand for, fp32."""
@@ -148,6 +152,8 @@ class Fp8Weight:
         q, scale = x
         _codes("x", q, scale, 1, self.index)
         rows, cols = q.shape
+        if self.c is None:
+            self.c = C.byref(FnFp8(self.q.data_ptr(), self.scale.data_ptr(), self.rows, self.cols))
         if cols != self.cols:
             raise ValueError(f"x: rows of {self.cols} columns are wanted")
         shape = (rows, self.rows)

@@ -30,9 +30,12 @@ class Logprobs(NamedTuple):
 
 
 def _make(rows, top, dev, tokens):
-    f, i = {"dtype": torch.float32, "device": dev}, {"dtype": torch.int32, "device": dev}
-    return Logprobs(torch.empty(rows, **f) if tokens else None, torch.empty(rows, **i) if tokens else None, torch.empty(rows, **f),
-                    torch.empty((rows, top), **i), torch.empty((rows, top), **f))
+    # one allocation: an empty tensor costs the host as much as two views of one
+    f = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=dev)
+    i = f.view(torch.int32)
+    one, wide, at = (rows,), (rows, top), 3 * rows
+    return Logprobs(f.as_strided(one, (1,), 0) if tokens else None, i.as_strided(one, (1,), rows) if tokens else None,
+                    f.as_strided(one, (1,), 2 * rows), i.as_strided(wide, (top, 1), at), f.as_strided(wide, (top, 1), at + rows * top))
 
 
 def token_logprobs(fn, logits, tokens=None, top: int = 0, out: Logprobs | None = None) -> Logprobs:
