@@ -265,27 +265,27 @@ template <> struct LpAcc<__nv_bfloat16> {
         const float y = far ? 0.0f : fmaf(b, LP_LOG2E, -c), f = lp_ex2(-y), z = s0 + s1;
         return LpSum{m, b, f * z, f * (t0 + t1 - y * z)};
     }
-    // how many entries are at least `bar`: counted in bf16, two at a time, from 128 on, where the next numbers up are 1 apart in value
-    // and in bits
+    // How many entries are at least `bar`, two at a time: a mask of ones for each that is, added up as 32-bit numbers. `low` masks in the
+    // low halves and `high` ones make 0xffff (low + 65536 high) = 65536 (low - high) - low, from which both are read back.
     struct Counter {
-        uint32_t n = 0x43004300u;
+        uint32_t n = 0;
         __device__ __forceinline__ void add(uint4 w, float bar) {
             const uint32_t v[4] = {w.x, w.y, w.z, w.w};
             const __nv_bfloat162 b = __floats2bfloat162_rn(bar, bar);  // (exact)
-            __nv_bfloat162 c;
-            memcpy(&c, &n, 4);
+            uint32_t k[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 __nv_bfloat162 x;
                 memcpy(&x, &v[i], 4);
-                c = __hadd2(c, __hge2(x, b));
+                k[i] = __hge2_mask(x, b);
             }
-            memcpy(&n, &c, 4);
+            n += k[0] + k[1];
+            n += k[2] + k[3];
         }
-        __device__ __forceinline__ void flush(int &before) {  // before 128 of a half
-            n -= 0x43004300u;
-            before += (n & 0xffff) + (n >> 16);
-            n = 0x43004300u;
+        __device__ __forceinline__ void flush(int &before) {  // before 65536 of a half
+            const uint32_t low = (0u - n) & 0xffff, high = (low - ((n + low) >> 16)) & 0xffff;
+            before += low + high;
+            n = 0;
         }
         __device__ __forceinline__ void end(int &before) { flush(before); }
     };
@@ -384,8 +384,13 @@ __device__ __forceinline__ LpSum lp_warp_join(LpSum a) {
     return a;
 }
 
+constexpr int LP_MAX_VOCAB = 1 << 28;  // so a segment has up to 2048 rounds, each with up to 16 entries of a half of the counter
+// CTAs of 256 threads on an SM: five where instructions bound it (bf16, 2048 rows of 151936: 138.5 us, by four 143.8; 200 rows, where
+// latency counts, 26.5 and 25.0), four where loads do (fp32, 1024 rows: 115 us, by five 122)
+constexpr int lp_ctas(int size) { return size == 2 ? 5 : 4; }
+
 // grid: rows x C CTAs in clusters of C (a power of two up to 8) for a row
-template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, 1024 / LP_T) k_logprobs(const LpArgs a, int C) {
+template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, LP_T == 1024 ? 1 : lp_ctas(sizeof(T))) k_logprobs(const LpArgs a, int C) {
     constexpr int N = LpAcc<T>::N, U = 4, LP_W = LP_T / 32, SEGMENTS = LpShared<LP_T>::SEGMENTS;  // entries of a word; words in flight per thread
     static_assert(LP_W >= LP_MAX_CLUSTER, "");
     __shared__ LpShared<LP_T> sh;
@@ -448,8 +453,8 @@ template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, 1024 / L
                         if (w + u * LP_T < w1) counter.add(r[u], w + u * LP_T < own_word ? given : above);
                 }
             }
-            if (known) counter.flush(before);
         }
+        if (known) counter.flush(before);
         if (a.top) sh.most[seg][tid] = lp_order(LpAcc<T>::value(most));
     }
     if (known) counter.end(before);
@@ -614,14 +619,14 @@ FN_API int fn_logprobs(uint32_t type, const void *logits, int64_t stride, int ro
                        int *rank, float *entropy, int top, int *top_ids, float *top_logprobs, void *stream) {
     return kv4_entry("logprobs", [&]() -> int {
         if (type != T_F32 && type != T_BF16) return fail("logprobs: logits must be F32 or BF16");
-        if (rows < 0 || vocab < 1 || vocab > 1 << 30) return fail("logprobs: bad row / vocabulary counts");
+        if (rows < 0 || vocab < 1 || vocab > LP_MAX_VOCAB) return fail("logprobs: bad row / vocabulary counts");
         if (top < 0 || top > LP_MAX_TOP) return fail("logprobs: top out of range (0..32)");
         if (rows == 0) return 0;
         if (!logits || (top && (!top_ids || !top_logprobs))) return fail("logprobs: null pointer");
         if (!tokens && (logprob || rank)) return fail("logprobs: log probabilities and ranks want tokens");
         if ((uintptr_t)logits % (type == T_F32 ? 4 : 2)) return fail("logprobs: logits must be aligned to their type");
         // rows that the SMs can take at once get CTAs of 1024 threads, and up to 8 of them (of 4096 entries and more) where they are fewer;
-        // else four CTAs of 256 share an SM
+        // else CTAs of 256 share an SM
         const bool large = rows <= num_sms();
         int C = 1;
         while (large && C < LP_MAX_CLUSTER && (int64_t)rows * C * 2 <= num_sms() && vocab / (2 * C) >= 4096) C *= 2;

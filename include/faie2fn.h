@@ -382,7 +382,7 @@ int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *scales,
 
 /* ---- scores of tokens (no counterpart in the reference, which answers with the argmax alone, engine/faie2fn.cu:1910-1935) --
  * Of every row of logits [rows][vocab] (device memory, F32 (0) or BF16 (30), `stride` elements from row to row, entries adjacent;
- * vocab 1..2^30), in one launch: logprob [rows] = logits[t] - ln sum e^logits of the row's token t = tokens[row]; rank [rows] =
+ * vocab 1..2^28), in one launch: logprob [rows] = logits[t] - ln sum e^logits of the row's token t = tokens[row]; rank [rows] =
  * the entries that stand before t, larger ones first, equal ones by the lower index (-0 equals +0); entropy [rows] = -sum p ln p;
  * top_ids, top_logprobs [rows][top] = the first `top` (0..32) entries of that order. Any of logprob, rank, entropy may be NULL;
  * tokens may be NULL if logprob and rank are. Entries at -inf have no probability and are no alternatives; places that stay empty

@@ -47,7 +47,7 @@ GOOD = dict(dtype=0, logits=4096, stride=10, rows=2, vocab=10, tokens=4096, logp
 
 @pytest.mark.parametrize("change, words", [
     (dict(dtype=1), "F32 or BF16"), (dict(dtype=12), "F32 or BF16"), (dict(rows=-1), "bad row"), (dict(vocab=0), "bad row"),
-    (dict(vocab=(1 << 30) + 1), "bad row"), (dict(top=-1), "top out of range"), (dict(top=33), "top out of range"),
+    (dict(vocab=(1 << 28) + 1), "bad row"), (dict(top=-1), "top out of range"), (dict(top=33), "top out of range"),
     (dict(logits=None), "null pointer"), (dict(top_ids=None), "null pointer"), (dict(top_logprobs=None), "null pointer"),
     (dict(tokens=None), "want tokens"), (dict(tokens=None, rank=None), "want tokens"), (dict(logits=4098), "aligned"),
     (dict(logits=4097, dtype=30), "aligned")])
