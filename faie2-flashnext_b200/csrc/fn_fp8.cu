@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "fn_fp8.h"
 
@@ -304,7 +305,8 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
                        float *scales, void *stream) {
     return kv4_entry("fp8 rows", [&]() -> int {
         if (type != T_F32 && type != T_BF16) return fail("fp8 rows: rows must be F32 or BF16");
-        if (rows < 0 || cols < 16 || cols % 16) return fail("fp8 rows: bad row count, or columns that are no multiple of 16");
+        if (rows < 0 || cols < 16 || cols % 16 || cols > FP8_MAX_COLS)
+            return fail("fp8 rows: bad row count, or columns that are no multiple of 16");
         if (rows == 0) return 0;
         if (!x || !codes != !scales) return fail("fp8 rows: null pointer");
         if (!codes && !total && !normed) return fail("fp8 rows: nothing to write");
@@ -313,6 +315,13 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
             return fail("fp8 rows: rows must be aligned to their type");
         if ((uintptr_t)weight % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4)
             return fail("fp8 rows: weight and codes must be 16-byte aligned");
+        const int64_t bytes = (int64_t)cols * size;
+        if (rows > 1 && ((total && total_stride < cols) || (normed && normed_stride < cols))) return fail("fp8 rows: rows that are written overlap");
+        for (const auto &[p, ps] : {std::pair(x, x_stride), std::pair(add, add_stride)})
+            if (fp8_mixed(total, total_stride * size, p, ps * size, rows, bytes) || fp8_mixed(normed, normed_stride * size, p, ps * size, rows, bytes))
+                return fail("fp8 rows: rows that are written lie over other rows that are read");
+        if (normed && (normed == total || fp8_mixed(total, total_stride * size, normed, normed_stride * size, rows, bytes)))
+            return fail("fp8 rows: total and normed lie over one another");
         const bool wide = ((uintptr_t)x | (uintptr_t)add | (uintptr_t)total | (uintptr_t)normed | (uint64_t)(x_stride * size) |
                            (uint64_t)(add_stride * size) | (uint64_t)(total_stride * size) | (uint64_t)(normed_stride * size)) % 16 == 0;
         int tpr = 32;
@@ -333,7 +342,8 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
 FN_API int fn_fp8_blocks(uint32_t type, const void *w, int64_t stride, int rows, int cols, uint8_t *codes, float *scales, void *stream) {
     return kv4_entry("fp8 blocks", [&]() -> int {
         if (type != T_F32 && type != T_BF16) return fail("fp8 blocks: weights must be F32 or BF16");
-        if (rows < 0 || cols < 16 || cols % 16) return fail("fp8 blocks: bad row count, or columns that are no multiple of 16");
+        if (rows < 0 || cols < 16 || cols % 16 || cols > FP8_MAX_COLS)
+            return fail("fp8 blocks: bad row count, or columns that are no multiple of 16");
         if (rows == 0) return 0;
         if (!w || !codes || !scales) return fail("fp8 blocks: null pointer");
         const int size = type == T_F32 ? 4 : 2;

@@ -756,7 +756,7 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
                           int64_t add_stride, void *out, int64_t out_stride, void *stream) {
     return kv4_entry("fp8 product", [&]() -> int {
         if (!w || !w->codes || !w->scales) return fail("fp8 product: no weight");
-        if (w->rows < 1 || w->rows > 1 << 28 || w->cols < 16 || w->cols % 16 || w->cols > 1 << 24)
+        if (w->rows < 1 || w->rows > 1 << 28 || w->cols < 16 || w->cols % 16 || w->cols > FP8_MAX_COLS)
             return fail("fp8 product: bad weight sizes (columns: multiples of 16)");
         if (type != T_F32 && type != T_BF16) return fail("fp8 product: outputs must be F32 or BF16");
         if (rows < 0 || rows > 1 << 28) return fail("fp8 product: bad row count");
@@ -765,6 +765,10 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
         if (((uintptr_t)w->codes | (uintptr_t)codes) % 16) return fail("fp8 product: codes must be 16-byte aligned");
         if (((uintptr_t)w->scales | (uintptr_t)scales) % 4 || ((uintptr_t)out | (uintptr_t)add) % (type == T_F32 ? 4 : 2))
             return fail("fp8 product: scales, add and out must be aligned to their types");
+        const int size = type == T_F32 ? 4 : 2;
+        if (rows > 1 && out_stride < w->rows) return fail("fp8 product: rows of out overlap");
+        if (fp8_mixed(out, out_stride * size, add, add_stride * size, rows, (int64_t)w->rows * size))
+            return fail("fp8 product: out lies over other rows of add");
         Fp8Args a{};
         a.ws = w->scales, a.xs = scales;
         a.m = rows, a.n = w->rows, a.groups = fp8_groups(w->cols);

@@ -66,7 +66,7 @@ def empty_rows(rows: int, cols: int, device="cuda") -> Fp8Rows:
 def quantise_rows(fn, x, add=None, total=None, weight=None, eps: float = 1e-6, normed=None, out: Fp8Rows | None = None) -> Fp8Rows:
     """x [rows][cols] fp32 or bf16 (any row stride) as 8-bit rows. add: rows added first (the sum is rounded to x's type); total: gets
     the sum (may be x or add); weight: fp32 [cols] of an RMSNorm of the sum, else none is taken; normed: gets the normed rows in x's
-    type. out: buffers of those sizes, written again."""
+    type (may be x or add, not total). out: buffers of those sizes, written again."""
     shape, dtype, index = x.shape, x.dtype, x.get_device()
     if len(shape) != 2 or dtype not in _TYPE or index < 0 or x.stride(1) != 1:
         _wants("x", x, None, None, -1)

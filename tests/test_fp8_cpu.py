@@ -89,6 +89,26 @@ def test_product_refuses(libpath, weight, change, words):
         FN(libpath).fp8_product(C.byref(FnFp8(*weight)), **{**PRODUCT, **change})
 
 
+@pytest.mark.parametrize("change, words", [
+    (dict(total_stride=60), "rows that are written overlap"), (dict(normed_stride=0), "rows that are written overlap"), (dict(normed=4096), "total and normed"),
+    (dict(total=4112), "lie over"), (dict(total=4096 + 256), "lie over"), (dict(normed=1 << 20, add=(1 << 20) - 16), "lie over"),
+    (dict(total=1 << 20, add=1 << 20, add_stride=0), "lie over"), (dict(normed=(1 << 20) + 128, total=1 << 20, total_stride=128, normed_stride=128), "total and normed"),
+    (dict(normed=(1 << 20) - 128, total=1 << 20, total_stride=128, normed_stride=128), "total and normed"), (dict(cols=(1 << 24) + 16), "bad row count")])
+def test_rows_refuse_to_overlap(libpath, change, words):
+    with pytest.raises(RuntimeError, match=words):
+        FN(libpath).fp8_rows(**{**ROWS, "normed": 1 << 16, **change})
+
+
+def test_more_refusals(libpath):
+    f = FN(libpath)
+    with pytest.raises(RuntimeError, match="bad row count"):
+        f.fp8_blocks(**{**BLOCKS, "cols": (1 << 24) + 16})
+    for change, words in ((dict(out_stride=63), "rows of out overlap"), (dict(add=4096 + 256), "other rows of add"), (dict(add=4080), "other rows of add"),
+                          (dict(add_stride=0), "other rows of add")):
+        with pytest.raises(RuntimeError, match=words):
+            f.fp8_product(C.byref(FnFp8(1 << 16, 1 << 16, 64, 64)), **{**PRODUCT, **change})
+
+
 def test_no_rows_is_no_work(libpath):
     f = FN(libpath)
     f.fp8_rows(**{**ROWS, "rows": 0})

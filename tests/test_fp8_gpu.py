@@ -1,6 +1,6 @@
 """GPU parity of 8-bit rows, weights and their product (flashnext/fp8.py over fn_fp8_*) against the float64 oracle (oracle/fp8.py).
 
-Tolerances. Codes, scales, sums and normed rows are equal: the oracle takes the kernels' quotients and products in fp32 (a row's factor
+Tolerances. Codes, scales, sums and normed rows are equal: the oracle takes the kernels' reciprocals and products in fp32 (a row's factor
 from a sum in 64 bits, rounded once). Products: of small whole numbers and powers of two every sum is exact, so they are equal. Of any
 numbers: a group's 128 products are exact, and an MMA adds 32 of them and the sum so far, aligned to the largest and cut no higher
 than 2^-23 of it; four MMAs a group, 33 terms each: below 4 * 33 * 2^-23 < 2^-15 of the sum of the terms' magnitudes. The scales' product
@@ -104,6 +104,51 @@ def test_rows_of_any_size(fn, fp8):
         # half a step of e4m3, or half the smallest one, and a last bit of the factors
         off = np.abs(np64(got.values())[r] - want[r])
         assert (off <= np.abs(want[r]) * (2.0 ** -4 + 2.0 ** -20) + O.spread(s, 1, 640, 1)[0] * 2.0 ** -9.9).all(), r
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, cols", [(1000, 512), (3, 4096), (400, 8192), (150, 8208)])
+def test_rows_in_place(fn, fp8, rows, cols, dtype):
+    """total over add and normed over x, columns of one buffer side by side, one row added to all."""
+    both = rand(rows, 2 * cols, dtype, 12)
+    add, w = rand(1, cols, dtype, 13)[0].expand(rows, cols), 1 + 0.1 * rand(1, cols, "f32", 14)[0]
+    h = (both[:, :cols].float() + add.float()).to(both.dtype)
+    want = fp8.quantise_rows(fn, h, weight=w, normed=(y := torch.empty_like(h)))
+    for norm, rows_ in ((w, want), (None, fp8.quantise_rows(fn, h))):
+        b, t = both.clone(), torch.empty_like(h)
+        got = fp8.quantise_rows(fn, b[:, :cols], add=add, total=b[:, cols:], weight=norm, normed=t)
+        assert torch.equal(b[:, cols:], h) and torch.equal(b[:, :cols], both[:, :cols]) and torch.equal(t, y if norm is not None else h)
+        x, a = both[:, :cols].clone(), add.clone()
+        again = fp8.quantise_rows(fn, x, add=a, total=a, weight=norm, normed=x)
+        assert torch.equal(a, h) and torch.equal(x, t)
+        x, a = both[:, :cols].clone(), add.clone()
+        third = fp8.quantise_rows(fn, a, add=x, weight=norm, normed=x)
+        assert torch.equal(x, t)
+        for r in (got, again, third):
+            assert torch.equal(r.scale, rows_.scale) and torch.equal(r.q.view(torch.uint8), rows_.q.view(torch.uint8))
+    with pytest.raises(RuntimeError, match="lie over"):
+        fp8.quantise_rows(fn, both[:, :cols], add=add, total=both[:, 16:16 + cols])
+    with pytest.raises(RuntimeError, match="overlap"):
+        fp8.quantise_rows(fn, both[:, :cols], add=add, total=add)
+
+
+@pytest.mark.parametrize("m, n", [(1, 16), (20, 5000), (40, 333), (600, 12352)])
+def test_product_into_part_of_a_buffer(fn, fp8, m, n):
+    """out among other columns, which stay as they were; one row added to all; add beside out."""
+    x, w = fp8.quantise_rows(fn, rand(m, 272, "f32", 15)), fp8.Fp8Weight.quantise(fn, rand(n, 272, "f32", 16))
+    bias, b = rand(1, n, "f32", 17)[0], rand(m, 2 * n + 8, "f32", 18)
+    old, want = b.clone(), w.product(x)
+    w.product(x, add=bias.expand(m, n), out=b[:, 4:4 + n])
+    assert torch.equal(b[:, 4:4 + n], w.product(x, add=bias.expand(m, n).contiguous()))
+    assert torch.equal(b[:, :4], old[:, :4]) and torch.equal(b[:, 4 + n:], old[:, 4 + n:])
+    assert ((b[:, 4:4 + n] - want - bias).abs() <= 2.0 ** -22 * (want.abs() + bias.abs())).all()
+    w.product(x, add=b[:, 4 + n:4 + 2 * n], out=b[:, 4:4 + n])
+    assert torch.equal(b[:, 4:4 + n], w.product(x, add=old[:, 4 + n:4 + 2 * n].contiguous())) and torch.equal(b[:, 4 + n:], old[:, 4 + n:])
+    if m > 1:
+        with pytest.raises(RuntimeError, match="other rows of add"):
+            w.product(x, add=b[:, :n], out=b[:, 4:4 + n])
+        with pytest.raises(RuntimeError, match="overlap"):
+            w.product(x, out=torch.empty(m, n, device="cuda")[:1].expand(m, n))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
