@@ -8,8 +8,8 @@
 // 448 is e4m3's largest number; 2^-116 keeps 448 / a and a / 448 normal numbers (a group of zeros has codes 0). A NaN in a group
 // makes its scale NaN, an infinity its scale infinite and its codes NaN: both read back as NaN.
 //
-// What bounds it is memory: every input is read once and kept in registers between the row's sum and its codes (rows up to 8192
-// columns; longer ones are read again, from L2). The sum of squares is held in 64 bits: an fp32 sum's last bits would move codes
+// What bounds it is memory, and close to it instruction issue (70%): every input is read once and kept in registers between the row's sum and
+// its codes (rows up to 8192 columns; longer ones are read again, from L2). 8192 x 4096 in bf16 with a residual: 40.2 us, 5.9 TB/s. The sum of squares is held in 64 bits: an fp32 sum's last bits would move codes
 // that lie next to a border, and squares of fp32 values leave that type's range.
 #include <cuda_bf16.h>
 
@@ -37,23 +37,37 @@ struct F8RowArgs {
     int tpr;  // threads of a row: 32, 64, 128 or 256
 };
 
+// the larger magnitude of three numbers; NaN if one is
+__device__ __forceinline__ float f8_max_nan(float a, float b, float c) {
+    float e;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(e) : "f"(a), "f"(b), "f"(c));
+    return e;
+}
 __device__ __forceinline__ float f8_max_nan(float a, float b) {
     float e;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(e) : "f"(a), "f"(b));
     return e;
 }
 __device__ __forceinline__ float f8_amax(const float (&y)[8]) {
-    float m = fabsf(y[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = f8_max_nan(m, fabsf(y[i]));
-    return m;
+    const float m = f8_max_nan(y[0], y[1], y[2]), n = f8_max_nan(y[3], y[4], y[5]);
+    return f8_max_nan(f8_max_nan(m, y[6], y[7]), n);
 }
-// eight codes, lowest byte first
-__device__ __forceinline__ uint2 f8_codes(const float (&y)[8], float inv) {
-    uint16_t p[4];
+// y *= b, two numbers an instruction
+__device__ __forceinline__ void f8_mul2(float &y0, float &y1, float b0, float b1) {
+    asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n mul.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}\n"
+        : "+f"(y0), "+f"(y1)
+        : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void f8_scale(float (&y)[8], float b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[i]) : "f"(y[2 * i + 1] * inv), "f"(y[2 * i] * inv));
+    for (int i = 0; i < 8; i += 2) f8_mul2(y[i], y[i + 1], b, b);
+}
+// eight codes of y inv, lowest byte first
+__device__ __forceinline__ uint2 f8_codes(float (&y)[8], float inv) {
+    uint16_t p[4];
+    f8_scale(y, inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[i]) : "f"(y[2 * i + 1]), "f"(y[2 * i]));
     return make_uint2((uint32_t)p[0] | (uint32_t)p[1] << 16, (uint32_t)p[2] | (uint32_t)p[3] << 16);
 }
 
@@ -81,33 +95,28 @@ template <typename T> __device__ __forceinline__ void f8_unpack(const F8Raw<T> &
         for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
-template <typename T, bool WIDE> __device__ __forceinline__ void f8_load(const T *p, float (&v)[8]) {
-    F8Raw<T> r;
-    f8_fetch<T, WIDE>(p, r);
-    f8_unpack<T>(r, v);
-}
-template <typename T, bool WIDE> __device__ __forceinline__ void f8_store(T *p, const float (&v)[8]) {
-    if constexpr (!WIDE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = (T)v[i];
-    } else if constexpr (sizeof(T) == 4) {
-        *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-        *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+// rounded to T
+template <typename T> __device__ __forceinline__ void f8_pack(const float (&v)[8], F8Raw<T> &r) {
+    if constexpr (sizeof(T) == 4) memcpy(&r, v, sizeof(r));
+    else {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
             memcpy(&u[i], &b, 4);
         }
-        *(uint4 *)p = make_uint4(u[0], u[1], u[2], u[3]);
+        r.w[0] = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
-// rounded to T
-template <typename T> __device__ __forceinline__ void f8_round(float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
+template <typename T, bool WIDE> __device__ __forceinline__ void f8_store(T *p, const F8Raw<T> &r) {
+    if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4 *)p)[j] = r.w[j];
+    } else {
+        T v[8];
+        memcpy(v, &r, sizeof(r));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = v[i];
     }
 }
 
@@ -118,73 +127,84 @@ __device__ __forceinline__ float f8_rsqrt(double v) {
     return (float)fma(0.5 * r, fma(-v * r, r, 1.0), r);
 }
 
+// rounds of 8 columns a thread that are on their way while others are worked on: 64 bytes a thread of x, and of add
+constexpr bool f8_ahead(int rounds, int size) { return rounds && rounds * size <= 8; }
+// CTAs that an SM holds
+constexpr int f8_ctas(int rounds, int size) { return !f8_ahead(rounds, size) ? 2 : rounds * size <= 2 ? 6 : rounds * size == 4 ? 4 : 3; }
+
 // 8 columns a thread, `tpr` threads a row, R rounds of them held in registers (0: any number, read twice if there is a norm). A CTA takes
-// rows at a stride of the grid, the next one's words on their way while one is summed and coded (R up to 2).
-template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T, R == 1 ? 6 : R == 2 ? 4 : 2) k_fp8_rows(const F8RowArgs a) {
-    constexpr bool AHEAD = R == 1 || R == 2;
+// rows at a stride of the grid, the next one's words on their way while one is summed and coded. F: whether there is something to add (1) and
+// a norm (2), or -1 for whatever there is. What lies past the last column or row reads the last ones' place, counts as zeros and is not
+// stored: with branches around it all a row of two rounds took a warp 537 instructions instead of 448.
+template <typename T, int R, bool WIDE, int F> __global__ void __launch_bounds__(F8_T, f8_ctas(R, sizeof(T))) k_fp8_rows(const F8RowArgs a) {
+    constexpr bool AHEAD = f8_ahead(R, sizeof(T));
+    const bool adds = F < 0 ? a.add != nullptr : F & 1, norm = F < 0 ? a.w != nullptr : F & 2;
     __shared__ double s_sum[2][F8_T / 32];
     const int t = threadIdx.x & (a.tpr - 1), warp = threadIdx.x >> 5, here = F8_T / a.tpr;  // rows a CTA at once
     const int span = a.tpr * 8, rounds = R ? R : (a.cols + span - 1) / span;
     pdl_wait();
     pdl_trigger();
     const T *x = (const T *)after_wait(a.x), *add = (const T *)after_wait(a.add);
-    F8Raw<T> rx[AHEAD ? R : 1], ra[AHEAD ? R : 1];
-    auto ahead = [&](int64_t row) {
-        if (row < a.rows) {
-#pragma unroll
-            for (int k = 0; k < (AHEAD ? R : 1); ++k) {
-                const int c = k * span + t * 8;
-                if (c < a.cols) {
-                    f8_fetch<T, WIDE>(x + row * a.xs + c, rx[k]);
-                    if (add) f8_fetch<T, WIDE>(add + row * a.adds + c, ra[k]);
-                }
-            }
-        }
+    auto fetch = [&](uint32_t row, int c, F8Raw<T> &wx, F8Raw<T> &wa) {
+        const int64_t at = min(row, (uint32_t)a.rows - 1);
+        const int cc = min(c, a.cols - 8);
+        f8_fetch<T, WIDE>(x + at * a.xs + cc, wx);
+        if (adds) f8_fetch<T, WIDE>(add + at * a.adds + cc, wa);
     };
-    const int64_t step = (int64_t)gridDim.x * here;
-    int64_t row = (int64_t)blockIdx.x * here + threadIdx.x / a.tpr;
-    if constexpr (AHEAD) ahead(row);
-    for (int turn = 0; row - threadIdx.x / a.tpr < a.rows; row += step, turn ^= 1) {
-        const bool live = row < a.rows;
-        T *total = a.total ? (T *)a.total + row * a.totals : nullptr, *normed = a.normed ? (T *)a.normed + row * a.normeds : nullptr;
-        uint8_t *codes = a.codes ? a.codes + row * a.cols : nullptr;
-        float h[R ? R : 1][8] = {};
-        // the row's sum h in columns c .. c + 7
-        auto fetch = [&](int c, float (&v)[8], const F8Raw<T> &wx, const F8Raw<T> &wa) {
-            f8_unpack<T>(wx, v);
-            if (add) {
-                float b[8];
+    F8Raw<T> rx[AHEAD ? R : 1], ra[AHEAD ? R : 1];
+    auto ahead = [&](uint32_t row) {
+#pragma unroll
+        for (int k = 0; k < (AHEAD ? R : 1); ++k) fetch(row, k * span + t * 8, rx[k], ra[k]);
+    };
+    const uint32_t step = gridDim.x * here, rows = a.rows;
+    uint32_t row0 = blockIdx.x * here;
+    if constexpr (AHEAD) ahead(row0 + threadIdx.x / a.tpr);
+    for (int turn = 0; row0 < rows; row0 += step, turn ^= 1) {
+        const uint32_t row32 = row0 + threadIdx.x / a.tpr;
+        const int64_t row = row32;
+        const int cols = row32 < rows ? a.cols : 0;
+        T *const total = (T *)a.total + row * a.totals, *const normed = (T *)a.normed + row * a.normeds;
+        F8Raw<T> h[R ? R : 1];  // the row's sum, rounded to T
+        auto sum = [&](const F8Raw<T> &wx, const F8Raw<T> &wa, bool in) {
+            F8Raw<T> r = wx;
+            if (adds) {
+                float v[8], b[8];
+                f8_unpack<T>(wx, v);
                 f8_unpack<T>(wa, b);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] += b[i];
-                f8_round<T>(v);
+                f8_pack<T>(v, r);
             }
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+                if (!in) r.w[j] = make_uint4(0, 0, 0, 0);
+            return r;
         };
-        auto read = [&](int c, float (&v)[8]) {
+        auto read = [&](int c) {
             F8Raw<T> wx, wa;
-            f8_fetch<T, WIDE>(x + row * a.xs + c, wx);
-            if (add) f8_fetch<T, WIDE>(add + row * a.adds + c, wa);
-            fetch(c, v, wx, wa);
+            fetch(row32, c, wx, wa);
+            return sum(wx, wa, c < cols);
         };
         float r = 1.0f;
-        if (R || a.w) {
+        if (R || norm) {
             double ss = 0.0;
 #pragma unroll
             for (int k = 0; k < rounds; ++k) {
                 const int c = k * span + t * 8;
-                float(&v)[8] = h[R ? k : 0];
-                if (live && c < a.cols) {
-                    if constexpr (AHEAD) fetch(c, v, rx[k], ra[k]);
-                    else read(c, v);
-                    if (total) f8_store<T, WIDE>(total + c, v);
-                    if (a.w) {
+                F8Raw<T> &w = h[R ? k : 0];
+                if constexpr (AHEAD) w = sum(rx[k], ra[k], c < cols);
+                else w = read(c);
+                if (a.total && c < cols) f8_store<T, WIDE>(total + c, w);
+                if (norm) {
+                    float v[8];
+                    f8_unpack<T>(w, v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
-                    }
+                    for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
                 }
             }
-            if constexpr (AHEAD) ahead(row + step);
-            if (a.w) {
+            if constexpr (AHEAD)
+                if (row0 + step < rows) ahead(row32 + step);
+            if (norm) {
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 if (a.tpr > 32) {
@@ -200,31 +220,37 @@ template <typename T, int R, bool WIDE> __global__ void __launch_bounds__(F8_T, 
 #pragma unroll
         for (int k = 0; k < rounds; ++k) {
             const int c = k * span + t * 8;
-            const bool in = live && c < a.cols;
-            float(&v)[8] = h[R ? k : 0];
-            if (!R && in) {
-                if (a.w && total) f8_load<T, WIDE>(total + c, v);  // (x may be total: its sum is there already)
-                else read(c, v);
-                if (!a.w && total) f8_store<T, WIDE>(total + c, v);
+            const bool in = c < cols;
+            if (!R) {
+                if (norm && a.total) {  // (x may be total: its sum is there already)
+                    if (in) f8_fetch<T, WIDE>(total + c, h[0]);
+                } else h[0] = read(c);
+                if (!norm && a.total && in) f8_store<T, WIDE>(total + c, h[0]);
             }
             float y[8];
+            f8_unpack<T>(h[R ? k : 0], y);
+            if (norm) {
+                F8Raw<float> w;
+                f8_fetch<float, true>(a.w + min(c, a.cols - 8), w);
+                float v[8];
+                f8_unpack<float>(w, v);
+                f8_scale(y, r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = in ? v[i] : 0.0f;
-            if (a.w && in) {
-                float w[8];
-                f8_load<float, true>(a.w + c, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
+                for (int i = 0; i < 8; i += 2) f8_mul2(y[i], y[i + 1], v[i], v[i + 1]);
             }
-            if (normed && in) f8_store<T, WIDE>(normed + c, y);
-            if (!codes) continue;
-            float m = f8_amax(y);
+            if (a.normed && in) {
+                F8Raw<T> w;
+                f8_pack<T>(y, w);
+                f8_store<T, WIDE>(normed + c, w);
+            }
+            if (!a.codes) continue;
+            float m = in ? f8_amax(y) : 0.0f;
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) m = f8_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
             m = f8_max_nan(m, F8_TINY);
-            if (!in) continue;
-            *(uint2 *)(codes + c) = f8_codes(y, F8_MAX * __frcp_rn(m));
-            if (t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m * F8_STEP;
+            const uint2 codes = f8_codes(y, F8_MAX * __frcp_rn(m));
+            if (in) *(uint2 *)(a.codes + row * a.cols + c) = codes;
+            if (in && t % 16 == 0) a.scales[row * a.groups + c / FP8_GROUP] = m * F8_STEP;
         }
     }
 }
@@ -288,12 +314,31 @@ template <typename T, bool WIDE> __global__ void __launch_bounds__(F8_BT, 2) k_f
     if (threadIdx.x == 0) a.scales[(int64_t)blockIdx.y * a.groups + blockIdx.x] = m * F8_STEP;
 }
 
-template <typename T, bool WIDE> static cudaError_t launch_rows(const F8RowArgs &a, dim3 grid, cudaStream_t s) {
+template <typename T, bool WIDE> static cudaError_t launch_rows(F8RowArgs a, cudaStream_t s) {
+    // As many threads a row as there are: 32 columns a thread and fewer threads a row take fewer instructions, but hold fewer CTAs (8192 x 4096
+    // bf16: 48.5 us, so 40.2).
+    a.tpr = 32;
+    while (a.tpr < F8_T && a.tpr * 8 < a.cols) a.tpr *= 2;
     const int per = a.tpr * 8;
-    if (a.cols <= per) return launch_k(k_fp8_rows<T, 1, WIDE>, grid, dim3(F8_T), 0, s, a);
-    if (a.cols <= 2 * per) return launch_k(k_fp8_rows<T, 2, WIDE>, grid, dim3(F8_T), 0, s, a);
-    if (a.cols <= 4 * per) return launch_k(k_fp8_rows<T, 4, WIDE>, grid, dim3(F8_T), 0, s, a);
-    return launch_k(k_fp8_rows<T, 0, WIDE>, grid, dim3(F8_T), 0, s, a);
+    auto grid = [&](int rounds) {
+        return std::min<int64_t>(((int64_t)a.rows * a.tpr + F8_T - 1) / F8_T, (int64_t)num_sms() * f8_ctas(rounds, sizeof(T)));
+    };
+    auto launch = [&](auto *k, int rounds) { return launch_k(k, dim3((unsigned)grid(rounds)), dim3(F8_T), 0, s, a); };
+    if constexpr (WIDE) {
+        if (a.cols <= 2 * per) {
+            switch ((a.add ? 1 : 0) + (a.w ? 2 : 0)) {
+            case 0: return a.cols <= per ? launch(k_fp8_rows<T, 1, true, 0>, 1) : launch(k_fp8_rows<T, 2, true, 0>, 2);
+            case 1: return a.cols <= per ? launch(k_fp8_rows<T, 1, true, 1>, 1) : launch(k_fp8_rows<T, 2, true, 1>, 2);
+            case 2: return a.cols <= per ? launch(k_fp8_rows<T, 1, true, 2>, 1) : launch(k_fp8_rows<T, 2, true, 2>, 2);
+            default: return a.cols <= per ? launch(k_fp8_rows<T, 1, true, 3>, 1) : launch(k_fp8_rows<T, 2, true, 3>, 2);
+            }
+        }
+    } else {
+        if (a.cols <= per) return launch(k_fp8_rows<T, 1, false, -1>, 1);
+        if (a.cols <= 2 * per) return launch(k_fp8_rows<T, 2, false, -1>, 2);
+    }
+    if (a.cols <= 4 * per) return launch(k_fp8_rows<T, 4, WIDE, -1>, 4);
+    return launch(k_fp8_rows<T, 0, WIDE, -1>, 0);
 }
 
 }  // namespace fn
@@ -324,16 +369,11 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
             return fail("fp8 rows: total and normed lie over one another");
         const bool wide = ((uintptr_t)x | (uintptr_t)add | (uintptr_t)total | (uintptr_t)normed | (uint64_t)(x_stride * size) |
                            (uint64_t)(add_stride * size) | (uint64_t)(total_stride * size) | (uint64_t)(normed_stride * size)) % 16 == 0;
-        int tpr = 32;
-        while (tpr < F8_T && tpr * 8 < cols) tpr *= 2;
-        // as many CTAs as the SMs hold (6 of 256 threads where a row's 8 columns a thread are one round, 4 else)
-        const int64_t grid = std::min<int64_t>(((int64_t)rows * tpr + F8_T - 1) / F8_T, (int64_t)num_sms() * (cols <= 8 * tpr ? 6 : 4));
         const F8RowArgs a{x, add, x_stride, add_stride, weight, eps, 1.0 / cols, rows, cols, fp8_groups(cols), total, normed, total_stride,
-                          normed_stride, codes, scales, tpr};
-        const dim3 g((unsigned)grid);
+                          normed_stride, codes, scales, 0};
         const cudaStream_t s = (cudaStream_t)stream;
-        const cudaError_t e = type == T_F32 ? (wide ? launch_rows<float, true>(a, g, s) : launch_rows<float, false>(a, g, s))
-                                            : (wide ? launch_rows<__nv_bfloat16, true>(a, g, s) : launch_rows<__nv_bfloat16, false>(a, g, s));
+        const cudaError_t e = type == T_F32 ? (wide ? launch_rows<float, true>(a, s) : launch_rows<float, false>(a, s))
+                                            : (wide ? launch_rows<__nv_bfloat16, true>(a, s) : launch_rows<__nv_bfloat16, false>(a, s));
         if (e != cudaSuccess) return fail(std::string("fp8 rows launch: ") + cudaGetErrorString(e));
         return 0;
     });
