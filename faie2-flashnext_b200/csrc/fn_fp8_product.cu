@@ -164,73 +164,135 @@ template <int N> __device__ __forceinline__ void fp_ld_wait(float (&v)[N]) {
 
 constexpr int FP_PITCH = 36;  // floats from row to row of a warp's 32 x 32 values on their way out (rows 4 banks apart)
 
-// A warp's 32 rows x W columns from shared memory into rows r0 .. < m, columns n0 .. < cols of out, plus those of `add`, rounded once; V
-// values a lane (V > 1: 16 bytes of T). Up to four rows' loads come before their stores, which for all the compiler knows might be to
-// the same place.
-template <typename T, int V, int W> __device__ __forceinline__ void fp_copy_out(const float *from, const T *add, int64_t adds, T *out,
-                                                                                int64_t outs, int r0, int m, int n0, int cols) {
-    constexpr int L = W / V, R = 32 / L, B = R * 4 <= 32 ? 4 : 32 / R;  // lanes a row, rows at once, times that before stores
-    const int lane = threadIdx.x & 31, n = n0 + lane % L * V, end = min(m, r0 + 32);
-    if (n >= cols) return;
-    int r = r0 + lane / L;
-    const float *x = from + lane / L * FP_PITCH + lane % L * V;
-    add = add ? add + (int64_t)r * adds + n : nullptr;
-    out += (int64_t)r * outs + n;
-#pragma unroll 1
-    for (; r < end; r += B * R, x += B * R * FP_PITCH, out += B * R * outs, add = add ? add + B * R * adds : nullptr) {
-        float v[B][V];
-        uint4 w[B];
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const bool in = r + b * R < end;
-            if constexpr (V == 1) {
-                v[b][0] = x[b * R * FP_PITCH];
-                w[b].x = add && in ? __float_as_uint((float)add[b * R * adds]) : 0u;
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j += 4) *(float4 *)&v[b][j] = *(const float4 *)(x + b * R * FP_PITCH + j);
-                w[b] = add && in ? *(const uint4 *)(add + b * R * adds) : make_uint4(0, 0, 0, 0);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            if (r + b * R >= end) break;
-            if constexpr (V == 1) out[b * R * outs] = (T)(v[b][0] + __uint_as_float(w[b].x));
-            else {
-                uint32_t u[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (V == 4) u[j] = __float_as_uint(v[b][j] + __uint_as_float(u[j]));
-                    else {
-                        const __nv_bfloat162 z = __floats2bfloat162_rn(v[b][2 * j] + __uint_as_float(u[j] << 16),
-                                                                       v[b][2 * j + 1] + __uint_as_float(u[j] & 0xffff0000u));
-                        memcpy(&u[j], &z, 4);
-                    }
-                }
-                *(uint4 *)(out + b * R * outs) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-        }
-    }
+// columns n0 .. < end of row `row` of `add` on their way into L2 before their tile ends (8192 x 12352, K 2048, bf16: 303 -> 287 us, fp32 413 ->
+// 384)
+template <typename T> __device__ __forceinline__ void fp_add_ahead(const Fp8Args &a, int row, int n0, int end) {
+    if (row >= a.m) return;
+    const T *const p = (const T *)a.add + row * a.adds;
+    for (int n = n0; n < end; n += 128 / (int)sizeof(T)) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p + n) : "memory");
 }
-// N sums a thread, its row's columns n0 .. < end of out, by way of shared memory, 32 rows x 32 columns at a time, so that a warp stores whole
-// lines. What is not unrolled here is for the instruction cache: unrolled, a tile's end took 14 us, its code fetched once a tile.
-template <typename T, int N> __device__ __forceinline__ void fp_tile_out(const Fp8Args &a, float *stage, const float (&sum)[N], int r0, int n0, int end) {
-    constexpr int W = N % 32 == 0 ? 32 : N % 16 == 0 ? 16 : 8;
-    float4 *mine = (float4 *)(stage + (threadIdx.x & 31) * FP_PITCH);
-#pragma unroll 1
-    for (int q = 0; q < N / W; ++q) {
-#pragma unroll
-        for (int u = 0; u < N / W; ++u)
-            if (q == u) {
-#pragma unroll
-                for (int j = 0; j < W / 4; ++j)
-                    mine[j] = make_float4(sum[u * W + 4 * j], sum[u * W + 4 * j + 1], sum[u * W + 4 * j + 2], sum[u * W + 4 * j + 3]);
-            }
-        __syncwarp();
-        if (a.wide) fp_copy_out<T, 16 / sizeof(T), W>(stage, (const T *)a.add, a.adds, (T *)a.out, a.outs, r0, a.m, n0 + q * W, end);
-        else fp_copy_out<T, 1, W>(stage, (const T *)a.add, a.adds, (T *)a.out, a.outs, r0, a.m, n0 + q * W, end);
-        __syncwarp();
+
+// A warp's 32 rows x W columns, from row r0 and column n0 on, on their way out: V values a lane (V > 1: 16 bytes of T), B rows at R a time.
+// `add` is read before the stores, which for all the compiler knows might be to the same place, for as many rows as registers hold: all of
+// them in whole words, whose reads (begin) run while the sums go through shared memory.
+template <typename T, int V, int W, bool ADD> struct FpOut {
+    static constexpr int L = W / V, R = 32 / L, B = V == 1 ? 16 / R : 32 / R;  // lanes a row, rows at once, times that before stores
+    uint4 w[ADD ? B : 1];
+    int lane, rows;
+    bool in;
+    const T *add;
+    T *out;
+    __device__ __forceinline__ void begin(const Fp8Args &a, int r0, int n0, int end) {
+        lane = threadIdx.x & 31;
+        const int n = n0 + lane % L * V, r = r0 + lane / L;
+        in = n < end && r < a.m;
+        rows = a.m - r;  // from this lane's first one on
+        out = (T *)a.out + (int64_t)r * a.outs + n;
+        if (ADD) {
+            add = (const T *)a.add + (int64_t)r * a.adds + n;
+            if (V > 1 && in) read(a.adds, 0);
+        }
     }
+    __device__ __forceinline__ void read(int64_t adds, int at) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const T *p = add + (at + b * R < rows ? at + b * R : 0) * adds;
+            if constexpr (V == 1) w[b].x = __float_as_uint((float)*p);
+            else w[b] = *(const uint4 *)p;
+        }
+    }
+    __device__ __forceinline__ void end(const Fp8Args &a, const float *stage) {
+        if (!in) return;
+        const float *x = stage + lane / L * FP_PITCH + lane % L * V;
+#pragma unroll 1
+        for (int at = 0; at < 32; at += B * R) {
+            if (ADD && V == 1) read(a.adds, at);
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                if (at + b * R >= rows) break;
+                T *const to = out + (at + b * R) * a.outs;
+                const float *from = x + (at + b * R) * FP_PITCH;
+                if constexpr (V == 1) *to = (T)(*from + (ADD ? __uint_as_float(w[b].x) : 0.0f));
+                else {
+                    float v[V];
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) *(float4 *)&v[j] = *(const float4 *)(from + j);
+                    uint32_t u[4];
+                    const uint32_t e[4] = {w[ADD ? b : 0].x, w[ADD ? b : 0].y, w[ADD ? b : 0].z, w[ADD ? b : 0].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (V == 4) u[j] = __float_as_uint(ADD ? v[j] + __uint_as_float(e[j]) : v[j]);
+                        else {
+                            if (ADD) v[2 * j] += __uint_as_float(e[j] << 16), v[2 * j + 1] += __uint_as_float(e[j] & 0xffff0000u);
+                            const __nv_bfloat162 z = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                            memcpy(&u[j], &z, 4);
+                        }
+                    }
+                    *(uint4 *)to = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            }
+        }
+    }
+};
+// N sums a thread, its row's columns n0 .. < end of out, by way of shared memory, 32 rows x up to 32 words at a time, so that a warp stores
+// whole lines. What is not unrolled here is for the instruction cache: unrolled, a tile's end took 14 us, its code fetched once a tile; kernels
+// with and without `add` for the same reason (8192 x 12352, K 2048, bf16: 237 -> 228 us). WIDE: rows in whole 16-byte words, -1: as a.wide says.
+template <typename T, int N, bool ADD, int WIDE = -1> __device__ __forceinline__ void fp_tile_out(const Fp8Args &a, float *stage, const float (&sum)[N], int r0, int n0, int end) {
+    if constexpr (!ADD && sizeof(T) == 2 && WIDE != 0) {
+        if (WIDE > 0 || a.wide) {  // rounded before, two values a word: half the way through shared memory (228 -> 207 us)
+            constexpr int M = N / 2, W = M % 32 == 0 ? 32 : M % 16 == 0 ? 16 : M % 8 == 0 ? 8 : 4, L = W / 4, R = 32 / L;  // words; lanes a row, rows at once
+            const int lane = threadIdx.x & 31, rows = min(a.m - r0, 32);
+            uint4 *mine = (uint4 *)(stage + lane * FP_PITCH);
+            const uint4 *from = (const uint4 *)(stage + lane / L * FP_PITCH) + lane % L;
+            T *out = (T *)a.out + (int64_t)(r0 + lane / L) * a.outs + n0 + lane % L * 8;
+#pragma unroll 1
+            for (int q = 0; q < M / W; ++q) {
+#pragma unroll
+                for (int u = 0; u < M / W; ++u)
+                    if (q == u) {
+#pragma unroll
+                        for (int j = 0; j < L; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const __nv_bfloat162 z = __floats2bfloat162_rn(sum[2 * (u * W + 4 * j + k)], sum[2 * (u * W + 4 * j + k) + 1]);
+                                memcpy(&w[k], &z, 4);
+                            }
+                            mine[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                __syncwarp();
+                if (n0 + 2 * (q * W) + lane % L * 8 < end) {
+#pragma unroll
+                    for (int b = 0; b < L; ++b)
+                        if (lane / L + b * R < rows) *(uint4 *)(out + 2 * (q * W) + b * R * a.outs) = from[b * R * (FP_PITCH / 4)];
+                }
+                __syncwarp();
+            }
+            return;
+        }
+    }
+    auto go = [&]<int V>() {
+        constexpr int W = N % 32 == 0 ? 32 : N % 16 == 0 ? 16 : 8;
+        float4 *mine = (float4 *)(stage + (threadIdx.x & 31) * FP_PITCH);
+#pragma unroll 1
+        for (int q = 0; q < N / W; ++q) {
+            FpOut<T, V, W, ADD> o;
+            o.begin(a, r0, n0 + q * W, end);
+#pragma unroll
+            for (int u = 0; u < N / W; ++u)
+                if (q == u) {
+#pragma unroll
+                    for (int j = 0; j < W / 4; ++j)
+                        mine[j] = make_float4(sum[u * W + 4 * j], sum[u * W + 4 * j + 1], sum[u * W + 4 * j + 2], sum[u * W + 4 * j + 3]);
+                }
+            __syncwarp();
+            o.end(a, stage);
+            __syncwarp();
+        }
+    };
+    if (WIDE < 0 ? a.wide : WIDE) go.template operator()<16 / (int)sizeof(T)>();
+    else go.template operator()<1>();
 }
 
 // ---- single SMs -----------------------------------------------------------------------------------------------------
@@ -253,7 +315,7 @@ template <int N, bool FEW> struct Fp8Shared {
     alignas(16) float both[2][FP_CHUNK][2][FEW ? N : 4];
 };
 
-template <typename T, int N, bool FEW>
+template <typename T, int N, bool FEW, bool ADD>
 __global__ void __launch_bounds__(128 + 128 * fp_sets(N, FEW), 1) k_fp8_product(const __grid_constant__ Fp8Args a) {
     constexpr int SETS = fp_sets(N, FEW), NC = N / SETS, U = FP_STEP, G = fp_stage(N), ACC = fp_acc(N);  // NC: columns of a thread
     constexpr uint32_t USED = ACC * U * N, COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
@@ -382,7 +444,16 @@ __global__ void __launch_bounds__(128 + 128 * fp_sets(N, FEW), 1) k_fp8_product(
         float *const out_stage = (float *)(ring + a.stages * stage) + (warp - 4) * (32 * FP_PITCH);
         int i = 0, c = 0;
         bool ok = true;
+        auto add_ahead = [&](int tile) {  // a thread a row of x
+            if (!ADD || tile >= a.tiles) return;
+            const int n0 = (FEW ? tile : tile / a.tiles_m) * a.width + col, end = min(min(n0 + NC, n0 - col + a.width), a.n);
+            if constexpr (FEW) {
+                if (warp == 4) fp_add_ahead<T>(a, lane, n0, min(n0 + a.width, a.n));
+            } else fp_add_ahead<T>(a, tile % a.tiles_m * 128 + row, n0, end);
+        };
+        add_ahead(blockIdx.x);
         for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+            add_ahead(tile + gridDim.x);
             const int r0 = (FEW ? 0 : tile % a.tiles_m * 128) + 32 * (warp & 3), first = (FEW ? tile : tile / a.tiles_m) * a.width;
             const int edge = (first / FP8_GROUP + 1) * FP8_GROUP - first;  // the tile's rows of the weight from it on are of the second block
             const int end = min(first + a.width, a.n);
@@ -451,9 +522,9 @@ __global__ void __launch_bounds__(128 + 128 * fp_sets(N, FEW), 1) k_fp8_product(
             }
             if (!ok) break;
             if constexpr (!FEW) {
-                if (live) fp_tile_out<T, NC>(a, out_stage, sum, r0, first + col, end);
+                if (live) fp_tile_out<T, NC, ADD>(a, out_stage, sum, r0, first + col, end);
             } else if (first + row < end) {
-                const T *add = a.add ? (const T *)a.add + first + row : nullptr;
+                const T *add = ADD ? (const T *)a.add + first + row : nullptr;
                 T *out = (T *)a.out + first + row;
                 // 16 rows at a time, not unrolled, for the instruction cache (the sums move down instead); loads before the stores, which
                 // for all the compiler knows might be to the same place
@@ -461,11 +532,11 @@ __global__ void __launch_bounds__(128 + 128 * fp_sets(N, FEW), 1) k_fp8_product(
                 for (int left = a.m; left > 0; left -= 16) {
                     float x[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = add && j < left ? (float)add[j * a.adds] : 0.0f;
+                    for (int j = 0; j < 16; ++j) x[j] = ADD && j < left ? (float)add[j * a.adds] : 0.0f;
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (j < left) out[j * a.outs] = (T)(sum[j] + x[j]);
-                    if (add) add += 16 * a.adds;
+                    if (ADD) add += 16 * a.adds;
                     out += 16 * a.outs;
 #pragma unroll
                     for (int j = 0; j + 16 < NC; ++j) sum[j] = sum[j + 16];
@@ -532,7 +603,7 @@ __device__ __forceinline__ void fw_commit_here(uint32_t bar) {  // arrives in th
 __device__ __forceinline__ void fw_arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
-template <typename T> __global__ void __launch_bounds__(FW_T, 1) k_fp8_product_wide(const __grid_constant__ Fp8Args a) {
+template <typename T, bool ADD, bool WIDE> __global__ void __launch_bounds__(FW_T, 1) k_fp8_product_wide(const __grid_constant__ Fp8Args a) {
     extern __shared__ uint8_t sm_fp8[];
     __shared__ Fp8WideShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -647,6 +718,7 @@ template <typename T> __global__ void __launch_bounds__(FW_T, 1) k_fp8_product_w
         bool ok = true;
         for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
             const int m0 = tile % a.tiles_m * 256 + (int)rank * 128, n0 = tile / a.tiles_m * 256 + half * 128;
+            if (ADD) fp_add_ahead<T>(a, m0 + row, n0, min(n0 + 128, a.n));
             float sum[128], v[2][32];
 #pragma unroll
             for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
@@ -684,7 +756,7 @@ template <typename T> __global__ void __launch_bounds__(FW_T, 1) k_fp8_product_w
                 fp_ld_wait<32>(v[0]);
             }
             if (!ok) break;
-            fp_tile_out<T, 128>(a, out_stage, sum, m0 + 32 * (warp & 3), n0, a.n);
+            fp_tile_out<T, 128, ADD, WIDE>(a, out_stage, sum, m0 + 32 * (warp & 3), n0, a.n);
         }
     }
     __syncwarp();
@@ -720,14 +792,15 @@ static bool fp_map(CUtensorMap *map, const uint8_t *codes, int rows, int cols, i
 }
 
 template <typename T> static cudaError_t fp_launch_wide(Fp8Args &a, cudaStream_t s) {
-    auto *k = k_fp8_product_wide<T>;
+    auto *k = a.add ? (a.wide ? k_fp8_product_wide<T, true, true> : k_fp8_product_wide<T, true, false>)
+                    : (a.wide ? k_fp8_product_wide<T, false, true> : k_fp8_product_wide<T, false, false>);
     const cudaError_t e = allow_max_dynamic_smem(k);
     if (e != cudaSuccess) return e;
     const size_t smem = FW_RING * FW_STAGE + 8 * 32 * FP_PITCH * sizeof(float) + 1024;
     return launch_kc(k, dim3((unsigned)(2 * std::min(a.tiles, num_sms() / 2))), dim3(FW_T), 2u, smem, s, a);
 }
 template <typename T, int N, bool FEW> static cudaError_t fp_launch(Fp8Args &a, cudaStream_t s) {
-    auto *k = k_fp8_product<T, N, FEW>;
+    auto *k = a.add ? k_fp8_product<T, N, FEW, true> : k_fp8_product<T, N, FEW, false>;
     const cudaError_t e = allow_max_dynamic_smem(k);
     if (e != cudaSuccess) return e;
     constexpr int sets = fp_sets(N, FEW), out = FEW ? 0 : 4 * sets * 32 * FP_PITCH * (int)sizeof(float);
@@ -778,9 +851,9 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
         a.wide = (((uintptr_t)out | (uintptr_t)add) % 16 | (uint64_t)a.n % per | (uint64_t)out_stride % per | (uint64_t)add_stride % per) == 0;
         const int64_t sms = num_sms(), tm = fp8_groups(rows), waves = (fp8_groups(a.n) * tm + sms - 1) / sms;  // of tiles of 128 x 128
         const int64_t wide_tiles = (int64_t)((rows + 255) / 256) * ((a.n + 255) / 256), wide_waves = (wide_tiles + sms / 2 - 1) / (sms / 2);
-        // A group takes a pair of SMs 0.44 us for 256 x 256, a single one 0.31 us for 128 x 128 (K 2048 and 4096 compared): pairs where
-        // their fewer waves save more than that. 768 x 12352: 25.7 us by pairs, 29.4 by single SMs; 512 x 12352: 24.6 and 22.7;
-        // 1024 x 2048, K 4096: 21.5 and 14.6; 2048 x 2048: 22.3 and 26.2.
+        // A group takes a pair of SMs 0.55 us for 256 x 256, a single one 0.37 us for 128 x 128 (K 4096): pairs where their fewer waves save
+        // more than that. 768 x 12352, K 2048, fp32: 25.3 us by pairs, 30.1 by single SMs; 512 x 12352: 24.3 and 23.0; 1024 x 2048, K 4096:
+        // 20.7 and 14.8; 2048 x 2048: 21.8 and 26.6.
         if (3 * wide_waves < 2 * waves && sms >= 2) {
             a.tiles_m = (rows + 255) / 256;
             if (wide_tiles * a.groups > INT32_MAX) return fail("fp8 product: too large");
