@@ -13,6 +13,10 @@
 // alternative of the CTA's part falls below, so only what can reach it is read again: the segments (of a thread's words) whose own
 // maximum does, about k of 4096, spread over all threads, which list what reaches it. (If equal entries are too many to be listed, every
 // warp keeps its best 32 sorted over its lanes.)
+//
+// What bounds it: with many rows in bf16 instruction issue (11.5 an entry in all; 2048 x 151936: 137 us with 20 alternatives and tokens, 113 with
+// neither, where the bytes take 95 at the copy rate), in fp32 the loads (1024 rows: 114 and 97); with few rows the chain of steps behind the
+// pass (32 rows of fp32: 11.5 us, without alternatives 8.0, where the bytes take 3).
 #include <cuda_bf16.h>
 
 #include "fn_argmax.cuh"
@@ -359,8 +363,8 @@ template <int THREADS> struct LpShared {
 // n keys (distinct, or 0) put in order: the first `top` into best, which holds zeros. THREADS / 256 neighbours count a key against the others.
 template <int THREADS> __device__ __noinline__ void lp_rank_keys(const unsigned long long *keys, int n, int top, unsigned long long *best) {
     constexpr int Q = THREADS / 256;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + threadIdx.x / Q;
+    for (int i0 = (threadIdx.x & ~31) / Q; i0 < n; i0 += 256) {  // (a warp without a key is done)
+        const int i = i0 + (threadIdx.x & 31) / Q;
         const unsigned long long k = i < n ? keys[i] : 0;
         int at = 0;
 #pragma unroll 4
@@ -385,7 +389,7 @@ __device__ __forceinline__ LpSum lp_warp_join(LpSum a) {
 }
 
 constexpr int LP_MAX_VOCAB = 1 << 28;  // so a segment has up to 2048 rounds, each with up to 16 entries of a half of the counter
-// CTAs of 256 threads on an SM: five where instructions bound it (bf16, 2048 rows of 151936: 138.5 us, by four 143.8; 200 rows, where
+// CTAs of 256 threads on an SM: five where instructions bound it (bf16, 2048 rows of 151936: 137 us, by four 143; 200 rows, where
 // latency counts, 26.5 and 25.0), four where loads do (fp32, 1024 rows: 115 us, by five 122)
 constexpr int lp_ctas(int size) { return size == 2 ? 5 : 4; }
 

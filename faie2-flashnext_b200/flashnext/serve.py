@@ -131,12 +131,12 @@ class ServeModel(BatchDecodeModel):
         need = [-(-(len(p) + n - 1) // self.page_size) for p, n in zip(prompts, n_new)]  # the last token is not fed
         if wait and max(need, default=0) + self.B - 1 > self.n_pages:
             raise ValueError("a request wants more pages than there are beside one for each other place")
+        if scores is not None and not 0 <= scores <= lp.MAX_TOP:
+            raise ValueError(f"scores: 0..{lp.MAX_TOP} alternatives are wanted")
         self.start(None, stream)
         waiting, place, seq = list(range(len(prompts))), [None] * self.B, [p.tolist() for p in prompts]
         at = [0] * self.B  # tokens fed of the place's request
         if scores is not None:
-            if not 0 <= scores <= lp.MAX_TOP:
-                raise ValueError(f"scores: 0..{lp.MAX_TOP} alternatives are wanted")
             said, kept, known = [[] for _ in prompts], None, np.full(self.B, -1, np.int32)  # known: the token that follows, if it is given
         inputs, drop = np.zeros(self.B, np.int32), np.full(self.B, -1, np.int32)
         while waiting or any(r is not None for r in place):
