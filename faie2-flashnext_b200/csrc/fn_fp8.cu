@@ -264,7 +264,7 @@ struct F8BlockArgs {
 };
 
 // one CTA per 128 x 128 block, its values in registers (as they are stored) between the maximum and the codes; 16 threads a row, 8
-// columns each, four rows a thread
+// columns each, four rows a thread. Memory bounds it (12352 x 2048 bf16: 13.6 us, 5.6 TB/s).
 constexpr int F8_BT = 512;
 template <typename T, bool WIDE> __global__ void __launch_bounds__(F8_BT, 2) k_fp8_blocks(const F8BlockArgs a) {
     __shared__ float s_max[F8_BT / 32];
