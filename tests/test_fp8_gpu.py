@@ -270,6 +270,27 @@ def test_a_row_is_the_same_in_any_batch(fn, fp8):
     sync(fn)
 
 
+def test_far_rows(fn, fp8):
+    """Codes and outputs whose offsets pass 32 bits."""
+    row = rand(1, 4096, "bf16", 19)
+    n = (1 << 20) + 3
+    got = fp8.quantise_rows(fn, row.expand(n, 4096))
+    want = fp8.quantise_rows(fn, row)
+    sync(fn)
+    for r in (0, 1, n // 2, n - 2, n - 1):
+        assert torch.equal(got.q[r].view(torch.uint8), want.q[0].view(torch.uint8)) and torch.equal(got.scale[r], want.scale[0])
+    del got
+    x, w = fp8.quantise_rows(fn, rand(17001, 128, "bf16", 20)), fp8.Fp8Weight.quantise(fn, rand(262152, 128, "bf16", 21))
+    out = w.product(x, dtype=torch.bfloat16)
+    sync(fn)
+    for lo in (0, 8000, 16900):
+        assert torch.equal(out[lo:lo + 101], w.product(fp8.Fp8Rows(x.q[lo:lo + 101], x.scale[lo:lo + 101]), dtype=torch.bfloat16))
+    h = fp8.Fp8Weight.quantise(fn, rand(3, 4096, "bf16", 22))
+    far = torch.empty(1 << 28, 20, device="cuda", dtype=torch.bfloat16)[::1 << 20, :3]  # rows 40 MB apart
+    assert torch.equal(h.product(fp8.Fp8Rows(want.q.expand(256, 4096).contiguous(), want.scale.expand(256, 32).contiguous()), out=far),
+                       h.product(want, dtype=torch.bfloat16).expand(256, 3))
+
+
 def test_streams_and_graphs(fn, fp8):
     """Weights quantised, rows normed and multiplied in one stream without waits, two streams at once, and a captured chain."""
     h, d = rand(40, 2048, "bf16", 1), rand(40, 2048, "bf16", 2)

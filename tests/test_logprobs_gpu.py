@@ -140,6 +140,26 @@ def test_far_rows(fn, lp):
     check(fn, lp, x, [4, 4999], 9)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_counts_of_long_rows(fn, lp, dtype):
+    """One long row, taken once and by as many rows as have small CTAs: ranks of millions are whole numbers. Two levels, e apart: n / 2
+    entries of each, so Z e^-1 = n / 2 (1 + 1 / e); the sums are of equal terms, off by 2^-24 a step of a thread's 2^18 at most."""
+    n, rows = 1 << 26, 200
+    x = torch.zeros(n, device="cuda", dtype=torch.float32 if dtype == "f32" else torch.bfloat16)
+    x[:n // 2] = 1
+    tokens = torch.arange(rows, device="cuda", dtype=torch.int32) * 331337 + 5
+    tokens[-1], tokens[-2], tokens[-3] = n - 1, n // 2, n // 2 - 1
+    z = np.log(n / 2) + np.log1p(np.exp(-1.0))
+    p = 1 / (1 + np.exp(-1.0))
+    for r in (rows, 1):
+        got = lp.token_logprobs(fn, x.expand(r, n), tokens[-r:].contiguous())
+        torch.cuda.synchronize()
+        assert torch.equal(got.rank, tokens[-r:])  # by value, then by index
+        want = np.where(tokens[-r:].cpu().numpy() < n // 2, 0.0, -1.0) - z
+        assert np.abs(got.logprob.double().cpu().numpy() - want).max() <= 2.0 ** -6
+        assert abs(float(got.entropy[0]) - (z + 1 - p)) <= 2.0 ** -5
+
+
 def test_streams_graphs_and_buffers(fn, lp):
     x, y = logits(8, 151936, "f32", seed=1), logits(700, 20000, "bf16", seed=2)
     tok = torch.arange(8, dtype=torch.int32, device="cuda")
