@@ -241,7 +241,8 @@ template <typename T, int V, int W, bool ADD> struct FpOut {
 // N sums a thread, its row's columns n0 .. < end of out, by way of shared memory, 32 rows x up to 32 words at a time, so that a warp stores
 // whole lines. What is not unrolled here is for the instruction cache: unrolled, a tile's end took 14 us, its code fetched once a tile; kernels
 // with and without `add` for the same reason (8192 x 12352, K 2048, bf16: 237 -> 228 us). WIDE: rows in whole 16-byte words, -1: as a.wide says.
-template <typename T, int N, bool ADD, int WIDE = -1> __device__ __forceinline__ void fp_tile_out(const Fp8Args &a, float *stage, const float (&sum)[N], int r0, int n0, int end) {
+template <typename T, int N, bool ADD, int WIDE = -1>
+__device__ __forceinline__ void fp_tile_out(const Fp8Args &a, float *stage, const float (&sum)[N], int r0, int n0, int end) {
     if constexpr (!ADD && sizeof(T) == 2 && WIDE != 0) {
         if (WIDE > 0 || a.wide) {  // rounded before, two values a word: half the way through shared memory (228 -> 207 us)
             constexpr int M = N / 2, W = M % 32 == 0 ? 32 : M % 16 == 0 ? 16 : M % 8 == 0 ? 8 : 4, L = W / 4, R = 32 / L;  // words; lanes a row, rows at once
