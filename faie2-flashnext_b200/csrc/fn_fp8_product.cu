@@ -635,82 +635,83 @@ template <typename T, bool ADD, bool WIDE> __global__ void __launch_bounds__(FW_
     pdl_trigger();
     const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), af = smem_u32(sh.af), base = smem_u32(ring);
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    // registers: 384 threads of 168 at launch become 128 of 72 and 256 of 216
-    if (warp == 0) {
+    // registers: 384 threads of 168 at launch become 128 of 72 and 256 of 216. All warps of a warpgroup change theirs by the same instruction
+    // (PTX leaves anything else undefined), before their roles part.
+    if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        // either CTA brings its own half of both operands; the copies complete on the first CTA's barrier
-        const bool lead = fp_elect();
-        const uint32_t full0 = fw_leader(sh.full);
-        int i = 0;
-        uint32_t s = 0, turn = 0;
-        bool ok = true;
-        for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
-            const int m0 = tile % a.tiles_m * 256 + (int)rank * 128, n0 = tile / a.tiles_m * 256 + (int)rank * 128;
-            for (int g = 0; g < a.groups; ++g, ++i) {
-                ok = fp_wait(empty + 8 * s, (turn & 1) ^ 1, s_fail, a.err);
-                if (!ok) break;
-                if (lead) {
-                    const uint32_t dst = base + s * FW_STAGE, bar = full0 + 8 * s;
-                    if (rank == 0) fp_expect(full + 8 * s, 2 * FW_STAGE);
-                    fw_tma(dst, &a.tx, g * FP8_GROUP, m0, bar);
-                    fw_tma(dst + FW_OP, &a.tw, g * FP8_GROUP, n0, bar);
-                }
-                if (++s == FW_RING) s = 0, ++turn;
-            }
-        }
-        if (!ok && rank == 0)
-            for (int j = max(0, i - FW_RING); j < i; ++j) mbar_park(&sh.full[j % FW_RING], (uint32_t)(j / FW_RING) & 1u);
-    } else if (warp == 1) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (rank == 0) {
-            constexpr uint32_t idesc = fp_idesc(256, 256);
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), ae = smem_u32(sh.ae);
-            const uint64_t ad0 = fp_desc(base), bd0 = fp_desc(base + FW_OP);
-            const int total = (a.tiles - pair + pairs - 1) / pairs * a.groups;
+        if (warp == 0) {
+            // either CTA brings its own half of both operands; the copies complete on the first CTA's barrier
             const bool lead = fp_elect();
+            const uint32_t full0 = fw_leader(sh.full);
+            int i = 0;
             uint32_t s = 0, turn = 0;
             bool ok = true;
-            for (int i = 0; i < total && ok; ++i) {
-                const uint32_t b = (uint32_t)i & 1, at = s * (FW_STAGE >> 4), parity = ((uint32_t)i / 2 & 1) ^ 1;
-                ok = fp_wait(full + 8 * s, turn & 1, ae + 8 * b, parity, s_fail, a.err);
-                if (!ok) break;
-                tc_fence_after();
-                if (lead) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) fw_mma(tm + b * 256, ad0 + at + 2u * k, bd0 + at + 2u * k, idesc, k > 0);
-                    fw_commit(af + 8 * b);
-                    fw_commit(empty + 8 * s);
+            for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
+                const int m0 = tile % a.tiles_m * 256 + (int)rank * 128, n0 = tile / a.tiles_m * 256 + (int)rank * 128;
+                for (int g = 0; g < a.groups; ++g, ++i) {
+                    ok = fp_wait(empty + 8 * s, (turn & 1) ^ 1, s_fail, a.err);
+                    if (!ok) break;
+                    if (lead) {
+                        const uint32_t dst = base + s * FW_STAGE, bar = full0 + 8 * s;
+                        if (rank == 0) fp_expect(full + 8 * s, 2 * FW_STAGE);
+                        fw_tma(dst, &a.tx, g * FP8_GROUP, m0, bar);
+                        fw_tma(dst + FW_OP, &a.tw, g * FP8_GROUP, n0, bar);
+                    }
+                    if (++s == FW_RING) s = 0, ++turn;
                 }
-                __syncwarp();
-                if (++s == FW_RING) s = 0, ++turn;
             }
-            if (lead) fw_commit_here(smem_u32(&sh.done));
-            __syncwarp();
-            mbar_park(&sh.done, 0);  // every MMA has read its operands (the other CTA waits for this one at the end)
-        }
-    } else if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int t64 = tid - 64;
-        int c = 0;
-        bool ok = true;
-        for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
-            const int m0 = tile % a.tiles_m * 256 + (int)rank * 128, b0 = tile / a.tiles_m * 2, b1 = min(b0 + 1, (a.n - 1) / FP8_GROUP);
-            for (int g0 = 0; g0 < a.groups; g0 += FP_CHUNK, ++c) {
-                const int n = min(FP_CHUNK, a.groups - g0), j0 = lane & (FP_CHUNK - 1);
-                const float w = a.ws[(int64_t)(lane < FP_CHUNK ? b0 : b1) * a.groups + g0 + min(j0, n - 1)];
-                float x[2][FP_CHUNK];
+            if (!ok && rank == 0)
+                for (int j = max(0, i - FW_RING); j < i; ++j) mbar_park(&sh.full[j % FW_RING], (uint32_t)(j / FW_RING) & 1u);
+        } else if (warp == 1) {
+            if (rank == 0) {
+                constexpr uint32_t idesc = fp_idesc(256, 256);
+                const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), ae = smem_u32(sh.ae);
+                const uint64_t ad0 = fp_desc(base), bd0 = fp_desc(base + FW_OP);
+                const int total = (a.tiles - pair + pairs - 1) / pairs * a.groups;
+                const bool lead = fp_elect();
+                uint32_t s = 0, turn = 0;
+                bool ok = true;
+                for (int i = 0; i < total && ok; ++i) {
+                    const uint32_t b = (uint32_t)i & 1, at = s * (FW_STAGE >> 4), parity = ((uint32_t)i / 2 & 1) ^ 1;
+                    ok = fp_wait(full + 8 * s, turn & 1, ae + 8 * b, parity, s_fail, a.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lead) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float *p = a.xs + (int64_t)min(m0 + t64 + 64 * u, a.m - 1) * a.groups + g0;
-#pragma unroll
-                    for (int j = 0; j < FP_CHUNK; ++j) x[u][j] = p[min(j, n - 1)];
+                        for (int k = 0; k < 4; ++k) fw_mma(tm + b * 256, ad0 + at + 2u * k, bd0 + at + 2u * k, idesc, k > 0);
+                        fw_commit(af + 8 * b);
+                        fw_commit(empty + 8 * s);
+                    }
+                    __syncwarp();
+                    if (++s == FW_RING) s = 0, ++turn;
                 }
-                ok = fp_wait(smem_u32(&sh.se[c & 1]), ((uint32_t)c / 2 & 1) ^ 1, s_fail, a.err);
-                if (!ok) break;
+                if (lead) fw_commit_here(smem_u32(&sh.done));
+                __syncwarp();
+                mbar_park(&sh.done, 0);  // every MMA has read its operands (the other CTA waits for this one at the end)
+            }
+        } else {
+            const int t64 = tid - 64;
+            int c = 0;
+            bool ok = true;
+            for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
+                const int m0 = tile % a.tiles_m * 256 + (int)rank * 128, b0 = tile / a.tiles_m * 2, b1 = min(b0 + 1, (a.n - 1) / FP8_GROUP);
+                for (int g0 = 0; g0 < a.groups; g0 += FP_CHUNK, ++c) {
+                    const int n = min(FP_CHUNK, a.groups - g0), j0 = lane & (FP_CHUNK - 1);
+                    const float w = a.ws[(int64_t)(lane < FP_CHUNK ? b0 : b1) * a.groups + g0 + min(j0, n - 1)];
+                    float x[2][FP_CHUNK];
 #pragma unroll
-                for (int j = 0; j < FP_CHUNK; ++j) sh.xsc[c & 1][j][t64] = x[0][j], sh.xsc[c & 1][j][t64 + 64] = x[1][j];
-                if (t64 < 2 * FP_CHUNK) sh.wsc[c & 1][j0][t64 / FP_CHUNK] = w;
-                tc_arrive(&sh.sf[c & 1]);
+                    for (int u = 0; u < 2; ++u) {
+                        const float *p = a.xs + (int64_t)min(m0 + t64 + 64 * u, a.m - 1) * a.groups + g0;
+#pragma unroll
+                        for (int j = 0; j < FP_CHUNK; ++j) x[u][j] = p[min(j, n - 1)];
+                    }
+                    ok = fp_wait(smem_u32(&sh.se[c & 1]), ((uint32_t)c / 2 & 1) ^ 1, s_fail, a.err);
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < FP_CHUNK; ++j) sh.xsc[c & 1][j][t64] = x[0][j], sh.xsc[c & 1][j][t64 + 64] = x[1][j];
+                    if (t64 < 2 * FP_CHUNK) sh.wsc[c & 1][j0][t64 / FP_CHUNK] = w;
+                    tc_arrive(&sh.sf[c & 1]);
+                }
             }
         }
     } else {
