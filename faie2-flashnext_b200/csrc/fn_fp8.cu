@@ -362,12 +362,11 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
             return fail("fp8 rows: rows must be aligned to their type");
         if ((uintptr_t)weight % 16 || (uintptr_t)codes % 16 || (uintptr_t)scales % 4)
             return fail("fp8 rows: weight and codes must be 16-byte aligned");
-        const int64_t bytes = (int64_t)cols * size;
         if (rows > 1 && ((total && total_stride < cols) || (normed && normed_stride < cols))) return fail("fp8 rows: rows that are written overlap");
         for (const auto &[p, ps] : {std::pair(x, x_stride), std::pair(add, add_stride)})
-            if (fp8_mixed(total, total_stride * size, p, ps * size, rows, bytes) || fp8_mixed(normed, normed_stride * size, p, ps * size, rows, bytes))
+            if (rows_mixed(total, total_stride, p, ps, rows, cols, size) || rows_mixed(normed, normed_stride, p, ps, rows, cols, size))
                 return fail("fp8 rows: rows that are written lie over other rows that are read");
-        if (normed && (normed == total || fp8_mixed(total, total_stride * size, normed, normed_stride * size, rows, bytes)))
+        if (normed && (normed == total || rows_mixed(total, total_stride, normed, normed_stride, rows, cols, size)))
             return fail("fp8 rows: total and normed lie over one another");
         const bool wide = ((uintptr_t)x | (uintptr_t)add | (uintptr_t)total | (uintptr_t)normed | (uint64_t)(x_stride * size) |
                            (uint64_t)(add_stride * size) | (uint64_t)(total_stride * size) | (uint64_t)(normed_stride * size)) % 16 == 0;

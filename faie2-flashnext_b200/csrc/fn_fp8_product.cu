@@ -846,7 +846,7 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
             return fail("fp8 product: scales, add and out must be aligned to their types");
         const int size = type == T_F32 ? 4 : 2;
         if (rows > 1 && out_stride < w->rows) return fail("fp8 product: rows of out overlap");
-        if (fp8_mixed(out, out_stride * size, add, add_stride * size, rows, (int64_t)w->rows * size))
+        if (rows_mixed(out, out_stride, add, add_stride, rows, w->rows, size))
             return fail("fp8 product: out lies over other rows of add");
         Fp8Args a{};
         a.ws = w->scales, a.xs = scales;

@@ -25,4 +25,11 @@ inline bool kv4_rows_meet(const void *a, int64_t a_token, int64_t a_head, const 
     return from < q.hi - q.lo || from + (p.hi - p.lo) > a_token;
 }
 
+// The same for rows of `cols` values (strides of either sign, in elements), but for rows that are the same ones in the same order, which a
+// kernel that reads an element before it writes it allows.
+inline bool rows_mixed(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int64_t rows, int64_t cols, int64_t size) {
+    if (!a || !b || (a == b && (a_stride == b_stride || rows == 1))) return false;
+    return kv4_rows_meet(a, a_stride, 0, b, b_stride, 0, rows, 1, cols, size);
+}
+
 }  // namespace fn
