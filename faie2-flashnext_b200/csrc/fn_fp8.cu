@@ -368,6 +368,17 @@ FN_API int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const voi
                 return fail("fp8 rows: rows that are written lie over other rows that are read");
         if (normed && (normed == total || rows_mixed(total, total_stride, normed, normed_stride, rows, cols, size)))
             return fail("fp8 rows: total and normed lie over one another");
+        const int64_t bytes = (int64_t)cols * size, n_codes = (int64_t)rows * cols, n_scales = (int64_t)rows * fp8_groups(cols) * 4, n_weight = (int64_t)cols * 4;
+        auto meets = [&](const void *q, int64_t n) {
+            return rows_meet_bytes(total, total_stride * size, rows, bytes, q, n) || rows_meet_bytes(normed, normed_stride * size, rows, bytes, q, n);
+        };
+        auto read = [&](const void *q, int64_t n) {
+            return rows_meet_bytes(x, x_stride * size, rows, bytes, q, n) || rows_meet_bytes(add, add_stride * size, rows, bytes, q, n) ||
+                   rows_meet_bytes(weight, 0, 1, n_weight, q, n);
+        };
+        if (meets(codes, n_codes) || meets(scales, n_scales) || read(codes, n_codes) || read(scales, n_scales) || meets(weight, n_weight) ||
+            rows_meet_bytes(codes, 0, 1, n_codes, scales, n_scales))
+            return fail("fp8 rows: codes, scales, weight and rows share memory");
         const bool wide = ((uintptr_t)x | (uintptr_t)add | (uintptr_t)total | (uintptr_t)normed | (uint64_t)(x_stride * size) |
                            (uint64_t)(add_stride * size) | (uint64_t)(total_stride * size) | (uint64_t)(normed_stride * size)) % 16 == 0;
         const F8RowArgs a{x, add, x_stride, add_stride, weight, eps, 1.0 / cols, rows, cols, fp8_groups(cols), total, normed, total_stride,
@@ -391,6 +402,10 @@ FN_API int fn_fp8_blocks(uint32_t type, const void *w, int64_t stride, int rows,
         if ((uintptr_t)w % size || (uintptr_t)codes % 16 || (uintptr_t)scales % 4)
             return fail("fp8 blocks: weights must be aligned to their type, codes to 16 bytes");
         if (fp8_groups(rows) > 65535) return fail("fp8 blocks: too many rows");
+        const int64_t n_codes = (int64_t)rows * cols, n_scales = (int64_t)fp8_groups(rows) * fp8_groups(cols) * 4;
+        if (rows_meet_bytes(w, stride * size, rows, (int64_t)cols * size, codes, n_codes) ||
+            rows_meet_bytes(w, stride * size, rows, (int64_t)cols * size, scales, n_scales) || rows_meet_bytes(codes, 0, 1, n_codes, scales, n_scales))
+            return fail("fp8 blocks: codes, scales and the weight share memory");
         const F8BlockArgs a{w, stride, rows, cols, fp8_groups(cols), codes, scales};
         const dim3 g((unsigned)a.groups, (unsigned)fp8_groups(rows));
         const bool wide = ((uintptr_t)w | (uint64_t)(stride * size)) % 16 == 0;

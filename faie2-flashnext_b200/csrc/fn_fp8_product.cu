@@ -848,6 +848,11 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
         if (rows > 1 && out_stride < w->rows) return fail("fp8 product: rows of out overlap");
         if (rows_mixed(out, out_stride, add, add_stride, rows, w->rows, size))
             return fail("fp8 product: out lies over other rows of add");
+        const int64_t groups = fp8_groups(w->cols);
+        auto meets = [&](const void *q, int64_t n) { return rows_meet_bytes(out, out_stride * size, rows, (int64_t)w->rows * size, q, n); };
+        if (meets(codes, (int64_t)rows * w->cols) || meets(scales, rows * groups * 4) || meets(w->codes, (int64_t)w->rows * w->cols) ||
+            meets(w->scales, fp8_groups(w->rows) * groups * 4))
+            return fail("fp8 product: out lies over codes or scales");
         Fp8Args a{};
         a.ws = w->scales, a.xs = scales;
         a.m = rows, a.n = w->rows, a.groups = fp8_groups(w->cols);

@@ -32,4 +32,15 @@ inline bool rows_mixed(const void *a, int64_t a_stride, const void *b, int64_t b
     return kv4_rows_meet(a, a_stride, 0, b, b_stride, 0, rows, 1, cols, size);
 }
 
+// Whether rows of `bytes` bytes, a step of `stride` bytes (of either sign) apart, share memory with the n bytes from q on. Null pointers
+// share none.
+inline bool rows_meet_bytes(const void *p, int64_t stride, int64_t rows, int64_t bytes, const void *q, int64_t n) {
+    if (!p || !q || rows < 1 || bytes < 1 || n < 1) return false;
+    int64_t at = (int64_t)((uintptr_t)q - (uintptr_t)p);  // where they begin, counted from the lowest row
+    if (stride < 0) at -= (rows - 1) * stride, stride = -stride;
+    if (stride == 0 || at < bytes) return at < bytes && at + n > 0;
+    const int64_t i = (at - bytes) / stride + 1;  // the first row that ends behind there
+    return i < rows && i * stride < at + n;
+}
+
 }  // namespace fn

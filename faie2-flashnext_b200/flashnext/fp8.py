@@ -66,7 +66,7 @@ def empty_rows(rows: int, cols: int, device="cuda") -> Fp8Rows:
 def quantise_rows(fn, x, add=None, total=None, weight=None, eps: float = 1e-6, normed=None, out: Fp8Rows | None = None) -> Fp8Rows:
     """x [rows][cols] fp32 or bf16 (any row stride) as 8-bit rows. add: rows added first (the sum is rounded to x's type); total: gets
     the sum (may be x or add); weight: fp32 [cols] of an RMSNorm of the sum, else none is taken; normed: gets the normed rows in x's
-    type (may be x or add, not total). out: buffers of those sizes, written again."""
+    type (may be x or add, not total). out: buffers of those sizes, apart from the others, written again."""
     shape, dtype, index = x.shape, x.dtype, x.get_device()
     if len(shape) != 2 or dtype not in _TYPE or index < 0 or x.stride(1) != 1:
         _wants("x", x, None, None, -1)
@@ -148,7 +148,7 @@ class Fp8Weight:
 
     def product(self, x: Fp8Rows, dtype=torch.float32, add=None, out=None):
         """x weight^T [rows][n], in out's type if it is given, else in dtype (fp32 or bf16); add: added before the one rounding, of
-        the result's type (may be out)."""
+        the result's type (may be out). out: apart from the rows' and the weight's codes and scales."""
         q, scale = x
         _codes("x", q, scale, 1, self.index)
         rows, cols = q.shape

@@ -369,15 +369,17 @@ typedef struct fn_fp8_t {  /* a weight */
  * what comes before: h = x + add (add NULL: h = x), rounded to the type and written to total (NULL: not written); with weight [cols]
  * (fp32, 16-byte aligned) y = h (mean h^2 + eps)^-1/2 weight, else y = h; y, rounded to the type, written to normed (NULL: not);
  * y unrounded as codes and scales (both NULL: not). The sum of squares is held in 64 bits. total and normed may be x or add, the same
- * rows; rows that are written and share memory in another way are refused. */
+ * rows; rows that are written and share memory in another way are refused (with other strides than theirs also rows that lie between
+ * them), and so are codes, scales and weights that share memory with rows or with one another. */
 int fn_fp8_rows(uint32_t type, const void *x, int64_t x_stride, const void *add, int64_t add_stride, const float *weight, float eps,
                 int rows, int cols, void *total, int64_t total_stride, void *normed, int64_t normed_stride, uint8_t *codes,
                 float *scales, void *stream);
-/* A weight [rows][cols] of `type` (row stride in elements) as codes and scales of 128 x 128 blocks. */
+/* A weight [rows][cols] of `type` (row stride in elements) as codes and scales of 128 x 128 blocks, in memory of their own. */
 int fn_fp8_blocks(uint32_t type, const void *w, int64_t stride, int rows, int cols, uint8_t *codes, float *scales, void *stream);
 /* out[i][j] = sum_g scales[i][g] w->scales[j / 128][g] sum_{k in group g} codes[i][k] w->codes[j][k] (+ add[i][j]) for i < rows,
  * j < w->rows, on the tensor cores: fp32 sums, `type` F32 or BF16 for out and add (row strides in elements, columns adjacent; add may
- * be NULL, or out itself, but no other rows of it). codes, scales: rows as fn_fp8_rows makes them, of w->cols columns. */
+ * be NULL, or out itself, but no other rows of it; out lies over no codes or scales). codes, scales: rows as fn_fp8_rows makes them, of
+ * w->cols columns. */
 int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *scales, int rows, uint32_t type, const void *add,
                    int64_t add_stride, void *out, int64_t out_stride, void *stream);
 
