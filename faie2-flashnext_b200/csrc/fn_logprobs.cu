@@ -19,6 +19,8 @@
 // pass (32 rows of fp32: 11.5 us, without alternatives 8.0, where the bytes take 3).
 #include <cuda_bf16.h>
 
+#include <utility>
+
 #include "fn_argmax.cuh"
 #include "fn_engine.h"
 #include "fn_kv4.h"
@@ -628,7 +630,11 @@ FN_API int fn_logprobs(uint32_t type, const void *logits, int64_t stride, int ro
         if (rows == 0) return 0;
         if (!logits || (top && (!top_ids || !top_logprobs))) return fail("logprobs: null pointer");
         if (!tokens && (logprob || rank)) return fail("logprobs: log probabilities and ranks want tokens");
-        if ((uintptr_t)logits % (type == T_F32 ? 4 : 2)) return fail("logprobs: logits must be aligned to their type");
+        const int64_t size = type == T_F32 ? 4 : 2, one = (int64_t)rows * 4;
+        if ((uintptr_t)logits % size) return fail("logprobs: logits must be aligned to their type");
+        for (const auto &[out, n] : {std::pair<const void *, int64_t>(logprob, one), {rank, one}, {entropy, one}, {top_ids, one * top}, {top_logprobs, one * top}})
+            if (rows_meet_bytes(logits, stride * size, rows, vocab * size, out, n) || ((out != tokens || n != one) && rows_meet_bytes(tokens, 0, 1, one, out, n)))
+                return fail("logprobs: results lie over logits or tokens");
         // rows that the SMs can take at once get CTAs of 1024 threads, and up to 8 of them (of 4096 entries and more) where they are fewer;
         // else CTAs of 256 share an SM
         const bool large = rows <= num_sms();

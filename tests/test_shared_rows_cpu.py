@@ -56,6 +56,19 @@ def test_products_over_what_they_read(libpath, change):
         FN(libpath).fp8_product(C.byref(FnFp8(c["weight"], c["w_scales"], 64, 64)), c["codes"], c["scales"], 3, 0, None, 0, AT, c["out_stride"])
 
 
+SCORES = dict(dtype=0, logits=AT, stride=128, rows=4, vocab=100, tokens=AT << 1, logprob=AT << 2, rank=AT << 3, entropy=AT << 4, top=3, top_ids=AT << 5,
+              top_logprobs=AT << 6)
+
+
+@pytest.mark.parametrize("change", [
+    dict(logprob=AT), dict(rank=AT - 12), dict(entropy=AT + 3 * 512 + 396), dict(top_ids=AT + 512), dict(top_logprobs=AT - 44), dict(dtype=30, rank=AT + 256),
+    dict(stride=-128, rank=AT - 3 * 512), dict(stride=0, top_ids=AT + 396), dict(logprob=(AT << 1) + 4), dict(rank=(AT << 1) - 4),
+    dict(top_ids=AT << 1), dict(top_logprobs=(AT << 1) - 44)])
+def test_scores_over_what_they_read(libpath, change):
+    with pytest.raises(RuntimeError, match="lie over logits or tokens"):
+        FN(libpath).logprobs(**{**SCORES, **change})
+
+
 def run(tmp_path, body):
     src = tmp_path / "t.cpp"
     src.write_text('#include <cstdio>\n#include <random>\n#include <set>\n#include "fn_rows.h"\nint main() {\n std::mt19937 r(1);\n'
