@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from fn import FnFp8
-from kv4 import _TYPE, _stream
+from kv4 import _TYPE, Fixed, _stream
 
 GROUP = 128  # columns (and weight rows) that share a scale
 CODES = torch.float8_e4m3fn
@@ -113,8 +113,10 @@ def add_norm(fn, x, add, weight, eps: float, total, normed) -> None:
                 total.stride(0), normed.data_ptr(), normed.stride(0), None, None, _stream(x.device))
 
 
-class Fp8Weight:
-    """A weight [n][k]: codes q (float8_e4m3fn) and scales of 128 x 128 blocks, fp32 [ceil(n / 128)][ceil(k / 128)]."""
+class Fp8Weight(Fixed):
+    """A weight [n][k]: codes q (float8_e4m3fn) and scales of 128 x 128 blocks, fp32 [ceil(n / 128)][ceil(k / 128)]. Their values may be
+    written anew (by q.copy_, say), the tensors stay these."""
+    FIXED = frozenset(("q", "scale", "rows", "cols"))
 
     def __init__(self, fn, q, scale):
         _codes("weight", q, scale, GROUP, q.get_device())

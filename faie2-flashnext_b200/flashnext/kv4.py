@@ -34,6 +34,16 @@ def record_bytes(hd: int, page_size: int) -> int:
     return 2 * page_size * (hd // 2 + hd // GROUP * 2)
 
 
+class Fixed:
+    """Attributes named in FIXED are set once: pointers that calls pass were taken from them."""
+    FIXED: frozenset = frozenset()
+
+    def __setattr__(self, name, value):
+        if name in self.FIXED and name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: make another {type(self).__name__}")
+        super().__setattr__(name, value)
+
+
 def _stream(dev) -> int:
     index = dev.index
     if torch.cuda.current_device() != index:  # kernels launch on the current device
