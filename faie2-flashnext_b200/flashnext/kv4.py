@@ -58,10 +58,11 @@ def _ints(name, t, shape, dev):
                          f"{tuple(t.shape)} on {t.device}")
 
 
-class KV4Plan:
+class KV4Plan(Fixed):
     """A planned step (device tensors): cu [n + 1], kv_len [n] (what attention reads: 0 for a refused request), ctx [n] (the lengths that
     requests go on with: a refused one's is unchanged), slots / positions / requests [max_tokens], free_count and status (refused
     requests), one value each."""
+    FIXED = frozenset(("cu", "kv_len", "ctx", "slots", "positions", "requests", "free_count", "status", "ptrs"))
 
     def __init__(self, n, max_tokens, dev):
         ints = torch.empty(3 * n + 3 + 2 * max_tokens, dtype=torch.int32, device=dev)
@@ -105,9 +106,10 @@ class KV4Planner:
         return out
 
 
-class KV4Workspace:
+class KV4Workspace(Fixed):
     """Scratch of the attention (split requests' partial results). Calls that may run at the same time, as on two
     streams, need one each."""
+    FIXED = frozenset(("tensor", "ptr", "bytes"))
 
     def __init__(self, fn, device="cuda"):
         self.bytes = fn.kv4_attn_workspace()
@@ -115,9 +117,10 @@ class KV4Workspace:
         self.ptr = self.tensor.data_ptr()
 
 
-class KV4Cache:
+class KV4Cache(Fixed):
     """Pages of one attention layer. pages: their number (a zeroed uint8 tensor [pages][nkv][record_bytes] is made), or
     that tensor."""
+    FIXED = frozenset(("pages", "nkv", "hd", "page_size"))
 
     def __init__(self, fn, nkv: int, hd: int, page_size: int, pages, workspace: KV4Workspace | None = None):
         if isinstance(pages, int):
