@@ -356,7 +356,8 @@ class BatchDecodeModel:
     def launch_step(self, s: int):
         """One decode step of every sequence on stream s (device pointers only; capturable)."""
         import torch
-        with torch.cuda.stream(torch.cuda.ExternalStream(s)):  # the layers over torch tensors launch on the current stream
+        # the layers over torch tensors launch on the current stream (ExternalStream takes 0 for no handle and makes a stream of its own)
+        with torch.cuda.stream(torch.cuda.ExternalStream(s) if s else torch.cuda.default_stream()):
             self._launch_step(s)
 
     def _launch_step(self, s: int):
