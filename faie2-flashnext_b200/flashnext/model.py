@@ -465,3 +465,10 @@ class BatchDecodeModel:
         for g in self.gdns:
             self.fn.gdn_free(g)
         self.tcs, self.moes, self.gdns = [], [], []
+        if self.dense == "fp8":  # weights and rows in torch's memory, which gives them to others at once
+            import torch
+            torch.cuda.synchronize()
+            for L in self.layers:
+                for name in ("w_in", "w_out", "w_qkv", "w_o"):
+                    L.pop(name, None)
+            self.head, self.rows8 = None, {}

@@ -1,5 +1,7 @@
 """GPU: what the models with 8-bit dense weights and scores keep and give back."""
 
+import gc
+
 import pytest
 import torch
 
@@ -29,3 +31,35 @@ def test_a_step_runs_on_the_stream_it_is_given(fn, small):
         assert at == [(0, 0)] * 2 + [(other.cuda_stream,) * 2] * 2
     finally:
         m.free()
+
+
+@pytest.mark.parametrize("serve", [False, True])
+@pytest.mark.parametrize("dense", ["gguf", "fp8"])
+def test_free_gives_the_dense_weights_back(fn, small, dense, serve):
+    from model import BatchDecodeModel
+    from serve import ServeModel
+    cfg, W = small
+
+    def make():
+        if serve:
+            return ServeModel(fn, cfg, W, batch=2, pages=4, max_ctx=16, page_size=16, dense=dense)
+        return BatchDecodeModel(fn, cfg, W, 2, max_ctx=16, dense=dense)
+
+    def held():
+        gc.collect()
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated()
+
+    make().free()  # (what a first model leaves: the planner's and the library's own)
+    m = make()
+    before = held()
+    dense_bytes = sum(t.numel() for t in weights(m)) if dense == "fp8" else 0
+    m.free()
+    assert before - held() >= dense_bytes
+    m.free()  # again is nothing
+
+
+def weights(m):
+    from fp8 import Fp8Weight
+    found = [m.head, *(v for L in m.layers for v in L.values())]
+    return [v.q for v in found if isinstance(v, Fp8Weight)]
