@@ -22,11 +22,12 @@ from model import HD, BatchDecodeModel
 
 
 class OutOfPages(RuntimeError):
-    """A step found too few free pages. outs: what generate would have returned, None for requests that were not finished."""
+    """A step found too few free pages. outs: what generate would have returned, None for requests that were not finished; scores: the same of
+    their Scores (None if none were asked for)."""
 
-    def __init__(self, message, outs):
+    def __init__(self, message, outs, scores=None):
         super().__init__(message)
-        self.outs = outs
+        self.outs, self.scores = outs, scores
 
 
 class Scores(NamedTuple):
@@ -138,6 +139,7 @@ class ServeModel(BatchDecodeModel):
         at = [0] * self.B  # tokens fed of the place's request
         if scores is not None:
             said, kept, known = [[] for _ in prompts], None, np.full(self.B, -1, np.int32)  # known: the token that follows, if it is given
+        finished = lambda r: Scores(*(np.array(v) for v in zip(*said[r])))  # noqa: E731
         inputs, drop = np.zeros(self.B, np.int32), np.full(self.B, -1, np.int32)
         while waiting or any(r is not None for r in place):
             for b in range(self.B):
@@ -161,7 +163,8 @@ class ServeModel(BatchDecodeModel):
             self.fn.sync(stream.cuda_stream)
             if int(self.plan.status):
                 done = [np.array(s, np.int32) if len(s) == len(p) + n else None for s, p, n in zip(seq, prompts, n_new)]
-                raise OutOfPages(f"out of pages: {int(self.plan.status)} of the batch found none (of {self.n_pages})", done)
+                raise OutOfPages(f"out of pages: {int(self.plan.status)} of the batch found none (of {self.n_pages})", done,
+                                 None if scores is None else [None if o is None else finished(r) for r, o in enumerate(done)])
             new = self.next.cpu().numpy()
             if scores is not None:
                 step = [t.cpu().numpy() for t in kept]
@@ -178,4 +181,4 @@ class ServeModel(BatchDecodeModel):
                 if len(seq[r]) == len(prompts[r]) + n_new[r]:
                     place[b] = None
         outs = [np.array(s, np.int32) for s in seq]
-        return outs if scores is None else (outs, [Scores(*(np.array(v) for v in zip(*t))) for t in said])
+        return outs if scores is None else (outs, [finished(r) for r in range(len(outs))])

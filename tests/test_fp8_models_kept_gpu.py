@@ -2,6 +2,7 @@
 
 import gc
 
+import numpy as np
 import pytest
 import torch
 
@@ -63,3 +64,24 @@ def weights(m):
     from fp8 import Fp8Weight
     found = [m.head, *(v for L in m.layers for v in L.values())]
     return [v.q for v in found if isinstance(v, Fp8Weight)]
+
+
+@pytest.mark.parametrize("top", [0, 3])
+def test_scores_of_what_was_finished_are_kept(fn, small, top):
+    from serve import OutOfPages, ServeModel
+    m, s = ServeModel(fn, *small, batch=3, pages=8, max_ctx=48, page_size=16), torch.cuda.Stream()
+    m.capture(s)
+    try:
+        with pytest.raises(OutOfPages, match="out of pages") as e:
+            m.generate([[1, 2], [1] * 40, [1] * 40, [1] * 40], [2, 8, 8, 8], s, scores=top)
+        outs, scores = e.value.outs, e.value.scores
+        alone, said = m.generate([[1, 2]], 2, s, scores=top)
+        assert len(scores) == 4 and scores[3] is None and [o is None for o in outs] == [q is None for q in scores]
+        assert np.array_equal(outs[0], alone[0])
+        for got, want in zip(scores[0], said[0]):
+            assert np.array_equal(got, want) and len(got) == 3
+        with pytest.raises(OutOfPages) as e:
+            m.generate([[1, 2], [1] * 40, [1] * 40, [1] * 40], [2, 8, 8, 8], s)
+        assert e.value.scores is None
+    finally:
+        m.free()
