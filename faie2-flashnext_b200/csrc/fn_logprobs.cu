@@ -165,6 +165,7 @@ template <> struct LpAcc<float> {
         if (x > m) raise(x);
         pair(x, -INFINITY);
     }
+    __device__ __forceinline__ void clear() { s = t = 0; }
     __device__ __forceinline__ LpSum sum() const {
         float s0, s1, t0, t1;
         lp_untwo(s, s0, s1);
@@ -267,6 +268,7 @@ template <> struct LpAcc<__nv_bfloat16> {
         if (far) equal(x);
         else pair(__float_as_uint(x) >> 16 | 0xff800000u);  // (beside -inf)
     }
+    __device__ __forceinline__ void clear() { s0 = s1 = t0 = t1 = 0.0f; }
     __device__ __forceinline__ LpSum sum() const {  // counted from b
         const float y = far ? 0.0f : fmaf(b, LP_LOG2E, -c), f = lp_ex2(-y), z = s0 + s1;
         return LpSum{m, b, f * z, f * (t0 + t1 - y * z)};
@@ -343,20 +345,42 @@ template <typename P> __device__ __forceinline__ void lp_store(P *p, uint32_t ra
     }
 }
 
+// Rounds of words that a thread's sums take in fp32 (up to 512 terms each, whose additions are off by 2^-15 of it at the very worst) before
+// they join sums in 64 bits: in fp32 alone rows of 2^26 entries lost up to 5e-4.
+constexpr int LP_FOLD = 32;
+template <int THREADS> struct LpFold {  // every thread's own: sums counted from b
+    double s[THREADS], t[THREADS];
+    float b[THREADS];
+    __device__ __forceinline__ void add(const LpSum &c, bool first) {
+        double s0 = 0.0, t0 = 0.0;
+        if (!first) {
+            const float y = fmaxf((b[threadIdx.x] - c.b) * LP_LOG2E, LP_FAR), f = lp_ex2(y);
+            s0 = f * s[threadIdx.x], t0 = f * (t[threadIdx.x] + y * s[threadIdx.x]);
+        }
+        s[threadIdx.x] = s0 + c.s, t[threadIdx.x] = t0 + c.t;
+        b[threadIdx.x] = c.b;
+    }
+};
+
 template <int THREADS> struct LpShared {
     static constexpr int W = THREADS / 32, SEGMENTS = 4096 / THREADS;
     LpSum sums[W];
     int before[W];
     uint32_t ends[2][W];
-    unsigned long long keys[W * LP_MAX_TOP];  // (as many as a cluster's at least)
+    union {
+        LpFold<THREADS> fold;  // while the words are read; then
+        struct {
+            unsigned long long keys[W * LP_MAX_TOP];  // (as many as a cluster's at least)
+            int columns[THREADS];                     // segments that are read again
+        };
+    };
     unsigned long long best[LP_MAX_TOP];  // this CTA's alternatives, in order
     LpSum sum;                            // the row's
     LpSum part[LP_MAX_CLUSTER];           // what the cluster's CTAs found
     int before_of[LP_MAX_CLUSTER];
     unsigned long long keys_of[LP_MAX_CLUSTER][LP_MAX_TOP];
     int count, n_keys, n_columns;
-    int columns[THREADS];                 // segments that are read again
-    uint32_t most[SEGMENTS][THREADS];     // the largest entry (in order) of every segment
+    uint32_t most[SEGMENTS][THREADS];  // the largest entry (in order) of every segment
 };
 
 // What a CTA does once a row is out of line and rolled where it is called more than once: of a short call's time a good part is fetching
@@ -427,6 +451,7 @@ template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, LP_T == 
         typename LpAcc<T>::Most most = LpAcc<T>::none();
 #pragma unroll 1
         for (const int end = min(rounds, i + per); i < end; ++i) {
+            if (i && i % LP_FOLD == 0) sh.fold.add(acc.sum(), i == LP_FOLD), acc.clear();
             const int w = w0 + i * U * LP_T + tid;
             const uint4 *p = v + w;
             uint4 r[U];
@@ -475,7 +500,11 @@ template <typename T, int LP_T> __global__ void __launch_bounds__(LP_T, LP_T == 
         acc.one(e);
         if (known) before += lp_stands_before(e, odd, token, given, above);
     }
-    const LpSum sum = acc.sum();
+    LpSum sum = acc.sum();
+    if (rounds > LP_FOLD) {
+        sh.fold.add(sum, false);
+        sum.s = (float)sh.fold.s[tid], sum.t = (float)sh.fold.t[tid];
+    }
     const uint32_t mine = lp_order(sum.m);
     const LpSum all = lp_warp_join(sum);
     before = __reduce_add_sync(0xffffffffu, before);

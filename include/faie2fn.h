@@ -391,7 +391,8 @@ int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *scales,
  * tokens may be NULL if logprob and rank are. Entries at -inf have no probability and are no alternatives; places that stay empty
  * hold -1 and -inf. tokens[row] < 0: no token, logprob 0 and rank -1; past the vocabulary: NaN and -1, reported by fn_sync. A row
  * with a NaN or +inf has logprob, entropy and top_logprobs NaN (a NaN is no alternative, and its rank is -1); a row of nothing but
- * -inf has log probabilities -inf and entropy 0. Sums are fp32. Results lie apart from logits and tokens (logprob, rank or entropy may be
+ * -inf has log probabilities -inf and entropy 0. Sums are fp32, those of long rows in parts that join in 64 bits: the logarithm of a
+ * row's sum is right within 2^-15 whatever the vocabulary. Results lie apart from logits and tokens (logprob, rank or entropy may be
  * tokens itself). Allocates nothing, keeps nothing: calls may overlap. */
 int fn_logprobs(uint32_t type, const void *logits, int64_t stride, int rows, int vocab, const int *tokens, float *logprob,
                 int *rank, float *entropy, int top, int *top_ids, float *top_logprobs, void *stream);
