@@ -125,8 +125,8 @@ class Fp8Weight(Fixed):
         self._keep(fn, q, scale)
 
     def _keep(self, fn, q, scale):
-        self.fn, self.q, self.scale, self.dev, self.index, self.c = fn, q, scale, q.device, q.get_device(), None
-        self.rows, self.cols = q.shape
+        rows, cols = q.shape  # (a dictionary's update: attributes one by one cost a weight's quantising 1.3 us)
+        self.__dict__.update(fn=fn, q=q, scale=scale, dev=q.device, index=q.get_device(), c=None, rows=rows, cols=cols)
 
     @classmethod
     def quantise(cls, fn, w):
