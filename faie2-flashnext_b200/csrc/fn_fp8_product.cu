@@ -862,9 +862,9 @@ FN_API int fn_fp8_product(const fn_fp8_t *w, const uint8_t *codes, const float *
         a.wide = (((uintptr_t)out | (uintptr_t)add) % 16 | (uint64_t)a.n % per | (uint64_t)out_stride % per | (uint64_t)add_stride % per) == 0;
         const int64_t sms = num_sms(), tm = fp8_groups(rows), waves = (fp8_groups(a.n) * tm + sms - 1) / sms;  // of tiles of 128 x 128
         const int64_t wide_tiles = (int64_t)((rows + 255) / 256) * ((a.n + 255) / 256), wide_waves = (wide_tiles + sms / 2 - 1) / (sms / 2);
-        // A group takes a pair of SMs 0.55 us for 256 x 256, a single one 0.37 us for 128 x 128 (K 4096): pairs where their fewer waves save
-        // more than that. 768 x 12352, K 2048, fp32: 25.3 us by pairs, 30.1 by single SMs; 512 x 12352: 24.3 and 23.0; 1024 x 2048, K 4096:
-        // 20.7 and 14.8; 2048 x 2048: 21.8 and 26.6.
+        // A group takes a pair of SMs 0.47 to 0.50 us for 256 x 256, a single one 0.33 us for 128 x 128 (K 4096 less K 2048): pairs where
+        // their fewer waves save more than that. 768 x 12352, K 2048, fp32: 25.3 us by pairs, 30.1 by single SMs; 512 x 12352: 24.3 and
+        // 23.0; 1024 x 2048, K 4096: 20.7 and 14.8; 2048 x 2048: 21.8 and 26.6.
         if (3 * wide_waves < 2 * waves && sms >= 2) {
             a.tiles_m = (rows + 255) / 256;
             if (wide_tiles * a.groups > INT32_MAX) return fail("fp8 product: too large");

@@ -14,8 +14,8 @@
 // maximum does, about k of 4096, spread over all threads, which list what reaches it. (If equal entries are too many to be listed, every
 // warp keeps its best 32 sorted over its lanes.)
 //
-// What bounds it: with many rows in bf16 instruction issue (11.5 an entry in all; 2048 x 151936: 137 us with 20 alternatives and tokens, 113 with
-// neither, where the bytes take 95 at the copy rate), in fp32 the loads (1024 rows: 114 and 97); with few rows the chain of steps behind the
+// What bounds it: with many rows in bf16 instruction issue (11.5 an entry in all; 2048 x 151936: 135 us with 20 alternatives and tokens, 109 with
+// neither, where the bytes take 95 at the copy rate), in fp32 the loads (1024 rows: 117, the bytes 95); with few rows the chain of steps behind the
 // pass (32 rows of fp32: 11.5 us, without alternatives 8.0, where the bytes take 3).
 #include <cuda_bf16.h>
 
@@ -415,8 +415,8 @@ __device__ __forceinline__ LpSum lp_warp_join(LpSum a) {
 }
 
 constexpr int LP_MAX_VOCAB = 1 << 28;  // so a segment has up to 2048 rounds, each with up to 16 entries of a half of the counter
-// CTAs of 256 threads on an SM: five where instructions bound it (bf16, 2048 rows of 151936: 137 us, by four 143; 200 rows, where
-// latency counts, 26.5 and 25.0), four where loads do (fp32, 1024 rows: 115 us, by five 122)
+// CTAs of 256 threads on an SM: five where instructions bound it (bf16, 2048 rows of 151936: 135 us, by four 145; 200 rows, where
+// latency counts, 27.2 and 26.9), four where loads do (fp32, 1024 rows: 117 us, by five 126)
 constexpr int lp_ctas(int size) { return size == 2 ? 5 : 4; }
 
 // grid: rows x C CTAs in clusters of C (a power of two up to 8) for a row
